@@ -294,6 +294,45 @@ int32_t ivb_batch_sample_merge(const uint32_t* keys, const int32_t* ids, int32_t
                                int64_t* history, int32_t history_len, const int32_t* step_counter, uint8_t* seen, int32_t v0,
                                int32_t vloc, void* stream);
 
+/* ---- 4-bit key/value cache ---------------------------------------------------------------------------
+ * Keys and values of `batch` sequences, `kv_heads` heads of `head_dim` (32, 64 or 128) values, `max_len`
+ * positions each, in 4 bits with one fp16 scale and offset per row of head_dim values:
+ *   offset = fp16(min x), scale = fp16((max x - offset) / 15), code = round((x - offset) / scale) in 0..15,
+ *   x ~ offset + scale * code; head_dim + 8 bytes per position and head for keys and values together.
+ * `data`: ivb_kv4_bytes bytes, 16-byte aligned: [batch][kv_heads][tiles of 16 positions, an even number]
+ * [key codes 8 head_dim bytes | value codes 8 head_dim bytes | 16 x (key scale, key offset, value scale,
+ * value offset) fp16], the order of the code words within a tile as csrc/ivb_kv4.cuh says. Bytes of positions
+ * that were never written are read by no result; they may hold anything.
+ *
+ * Rows of a call: sequence b holds rows starts[b] .. starts[b + 1] - 1 (device int32 [batch + 1], ascending)
+ * at positions positions[b], positions[b] + 1, ... (device int64 [batch]); starts NULL: row b is sequence
+ * b's only row (rows == batch). `rows` is the number of rows that the arrays have; rows from starts[batch]
+ * on are left as they are. A row at a negative position is idle: it is not written, not read, and attends to
+ * nothing (zeros). A row at max_len or beyond sets *error (device word, may be NULL) to IVB_ECAPACITY and is
+ * treated the same way. `dtype` is IVB_F32, IVB_F16 or IVB_BF16; strides are in values, channels contiguous.
+ * Nothing is allocated and nothing is kept between calls; calls on one cache are ordered by their stream. */
+enum { IVB_F32 = 0, IVB_F16 = 1, IVB_BF16 = 2 };
+typedef struct IvbKv4Cache {
+  void* data;
+  int32_t batch, kv_heads, head_dim, max_len;
+} IvbKv4Cache;
+uint64_t ivb_kv4_bytes(int32_t batch, int32_t kv_heads, int32_t head_dim, int32_t max_len);
+/* Quantises key and value rows k, v [rows][kv_heads][head_dim] into the cache. A row with an infinity or a
+ * NaN reads back as NaN; values beyond +-65504 are clipped. */
+int32_t ivb_kv4_append(const IvbKv4Cache* c, const void* k, const void* v, int32_t dtype, int64_t k_row, int64_t k_head,
+                       int64_t v_row, int64_t v_head, const int32_t* starts, const int64_t* positions, int32_t rows,
+                       uint32_t* error, void* stream);
+/* The rows as the cache holds them, into k, v [rows][kv_heads][head_dim]. */
+int32_t ivb_kv4_read(const IvbKv4Cache* c, void* k, void* v, int32_t dtype, int64_t k_row, int64_t k_head, int64_t v_row,
+                     int64_t v_head, const int32_t* starts, const int64_t* positions, int32_t rows, uint32_t* error,
+                     void* stream);
+/* Attention of the rows' queries q [rows][heads][head_dim] over their sequences' caches into out (same shape
+ * and type); query head h reads key/value head h / (heads / kv_heads). The row at position p sees positions
+ * j <= p with j > p - window or j < sinks (window 0: all j <= p). out = sum_j softmax_j(scale q.k_j) v_j. */
+int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
+                          const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,
+                          int32_t sinks, void* out, int64_t o_row, int64_t o_head, uint32_t* error, void* stream);
+
 /* Per-row max |x| (rows x n fp32) into amax [rows]; with ivb_quantize_rows_amax the quantisation of a
  * row-parallel shard uses the amax of the whole row (after an all-reduce MAX), so every shard's codes
  * equal the unsharded quantiser's: scale = max(amax / 127, act_eps), code = rint(x / scale). */

@@ -20,6 +20,7 @@ IVB_ABI_VERSION = 2
 IVB_OK, IVB_EINVAL, IVB_ECUDA, IVB_ETIMEOUT, IVB_ECAPACITY, IVB_EUNSUPPORTED = range(6)
 IVB_EPI_STORE, IVB_EPI_RESIDUAL, IVB_EPI_SILU_PAIR = range(3)
 IVB_MAMBA, IVB_MLA = 0, 1
+IVB_F32, IVB_F16, IVB_BF16 = range(3)
 IVB_RUN_SAMPLE, IVB_RUN_SAMPLE_ONLY, IVB_RUN_HEAD_ALL = 1, 2, 4
 
 
@@ -143,6 +144,16 @@ class IvbBatch(Structure):
     ]
 
 
+class IvbKv4Cache(Structure):
+    _fields_ = [
+        ("data", c_void_p),
+        ("batch", c_int32),
+        ("kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("max_len", c_int32),
+    ]
+
+
 SIGNATURES = {
     "ivb_abi_version": (c_int32, []),
     "ivb_last_error": (c_char_p, []),
@@ -182,6 +193,13 @@ SIGNATURES = {
                                          c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
     "ivb_rows_amax": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
     "ivb_quantize_rows_amax": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_float, c_void_p, c_int32, c_void_p, c_void_p]),
+    "ivb_kv4_bytes": (c_uint64, [c_int32, c_int32, c_int32, c_int32]),
+    "ivb_kv4_append": (c_int32, [POINTER(IvbKv4Cache), c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                 c_void_p, c_int32, c_void_p, c_void_p]),
+    "ivb_kv4_read": (c_int32, [POINTER(IvbKv4Cache), c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                               c_void_p, c_int32, c_void_p, c_void_p]),
+    "ivb_kv4_attention": (c_int32, [POINTER(IvbKv4Cache), c_void_p, c_int32, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_int32,
+                                    c_float, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
     "ivb_decoder_check": (c_int32, [c_void_p, c_void_p]),
 }
 
