@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <atomic>
 #include <type_traits>
 
@@ -66,16 +67,23 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// (a & b) | c in one instruction (two constants keep the compiler from it).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
+  return y;
+}
+
 // Two nibbles of a word as fp16 values u - 8: the bits under 0x6400 give 1024 + u and 1024 + 16 u, the rest is exact. The
 // bare bits, fp16 subnormals u 2^-24, would save this instruction, but the tensor cores align products by the operands'
 // exponent fields and cut 7 to 10 bits more of a subnormal's: 5e-5 of the output, measured.
 __device__ __forceinline__ uint32_t codes_low(uint32_t w) {
-  const uint32_t x = (w & 0x000f000fu) | 0x64006400u;
+  const uint32_t x = and_or(w, 0x000f000fu, 0x64006400u);
   const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(-1032.0f, -1032.0f));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 __device__ __forceinline__ uint32_t codes_high(uint32_t w) {
-  const uint32_t x = (w & 0x00f000f0u) | 0x64006400u;
+  const uint32_t x = and_or(w, 0x00f000f0u, 0x64006400u);
   const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-72.0f, -72.0f));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
@@ -103,39 +111,49 @@ __device__ __forceinline__ PositionTerms position_terms(uint2 par, float score_u
   return t;
 }
 
-// ---- few rows: one token per sequence, a few drafted ones, or any number in tiles of 16 (8 for fp32) rows -----------------
-// One cluster of C CTAs per (sequence, key/value head, tile of rows); row i of a sequence's head group is token i / group,
-// query head i % group of the group. The 32-position groups of the cache that a row of the tile sees are dealt out to the
-// cluster's warps in turn; each warp streams its own through a ring of cp.async stages, holds its scores and its online
-// softmax in registers (scores in the C fragment's layout are weights in the A fragment's), and the partial (reference,
-// sum, output) join in shared memory, then over the cluster's.
-template <int D, typename T>
+// ---- few rows: one token per sequence, a few drafted ones, or any number in tiles -----------------------------------------
+// One cluster of C CTAs of W warps per (sequence, key/value head, tile of rows); row i of a sequence's head group is token
+// i / group, query head i % group of the group. The 32-position groups of the cache that a row of the tile sees are dealt
+// out to the cluster's warps in turn; each warp streams its own through a ring of cp.async stages and joins what it found
+// with the others' in shared memory, then over the cluster's.
+//
+// The codes are the A operands, 16 positions (keys) or 16 channels (values) a product, and the rows are the columns of B: with
+// one to four rows half the products of the other order are needed, and half its accumulators. Scores leave the
+// first product as positions x rows in the C layout; an 8x8 transposition (movmatrix) makes them the second one's B.
+// Columns hold, per tile of 8: kSplit 4 rows, each as the fp16 of its values and next to it the remainder's; else 8 rows.
+template <int D, bool kSplit, int kTiles>
 struct RowsGeometry {
-  static constexpr bool split = std::is_same<T, float>::value;
-  static constexpr int rows = split ? 8 : 16;
-  static constexpr int warps = 8;
-  static constexpr int stages = D == 128 ? 2 : 4;
+  static constexpr int rows = (kSplit ? 4 : 8) * kTiles;
+  static constexpr int stages = D == 128 ? 2 : 3;
   static constexpr int group_bytes = kKv4Group * (D + 8);
-
-  static constexpr int ring_bytes = warps * stages * group_bytes;
+  static constexpr int warp_bytes = stages * group_bytes;
   static constexpr int comb_floats = rows * D + 3 * rows;
-  static constexpr int smem = ring_bytes + warps * kKv4Group * 24 + comb_floats * 4 + warps * rows * 3 * 4;
+  static constexpr int term_bytes = kKv4Group * 24;  // a float4 and a float2 for each position
+  static constexpr int smem(int warps) { return warps * (warp_bytes + term_bytes + rows * 12) + comb_floats * 4; }
 };
 
-template <int D, typename T>
-__global__ void __launch_bounds__(256, D == 128 ? 2 : 2) kv4_rows_kernel(Kv4Attention A, int tiles_per_sequence) {
-  using G = RowsGeometry<D, T>;
-  constexpr int R = G::rows, W = G::warps, kSteps = D / 16, kTile = kv4_tile_bytes(D), kSets = G::split ? 1 : 2;
-  constexpr int kOut = D / 8;  // column tiles of the output
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <int D, typename T, bool kSplit, int kTiles>
+__global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int tiles_per_sequence) {
+  using G = RowsGeometry<D, kSplit, kTiles>;
+  constexpr int R = G::rows, kSteps = D / 16, kTile = kv4_tile_bytes(D);
+  constexpr int kPer = kSplit ? 1 : 2;        // rows of a lane in a column tile
+  constexpr int kSets = kPer * kTiles;        // rows of a lane
+  constexpr int kOut = D / 16;                // 16-channel tiles of the output
   extern __shared__ __align__(128) unsigned char smem[];
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank()), W = blockDim.x >> 5;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  unsigned char* const ring = smem + warp * G::stages * G::group_bytes;
-  float4* const terms4 = reinterpret_cast<float4*>(smem + G::ring_bytes) + warp * kKv4Group;
-  float2* const terms2 = reinterpret_cast<float2*>(smem + G::ring_bytes + W * kKv4Group * 16) + warp * kKv4Group;
-  float* const comb = reinterpret_cast<float*>(smem + G::ring_bytes + W * kKv4Group * 24);  // [R][D], then ref, sum, offset [R]
-  float* const stats = comb + G::comb_floats;                                              // [W][R][3]
+  unsigned char* const ring = smem + warp * G::warp_bytes;
+  float4* const terms4 = reinterpret_cast<float4*>(smem + W * G::warp_bytes + warp * G::term_bytes);
+  float2* const terms2 = reinterpret_cast<float2*>(terms4 + kKv4Group);
+  float* const comb = reinterpret_cast<float*>(smem + W * (G::warp_bytes + G::term_bytes));  // [R][D], then ref, sum, offset [R]
+  float* const stats = comb + G::comb_floats;                                               // [W][R][3]
 
   // which rows
   const int64_t cluster_id = blockIdx.x / C;
@@ -154,13 +172,13 @@ __global__ void __launch_bounds__(256, D == 128 ? 2 : 2) kv4_rows_kernel(Kv4Atte
   const int64_t base = __ldg(A.positions + b);
   const int64_t first = base + i0 / A.group, last = base + (i0 + live - 1) / A.group;
   const int max_len = A.cache.max_len;
-  // position of this lane's rows (-1: sees nothing)
-  int at[kSets], sum_row[kSets];
+  // row of the tile that set s of this lane holds, and its position (-1: sees nothing)
+  auto row_of = [&](int s) { return kSplit ? 4 * s + c : 8 * (s >> 1) + 2 * c + (s & 1); };
+  int at[kSets];
 #pragma unroll
   for (int s = 0; s < kSets; ++s) {
-    const int64_t p = base + (i0 + r + 8 * s) / A.group;
-    at[s] = r + 8 * s < live && p >= 0 && p < max_len ? static_cast<int>(p) : -1;
-    sum_row[s] = r + 8 * s;
+    const int64_t p = base + (i0 + row_of(s)) / A.group;
+    at[s] = row_of(s) < live && p >= 0 && p < max_len ? static_cast<int>(p) : -1;
   }
   if (last >= max_len && threadIdx.x == 0 && rank == 0 && A.error != nullptr) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
   // the groups of 32 positions that some row sees: the sinks' below the window, then the window's
@@ -174,74 +192,83 @@ __global__ void __launch_bounds__(256, D == 128 ? 2 : 2) kv4_rows_kernel(Kv4Atte
   const int steps = groups > mine ? (groups - mine + lanes_in - 1) / lanes_in : 0;
 
   const unsigned char* const codes = static_cast<const unsigned char*>(A.cache.data) +
-                                     (static_cast<int64_t>(b) * A.cache.kv_heads + kvh) * kv4_tiles(max_len) * kTile;
+                                     (static_cast<int64_t>(b) * A.cache.kv_heads + kvh) * kv4_tiles(max_len) * kTile + lane * 16;
   auto group_of = [&](int step) {
     const int i = mine + step * lanes_in;
     return i < sink_groups ? i : window_group + i - sink_groups;
   };
-  auto issue = [&](int step) {
+  auto issue = [&](int step, int stage) {
     if (step < steps) {
       const unsigned char* src = codes + static_cast<int64_t>(group_of(step)) * G::group_bytes;
-      unsigned char* dst = ring + step % G::stages * G::group_bytes;
+      unsigned char* dst = ring + stage * G::group_bytes + lane * 16;
 #pragma unroll
       for (int o = 0; o < G::group_bytes; o += 512)
-        if (o + lane * 16 < G::group_bytes) cp_async16(dst + o + lane * 16, src + o + lane * 16);
+        if (o + 512 <= G::group_bytes || lane * 16 < G::group_bytes - o) cp_async16(dst + o, src + o);
     }
     cp_async_commit();
   };
 #pragma unroll
-  for (int s = 0; s < G::stages - 1; ++s) issue(s);
+  for (int s = 0; s < G::stages - 1; ++s) issue(s, s);
 
-  // queries as A fragments, scaled by a power of two that brings the largest to 2^13: channels D/4 c + 4 s + {0, 1} and
-  // {2, 3}
-  float amax = 0.0f, sum_q[kSets];
-  float qv[kSets][D / 4];
+  // queries as B fragments (this lane: column r, channels D/4 c .. of its row), scaled by a power of two that brings the
+  // largest to 2^13
+  uint32_t qf[kTiles][kSteps][2];
+  float sum_q[kSets];
+  float score_unit, offset_unit;
+  {
+    float qv[kTiles][D / 4];
+    float amax = 0.0f, total[kTiles];
 #pragma unroll
-  for (int s = 0; s < kSets; ++s) {
-    sum_q[s] = 0.0f;
+    for (int n = 0; n < kTiles; ++n) {
+      const int row = kSplit ? 4 * n + (r >> 1) : 8 * n + r;
 #pragma unroll
-    for (int j = 0; j < D / 4; ++j) qv[s][j] = 0.0f;
-    const int64_t i = i0 + sum_row[s];
-    if (sum_row[s] < live) {
-      const int64_t t = i / A.group;
-      const int h = kvh * A.group + static_cast<int>(i - t * A.group);
-      load_values<T, D / 4>(static_cast<const T*>(A.q) + (row0 + t) * A.q_row + h * A.q_head + D / 4 * c, A.q_vec, qv[s]);
-    }
-#pragma unroll
-    for (int j = 0; j < D / 4; ++j) {
-      sum_q[s] += qv[s][j];
-      const float m = fabsf(qv[s][j]);
-      if (m <= 3.402823466e38f) amax = fmaxf(amax, m);
-    }
-    sum_q[s] += __shfl_xor_sync(0xFFFFFFFFu, sum_q[s], 1);
-    sum_q[s] += __shfl_xor_sync(0xFFFFFFFFu, sum_q[s], 2);
-  }
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
-  int up = 13 - (static_cast<int>(__float_as_uint(amax) >> 23) - 127);
-  up = amax == 0.0f ? 0 : min(max(up, -100), 100);
-  const float q_unit = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-  const float score_unit = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * A.scale * kLog2e;
-  const float offset_unit = A.scale * kLog2e;
-  uint32_t qf[kSteps][4];
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float x0 = qv[0][4 * s + 2 * e] * q_unit, x1 = qv[0][4 * s + 2 * e + 1] * q_unit;
-      qf[s][2 * e] = pack_f16(x0, x1);
-      if constexpr (G::split) {
-        const float2 hi = unpack_f16(qf[s][2 * e]);
-        qf[s][2 * e + 1] = pack_f16(x0 - hi.x, x1 - hi.y);
-      } else {
-        qf[s][2 * e + 1] = pack_f16(qv[kSets - 1][4 * s + 2 * e] * q_unit, qv[kSets - 1][4 * s + 2 * e + 1] * q_unit);
+      for (int j = 0; j < D / 4; ++j) qv[n][j] = 0.0f;
+      if (row < live) {
+        const int64_t t = (i0 + row) / A.group;
+        const int h = kvh * A.group + static_cast<int>(i0 + row - t * A.group);
+        load_values<T, D / 4>(static_cast<const T*>(A.q) + (row0 + t) * A.q_row + h * A.q_head + D / 4 * c, A.q_vec, qv[n]);
       }
+      total[n] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < D / 4; ++j) {
+        total[n] += qv[n][j];
+        const float m = fabsf(qv[n][j]);
+        if (m <= 3.402823466e38f) amax = fmaxf(amax, m);
+      }
+      total[n] += __shfl_xor_sync(0xFFFFFFFFu, total[n], 1);
+      total[n] += __shfl_xor_sync(0xFFFFFFFFu, total[n], 2);
     }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
+#pragma unroll
+    for (int s = 0; s < kSets; ++s)  // from the lanes that hold the row as a column
+      sum_q[s] = __shfl_sync(0xFFFFFFFFu, total[kSplit ? s : s >> 1], kSplit ? 8 * c : 4 * (2 * c + (s & 1)));
+    int up = 13 - (static_cast<int>(__float_as_uint(amax) >> 23) - 127);
+    up = amax == 0.0f ? 0 : min(max(up, -100), 100);
+    const float q_unit = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+    offset_unit = A.scale * kLog2e;
+    score_unit = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * offset_unit;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x0 = qv[n][4 * s + 2 * e] * q_unit, x1 = qv[n][4 * s + 2 * e + 1] * q_unit;
+          uint32_t w = pack_f16(x0, x1);
+          if (kSplit && (r & 1)) {
+            const float2 hi = unpack_f16(w);
+            w = pack_f16(x0 - hi.x, x1 - hi.y);
+          }
+          qf[n][s][e] = w;
+        }
   }
 
-  float acc[kOut][4];
+  float acc[kTiles][kOut][4];
 #pragma unroll
-  for (int i = 0; i < kOut; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+  for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.0f;
   float ref[kSets], sum[kSets], off[kSets];
 #pragma unroll
   for (int s = 0; s < kSets; ++s) {
@@ -249,10 +276,11 @@ __global__ void __launch_bounds__(256, D == 128 ? 2 : 2) kv4_rows_kernel(Kv4Atte
     sum[s] = off[s] = 0.0f;
   }
 
+  int at_stage = 0, to_stage = G::stages - 1;
   for (int step = 0; step < steps; ++step) {
     cp_async_wait<G::stages - 2>();
     __syncwarp();
-    const unsigned char* const stage = ring + step % G::stages * G::group_bytes;
+    const unsigned char* const stage = ring + at_stage * G::group_bytes;
     const int p0 = group_of(step) * kKv4Group;
     {
       const uint2 par = *reinterpret_cast<const uint2*>(stage + (lane >> 4) * kTile + 16 * D + (lane & 15) * 8);
@@ -261,13 +289,14 @@ __global__ void __launch_bounds__(256, D == 128 ? 2 : 2) kv4_rows_kernel(Kv4Atte
       terms2[lane] = make_float2(t.unbias, t.value_offset);
     }
     __syncwarp();
-    // scores of 8 positions per lane and set: x[set][4 tile + i] is position p0 + 16 tile + 4 c + i
-    float x[kSets][8];
+    // scores: x[set][2 tile + half] is position p0 + 16 tile + 4 (r / 2) + r % 2 + 2 half
+    const int mine_of = 4 * (r >> 1) + (r & 1);
+    float x[kSets][4], mantissa[4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      float s2[2][4];
+      float s2[kTiles][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) s2[h][0] = s2[h][1] = s2[h][2] = s2[h][3] = 0.0f;
+      for (int n = 0; n < kTiles; ++n) s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.0f;
       uint32_t w[2][D / 32];
       const uint32_t* kw = reinterpret_cast<const uint32_t*>(stage + t * kTile);
       if constexpr (D == 32) {
@@ -291,21 +320,20 @@ __global__ void __launch_bounds__(256, D == 128 ? 2 : 2) kv4_rows_kernel(Kv4Atte
         }
       }
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
+      for (int s = 0; s < kSteps; ++s) {
+        const uint32_t v0 = s & 1 ? w[0][s >> 1] >> 8 : w[0][s >> 1], v1 = s & 1 ? w[1][s >> 1] >> 8 : w[1][s >> 1];
+        const uint32_t a0 = codes_low(v0), a1 = codes_low(v1), a2 = codes_high(v0), a3 = codes_high(v1);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t v = s & 1 ? w[h][s >> 1] >> 8 : w[h][s >> 1];
-          mma_f16(s2[h], qf[s][0], qf[s][1], qf[s][2], qf[s][3], codes_low(v), codes_high(v));
-        }
+        for (int n = 0; n < kTiles; ++n) mma_f16(s2[n], a0, a1, a2, a3, qf[n][s][0], qf[n][s][1]);
+      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 pt = terms4[16 * t + 4 * c + i];
-        const int h = i >> 1, e = i & 1;
-        if constexpr (G::split) {
-          x[0][4 * t + i] = fmaf(s2[h][e] + s2[h][e + 2], pt.x, fmaf(sum_q[0], pt.y, pt.z));
-        } else {
-          x[0][4 * t + i] = fmaf(s2[h][e], pt.x, fmaf(sum_q[0], pt.y, pt.z));
-          x[kSets - 1][4 * t + i] = fmaf(s2[h][e + 2], pt.x, fmaf(sum_q[kSets - 1], pt.y, pt.z));
+      for (int h = 0; h < 2; ++h) {
+        const float4 pt = terms4[16 * t + mine_of + 2 * h];
+        mantissa[2 * t + h] = pt.w;
+#pragma unroll
+        for (int s = 0; s < kSets; ++s) {
+          const float dot = kSplit ? s2[s][2 * h] + s2[s][2 * h + 1] : s2[s >> 1][2 * h + (s & 1)];
+          x[s][2 * t + h] = fmaf(dot, pt.x, fmaf(sum_q[s], pt.y, pt.z));
         }
       }
     }
@@ -315,8 +343,8 @@ __global__ void __launch_bounds__(256, D == 128 ? 2 : 2) kv4_rows_kernel(Kv4Atte
 #pragma unroll
       for (int s = 0; s < kSets; ++s)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int p = p0 + 16 * (i >> 2) + 4 * c + (i & 3);
+        for (int i = 0; i < 4; ++i) {
+          const int p = p0 + 16 * (i >> 1) + mine_of + 2 * (i & 1);
           const bool seen = p <= at[s] && (A.window <= 0 || p > at[s] - A.window || p < A.sinks);
           if (!seen) x[s][i] = -INFINITY;
         }
@@ -325,170 +353,216 @@ __global__ void __launch_bounds__(256, D == 128 ? 2 : 2) kv4_rows_kernel(Kv4Atte
     float next[kSets];
 #pragma unroll
     for (int s = 0; s < kSets; ++s) {
-      float m = fmaxf(fmaxf(fmaxf(x[s][0], x[s][1]), fmaxf(x[s][2], x[s][3])), fmaxf(fmaxf(x[s][4], x[s][5]), fmaxf(x[s][6], x[s][7])));
-      m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+      float m = fmaxf(fmaxf(x[s][0], x[s][1]), fmaxf(x[s][2], x[s][3]));
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
       next[s] = fmaxf(ref[s], m);
       raise |= next[s] > ref[s];
     }
     if (__any_sync(0xFFFFFFFFu, raise)) {
-      float corr[kSets];
 #pragma unroll
       for (int s = 0; s < kSets; ++s) {
-        corr[s] = next[s] > ref[s] ? ex2(ref[s] - next[s]) : 1.0f;
+        const float corr = next[s] > ref[s] ? ex2(ref[s] - next[s]) : 1.0f;
         ref[s] = next[s];
-        sum[s] *= corr[s];
-        off[s] *= corr[s];
-      }
+        sum[s] *= corr;
+        off[s] *= corr;
 #pragma unroll
-      for (int i = 0; i < kOut; ++i) {
-        acc[i][0] *= corr[0];
-        acc[i][1] *= corr[0];
-        acc[i][2] *= corr[kSets - 1];
-        acc[i][3] *= corr[kSets - 1];
+        for (int i = 0; i < kOut; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if constexpr (kSplit) {
+              acc[s][i][2 * j] *= corr;
+              acc[s][i][2 * j + 1] *= corr;
+            } else {
+              acc[s >> 1][i][2 * j + (s & 1)] *= corr;
+            }
+          }
       }
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      float wgt[kSets][4];
+      uint32_t bw[kTiles][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float mantissa = terms4[16 * t + 4 * c + i].w;
-        const float2 pt = terms2[16 * t + 4 * c + i];
+      for (int h = 0; h < 2; ++h) {
+        const float2 pt = terms2[16 * t + mine_of + 2 * h];
+        float wgt[kSets];
 #pragma unroll
         for (int s = 0; s < kSets; ++s) {
-          const float xi = x[s][4 * t + i];
+          const float xi = x[s][2 * t + h];
           const float pw = ex2(xi - ref[s]);
           if (whole) {
             sum[s] = fmaf(pw, pt.x, sum[s]);
             off[s] = fmaf(pw, pt.y, off[s]);
-            wgt[s][i] = pw * mantissa;
+            wgt[s] = pw * mantissa[2 * t + h];
           } else {  // a masked position's terms may hold anything
             const bool seen = xi != -INFINITY;
             sum[s] = seen ? fmaf(pw, pt.x, sum[s]) : sum[s];
             off[s] = seen ? fmaf(pw, pt.y, off[s]) : off[s];
-            wgt[s][i] = seen ? pw * mantissa : 0.0f;
+            wgt[s] = seen ? pw * mantissa[2 * t + h] : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          if constexpr (kSplit) {
+            const __half hi = __float2half_rn(wgt[n]);
+            const __half2 both = __halves2half2(hi, __float2half_rn(wgt[n] - __half2float(hi)));
+            bw[n][h] = transpose8(*reinterpret_cast<const uint32_t*>(&both));
+          } else {
+            bw[n][h] = transpose8(pack_f16(wgt[2 * n], wgt[2 * n + 1]));
           }
         }
       }
-      uint32_t a[4];
-      a[0] = pack_f16(wgt[0][0], wgt[0][1]);
-      a[2] = pack_f16(wgt[0][2], wgt[0][3]);
-      if constexpr (G::split) {
-        const float2 h0 = unpack_f16(a[0]), h1 = unpack_f16(a[2]);
-        a[1] = pack_f16(wgt[0][0] - h0.x, wgt[0][1] - h0.y);
-        a[3] = pack_f16(wgt[0][2] - h1.x, wgt[0][3] - h1.y);
-      } else {
-        a[1] = pack_f16(wgt[kSets - 1][0], wgt[kSets - 1][1]);
-        a[3] = pack_f16(wgt[kSets - 1][2], wgt[kSets - 1][3]);
-      }
       const uint4* vw = reinterpret_cast<const uint4*>(stage + t * kTile + 8 * D);
-      constexpr int planes = D == 128 ? 2 : 1;
+      if constexpr (D == 32) {
+        const uint4 v = vw[4 * (r >> 1) + c];
+        const unsigned sel = r & 1 ? 0x7632u : 0x5410u;
+        const uint32_t x01 = __byte_perm(v.x, v.y, sel), x23 = __byte_perm(v.z, v.w, sel);
 #pragma unroll
-      for (int h = 0; h < planes; ++h) {
-        if constexpr (D == 32) {
-          const uint4 v = vw[4 * (r >> 1) + c];
-          const unsigned sel = r & 1 ? 0x7632u : 0x5410u;
-          const uint32_t x01 = __byte_perm(v.x, v.y, sel), x23 = __byte_perm(v.z, v.w, sel);
-          mma_f16(acc[0], a[0], a[1], a[2], a[3], codes_low(x01), codes_low(x23));
-          mma_f16(acc[1], a[0], a[1], a[2], a[3], codes_high(x01), codes_high(x23));
-          mma_f16(acc[2], a[0], a[1], a[2], a[3], codes_low(x01 >> 8), codes_low(x23 >> 8));
-          mma_f16(acc[3], a[0], a[1], a[2], a[3], codes_high(x01 >> 8), codes_high(x23 >> 8));
-        } else {
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t y01 = i ? x01 >> 8 : x01, y23 = i ? x23 >> 8 : x23;
+          const uint32_t a0 = codes_low(y01), a1 = codes_high(y01), a2 = codes_low(y23), a3 = codes_high(y23);
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) mma_f16(acc[n][i], a0, a1, a2, a3, bw[n][0], bw[n][1]);
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
           const uint4 v = vw[32 * h + lane];
+          uint32_t l01 = __byte_perm(v.x, v.y, 0x5410u), l23 = __byte_perm(v.z, v.w, 0x5410u);
+          uint32_t h01 = __byte_perm(v.x, v.y, 0x7632u), h23 = __byte_perm(v.z, v.w, 0x7632u);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const unsigned sel = e ? 0x7632u : 0x5410u;
-            const uint32_t x01 = __byte_perm(v.x, v.y, sel), x23 = __byte_perm(v.z, v.w, sel);
-            float(&o)[4] = acc[8 * h + 4 * e];
-            mma_f16(o, a[0], a[1], a[2], a[3], codes_low(x01), codes_low(x23));
-            mma_f16(acc[8 * h + 4 * e + 1], a[0], a[1], a[2], a[3], codes_high(x01), codes_high(x23));
-            mma_f16(acc[8 * h + 4 * e + 2], a[0], a[1], a[2], a[3], codes_low(x01 >> 8), codes_low(x23 >> 8));
-            mma_f16(acc[8 * h + 4 * e + 3], a[0], a[1], a[2], a[3], codes_high(x01 >> 8), codes_high(x23 >> 8));
+          for (int i = 0; i < 4; ++i) {
+            if (i == 2) {
+              l01 >>= 8;
+              l23 >>= 8;
+              h01 >>= 8;
+              h23 >>= 8;
+            }
+            const uint32_t a0 = i & 1 ? codes_high(l01) : codes_low(l01), a1 = i & 1 ? codes_high(h01) : codes_low(h01);
+            const uint32_t a2 = i & 1 ? codes_high(l23) : codes_low(l23), a3 = i & 1 ? codes_high(h23) : codes_low(h23);
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) mma_f16(acc[n][4 * h + i], a0, a1, a2, a3, bw[n][0], bw[n][1]);
           }
         }
       }
     }
     __syncwarp();
-    issue(step + G::stages - 1);
+    issue(step + G::stages - 1, to_stage);
+    at_stage = at_stage + 1 == G::stages ? 0 : at_stage + 1;
+    to_stage = to_stage + 1 == G::stages ? 0 : to_stage + 1;
   }
   cp_async_wait<0>();
   __syncwarp();
 
-  // this warp's part: reference, sum and offset sum per row, and its output over the ring it no longer needs
-  float* const part = reinterpret_cast<float*>(ring);
+  // the lane's rows: their sums over the 8 lanes that hold other positions, and 8 neighbouring channels a plane of 64 (or 32)
 #pragma unroll
-  for (int s = 0; s < kSets; ++s) {
-    sum[s] += __shfl_xor_sync(0xFFFFFFFFu, sum[s], 1);
-    sum[s] += __shfl_xor_sync(0xFFFFFFFFu, sum[s], 2);
-    off[s] += __shfl_xor_sync(0xFFFFFFFFu, off[s], 1);
-    off[s] += __shfl_xor_sync(0xFFFFFFFFu, off[s], 2);
-    if (c == 0) {
-      float* st = stats + (warp * R + r + 8 * s) * 3;
-      st[0] = ref[s];
-      st[1] = sum[s];
-      st[2] = off[s];
+  for (int s = 0; s < kSets; ++s)
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) {
+      sum[s] += __shfl_xor_sync(0xFFFFFFFFu, sum[s], d);
+      off[s] += __shfl_xor_sync(0xFFFFFFFFu, off[s], d);
     }
-    if (r + 8 * s < live) {
+  constexpr int kPlanes = D == 128 ? 2 : 1, kRun = D == 32 ? 4 : 8;  // channels of a lane in a plane
+  float o[kSets][kPlanes][kRun];
 #pragma unroll
-      for (int i = 0; i < kOut; ++i)
+  for (int s = 0; s < kSets; ++s)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          // column 2 c + e of column tile i
-          const int j = i & 3;
-          const int ch = D == 32 ? 8 * c + 2 * j + e : 64 * (i >> 3) + 8 * (2 * c + e) + 2 * j + ((i >> 2) & 1);
-          const float v = G::split ? acc[i][e] + acc[i][e + 2] : acc[i][2 * s + e];
-          part[(r + 8 * s) * D + ch] = v * 0.00006103515625f;  // the weights' 2^14
+    for (int h = 0; h < kPlanes; ++h)
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        const int i = 4 * h + (j >> 1), e = 2 * (j & 1);
+        const float v = kSplit ? acc[s][i][e] + acc[s][i][e + 1] : acc[s >> 1][i][e + (s & 1)];
+        o[s][h][j] = v * 0.00006103515625f;  // the weights' 2^14
+      }
+  // channel of value j: D = 32: 8 (r / 2) + r % 2 + 2 j, else 64 plane + 8 r + j
+  auto channel = [&](int h, int j) { return D == 32 ? 8 * (r >> 1) + (r & 1) + 2 * j : 64 * h + 8 * r + j; };
+  auto place = [&](int row) {
+    const int64_t t = (i0 + row) / A.group;
+    return static_cast<T*>(A.out) + (row0 + t) * A.o_row + (kvh * A.group + (i0 + row - t * A.group)) * A.o_head;
+  };
+  if (C * W == 1) {
+#pragma unroll
+    for (int s = 0; s < kSets; ++s)
+      if (row_of(s) < live) {
+        T* out = place(row_of(s));
+        const float inv = sum[s] == 0.0f ? 0.0f : 1.0f / sum[s];
+#pragma unroll
+        for (int h = 0; h < kPlanes; ++h) {
+          float y[kRun];
+#pragma unroll
+          for (int j = 0; j < kRun; ++j) y[j] = sum[s] == 0.0f ? 0.0f : (o[s][h][j] + off[s]) * inv;
+          if constexpr (D == 32) {
+#pragma unroll
+            for (int j = 0; j < kRun; ++j) out[channel(h, j)] = from_f32<T>(y[j]);
+          } else {
+            store_values<T, kRun>(out + channel(h, 0), A.o_vec, y);
+          }
         }
-    }
+      }
+    return;
   }
+  float* const part = reinterpret_cast<float*>(ring);  // the warp's ring is free
+#pragma unroll
+  for (int s = 0; s < kSets; ++s)
+    if (row_of(s) < live) {
+      if (r == 0) {
+        float* st = stats + (warp * R + row_of(s)) * 3;
+        st[0] = ref[s];
+        st[1] = sum[s];
+        st[2] = off[s];
+      }
+#pragma unroll
+      for (int h = 0; h < kPlanes; ++h)
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) part[row_of(s) * D + channel(h, j)] = o[s][h][j];
+    }
   __syncthreads();
   float* const cref = comb + R * D;
   for (int i = threadIdx.x; i < live * D; i += 32 * W) {
     const int row = i / D;
     float top = -INFINITY;
-#pragma unroll
     for (int w = 0; w < W; ++w) top = fmaxf(top, stats[(w * R + row) * 3]);
-    float o = 0.0f, l = 0.0f, m = 0.0f;
-#pragma unroll
+    float v = 0.0f, l = 0.0f, m = 0.0f;
     for (int w = 0; w < W; ++w) {
       const float* st = stats + (w * R + row) * 3;
       if (st[1] != 0.0f) {  // zero: the warp saw nothing for this row
         const float f = ex2(st[0] - top);
-        o = fmaf(reinterpret_cast<const float*>(smem + w * G::stages * G::group_bytes)[i], f, o);
+        v = fmaf(reinterpret_cast<const float*>(smem + w * G::warp_bytes)[i], f, v);
         l = fmaf(st[1], f, l);
         m = fmaf(st[2], f, m);
       }
     }
-    comb[i] = o;
-    if (i - row * D == 0) {
-      cref[row] = top;
-      cref[R + row] = l;
-      cref[2 * R + row] = m;
+    if (C == 1) {
+      place(row)[i - row * D] = from_f32<T>(l == 0.0f ? 0.0f : (v + m) / l);
+    } else {
+      comb[i] = v;
+      if (i - row * D == 0) {
+        cref[row] = top;
+        cref[R + row] = l;
+        cref[2 * R + row] = m;
+      }
     }
   }
-  if (C > 1) cluster.sync();
-  else __syncthreads();
+  if (C == 1) return;
+  cluster.sync();
   // the cluster's parts: every CTA writes its share of the rows' values
   for (int i = rank * 32 * W + threadIdx.x; i < live * D; i += C * 32 * W) {
     const int row = i / D;
     float top = -INFINITY;
     for (int k = 0; k < C; ++k) top = fmaxf(top, cluster.map_shared_rank(comb, k)[R * D + row]);
-    float o = 0.0f, l = 0.0f;
+    float v = 0.0f, l = 0.0f;
     for (int k = 0; k < C; ++k) {
       const float* other = cluster.map_shared_rank(comb, k);
       const float part_sum = other[R * D + R + row];
       if (part_sum != 0.0f) {
         const float f = ex2(other[R * D + row] - top);
-        o = fmaf(other[i] + other[R * D + 2 * R + row], f, o);
+        v = fmaf(other[i] + other[R * D + 2 * R + row], f, v);
         l = fmaf(part_sum, f, l);
       }
     }
-    const int64_t item = i0 + row, t = item / A.group;
-    const int h = kvh * A.group + static_cast<int>(item - t * A.group);
-    static_cast<T*>(A.out)[(row0 + t) * A.o_row + h * A.o_head + (i - row * D)] = from_f32<T>(l == 0.0f ? 0.0f : o / l);
+    place(row)[i - row * D] = from_f32<T>(l == 0.0f ? 0.0f : v / l);
   }
-  if (C > 1) cluster.sync();  // no CTA leaves while another reads its shared memory
+  cluster.sync();  // no CTA leaves while another reads its shared memory
 }
 
 // Opt-in shared memory, once per device and kernel.
@@ -503,21 +577,26 @@ int32_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
   return IVB_OK;
 }
 
-template <int D, typename T>
+template <int D, typename T, bool kSplit, int kTiles>
 int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
-  using G = RowsGeometry<D, T>;
+  using G = RowsGeometry<D, kSplit, kTiles>;
+  constexpr int kMostWarps = 8;
   static std::atomic<uint64_t> done{0};
-  if (int32_t rc = allow_smem(kv4_rows_kernel<D, T>, G::smem, done)) return rc;
+  if (int32_t rc = allow_smem(kv4_rows_kernel<D, T, kSplit, kTiles>, G::smem(kMostWarps), done)) return rc;
   const int64_t most = static_cast<int64_t>(A.starts == nullptr ? 1 : A.rows) * A.group;
   const int64_t tiles = (most + G::rows - 1) / G::rows;
   const int64_t base = tiles * A.cache.kv_heads * A.cache.batch;
-  int C = 1;
-  while (C < 8 && base * C * 2 <= 2 * 148 && A.cache.max_len > C * G::warps * kKv4Group) C *= 2;
+  const int64_t slots = 148 * 16;  // warps of this kernel that the GPU holds
+  int W = 1, C = 1;
+  while (W < kMostWarps && base * W < 2 * slots && A.cache.max_len > W * kKv4Group) W *= 2;
+  while (C < 8 && W == kMostWarps && base * W * C * 2 <= slots && A.cache.max_len > C * W * kKv4Group) C *= 2;
+  if (getenv("KV4_W")) W = atoi(getenv("KV4_W"));
+  if (getenv("KV4_C")) C = atoi(getenv("KV4_C"));
   if (base * C > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(base));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(base * C));
-  cfg.blockDim = dim3(32 * G::warps);
-  cfg.dynamicSmemBytes = G::smem;
+  cfg.blockDim = dim3(32 * W);
+  cfg.dynamicSmemBytes = G::smem(W);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -526,18 +605,33 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_rows_kernel<D, T>, A, static_cast<int>(tiles)));
+  IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_rows_kernel<D, T, kSplit, kTiles>, A, static_cast<int>(tiles)));
   return IVB_OK;
+}
+
+// Rows of a tile by what a sequence can have: four as pairs of fp16 (for every type: no less exact, and as fast), then
+// eight; 16-bit queries with more in columns of their own.
+template <int D, typename T>
+int32_t launch_dim(const Kv4Attention& A, cudaStream_t stream) {
+  const bool one = A.starts == nullptr;
+  if (one && A.group <= 4) return launch_rows_attention<D, T, true, 1>(A, stream);
+  if constexpr (std::is_same<T, float>::value) {
+    return launch_rows_attention<D, T, true, 2>(A, stream);
+  } else {
+    if (one && A.group <= 8) return launch_rows_attention<D, T, false, 1>(A, stream);
+    return launch_rows_attention<D, T, false, 2>(A, stream);
+  }
 }
 
 template <typename T>
 int32_t launch_attention(Kv4Attention& A, cudaStream_t stream) {
   const int size = static_cast<int>(sizeof(T)), chunk = std::min(16, A.cache.head_dim / 4 * size);
   A.q_vec = reinterpret_cast<uintptr_t>(A.q) % chunk == 0 && A.q_row * size % chunk == 0 && A.q_head * size % chunk == 0;
+  A.o_vec = reinterpret_cast<uintptr_t>(A.out) % 16 == 0 && A.o_row * size % 16 == 0 && A.o_head * size % 16 == 0;
   switch (A.cache.head_dim) {
-    case 32: return launch_rows_attention<32, T>(A, stream);
-    case 64: return launch_rows_attention<64, T>(A, stream);
-    default: return launch_rows_attention<128, T>(A, stream);
+    case 32: return launch_dim<32, T>(A, stream);
+    case 64: return launch_dim<64, T>(A, stream);
+    default: return launch_dim<128, T>(A, stream);
   }
 }
 
