@@ -1,11 +1,5 @@
-// Causal attention over the 4-bit key/value cache, with a sliding window and visible first tokens (sinks).
-//
-// With k_j = m_j + s_j u_j (codes u_j) the score is  a q.k_j = a s_j (q.u_j) + a m_j sum(q), and with v_j = m'_j + s'_j u'_j the
-// output is  sum_j p_j v_j = sum_j (p_j s'_j) u'_j + sum_j p_j m'_j : both products run on the codes themselves, and scales and
-// offsets are applied to scores and weights in 32 bits, one multiply-add per score. The operands are u - 8, exact in
-// fp16, with m + 8 s in the offsets' place: the tensor cores cut their sums towards zero, which adds up over a long axis
-// where all terms have one sign (3e-6 of the output at 2000 positions with u, 5e-7 with u - 8). fp32 queries and weights are split in two fp16 (x = hi + lo, 22 bits); fp16 and bf16
-// queries are exact in fp16 after a common power of two, and weights are rounded once to fp16.
+// Causal attention over the 4-bit key/value cache, with a sliding window and visible first tokens (sinks): few rows a sequence
+// (the prompts are in ivb_kv4_prompt.cu), and the entry point.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -14,8 +8,7 @@
 #include <atomic>
 #include <type_traits>
 
-#include "ivb_common.h"
-#include "ivb_kv4.cuh"
+#include "ivb_kv4_attention.cuh"
 
 namespace ivb {
 
@@ -26,21 +19,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct Kv4Attention {
-  IvbKv4Cache cache;
-  const void* q;
-  void* out;
-  int64_t q_row, q_head, o_row, o_head;
-  const int32_t* starts;
-  const int64_t* positions;
-  uint32_t* error;
-  float scale;
-  int heads, group;  // query heads, query heads per key/value head
-  int rows, window, sinks;
-  bool q_vec, o_vec;
-};
+constexpr int kFewItems = 32;  // tokens x query heads of a group
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -56,61 +35,6 @@ template <int n>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
 }
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// (a & b) | c in one instruction (two constants keep the compiler from it).
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t y;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
-  return y;
-}
-
-// Two nibbles of a word as fp16 values u - 8: the bits under 0x6400 give 1024 + u and 1024 + 16 u, the rest is exact. The
-// bare bits, fp16 subnormals u 2^-24, would save this instruction, but the tensor cores align products by the operands'
-// exponent fields and cut 7 to 10 bits more of a subnormal's: 5e-5 of the output, measured.
-__device__ __forceinline__ uint32_t codes_low(uint32_t w) {
-  const uint32_t x = and_or(w, 0x000f000fu, 0x64006400u);
-  const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(-1032.0f, -1032.0f));
-  return *reinterpret_cast<const uint32_t*>(&y);
-}
-__device__ __forceinline__ uint32_t codes_high(uint32_t w) {
-  const uint32_t x = and_or(w, 0x00f000f0u, 0x64006400u);
-  const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-72.0f, -72.0f));
-  return *reinterpret_cast<const uint32_t*>(&y);
-}
-
-// What the softmax needs of one position: x = S key_scale + sum(q) key_offset + bias, with bias the exponent of the value
-// scale, so that the running reference is the maximum of weight times value scale and neither overflows fp16, whatever the
-// scales; the weight is then 2^(x - ref) = p 2^bias, its product with the mantissa the A operand of the value product, and
-// p = weight * unbias enters the sum.
-struct PositionTerms {
-  float key_scale, key_offset, bias, mantissa;  // mantissa of the value scale, times 2^14
-  float unbias, value_offset;                   // 2^-bias, value offset times 2^-bias (offsets are of u - 8)
-};
-
-__device__ __forceinline__ PositionTerms position_terms(uint2 par, float score_unit, float offset_unit) {
-  const float2 key = unpack_f16(par.x), value = unpack_f16(par.y);
-  PositionTerms t;
-  t.key_scale = key.x * score_unit;
-  t.key_offset = fmaf(8.0f, key.x, key.y) * offset_unit;
-  const uint32_t bits = __float_as_uint(value.x) & 0x7f800000u;
-  const uint32_t e = bits == 0x7f800000u ? 0x3f800000u : max(bits, 0x33800000u);  // 2^-24 is the least scale above zero
-  t.bias = static_cast<float>(static_cast<int>(e >> 23) - 127);
-  t.unbias = __uint_as_float(0x7f000000u - e);
-  t.mantissa = value.x * t.unbias * 16384.0f;
-  t.value_offset = fmaf(8.0f, value.x, value.y) * t.unbias;
-  return t;
-}
-
 // ---- few rows: one token per sequence, a few drafted ones, or any number in tiles -----------------------------------------
 // One cluster of C CTAs of W warps per (sequence, key/value head, tile of rows); row i of a sequence's head group is token
 // i / group, query head i % group of the group. The 32-position groups of the cache that a row of the tile sees are dealt
@@ -155,36 +79,38 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
   float* const comb = reinterpret_cast<float*>(smem + W * (G::warp_bytes + G::term_bytes));  // [R][D], then ref, sum, offset [R]
   float* const stats = comb + G::comb_floats;                                               // [W][R][3]
 
-  // which rows
-  const int64_t cluster_id = blockIdx.x / C;
-  const int tile = static_cast<int>(cluster_id % tiles_per_sequence);
-  const int64_t sh = cluster_id / tiles_per_sequence;
-  const int kvh = static_cast<int>(sh % A.cache.kv_heads), b = static_cast<int>(sh / A.cache.kv_heads);
+  // which rows (rows x heads is below 2^31)
+  const unsigned cluster_id = blockIdx.x / static_cast<unsigned>(C), group_size = static_cast<unsigned>(A.group);
+  const int tile = static_cast<int>(cluster_id % static_cast<unsigned>(tiles_per_sequence));
+  const unsigned sh = cluster_id / static_cast<unsigned>(tiles_per_sequence);
+  const int b = static_cast<int>(sh / static_cast<unsigned>(A.cache.kv_heads)), kvh = static_cast<int>(sh) - b * A.cache.kv_heads;
   int row0 = b, count = 1;
   if (A.starts != nullptr) {
     row0 = max(0, __ldg(A.starts + b));
     count = min(A.rows, __ldg(A.starts + b + 1)) - row0;
   }
-  const int64_t items = static_cast<int64_t>(max(count, 0)) * A.group;
-  const int64_t i0 = static_cast<int64_t>(tile) * R;
-  if (i0 >= items) return;  // the whole cluster
-  const int live = static_cast<int>(min(static_cast<int64_t>(R), items - i0));
+  const int items = max(count, 0) * A.group, i0 = tile * R;
+  if (i0 >= items || items > A.few) return;  // the whole cluster
+  const int live = min(R, items - i0);
   const int64_t base = __ldg(A.positions + b);
-  const int64_t first = base + i0 / A.group, last = base + (i0 + live - 1) / A.group;
   const int max_len = A.cache.max_len;
+  // token and query head of an item of the sequence's head group
+  auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };
+  // positions of the tile's first and last rows, -1 where idle and max_len where beyond the capacity
+  auto clamp_position = [&](int64_t p) { return static_cast<int>(max(static_cast<int64_t>(-1), min(p, static_cast<int64_t>(max_len)))); };
+  const int first = clamp_position(base + token_of(i0)), last = clamp_position(base + token_of(i0 + live - 1));
   // row of the tile that set s of this lane holds, and its position (-1: sees nothing)
   auto row_of = [&](int s) { return kSplit ? 4 * s + c : 8 * (s >> 1) + 2 * c + (s & 1); };
   int at[kSets];
 #pragma unroll
   for (int s = 0; s < kSets; ++s) {
-    const int64_t p = base + (i0 + row_of(s)) / A.group;
-    at[s] = row_of(s) < live && p >= 0 && p < max_len ? static_cast<int>(p) : -1;
+    const int p = clamp_position(base + token_of(i0 + row_of(s)));
+    at[s] = row_of(s) < live && p < max_len ? p : -1;
   }
   if (last >= max_len && threadIdx.x == 0 && rank == 0 && A.error != nullptr) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
   // the groups of 32 positions that some row sees: the sinks' below the window, then the window's
-  const int high = static_cast<int>(min(last, static_cast<int64_t>(max_len) - 1));  // negative: none
-  const int lowest = static_cast<int>(min(max(first, static_cast<int64_t>(0)), static_cast<int64_t>(max_len)));
-  const int low = A.window > 0 ? max(0, lowest - A.window + 1) : 0;
+  const int high = min(last, max_len - 1);  // negative: none
+  const int low = A.window > 0 ? max(0, max(first, 0) - A.window + 1) : 0;
   const int window_group = low / kKv4Group;
   const int sink_groups = A.window > 0 ? min((min(A.sinks, low) + kKv4Group - 1) / kKv4Group, window_group) : 0;
   const int groups = high < 0 ? 0 : sink_groups + high / kKv4Group - window_group + 1;
@@ -224,8 +150,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
 #pragma unroll
       for (int j = 0; j < D / 4; ++j) qv[n][j] = 0.0f;
       if (row < live) {
-        const int64_t t = (i0 + row) / A.group;
-        const int h = kvh * A.group + static_cast<int>(i0 + row - t * A.group);
+        const int t = token_of(i0 + row), h = kvh * A.group + i0 + row - t * A.group;
         load_values<T, D / 4>(static_cast<const T*>(A.q) + (row0 + t) * A.q_row + h * A.q_head + D / 4 * c, A.q_vec, qv[n]);
       }
       total[n] = 0.0f;
@@ -284,7 +209,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
     const int p0 = group_of(step) * kKv4Group;
     {
       const uint2 par = *reinterpret_cast<const uint2*>(stage + (lane >> 4) * kTile + 16 * D + (lane & 15) * 8);
-      const PositionTerms t = position_terms(par, score_unit, offset_unit);
+      const PositionTerms t = position_terms(par, score_unit, offset_unit, 16384.0f);
       terms4[lane] = make_float4(t.key_scale, t.key_offset, t.bias, t.mantissa);
       terms2[lane] = make_float2(t.unbias, t.value_offset);
     }
@@ -338,7 +263,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
       }
     }
     // a group that every row sees whole needs no masks
-    const bool whole = first >= p0 + kKv4Group - 1 && last < max_len && (A.window <= 0 || p0 > last - A.window || p0 + kKv4Group <= A.sinks);
+    const bool whole = first >= p0 + kKv4Group - 1 && last < max_len && (A.window <= 0 || p0 > last - A.window || p0 <= A.sinks - kKv4Group);
     if (!whole) {
 #pragma unroll
       for (int s = 0; s < kSets; ++s)
@@ -477,8 +402,8 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
   // channel of value j: D = 32: 8 (r / 2) + r % 2 + 2 j, else 64 plane + 8 r + j
   auto channel = [&](int h, int j) { return D == 32 ? 8 * (r >> 1) + (r & 1) + 2 * j : 64 * h + 8 * r + j; };
   auto place = [&](int row) {
-    const int64_t t = (i0 + row) / A.group;
-    return static_cast<T*>(A.out) + (row0 + t) * A.o_row + (kvh * A.group + (i0 + row - t * A.group)) * A.o_head;
+    const int t = token_of(i0 + row);
+    return static_cast<T*>(A.out) + (row0 + t) * A.o_row + (kvh * A.group + i0 + row - t * A.group) * A.o_head;
   };
   if (C * W == 1) {
 #pragma unroll
@@ -583,13 +508,13 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   constexpr int kMostWarps = 8;
   static std::atomic<uint64_t> done{0};
   if (int32_t rc = allow_smem(kv4_rows_kernel<D, T, kSplit, kTiles>, G::smem(kMostWarps), done)) return rc;
-  const int64_t most = static_cast<int64_t>(A.starts == nullptr ? 1 : A.rows) * A.group;
+  const int64_t most = std::min<int64_t>(A.few, static_cast<int64_t>(A.starts == nullptr ? 1 : A.rows) * A.group);
   const int64_t tiles = (most + G::rows - 1) / G::rows;
   const int64_t base = tiles * A.cache.kv_heads * A.cache.batch;
   const int64_t slots = 148 * 16;  // warps of this kernel that the GPU holds
   int W = 1, C = 1;
   while (W < kMostWarps && base * W < 2 * slots && A.cache.max_len > W * kKv4Group) W *= 2;
-  while (C < 8 && W == kMostWarps && base * W * C * 2 <= slots && A.cache.max_len > C * W * kKv4Group) C *= 2;
+  while (C < 8 && W == kMostWarps && base * W * C * 2 <= slots && A.cache.max_len > 4 * C * W * kKv4Group) C *= 2;
   if (getenv("KV4_W")) W = atoi(getenv("KV4_W"));
   if (getenv("KV4_C")) C = atoi(getenv("KV4_C"));
   if (base * C > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(base));
@@ -624,10 +549,7 @@ int32_t launch_dim(const Kv4Attention& A, cudaStream_t stream) {
 }
 
 template <typename T>
-int32_t launch_attention(Kv4Attention& A, cudaStream_t stream) {
-  const int size = static_cast<int>(sizeof(T)), chunk = std::min(16, A.cache.head_dim / 4 * size);
-  A.q_vec = reinterpret_cast<uintptr_t>(A.q) % chunk == 0 && A.q_row * size % chunk == 0 && A.q_head * size % chunk == 0;
-  A.o_vec = reinterpret_cast<uintptr_t>(A.out) % 16 == 0 && A.o_row * size % 16 == 0 && A.o_head * size % 16 == 0;
+int32_t launch_attention(const Kv4Attention& A, cudaStream_t stream) {
   switch (A.cache.head_dim) {
     case 32: return launch_dim<32, T>(A, stream);
     case 64: return launch_dim<64, T>(A, stream);
@@ -646,6 +568,7 @@ extern "C" int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_
   if (int32_t rc = check_kv4_rows(c, starts, positions, rows, dtype, "ivb_kv4_attention")) return rc;
   if (heads <= 0 || heads % c->kv_heads != 0) return fail(IVB_EINVAL, "ivb_kv4_attention: %d query heads over %d key/value heads", heads, c->kv_heads);
   if (window < 0 || sinks < 0) return fail(IVB_EINVAL, "ivb_kv4_attention: window %d, sinks %d", window, sinks);
+  if (static_cast<int64_t>(rows) * heads > 0x7fffffff - 1024) return fail(IVB_EINVAL, "ivb_kv4_attention: %d rows of %d heads", rows, heads);
   if (rows == 0) return IVB_OK;
   if (q == nullptr || out == nullptr) return fail(IVB_EINVAL, "ivb_kv4_attention: null queries or output");
   Kv4Attention A{};
@@ -665,7 +588,19 @@ extern "C" int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_
   A.rows = rows;
   A.window = window;
   A.sinks = sinks;
+  const int size = dtype == IVB_F32 ? 4 : 2;
+  auto aligned = [&](const void* p, int64_t row, int64_t head) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row * size % 16 == 0 && head * size % 16 == 0;
+  };
+  A.q_vec = aligned(q, q_row, q_head);
+  A.o_vec = aligned(out, o_row, o_head);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // sequences of more than `few` items go to the prompt kernel; a lone sequence all of its rows, if it can have so many
+  const int64_t items = static_cast<int64_t>(rows) * A.group;
+  A.few = starts == nullptr || items <= kFewItems ? 0x7fffffff : c->batch == 1 ? 0 : kFewItems;
+  if (A.few != 0x7fffffff)
+    if (int32_t rc = launch_kv4_prompts(A, dtype, A.few, s)) return rc;
+  if (A.few == 0) return IVB_OK;
   if (dtype == IVB_F32) return launch_attention<float>(A, s);
   if (dtype == IVB_F16) return launch_attention<__half>(A, s);
   return launch_attention<__nv_bfloat16>(A, s);

@@ -1,0 +1,91 @@
+// What the kernels of the attention over the 4-bit cache share.
+//
+// With k_j = m_j + s_j u_j (codes u_j) the score is  a q.k_j = a s_j (q.u_j) + a m_j sum(q), and with v_j = m'_j + s'_j u'_j the
+// output is  sum_j p_j v_j = sum_j (p_j s'_j) u'_j + sum_j p_j m'_j : both products run on the codes themselves, and scales and
+// offsets are applied to scores and weights in 32 bits, one multiply-add per score. The operands are u - 8, exact in
+// fp16, with m + 8 s in the offsets' place: the tensor cores cut their sums towards zero, which adds up over a long axis
+// where all terms have one sign (3e-6 of the output at 2000 positions with u, 5e-7 with u - 8). fp32 queries and weights are split in two fp16 (x = hi + lo, 22 bits); fp16 and bf16
+// queries are exact in fp16 after a common power of two, and weights are rounded once to fp16.
+#pragma once
+
+#include "ivb_common.h"
+#include "ivb_kv4.cuh"
+
+namespace ivb {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Kv4Attention {
+  IvbKv4Cache cache;
+  const void* q;
+  void* out;
+  int64_t q_row, q_head, o_row, o_head;
+  const int32_t* starts;
+  const int64_t* positions;
+  uint32_t* error;
+  float scale;
+  int heads, group;  // query heads, query heads per key/value head
+  int rows, window, sinks;
+  int few;             // sequences with more items (tokens x group) are prompts
+  bool q_vec, o_vec;   // rows begin on 16 bytes
+};
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// (a & b) | c in one instruction (two constants keep the compiler from it).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
+  return y;
+}
+
+// Two nibbles of a word as fp16 values u - 8: the bits under 0x6400 give 1024 + u and 1024 + 16 u, the rest is exact. The
+// bare bits, fp16 subnormals u 2^-24, would save this instruction, but the tensor cores align products by the operands'
+// exponent fields and cut 7 to 10 bits more of a subnormal's: 5e-5 of the output, measured.
+__device__ __forceinline__ uint32_t codes_low(uint32_t w) {
+  const uint32_t x = and_or(w, 0x000f000fu, 0x64006400u);
+  const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(-1032.0f, -1032.0f));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+__device__ __forceinline__ uint32_t codes_high(uint32_t w) {
+  const uint32_t x = and_or(w, 0x00f000f0u, 0x64006400u);
+  const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-72.0f, -72.0f));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// What the softmax needs of one position: x = S key_scale + sum(q) key_offset + bias, with bias the exponent of the value
+// scale, so that the running reference is the maximum of weight times value scale and neither overflows fp16, whatever the
+// scales; the weight is then 2^(x - ref) = p 2^bias, its product with the mantissa the A operand of the value product, and
+// p = weight * unbias enters the sum.
+struct PositionTerms {
+  float key_scale, key_offset, bias, mantissa;  // mantissa of the value scale, times weight_unit
+  float unbias, value_offset;                   // 2^-bias, value offset times 2^-bias (offsets are of u - 8)
+};
+
+__device__ __forceinline__ PositionTerms position_terms(uint2 par, float score_unit, float offset_unit, float weight_unit) {
+  const float2 key = unpack_f16(par.x), value = unpack_f16(par.y);
+  PositionTerms t;
+  t.key_scale = key.x * score_unit;
+  t.key_offset = fmaf(8.0f, key.x, key.y) * offset_unit;
+  const uint32_t bits = __float_as_uint(value.x) & 0x7f800000u;
+  const uint32_t e = bits == 0x7f800000u ? 0x3f800000u : max(bits, 0x33800000u);  // 2^-24 is the least scale above zero
+  t.bias = static_cast<float>(static_cast<int>(e >> 23) - 127);
+  t.unbias = __uint_as_float(0x7f000000u - e);
+  t.mantissa = value.x * t.unbias * weight_unit;
+  t.value_offset = fmaf(8.0f, value.x, value.y) * t.unbias;
+  return t;
+}
+
+// Prompts: every sequence of the call with more than `few` items (tokens x query heads of a group).
+int32_t launch_kv4_prompts(const Kv4Attention& A, int32_t dtype, int few, cudaStream_t stream);
+
+}  // namespace ivb

@@ -1,0 +1,607 @@
+// Causal attention over the 4-bit key/value cache for prompts: many rows a sequence, on the 5th-generation tensor cores.
+//
+// One CTA per (sequence, key/value head, 256 rows), 13 warps. Row i of a sequence's head group is token i / group, query head
+// i % group; rows 0..127 and 128..255 are two tiles X of the tensor cores' 128 lanes. Per tile of 64 positions:
+//   warps 8..11 (producers) read the codes, expand them to fp16 u - 8 in shared memory (keys as a K-major operand, values as an
+//     MN-major one: both are position rows of 16-byte channel chunks, so neither is transposed) and compute each
+//     position's terms (scales and offsets; ivb_kv4_attention.cuh);
+//   warp 12 (one thread) issues S_X = Q_X U^T and O_X += P_X U'^T, fp32 in tensor memory, P_X from tensor memory;
+//   warps 0..7 (a thread owns one row, which is its tensor-memory lane) turn S_X into weights: online softmax in 32 bits, the
+//     reference raised only when the maximum passes it by 2^8, and O_X rescaled in tensor memory then.
+// fp32 queries and weights are hi + lo fp16 pairs: two products each. S_X(it + 1) is issued as soon as S_X(it) has been read,
+// so the tensor pipe works while the softmax does. What bounds it is the softmax's issue slots (about 7 per score, with
+// paired fp32 instructions) and, at D = 128, the tensor pipe beside it.
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <type_traits>
+
+#include "ivb_decode.cuh"
+#include "ivb_kv4_attention.cuh"
+#include "ivb_tc.cuh"
+
+namespace ivb {
+namespace {
+
+constexpr int kRowsX = 128, kRowsCta = 256, kPos = 64;
+constexpr int kSoftmaxThreads = 256, kProducers = 128, kPromptThreads = kSoftmaxThreads + kProducers + 32;
+constexpr unsigned long long kPromptTimeout = 2000000000ull;
+constexpr float kWeightUnit = 64.0f;  // weights are at most 2 * 64 * 2^8 in fp16
+constexpr float kRaise = 8.0f;
+
+template <int D, bool kSplit>
+struct PromptGeometry {
+  static constexpr int parts = kSplit ? 2 : 1;
+  static constexpr int q_bytes = kRowsX * D * 2;    // one part of one row tile
+  static constexpr int kv_bytes = kPos * D * 2;     // keys or values of a stage
+  static constexpr int term_bytes = kPos * 24;
+  static constexpr int q_at = 0, kv_at = 2 * parts * q_bytes, terms_at = kv_at + 4 * kv_bytes;
+  static constexpr int smem = terms_at + 2 * term_bytes;
+  // tensor memory columns
+  static constexpr int s_at = 0, p_at = 2 * kPos, o_at = p_at + 2 * parts * (kPos / 2), columns_used = o_at + 2 * D;
+  static constexpr int columns = columns_used <= 256 ? 256 : 512;
+  static_assert(columns_used <= 512, "tensor memory");
+};
+
+// kind::f16, fp32 result, A K-major, B MN-major.
+__host__ __device__ constexpr uint32_t idesc_f16_bt(int m, int n) { return idesc_f16(m, n) | (1u << 16); }
+
+// Descriptor of an MN-major operand without swizzle: core matrices of 8 K rows x 8 channels (16 bytes a row), the next 8
+// channels 128 bytes on, the next 8 K rows `k_step` bytes on.
+__device__ __forceinline__ uint64_t smem_desc_mn(unsigned addr, unsigned k_step) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((k_step >> 4) & 0x3FFFu) << 16) |
+         (static_cast<uint64_t>(128 >> 4) << 32) | (1ull << 46);
+}
+
+// Byte offset of channel chunk i (8 channels) of row p in core matrices of 8 rows x 16 bytes, D / 8 chunks a row.
+template <int D>
+__device__ __forceinline__ int chunk_at(int p, int i) {
+  return ((p >> 3) * (D / 8) + i) * 128 + (p & 7) * 16;
+}
+
+__device__ __forceinline__ uint4 expand(uint32_t w) { return make_uint4(codes_low(w), codes_high(w), codes_low(w >> 8), codes_high(w >> 8)); }
+
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(f32x2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+struct PromptBarriers {
+  unsigned long long kv_full[2], kv_free[2], s_full[2], s_free[2], p_full[2], p_free[2], drain;
+};
+
+// Raw codes of one 64-position tile that a producer thread holds: what it expands itself.
+template <int D>
+struct RawTile {
+  static constexpr int key_chunks = D == 128 ? 2 : 1, value_chunks = D == 128 ? 2 : 1;
+  uint4 key[key_chunks], value[value_chunks];
+  uint2 par;
+};
+
+// Producer thread j (0..127): tile j / 32 of 16 positions (D = 32: values of threads 0..63), so that 8 neighbouring threads
+// write the 8 rows of a core matrix, without bank conflicts.
+template <int D>
+__device__ __forceinline__ void load_raw(const unsigned char* tiles16, int valid, int j, RawTile<D>& raw) {
+  constexpr int kTile = kv4_tile_bytes(D);
+  const int t = j >> 5;
+  const bool in = t < valid;
+  const unsigned char* at = tiles16 + static_cast<int64_t>(in ? t : 0) * kTile;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  if constexpr (D == 128) {
+    const int h = (j >> 2) & 1, c = (j >> 3) & 3;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) raw.key[k] = in ? __ldg(reinterpret_cast<const uint4*>(at + 512 * h + (((j & 3) + 4 * k) * 4 + c) * 16)) : zero;
+  } else {
+    const int r = j & 7, c = (j >> 3) & 3;
+    if constexpr (D == 64) {
+      raw.key[0] = in ? __ldg(reinterpret_cast<const uint4*>(at + (r * 4 + c) * 16)) : zero;
+    } else {
+      const uint2 v = in ? __ldg(reinterpret_cast<const uint2*>(at + (r * 4 + c) * 8)) : make_uint2(0u, 0u);
+      raw.key[0] = make_uint4(v.x, v.y, 0u, 0u);
+    }
+  }
+  if constexpr (D == 32) {
+    const int r = j & 3, c = ((j >> 2) & 1) + 2 * ((j >> 3) & 1), tv = (j >> 4) & 3;
+    raw.value[0] = j < 64 && tv < valid ? __ldg(reinterpret_cast<const uint4*>(tiles16 + static_cast<int64_t>(tv) * kTile + 8 * D + (r * 4 + c) * 16)) : zero;
+  } else {
+    const int r = (j & 3) + 4 * ((j >> 4) & 1), c = ((j >> 2) & 1) + 2 * ((j >> 3) & 1);
+#pragma unroll
+    for (int k = 0; k < RawTile<D>::value_chunks; ++k)
+      raw.value[k] = in ? __ldg(reinterpret_cast<const uint4*>(at + 8 * D + 512 * k + (r * 4 + c) * 16)) : zero;
+  }
+  if (j < kPos) raw.par = (j >> 4) < valid ? __ldg(reinterpret_cast<const uint2*>(tiles16 + static_cast<int64_t>(j >> 4) * kTile + 16 * D + (j & 15) * 8)) : make_uint2(0u, 0u);
+}
+
+template <int D>
+__device__ __forceinline__ void store_raw(const RawTile<D>& raw, int j, unsigned char* keys, unsigned char* values, float* terms,
+                                          float score_unit, float offset_unit) {
+  const int t = j >> 5;
+  if constexpr (D == 128) {
+    const int h = (j >> 2) & 1, c = (j >> 3) & 3;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = (j & 3) + 4 * k, p = 16 * t + 4 * (r >> 1) + (r & 1) + 2 * h;
+      const uint32_t w[4] = {raw.key[k].x, raw.key[k].y, raw.key[k].z, raw.key[k].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(keys + chunk_at<D>(p, 4 * c + i)) = expand(w[i]);
+    }
+  } else {
+    const int r = j & 7, c = (j >> 3) & 3, other = r >> 2;  // the upper four rows' lanes take their two positions in the other order
+    const int p = 16 * t + 4 * (r >> 1) + (r & 1);
+    if constexpr (D == 64) {
+      const uint2 a = other ? make_uint2(raw.key[0].z, raw.key[0].w) : make_uint2(raw.key[0].x, raw.key[0].y);
+      const uint2 b = other ? make_uint2(raw.key[0].x, raw.key[0].y) : make_uint2(raw.key[0].z, raw.key[0].w);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, 2 * c)) = expand(a.x);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, 2 * c + 1)) = expand(a.y);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, 2 * c)) = expand(b.x);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, 2 * c + 1)) = expand(b.y);
+    } else {
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, c)) = expand(other ? raw.key[0].y : raw.key[0].x);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, c)) = expand(other ? raw.key[0].x : raw.key[0].y);
+    }
+  }
+  if (D != 32 || j < 64) {
+    const int turn = j & 3, c = ((j >> 2) & 1) + 2 * ((j >> 3) & 1);
+    const int r = D == 32 ? j & 3 : (j & 3) + 4 * ((j >> 4) & 1), tv = D == 32 ? (j >> 4) & 3 : t;
+#pragma unroll
+    for (int k = 0; k < RawTile<D>::value_chunks; ++k) {
+      uint4 v = raw.value[k];  // word i of the lane is position 4 c + i: each lane begins with another one
+      if (turn & 1) v = make_uint4(v.y, v.z, v.w, v.x);
+      if (turn & 2) v = make_uint4(v.z, v.w, v.x, v.y);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(values + chunk_at<D>(16 * tv + 4 * c + ((i + turn) & 3), 8 * k + r)) = expand(w[i]);
+    }
+  }
+  if (j < kPos) {
+    const PositionTerms p = position_terms(raw.par, score_unit, offset_unit, kWeightUnit);
+    float* at = terms + 12 * (j >> 1) + (j & 1);
+    at[0] = p.key_scale;
+    at[2] = p.key_offset;
+    at[4] = p.bias;
+    at[6] = p.mantissa;
+    at[8] = p.unbias;
+    at[10] = p.value_offset;
+  }
+}
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attention A, int few) {
+  constexpr bool kSplit = std::is_same<T, float>::value;
+  using G = PromptGeometry<D, kSplit>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ PromptBarriers bar;
+  __shared__ unsigned tmem_base;
+  __shared__ float largest[kSoftmaxThreads / 32];
+  __shared__ int which[3];  // sequence, tile of its rows; and whether a wait ran out
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  // which rows: the call's tiles of 256 items in the order of the sequences, the last ones (the longest rows) first
+  const int kvh = blockIdx.x % A.cache.kv_heads;
+  const int order = static_cast<int>(gridDim.x) / A.cache.kv_heads - 1 - blockIdx.x / A.cache.kv_heads;
+  if (warp == 0) {
+    int seen = 0, found = -1, tile = 0;
+    for (int b0 = 0; b0 < A.cache.batch && found < 0; b0 += 32) {
+      const int b = b0 + lane;
+      int n = 0;
+      if (b < A.cache.batch) {
+        int count = 1;
+        if (A.starts != nullptr) count = max(0, min(A.rows, __ldg(A.starts + b + 1)) - max(0, __ldg(A.starts + b)));
+        const int items = count * A.group;
+        n = items > few ? (items + kRowsCta - 1) / kRowsCta : 0;
+      }
+      int upto = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+        if (lane >= d) upto += o;
+      }
+      const unsigned hit = __ballot_sync(0xFFFFFFFFu, seen + upto > order);
+      if (hit != 0u) {
+        const int l = __ffs(hit) - 1;
+        found = b0 + l;
+        tile = order - (seen + __shfl_sync(0xFFFFFFFFu, upto, l) - __shfl_sync(0xFFFFFFFFu, n, l));
+      }
+      seen += __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    if (lane == 0) {
+      which[0] = found;
+      which[1] = tile;
+      which[2] = 0;
+    }
+  }
+  if (tid == 32) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.kv_full[i], kProducers);
+      mbar_init(&bar.kv_free[i], 1);
+      mbar_init(&bar.s_full[i], 1);
+      mbar_init(&bar.s_free[i], kRowsX);
+      mbar_init(&bar.p_full[i], kRowsX);
+      mbar_init(&bar.p_free[i], 1);
+    }
+    mbar_init(&bar.drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  const int b = which[0];
+  if (b < 0) return;
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)), "r"(G::columns));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  int row0 = b, count = 1;
+  if (A.starts != nullptr) {
+    row0 = max(0, __ldg(A.starts + b));
+    count = min(A.rows, __ldg(A.starts + b + 1)) - row0;
+  }
+  const int i0 = which[1] * kRowsCta, live = min(kRowsCta, count * A.group - i0), row_tiles = live > kRowsX ? 2 : 1;
+  const int64_t base = __ldg(A.positions + b);
+  const int max_len = A.cache.max_len;
+  const unsigned group_size = static_cast<unsigned>(A.group);
+  auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };
+  auto clamp_position = [&](int64_t p) { return static_cast<int>(max(static_cast<int64_t>(-1), min(p, static_cast<int64_t>(max_len)))); };
+  const int first = clamp_position(base + token_of(i0)), last = clamp_position(base + token_of(i0 + live - 1));
+  if (last >= max_len && tid == 0 && A.error != nullptr) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
+  // the tiles of 64 positions that some row sees: the sinks' below the window, then the window's
+  const int high = min(last, max_len - 1);
+  const int low = A.window > 0 ? max(0, max(first, 0) - A.window + 1) : 0;
+  const int window_tile = low / kPos;
+  const int sink_tiles = A.window > 0 ? min((min(A.sinks, low) + kPos - 1) / kPos, window_tile) : 0;
+  const int tiles = high < 0 ? 0 : sink_tiles + high / kPos - window_tile + 1;
+  auto tile_of = [&](int it) { return it < sink_tiles ? it : window_tile + it - sink_tiles; };
+
+  // queries: the largest, then hi (and lo) parts as K-major operands, scaled by a power of two that brings it to 2^13
+  const int x = warp >> 2, row = tid & 127;  // row tile and row of a softmax thread
+  const int item = i0 + tid;
+  const bool mine = tid < live;
+  const T* q = nullptr;
+  int at = -1;
+  float sum_q = 0.0f;
+  if (tid < kSoftmaxThreads) {
+    float most = 0.0f;
+    if (mine) {
+      const int t = token_of(item), h = kvh * A.group + item - t * A.group;
+      q = static_cast<const T*>(A.q) + (row0 + t) * A.q_row + h * A.q_head;
+      const int p = clamp_position(base + t);
+      at = p < max_len ? p : -1;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        float v[8];
+        load_values<T, 8>(q + 8 * c, A.q_vec, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float m = fabsf(v[j]);
+          if (m <= 3.402823466e38f) most = fmaxf(most, m);
+          sum_q += v[j];
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+    if (lane == 0) largest[warp] = most;
+  }
+  __syncthreads();
+  float most = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kSoftmaxThreads / 32; ++w) most = fmaxf(most, largest[w]);
+  int up = 13 - (static_cast<int>(__float_as_uint(most) >> 23) - 127);
+  up = most == 0.0f ? 0 : min(max(up, -100), 100);
+  const float offset_unit = A.scale * kLog2e;
+  const float score_unit = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * offset_unit;
+  if (tid < kSoftmaxThreads && x < row_tiles) {
+    const float unit = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+    unsigned char* dst = smem + G::q_at + x * G::parts * G::q_bytes;
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+      if (mine) load_values<T, 8>(q + 8 * c, A.q_vec, v);
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = v[2 * j] * unit, c2 = v[2 * j + 1] * unit;
+        hi[j] = pack_f16(a, c2);
+        if constexpr (kSplit) {
+          const float2 h = unpack_f16(hi[j]);
+          lo[j] = pack_f16(a - h.x, c2 - h.y);
+        }
+      }
+      *reinterpret_cast<uint4*>(dst + chunk_at<D>(row, c)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      if constexpr (kSplit) *reinterpret_cast<uint4*>(dst + G::q_bytes + chunk_at<D>(row, c)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+  }
+  fence_proxy_async();  // the tensor cores read what the threads wrote
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = tmem_base;
+  auto keys_of = [&](int stage) { return smem + G::kv_at + stage * 2 * G::kv_bytes; };
+  auto terms_of = [&](int stage) { return reinterpret_cast<float*>(smem + G::terms_at + stage * G::term_bytes); };
+  bool ok = true;
+
+  if (warp >= 8 && warp < 12) {
+    // ---- producers ----
+    const int j = tid - kSoftmaxThreads;
+    const int64_t tiles16 = kv4_tiles(max_len);
+    const unsigned char* codes = static_cast<const unsigned char*>(A.cache.data) +
+                                 (static_cast<int64_t>(b) * A.cache.kv_heads + kvh) * tiles16 * kv4_tile_bytes(D);
+    RawTile<D> raw;
+    auto fetch = [&](int it) {
+      const int64_t t16 = static_cast<int64_t>(tile_of(it)) * (kPos / 16);
+      load_raw<D>(codes + t16 * kv4_tile_bytes(D), static_cast<int>(min(static_cast<int64_t>(4), tiles16 - t16)), j, raw);
+    };
+    if (tiles > 0) fetch(0);
+    for (int it = 0; it < tiles; ++it) {
+      const int st = it & 1;
+      if (it >= 2 && !mbar_wait_bounded(&bar.kv_free[st], ((it >> 1) - 1) & 1, kPromptTimeout)) {
+        ok = false;
+        break;
+      }
+      store_raw<D>(raw, j, keys_of(st), keys_of(st) + G::kv_bytes, terms_of(st), score_unit, offset_unit);
+      fence_proxy_async();
+      mbar_arrive(&bar.kv_full[st]);
+      if (it + 1 < tiles) fetch(it + 1);
+    }
+  } else if (warp == 12) {
+    // ---- the thread that issues the products ----
+    if (lane == 0) {
+      const unsigned q0 = smem_addr(smem + G::q_at);
+      auto issue_s = [&](int it, int xx) {
+        const unsigned ka = smem_addr(keys_of(it & 1)), qa = q0 + xx * G::parts * G::q_bytes;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+          for (int part = 0; part < G::parts; ++part)
+            umma_f16_ss(tmem + G::s_at + xx * kPos, smem_desc(qa + part * G::q_bytes + kk * 256, D / 8 * 128),
+                        smem_desc(ka + kk * 256, D / 8 * 128), idesc_f16(kRowsX, kPos), kk + part > 0);
+        umma_commit(&bar.s_full[xx]);
+      };
+      auto issue_o = [&](int it, int xx) {
+        const unsigned va = smem_addr(keys_of(it & 1)) + G::kv_bytes;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < kPos / 16; ++kk)
+#pragma unroll
+          for (int part = 0; part < G::parts; ++part)
+            umma_f16_ts(tmem + G::o_at + xx * D, tmem + G::p_at + (xx * G::parts + part) * (kPos / 2) + kk * 8,
+                        smem_desc_mn(va + kk * 2 * (D / 8) * 128, D / 8 * 128), idesc_f16_bt(kRowsX, D), it > 0 || kk + part > 0);
+        umma_commit(&bar.p_free[xx]);
+      };
+      if (tiles > 0) {
+        ok = mbar_wait_bounded(&bar.kv_full[0], 0, kPromptTimeout);
+        if (ok)
+          for (int xx = 0; xx < row_tiles; ++xx) issue_s(0, xx);
+      }
+      for (int it = 0; it < tiles && ok; ++it) {
+        if (it + 1 < tiles) {
+          ok = mbar_wait_bounded(&bar.kv_full[(it + 1) & 1], ((it + 1) >> 1) & 1, kPromptTimeout);
+          for (int xx = 0; xx < row_tiles && ok; ++xx) {
+            ok = mbar_wait_bounded(&bar.s_free[xx], it & 1, kPromptTimeout);
+            if (ok) issue_s(it + 1, xx);
+          }
+        }
+        for (int xx = 0; xx < row_tiles && ok; ++xx) {
+          ok = mbar_wait_bounded(&bar.p_full[xx], it & 1, kPromptTimeout);
+          if (ok) issue_o(it, xx);
+        }
+        if (ok) umma_commit(&bar.kv_free[it & 1]);
+      }
+      if (!ok) {  // let what was issued finish before shared and tensor memory go
+        umma_commit(&bar.drain);
+        mbar_wait_bounded(&bar.drain, 0, kPromptTimeout);
+      }
+    }
+  } else if (x < row_tiles) {
+    // ---- softmax: one row a thread ----
+    const unsigned lanes = static_cast<unsigned>(32 * (warp & 3)) << 16;
+    const unsigned ts = tmem + lanes + G::s_at + x * kPos, tp = tmem + lanes + G::p_at + x * G::parts * (kPos / 2), to = tmem + lanes + G::o_at + x * D;
+    const f32x2 q2 = pair(sum_q, sum_q);
+    float ref = -INFINITY;
+    f32x2 sum2 = pair(0.0f, 0.0f), off2 = pair(0.0f, 0.0f);
+    for (int it = 0; it < tiles; ++it) {
+      const int p0 = tile_of(it) * kPos;
+      const float4* terms = reinterpret_cast<const float4*>(terms_of(it & 1));
+      ok = mbar_wait_bounded(&bar.kv_full[it & 1], (it >> 1) & 1, kPromptTimeout) && mbar_wait_bounded(&bar.s_full[x], it & 1, kPromptTimeout);
+      if (!__all_sync(0xFFFFFFFFu, ok)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t s0[32], s1[32];
+      tmem_ld32(ts, s0);
+      tmem_ld32(ts + 32, s1);
+      tc_fence_before();
+      mbar_arrive(&bar.s_free[x]);
+      const bool all = at >= p0 + kPos - 1 && (A.window <= 0 || p0 > at - A.window || p0 <= A.sinks - kPos);
+      const bool whole = __all_sync(0xFFFFFFFFu, all || !mine);
+      float xs[kPos];
+#pragma unroll
+      for (int j = 0; j < kPos / 2; ++j) {
+        const float4 k = terms[3 * j];
+        const float2 e = *reinterpret_cast<const float2*>(&terms[3 * j + 1]);
+        const f32x2 s = j < 16 ? pair(__uint_as_float(s0[(2 * j) & 31]), __uint_as_float(s0[(2 * j + 1) & 31]))
+                               : pair(__uint_as_float(s1[(2 * j) & 31]), __uint_as_float(s1[(2 * j + 1) & 31]));
+        const float2 v = unpair(fma2(s, pair(k.x, k.y), fma2(q2, pair(k.z, k.w), pair(e.x, e.y))));
+        xs[2 * j] = v.x;
+        xs[2 * j + 1] = v.y;
+      }
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < kPos; ++j) {
+          const int p = p0 + j;
+          const bool seen = p <= at && (A.window <= 0 || p > at - A.window || p < A.sinks);
+          if (!seen) xs[j] = -INFINITY;
+        }
+      }
+      float m[4] = {xs[0], xs[1], xs[2], xs[3]};
+#pragma unroll
+      for (int j = 4; j < kPos; ++j) m[j & 3] = fmaxf(m[j & 3], xs[j]);
+      const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      const bool raise = __any_sync(0xFFFFFFFFu, top > ref + kRaise);  // the first seen position too: ref is -inf
+      if (it > 0) {
+        ok = mbar_wait_bounded(&bar.p_free[x], (it - 1) & 1, kPromptTimeout);  // P and O are at rest
+        if (!__all_sync(0xFFFFFFFFu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+      }
+      if (raise) {
+        const float next = fmaxf(ref, top);
+        const float corr = next > ref ? ex2(ref - next) : 1.0f;
+        ref = next;
+        sum2 = mul2(sum2, pair(corr, corr));
+        off2 = mul2(off2, pair(corr, corr));
+        if (it > 0) {
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t o[32];
+            tmem_ld32(to + c0, o);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+            tmem_st32(to + c0, o);
+          }
+        }
+      }
+      const f32x2 minus = pair(-ref, -ref);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = 16 * half + i;
+          const float4 mu = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(terms) + 12 * j + 4);
+          const float4 uo = terms[3 * j + 2];
+          const float2 d = unpair(add2(pair(xs[2 * j], xs[2 * j + 1]), minus));
+          f32x2 pw = pair(ex2(d.x), ex2(d.y));
+          f32x2 w;
+          if (whole) {
+            sum2 = fma2(pw, pair(uo.x, uo.y), sum2);
+            off2 = fma2(pw, pair(uo.z, uo.w), off2);
+            w = mul2(pw, pair(mu.z, mu.w));
+          } else {  // a masked position's terms may hold anything
+            const bool a = xs[2 * j] != -INFINITY, c = xs[2 * j + 1] != -INFINITY;
+            const float2 v = unpair(pw);
+            pw = pair(a ? v.x : 0.0f, c ? v.y : 0.0f);
+            sum2 = fma2(pw, pair(a ? uo.x : 0.0f, c ? uo.y : 0.0f), sum2);
+            off2 = fma2(pw, pair(a ? uo.z : 0.0f, c ? uo.w : 0.0f), off2);
+            w = mul2(pw, pair(a ? mu.z : 0.0f, c ? mu.w : 0.0f));
+          }
+          const float2 wv = unpair(w);
+          hi[i] = pack_f16(wv.x, wv.y);
+          if constexpr (kSplit) {
+            const float2 h = unpack_f16(hi[i]);
+            lo[i] = pack_f16(wv.x - h.x, wv.y - h.y);
+          }
+        }
+        tmem_st16(tp + 16 * half, hi);
+        if constexpr (kSplit) tmem_st16(tp + kPos / 2 + 16 * half, lo);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&bar.p_full[x]);
+    }
+    if (tiles > 0 && ok) {
+      ok = mbar_wait_bounded(&bar.p_free[x], (tiles - 1) & 1, kPromptTimeout);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+    }
+    tc_fence_after();
+    if (ok) {
+      const float2 s = unpair(sum2), f = unpair(off2);
+      const float total = s.x + s.y, inv = total == 0.0f ? 0.0f : 1.0f / total, offset = f.x + f.y;
+      T* out = nullptr;
+      if (mine) {
+        const int t = token_of(item), h = kvh * A.group + item - t * A.group;
+        out = static_cast<T*>(A.out) + (row0 + t) * A.o_row + h * A.o_head;
+      }
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t o[32];
+        if (tiles > 0) tmem_ld32(to + c0, o);
+        if (mine) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = total == 0.0f ? 0.0f : fmaf(__uint_as_float(o[8 * c + j]), 1.0f / kWeightUnit, offset) * inv;
+            store_values<T, 8>(out + c0 + 8 * c, A.o_vec, y);
+          }
+        }
+      }
+    }
+  }
+  if (!ok) which[2] = 1;
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && which[2] != 0 && A.error != nullptr) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ETIMEOUT));
+  if (warp == 12) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::columns));
+  }
+}
+
+template <int D, typename T>
+int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
+  using G = PromptGeometry<D, std::is_same<T, float>::value>;
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  IVB_CUDA(cudaGetDevice(&device));
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if ((done.load(std::memory_order_relaxed) & bit) == 0) {
+    IVB_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem));
+    done.fetch_or(bit, std::memory_order_relaxed);
+  }
+  // as many tiles as the rows can make: each sequence of the call may leave one unfilled
+  const int64_t items = static_cast<int64_t>(A.rows) * A.group;
+  const int64_t sequences = std::min<int64_t>(A.cache.batch, items / (few + 1));
+  const int64_t tiles = items / kRowsCta + sequences;
+  if (sequences == 0) return IVB_OK;
+  if (tiles * A.cache.kv_heads > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(tiles));
+  kv4_prompt_kernel<D, T><<<static_cast<unsigned>(tiles * A.cache.kv_heads), kPromptThreads, G::smem, stream>>>(A, few);
+  IVB_CUDA(cudaGetLastError());
+  return IVB_OK;
+}
+
+template <typename T>
+int32_t launch_dim(const Kv4Attention& A, int few, cudaStream_t stream) {
+  switch (A.cache.head_dim) {
+    case 32: return launch_prompts<32, T>(A, few, stream);
+    case 64: return launch_prompts<64, T>(A, few, stream);
+    default: return launch_prompts<128, T>(A, few, stream);
+  }
+}
+
+}  // namespace
+
+int32_t launch_kv4_prompts(const Kv4Attention& A, int32_t dtype, int few, cudaStream_t stream) {
+  if (dtype == IVB_F32) return launch_dim<float>(A, few, stream);
+  if (dtype == IVB_F16) return launch_dim<__half>(A, few, stream);
+  return launch_dim<__nv_bfloat16>(A, few, stream);
+}
+
+}  // namespace ivb
