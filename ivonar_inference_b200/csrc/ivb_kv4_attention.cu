@@ -304,6 +304,9 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
           }
       }
     }
+    float from[kSets];  // a row that has seen nothing yet: any number, so that its weights are 2^-inf
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) from[s] = ref[s] == -INFINITY ? 0.0f : ref[s];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       uint32_t bw[kTiles][2];
@@ -313,18 +316,10 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
         float wgt[kSets];
 #pragma unroll
         for (int s = 0; s < kSets; ++s) {
-          const float xi = x[s][2 * t + h];
-          const float pw = ex2(xi - ref[s]);
-          if (whole) {
-            sum[s] = fmaf(pw, pt.x, sum[s]);
-            off[s] = fmaf(pw, pt.y, off[s]);
-            wgt[s] = pw * mantissa[2 * t + h];
-          } else {  // a masked position's terms may hold anything
-            const bool seen = xi != -INFINITY;
-            sum[s] = seen ? fmaf(pw, pt.x, sum[s]) : sum[s];
-            off[s] = seen ? fmaf(pw, pt.y, off[s]) : off[s];
-            wgt[s] = seen ? pw * mantissa[2 * t + h] : 0.0f;
-          }
+          const float pw = ex2(x[s][2 * t + h] - from[s]);
+          sum[s] = fmaf(pw, pt.x, sum[s]);
+          off[s] = fmaf(pw, pt.y, off[s]);
+          wgt[s] = pw * mantissa[2 * t + h];
         }
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {

@@ -65,7 +65,8 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t w) {
 // What the softmax needs of one position: x = S key_scale + sum(q) key_offset + bias, with bias the exponent of the value
 // scale, so that the running reference is the maximum of weight times value scale and neither overflows fp16, whatever the
 // scales; the weight is then 2^(x - ref) = p 2^bias, its product with the mantissa the A operand of the value product, and
-// p = weight * unbias enters the sum.
+// p = weight * unbias enters the sum. A position whose value scale or offset is no number has a score that is none, and
+// value terms of zero: it makes the rows that see it NaN, and a masked one's weight of zero stays zero whatever it holds.
 struct PositionTerms {
   float key_scale, key_offset, bias, mantissa;  // mantissa of the value scale, times weight_unit
   float unbias, value_offset;                   // 2^-bias, value offset times 2^-bias (offsets are of u - 8)
@@ -76,12 +77,12 @@ __device__ __forceinline__ PositionTerms position_terms(uint2 par, float score_u
   PositionTerms t;
   t.key_scale = key.x * score_unit;
   t.key_offset = fmaf(8.0f, key.x, key.y) * offset_unit;
-  const uint32_t bits = __float_as_uint(value.x) & 0x7f800000u;
-  const uint32_t e = bits == 0x7f800000u ? 0x3f800000u : max(bits, 0x33800000u);  // 2^-24 is the least scale above zero
-  t.bias = static_cast<float>(static_cast<int>(e >> 23) - 127);
-  t.unbias = __uint_as_float(0x7f000000u - e);
-  t.mantissa = value.x * t.unbias * weight_unit;
-  t.value_offset = fmaf(8.0f, value.x, value.y) * t.unbias;
+  const bool number = (par.y & 0x7c00u) != 0x7c00u && (par.y & 0x7c000000u) != 0x7c000000u;
+  const uint32_t e = max(__float_as_uint(value.x) & 0x7f800000u, 0x33800000u);  // 2^-24 is the least scale above zero
+  t.bias = number ? static_cast<float>(static_cast<int>(e >> 23) - 127) : __uint_as_float(0x7fffffffu);
+  t.unbias = number ? __uint_as_float(0x7f000000u - e) : 0.0f;
+  t.mantissa = number ? value.x * t.unbias * weight_unit : 0.0f;
+  t.value_offset = number ? fmaf(8.0f, value.x, value.y) * t.unbias : 0.0f;
   return t;
 }
 

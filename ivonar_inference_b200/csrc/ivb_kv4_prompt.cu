@@ -432,23 +432,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         break;
       }
       tc_fence_after();
-      uint32_t s0[32], s1[32];
-      tmem_ld32(ts, s0);
-      tmem_ld32(ts + 32, s1);
-      tc_fence_before();
-      mbar_arrive(&bar.s_free[x]);
       const bool all = at >= p0 + kPos - 1 && (A.window <= 0 || p0 > at - A.window || p0 <= A.sinks - kPos);
       const bool whole = __all_sync(0xFFFFFFFFu, all || !mine);
       float xs[kPos];
 #pragma unroll
-      for (int j = 0; j < kPos / 2; ++j) {
-        const float4 k = terms[3 * j];
-        const float2 e = *reinterpret_cast<const float2*>(&terms[3 * j + 1]);
-        const f32x2 s = j < 16 ? pair(__uint_as_float(s0[(2 * j) & 31]), __uint_as_float(s0[(2 * j + 1) & 31]))
-                               : pair(__uint_as_float(s1[(2 * j) & 31]), __uint_as_float(s1[(2 * j + 1) & 31]));
-        const float2 v = unpair(fma2(s, pair(k.x, k.y), fma2(q2, pair(k.z, k.w), pair(e.x, e.y))));
-        xs[2 * j] = v.x;
-        xs[2 * j + 1] = v.y;
+      for (int half = 0; half < 2; ++half) {
+        uint32_t s[32];
+        tmem_ld32(ts + 32 * half, s);
+        if (half == 1) {
+          tc_fence_before();
+          mbar_arrive(&bar.s_free[x]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = 16 * half + i;
+          const float4 k = terms[3 * j];
+          const float2 e = *reinterpret_cast<const float2*>(&terms[3 * j + 1]);
+          const float2 v = unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), pair(k.x, k.y),
+                                       fma2(q2, pair(k.z, k.w), pair(e.x, e.y))));
+          xs[2 * j] = v.x;
+          xs[2 * j + 1] = v.y;
+        }
       }
       if (!whole) {
 #pragma unroll
@@ -488,30 +492,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           }
         }
       }
-      const f32x2 minus = pair(-ref, -ref);
+      const float from = ref == -INFINITY ? 0.0f : -ref;  // a row that has seen nothing yet: its weights are 2^-inf
+      const f32x2 minus = pair(from, from);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int j = 16 * half + i;
-          const float4 mu = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(terms) + 12 * j + 4);
+          const float2 mu = reinterpret_cast<const float2*>(terms)[6 * j + 3];
           const float4 uo = terms[3 * j + 2];
           const float2 d = unpair(add2(pair(xs[2 * j], xs[2 * j + 1]), minus));
-          f32x2 pw = pair(ex2(d.x), ex2(d.y));
-          f32x2 w;
-          if (whole) {
-            sum2 = fma2(pw, pair(uo.x, uo.y), sum2);
-            off2 = fma2(pw, pair(uo.z, uo.w), off2);
-            w = mul2(pw, pair(mu.z, mu.w));
-          } else {  // a masked position's terms may hold anything
-            const bool a = xs[2 * j] != -INFINITY, c = xs[2 * j + 1] != -INFINITY;
-            const float2 v = unpair(pw);
-            pw = pair(a ? v.x : 0.0f, c ? v.y : 0.0f);
-            sum2 = fma2(pw, pair(a ? uo.x : 0.0f, c ? uo.y : 0.0f), sum2);
-            off2 = fma2(pw, pair(a ? uo.z : 0.0f, c ? uo.w : 0.0f), off2);
-            w = mul2(pw, pair(a ? mu.z : 0.0f, c ? mu.w : 0.0f));
-          }
+          const f32x2 pw = pair(ex2(d.x), ex2(d.y));
+          sum2 = fma2(pw, pair(uo.x, uo.y), sum2);
+          off2 = fma2(pw, pair(uo.z, uo.w), off2);
+          const f32x2 w = mul2(pw, pair(mu.x, mu.y));
           const float2 wv = unpair(w);
           hi[i] = pack_f16(wv.x, wv.y);
           if constexpr (kSplit) {
