@@ -1,16 +1,16 @@
 // Causal attention over the 4-bit key/value cache for prompts: many rows a sequence, on the 5th-generation tensor cores.
 //
-// One CTA per (sequence, key/value head, 256 rows), 13 warps. Row i of a sequence's head group is token i / group, query head
-// i % group; rows 0..127 and 128..255 are two tiles X of the tensor cores' 128 lanes. Per tile of 64 positions:
-//   warps 8..11 (producers) read the codes, expand them to fp16 u - 8 in shared memory (keys as a K-major operand, values as an
+// One CTA per (sequence, key/value head, 256 rows), 12 warps. Row i of a sequence's head group is token i / group, query head
+// i % group; rows 0..127 and 128..255 are two tiles X of the tensor cores' 128 lanes. Per tile of 128 positions:
+//   warps 8..10 (producers) read the codes, expand them to fp16 u - 8 in shared memory (keys as a K-major operand, values as an
 //     MN-major one: both are position rows of 16-byte channel chunks, so neither is transposed) and compute each
 //     position's terms (scales and offsets; ivb_kv4_attention.cuh);
-//   warp 12 (one thread) issues S_X = Q_X U^T and O_X += P_X U'^T, fp32 in tensor memory, P_X from tensor memory;
+//   warp 11 (one thread) issues S_X = Q_X U^T and O_X += P_X U'^T, fp32 in tensor memory;
 //   warps 0..7 (a thread owns one row, which is its tensor-memory lane) turn S_X into weights: online softmax in 32 bits, the
-//     reference raised only when the maximum passes it by 2^8, and O_X rescaled in tensor memory then.
-// fp32 queries and weights are hi + lo fp16 pairs: two products each. S_X(it + 1) is issued as soon as S_X(it) has been read,
-// so the tensor pipe works while the softmax does. What bounds it is the softmax's issue slots (about 7 per score, with
-// paired fp32 instructions) and, at D = 128, the tensor pipe beside it.
+//     reference raised only when the maximum passes it by 2^8, and O_X rescaled in tensor memory then. The weights P_X take
+//     S_X's place as the fp16 A operand, so S_X(it + 1) follows P_X(it)'s product; while one X waits for it the other computes.
+// fp32 queries and weights are hi + lo fp16 pairs: two products each. 128 positions because a product from shared memory takes
+// 70 cycles for 64 columns as for 128 (measured). What bounds it is the softmax's issue slots, then the tensor pipe (D = 128).
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -23,8 +23,10 @@
 namespace ivb {
 namespace {
 
-constexpr int kRowsX = 128, kRowsCta = 256, kPos = 64;
-constexpr int kSoftmaxThreads = 256, kProducers = 128, kPromptThreads = kSoftmaxThreads + kProducers + 32;
+constexpr int kRowsX = 128, kRowsCta = 256, kPos = 128;
+// 12 warps: with three on each of the SM's four parts a thread has 168 registers, enough for its 128 scores
+constexpr int kSoftmaxThreads = 256, kProducerWarps = 3, kProducers = 32 * kProducerWarps, kPromptThreads = kSoftmaxThreads + kProducers + 32;
+constexpr int kTermSets = 3;  // terms(it + 2) are written when S(it) is done, so when nobody reads terms(it - 1) any more
 constexpr unsigned long long kPromptTimeout = 2000000000ull;
 constexpr float kWeightUnit = 64.0f;  // weights are at most 2 * 64 * 2^8 in fp16
 constexpr float kRaise = 8.0f;
@@ -32,15 +34,15 @@ constexpr float kRaise = 8.0f;
 template <int D, bool kSplit>
 struct PromptGeometry {
   static constexpr int parts = kSplit ? 2 : 1;
-  static constexpr int q_bytes = kRowsX * D * 2;    // one part of one row tile
-  static constexpr int kv_bytes = kPos * D * 2;     // keys or values of a stage
+  static constexpr int stages = kSplit && D == 128 ? 1 : 2;  // of keys and of values
+  static constexpr int q_bytes = kRowsX * D * 2;             // one part of one row tile
+  static constexpr int kv_bytes = kPos * D * 2;              // keys or values of a stage
   static constexpr int term_bytes = kPos * 24;
-  static constexpr int q_at = 0, kv_at = 2 * parts * q_bytes, terms_at = kv_at + 4 * kv_bytes;
-  static constexpr int smem = terms_at + 2 * term_bytes;
-  // tensor memory columns
-  static constexpr int s_at = 0, p_at = 2 * kPos, o_at = p_at + 2 * parts * (kPos / 2), columns_used = o_at + 2 * D;
-  static constexpr int columns = columns_used <= 256 ? 256 : 512;
-  static_assert(columns_used <= 512, "tensor memory");
+  static constexpr int q_at = 0, k_at = 2 * parts * q_bytes, v_at = k_at + stages * kv_bytes, terms_at = v_at + stages * kv_bytes;
+  static constexpr int smem = terms_at + kTermSets * term_bytes;
+  // tensor memory columns: S_X, then P_X in its place (of every 32 columns 16 hi, 16 lo), and O_X
+  static constexpr int s_at = 0, o_at = 2 * kPos, columns = 512;
+  static_assert(o_at + 2 * D <= columns, "tensor memory");
 };
 
 // kind::f16, fp32 result, A K-major, B MN-major.
@@ -89,101 +91,83 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
 }
 
 struct PromptBarriers {
-  unsigned long long kv_full[2], kv_free[2], s_full[2], s_free[2], p_full[2], p_free[2], drain;
+  unsigned long long k_full[2], k_free[2], v_full[2], v_free[2], terms_full[kTermSets], s_full[2], p_full[2], p_free[2], drain;
 };
 
-// Raw codes of one 64-position tile that a producer thread holds: what it expands itself.
+// What a lane of a producer warp holds of the keys or values of one tile of 16 positions (D = 32: values in lanes 0..15), dealt
+// out so that 8 neighbouring lanes write the 8 rows of a core matrix, without bank conflicts.
 template <int D>
-struct RawTile {
-  static constexpr int key_chunks = D == 128 ? 2 : 1, value_chunks = D == 128 ? 2 : 1;
-  uint4 key[key_chunks], value[value_chunks];
-  uint2 par;
+struct RawChunks {
+  static constexpr int n = D == 128 ? 2 : 1;
+  uint4 v[n];
 };
 
-// Producer thread j (0..127): tile j / 32 of 16 positions (D = 32: values of threads 0..63), so that 8 neighbouring threads
-// write the 8 rows of a core matrix, without bank conflicts.
 template <int D>
-__device__ __forceinline__ void load_raw(const unsigned char* tiles16, int valid, int j, RawTile<D>& raw) {
-  constexpr int kTile = kv4_tile_bytes(D);
-  const int t = j >> 5;
-  const bool in = t < valid;
-  const unsigned char* at = tiles16 + static_cast<int64_t>(in ? t : 0) * kTile;
+__device__ __forceinline__ void load_keys(const unsigned char* tile, bool in, int lane, RawChunks<D>& raw) {
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   if constexpr (D == 128) {
-    const int h = (j >> 2) & 1, c = (j >> 3) & 3;
+    const int h = (lane >> 2) & 1, c = lane >> 3;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) raw.key[k] = in ? __ldg(reinterpret_cast<const uint4*>(at + 512 * h + (((j & 3) + 4 * k) * 4 + c) * 16)) : zero;
+    for (int k = 0; k < 2; ++k) raw.v[k] = in ? __ldg(reinterpret_cast<const uint4*>(tile + 512 * h + (((lane & 3) + 4 * k) * 4 + c) * 16)) : zero;
   } else {
-    const int r = j & 7, c = (j >> 3) & 3;
+    const int r = lane & 7, c = lane >> 3;
     if constexpr (D == 64) {
-      raw.key[0] = in ? __ldg(reinterpret_cast<const uint4*>(at + (r * 4 + c) * 16)) : zero;
+      raw.v[0] = in ? __ldg(reinterpret_cast<const uint4*>(tile + (r * 4 + c) * 16)) : zero;
     } else {
-      const uint2 v = in ? __ldg(reinterpret_cast<const uint2*>(at + (r * 4 + c) * 8)) : make_uint2(0u, 0u);
-      raw.key[0] = make_uint4(v.x, v.y, 0u, 0u);
+      const uint2 v = in ? __ldg(reinterpret_cast<const uint2*>(tile + (r * 4 + c) * 8)) : make_uint2(0u, 0u);
+      raw.v[0] = make_uint4(v.x, v.y, 0u, 0u);
     }
   }
-  if constexpr (D == 32) {
-    const int r = j & 3, c = ((j >> 2) & 1) + 2 * ((j >> 3) & 1), tv = (j >> 4) & 3;
-    raw.value[0] = j < 64 && tv < valid ? __ldg(reinterpret_cast<const uint4*>(tiles16 + static_cast<int64_t>(tv) * kTile + 8 * D + (r * 4 + c) * 16)) : zero;
-  } else {
-    const int r = (j & 3) + 4 * ((j >> 4) & 1), c = ((j >> 2) & 1) + 2 * ((j >> 3) & 1);
+}
+template <int D>
+__device__ __forceinline__ void load_codes_of_values(const unsigned char* tile, bool in, int lane, RawChunks<D>& raw) {
+  const int r = D == 32 ? lane & 3 : (lane & 3) + 4 * (lane >> 4), c = (lane >> 2) & 3;
+  in = in && (D != 32 || lane < 16);
 #pragma unroll
-    for (int k = 0; k < RawTile<D>::value_chunks; ++k)
-      raw.value[k] = in ? __ldg(reinterpret_cast<const uint4*>(at + 8 * D + 512 * k + (r * 4 + c) * 16)) : zero;
-  }
-  if (j < kPos) raw.par = (j >> 4) < valid ? __ldg(reinterpret_cast<const uint2*>(tiles16 + static_cast<int64_t>(j >> 4) * kTile + 16 * D + (j & 15) * 8)) : make_uint2(0u, 0u);
+  for (int k = 0; k < RawChunks<D>::n; ++k)
+    raw.v[k] = in ? __ldg(reinterpret_cast<const uint4*>(tile + 8 * D + 512 * k + (r * 4 + c) * 16)) : make_uint4(0u, 0u, 0u, 0u);
 }
 
+// `keys`, `values`: the tile's 16 position rows.
 template <int D>
-__device__ __forceinline__ void store_raw(const RawTile<D>& raw, int j, unsigned char* keys, unsigned char* values, float* terms,
-                                          float score_unit, float offset_unit) {
-  const int t = j >> 5;
+__device__ __forceinline__ void store_keys(const RawChunks<D>& raw, int lane, unsigned char* keys) {
   if constexpr (D == 128) {
-    const int h = (j >> 2) & 1, c = (j >> 3) & 3;
+    const int h = (lane >> 2) & 1, c = lane >> 3;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int r = (j & 3) + 4 * k, p = 16 * t + 4 * (r >> 1) + (r & 1) + 2 * h;
-      const uint32_t w[4] = {raw.key[k].x, raw.key[k].y, raw.key[k].z, raw.key[k].w};
+      const int r = (lane & 3) + 4 * k, p = 4 * (r >> 1) + (r & 1) + 2 * h;
+      const uint32_t w[4] = {raw.v[k].x, raw.v[k].y, raw.v[k].z, raw.v[k].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(keys + chunk_at<D>(p, 4 * c + i)) = expand(w[i]);
     }
   } else {
-    const int r = j & 7, c = (j >> 3) & 3, other = r >> 2;  // the upper four rows' lanes take their two positions in the other order
-    const int p = 16 * t + 4 * (r >> 1) + (r & 1);
+    const int r = lane & 7, c = lane >> 3, other = r >> 2;  // the upper four rows' lanes take their two positions in the other order
+    const int p = 4 * (r >> 1) + (r & 1);
     if constexpr (D == 64) {
-      const uint2 a = other ? make_uint2(raw.key[0].z, raw.key[0].w) : make_uint2(raw.key[0].x, raw.key[0].y);
-      const uint2 b = other ? make_uint2(raw.key[0].x, raw.key[0].y) : make_uint2(raw.key[0].z, raw.key[0].w);
+      const uint2 a = other ? make_uint2(raw.v[0].z, raw.v[0].w) : make_uint2(raw.v[0].x, raw.v[0].y);
+      const uint2 b = other ? make_uint2(raw.v[0].x, raw.v[0].y) : make_uint2(raw.v[0].z, raw.v[0].w);
       *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, 2 * c)) = expand(a.x);
       *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, 2 * c + 1)) = expand(a.y);
       *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, 2 * c)) = expand(b.x);
       *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, 2 * c + 1)) = expand(b.y);
     } else {
-      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, c)) = expand(other ? raw.key[0].y : raw.key[0].x);
-      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, c)) = expand(other ? raw.key[0].x : raw.key[0].y);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, c)) = expand(other ? raw.v[0].y : raw.v[0].x);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, c)) = expand(other ? raw.v[0].x : raw.v[0].y);
     }
   }
-  if (D != 32 || j < 64) {
-    const int turn = j & 3, c = ((j >> 2) & 1) + 2 * ((j >> 3) & 1);
-    const int r = D == 32 ? j & 3 : (j & 3) + 4 * ((j >> 4) & 1), tv = D == 32 ? (j >> 4) & 3 : t;
+}
+template <int D>
+__device__ __forceinline__ void store_codes_of_values(const RawChunks<D>& raw, int lane, unsigned char* values) {
+  if (D == 32 && lane >= 16) return;
+  const int turn = lane & 3, c = (lane >> 2) & 3, r = D == 32 ? lane & 3 : (lane & 3) + 4 * (lane >> 4);
 #pragma unroll
-    for (int k = 0; k < RawTile<D>::value_chunks; ++k) {
-      uint4 v = raw.value[k];  // word i of the lane is position 4 c + i: each lane begins with another one
-      if (turn & 1) v = make_uint4(v.y, v.z, v.w, v.x);
-      if (turn & 2) v = make_uint4(v.z, v.w, v.x, v.y);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  for (int k = 0; k < RawChunks<D>::n; ++k) {
+    uint4 v = raw.v[k];  // word i of the lane is position 4 c + i: each lane begins with another one
+    if (turn & 1) v = make_uint4(v.y, v.z, v.w, v.x);
+    if (turn & 2) v = make_uint4(v.z, v.w, v.x, v.y);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(values + chunk_at<D>(16 * tv + 4 * c + ((i + turn) & 3), 8 * k + r)) = expand(w[i]);
-    }
-  }
-  if (j < kPos) {
-    const PositionTerms p = position_terms(raw.par, score_unit, offset_unit, kWeightUnit);
-    float* at = terms + 12 * (j >> 1) + (j & 1);
-    at[0] = p.key_scale;
-    at[2] = p.key_offset;
-    at[4] = p.bias;
-    at[6] = p.mantissa;
-    at[8] = p.unbias;
-    at[10] = p.value_offset;
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(values + chunk_at<D>(4 * c + ((i + turn) & 3), 8 * k + r)) = expand(w[i]);
   }
 }
 
@@ -235,20 +219,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   if (tid == 32) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.kv_full[i], kProducers);
-      mbar_init(&bar.kv_free[i], 1);
+      mbar_init(&bar.k_full[i], kProducers);
+      mbar_init(&bar.k_free[i], 1);
+      mbar_init(&bar.v_full[i], kProducers);
+      mbar_init(&bar.v_free[i], 1);
       mbar_init(&bar.s_full[i], 1);
-      mbar_init(&bar.s_free[i], kRowsX);
       mbar_init(&bar.p_full[i], kRowsX);
       mbar_init(&bar.p_free[i], 1);
     }
+#pragma unroll
+    for (int i = 0; i < kTermSets; ++i) mbar_init(&bar.terms_full[i], kProducers);
     mbar_init(&bar.drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
   const int b = which[0];
   if (b < 0) return;
-  if (warp == 12) {
+  if (warp == kPromptThreads / 32 - 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)), "r"(G::columns));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -265,7 +252,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   auto clamp_position = [&](int64_t p) { return static_cast<int>(max(static_cast<int64_t>(-1), min(p, static_cast<int64_t>(max_len)))); };
   const int first = clamp_position(base + token_of(i0)), last = clamp_position(base + token_of(i0 + live - 1));
   if (last >= max_len && tid == 0 && A.error != nullptr) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
-  // the tiles of 64 positions that some row sees: the sinks' below the window, then the window's
+  // the tiles of 128 positions that some row sees: the sinks' below the window, then the window's
   const int high = min(last, max_len - 1);
   const int low = A.window > 0 ? max(0, max(first, 0) - A.window + 1) : 0;
   const int window_tile = low / kPos;
@@ -339,39 +326,85 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = tmem_base;
-  auto keys_of = [&](int stage) { return smem + G::kv_at + stage * 2 * G::kv_bytes; };
-  auto terms_of = [&](int stage) { return reinterpret_cast<float*>(smem + G::terms_at + stage * G::term_bytes); };
+  auto keys_of = [&](int it) { return smem + G::k_at + it % G::stages * G::kv_bytes; };
+  auto values_of = [&](int it) { return smem + G::v_at + it % G::stages * G::kv_bytes; };
+  auto terms_of = [&](int it) { return reinterpret_cast<float*>(smem + G::terms_at + it % kTermSets * G::term_bytes); };
+  auto turn_of = [&](int it) { return static_cast<unsigned>(it / G::stages) & 1u; };  // parity of a stage's use
   bool ok = true;
 
-  if (warp >= 8 && warp < 12) {
-    // ---- producers ----
-    const int j = tid - kSoftmaxThreads;
+  if (warp >= kSoftmaxThreads / 32 && warp < kPromptThreads / 32 - 1) {
+    // ---- producers: 16-position tiles in turn ----
+    constexpr int kTile = kv4_tile_bytes(D), kUnits = kPos / 16, kMine = (kUnits + kProducerWarps - 1) / kProducerWarps;
+    const int unit0 = warp - kSoftmaxThreads / 32;
     const int64_t tiles16 = kv4_tiles(max_len);
-    const unsigned char* codes = static_cast<const unsigned char*>(A.cache.data) +
-                                 (static_cast<int64_t>(b) * A.cache.kv_heads + kvh) * tiles16 * kv4_tile_bytes(D);
-    RawTile<D> raw;
-    auto fetch = [&](int it) {
-      const int64_t t16 = static_cast<int64_t>(tile_of(it)) * (kPos / 16);
-      load_raw<D>(codes + t16 * kv4_tile_bytes(D), static_cast<int>(min(static_cast<int64_t>(4), tiles16 - t16)), j, raw);
+    const unsigned char* codes = static_cast<const unsigned char*>(A.cache.data) + (static_cast<int64_t>(b) * A.cache.kv_heads + kvh) * tiles16 * kTile;
+    RawChunks<D> key[kMine], value[kMine];
+    uint2 par[kMine];
+    auto fetch = [&](int it, bool keys) {
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) {
+        const int u = unit0 + k * kProducerWarps;
+        const int64_t t = static_cast<int64_t>(tile_of(it)) * kUnits + u;
+        const bool in = u < kUnits && t < tiles16;
+        const unsigned char* tile = codes + (in ? t : 0) * kTile;
+        if (keys) {
+          load_keys<D>(tile, in, lane, key[k]);
+          par[k] = in && lane < 16 ? __ldg(reinterpret_cast<const uint2*>(tile + 16 * D + lane * 8)) : make_uint2(0u, 0u);
+        } else {
+          load_codes_of_values<D>(tile, in, lane, value[k]);
+        }
+      }
     };
-    if (tiles > 0) fetch(0);
+    if (tiles > 0) fetch(0, true);
     for (int it = 0; it < tiles; ++it) {
-      const int st = it & 1;
-      if (it >= 2 && !mbar_wait_bounded(&bar.kv_free[st], ((it >> 1) - 1) & 1, kPromptTimeout)) {
+      fetch(it, false);
+      if (it >= G::stages && !mbar_wait_bounded(&bar.k_free[it % G::stages], turn_of(it) ^ 1u, kPromptTimeout)) {
         ok = false;
         break;
       }
-      store_raw<D>(raw, j, keys_of(st), keys_of(st) + G::kv_bytes, terms_of(st), score_unit, offset_unit);
+      if (lane < 16) {
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+          const int u = unit0 + k * kProducerWarps;
+          if (u < kUnits) {
+            const PositionTerms p = position_terms(par[k], score_unit, offset_unit, kWeightUnit);
+            float* at_terms = terms_of(it) + 12 * (8 * u + (lane >> 1)) + (lane & 1);
+            at_terms[0] = p.key_scale;
+            at_terms[2] = p.key_offset;
+            at_terms[4] = p.bias;
+            at_terms[6] = p.mantissa;
+            at_terms[8] = p.unbias;
+            at_terms[10] = p.value_offset;
+          }
+        }
+      }
+      mbar_arrive(&bar.terms_full[it % kTermSets]);
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) {
+        const int u = unit0 + k * kProducerWarps;
+        if (u < kUnits) store_keys<D>(key[k], lane, keys_of(it) + u * 16 * D * 2);
+      }
       fence_proxy_async();
-      mbar_arrive(&bar.kv_full[st]);
-      if (it + 1 < tiles) fetch(it + 1);
+      mbar_arrive(&bar.k_full[it % G::stages]);
+      if (it + 1 < tiles) fetch(it + 1, true);
+      if (it >= G::stages && !mbar_wait_bounded(&bar.v_free[it % G::stages], turn_of(it) ^ 1u, kPromptTimeout)) {
+        ok = false;
+        break;
+      }
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) {
+        const int u = unit0 + k * kProducerWarps;
+        if (u < kUnits) store_codes_of_values<D>(value[k], lane, values_of(it) + u * 16 * D * 2);
+      }
+      fence_proxy_async();
+      mbar_arrive(&bar.v_full[it % G::stages]);
     }
-  } else if (warp == 12) {
+  } else if (warp == kPromptThreads / 32 - 1) {
     // ---- the thread that issues the products ----
     if (lane == 0) {
       const unsigned q0 = smem_addr(smem + G::q_at);
       auto issue_s = [&](int it, int xx) {
-        const unsigned ka = smem_addr(keys_of(it & 1)), qa = q0 + xx * G::parts * G::q_bytes;
+        const unsigned ka = smem_addr(keys_of(it)), qa = q0 + xx * G::parts * G::q_bytes;
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
@@ -382,34 +415,38 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         umma_commit(&bar.s_full[xx]);
       };
       auto issue_o = [&](int it, int xx) {
-        const unsigned va = smem_addr(keys_of(it & 1)) + G::kv_bytes;
+        const unsigned va = smem_addr(values_of(it));
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < kPos / 16; ++kk)
 #pragma unroll
           for (int part = 0; part < G::parts; ++part)
-            umma_f16_ts(tmem + G::o_at + xx * D, tmem + G::p_at + (xx * G::parts + part) * (kPos / 2) + kk * 8,
+            umma_f16_ts(tmem + G::o_at + xx * D, tmem + G::s_at + xx * kPos + (kk >> 1) * 32 + part * 16 + (kk & 1) * 8,
                         smem_desc_mn(va + kk * 2 * (D / 8) * 128, D / 8 * 128), idesc_f16_bt(kRowsX, D), it > 0 || kk + part > 0);
         umma_commit(&bar.p_free[xx]);
       };
       if (tiles > 0) {
-        ok = mbar_wait_bounded(&bar.kv_full[0], 0, kPromptTimeout);
-        if (ok)
+        ok = mbar_wait_bounded(&bar.k_full[0], 0, kPromptTimeout);
+        if (ok) {
           for (int xx = 0; xx < row_tiles; ++xx) issue_s(0, xx);
+          umma_commit(&bar.k_free[0]);
+        }
       }
       for (int it = 0; it < tiles && ok; ++it) {
-        if (it + 1 < tiles) {
-          ok = mbar_wait_bounded(&bar.kv_full[(it + 1) & 1], ((it + 1) >> 1) & 1, kPromptTimeout);
-          for (int xx = 0; xx < row_tiles && ok; ++xx) {
-            ok = mbar_wait_bounded(&bar.s_free[xx], it & 1, kPromptTimeout);
-            if (ok) issue_s(it + 1, xx);
-          }
-        }
+        ok = mbar_wait_bounded(&bar.v_full[it % G::stages], turn_of(it), kPromptTimeout);
         for (int xx = 0; xx < row_tiles && ok; ++xx) {
           ok = mbar_wait_bounded(&bar.p_full[xx], it & 1, kPromptTimeout);
-          if (ok) issue_o(it, xx);
+          if (!ok) break;
+          issue_o(it, xx);
+          if (xx == row_tiles - 1) umma_commit(&bar.v_free[it % G::stages]);
+          if (it + 1 < tiles) {
+            ok = (xx > 0 || mbar_wait_bounded(&bar.k_full[(it + 1) % G::stages], turn_of(it + 1), kPromptTimeout)) &&
+                 mbar_wait_bounded(&bar.p_free[xx], it & 1, kPromptTimeout);  // S takes the place of P
+            if (!ok) break;
+            issue_s(it + 1, xx);
+            if (xx == row_tiles - 1) umma_commit(&bar.k_free[(it + 1) % G::stages]);
+          }
         }
-        if (ok) umma_commit(&bar.kv_free[it & 1]);
       }
       if (!ok) {  // let what was issued finish before shared and tensor memory go
         umma_commit(&bar.drain);
@@ -419,70 +456,70 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   } else if (x < row_tiles) {
     // ---- softmax: one row a thread ----
     const unsigned lanes = static_cast<unsigned>(32 * (warp & 3)) << 16;
-    const unsigned ts = tmem + lanes + G::s_at + x * kPos, tp = tmem + lanes + G::p_at + x * G::parts * (kPos / 2), to = tmem + lanes + G::o_at + x * D;
+    const unsigned ts = tmem + lanes + G::s_at + x * kPos, to = tmem + lanes + G::o_at + x * D;
     const f32x2 q2 = pair(sum_q, sum_q);
     float ref = -INFINITY;
     f32x2 sum2 = pair(0.0f, 0.0f), off2 = pair(0.0f, 0.0f);
     for (int it = 0; it < tiles; ++it) {
       const int p0 = tile_of(it) * kPos;
-      const float4* terms = reinterpret_cast<const float4*>(terms_of(it & 1));
-      ok = mbar_wait_bounded(&bar.kv_full[it & 1], (it >> 1) & 1, kPromptTimeout) && mbar_wait_bounded(&bar.s_full[x], it & 1, kPromptTimeout);
+      const float* terms = terms_of(it);
+      // S is full: the last product with P is done too, so O and P are at rest
+      ok = mbar_wait_bounded(&bar.terms_full[it % kTermSets], static_cast<unsigned>(it / kTermSets) & 1u, kPromptTimeout) &&
+           mbar_wait_bounded(&bar.s_full[x], it & 1, kPromptTimeout);
       if (!__all_sync(0xFFFFFFFFu, ok)) {
         ok = false;
         break;
       }
       tc_fence_after();
       const bool all = at >= p0 + kPos - 1 && (A.window <= 0 || p0 > at - A.window || p0 <= A.sinks - kPos);
+      const bool none = at < p0 || (A.window > 0 && p0 + kPos - 1 <= at - A.window && p0 >= A.sinks);
+      if (__all_sync(0xFFFFFFFFu, none || !mine)) {  // nothing of the tile for this warp's rows
+#pragma unroll
+        for (int c = 0; c < kPos; c += 32) tmem_fill32(ts + c, 0u);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bar.p_full[x]);
+        continue;
+      }
       const bool whole = __all_sync(0xFFFFFFFFu, all || !mine);
       float xs[kPos];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int c = 0; c < kPos; c += 32) {
         uint32_t s[32];
-        tmem_ld32(ts + 32 * half, s);
-        if (half == 1) {
-          tc_fence_before();
-          mbar_arrive(&bar.s_free[x]);
-        }
+        tmem_ld32(ts + c, s);
+        const float4* t4 = reinterpret_cast<const float4*>(terms + 6 * c);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int j = 16 * half + i;
-          const float4 k = terms[3 * j];
-          const float2 e = *reinterpret_cast<const float2*>(&terms[3 * j + 1]);
+          const float4 k = t4[3 * i];
+          const float2 e = *reinterpret_cast<const float2*>(&t4[3 * i + 1]);
           const float2 v = unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), pair(k.x, k.y),
                                        fma2(q2, pair(k.z, k.w), pair(e.x, e.y))));
-          xs[2 * j] = v.x;
-          xs[2 * j + 1] = v.y;
+          xs[c + 2 * i] = v.x;
+          xs[c + 2 * i + 1] = v.y;
         }
       }
       if (!whole) {
 #pragma unroll
         for (int j = 0; j < kPos; ++j) {
           const int p = p0 + j;
-          const bool seen = p <= at && (A.window <= 0 || p > at - A.window || p < A.sinks);
-          if (!seen) xs[j] = -INFINITY;
+          if (!(p <= at && (A.window <= 0 || p > at - A.window || p < A.sinks))) xs[j] = -INFINITY;
         }
       }
       float m[4] = {xs[0], xs[1], xs[2], xs[3]};
 #pragma unroll
-      for (int j = 4; j < kPos; ++j) m[j & 3] = fmaxf(m[j & 3], xs[j]);
-      const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-      const bool raise = __any_sync(0xFFFFFFFFu, top > ref + kRaise);  // the first seen position too: ref is -inf
-      if (it > 0) {
-        ok = mbar_wait_bounded(&bar.p_free[x], (it - 1) & 1, kPromptTimeout);  // P and O are at rest
-        if (!__all_sync(0xFFFFFFFFu, ok)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+      for (int j = 4; j < kPos; j += 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = fmaxf(m[i], fmaxf(xs[j + i], j + 4 + i < kPos ? xs[j + 4 + i] : xs[j + i]));
       }
-      if (raise) {
+      const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      if (__any_sync(0xFFFFFFFFu, top > ref + kRaise)) {  // the first seen position too: ref is -inf
         const float next = fmaxf(ref, top);
         const float corr = next > ref ? ex2(ref - next) : 1.0f;
         ref = next;
         sum2 = mul2(sum2, pair(corr, corr));
         off2 = mul2(off2, pair(corr, corr));
         if (it > 0) {
-#pragma unroll
+#pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 32) {
             uint32_t o[32];
             tmem_ld32(to + c0, o);
@@ -495,27 +532,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       const float from = ref == -INFINITY ? 0.0f : -ref;  // a row that has seen nothing yet: its weights are 2^-inf
       const f32x2 minus = pair(from, from);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int c = 0; c < kPos; c += 32) {
         uint32_t hi[16], lo[16];
+        const float4* t4 = reinterpret_cast<const float4*>(terms + 6 * c);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int j = 16 * half + i;
-          const float2 mu = reinterpret_cast<const float2*>(terms)[6 * j + 3];
-          const float4 uo = terms[3 * j + 2];
-          const float2 d = unpair(add2(pair(xs[2 * j], xs[2 * j + 1]), minus));
+          const float2 mu = reinterpret_cast<const float2*>(t4)[6 * i + 3];
+          const float4 uo = t4[3 * i + 2];
+          const float2 d = unpair(add2(pair(xs[c + 2 * i], xs[c + 2 * i + 1]), minus));
           const f32x2 pw = pair(ex2(d.x), ex2(d.y));
           sum2 = fma2(pw, pair(uo.x, uo.y), sum2);
           off2 = fma2(pw, pair(uo.z, uo.w), off2);
-          const f32x2 w = mul2(pw, pair(mu.x, mu.y));
-          const float2 wv = unpair(w);
-          hi[i] = pack_f16(wv.x, wv.y);
+          const float2 w = unpair(mul2(pw, pair(mu.x, mu.y)));
+          hi[i] = pack_f16(w.x, w.y);
           if constexpr (kSplit) {
             const float2 h = unpack_f16(hi[i]);
-            lo[i] = pack_f16(wv.x - h.x, wv.y - h.y);
+            lo[i] = pack_f16(w.x - h.x, w.y - h.y);
           }
         }
-        tmem_st16(tp + 16 * half, hi);
-        if constexpr (kSplit) tmem_st16(tp + kPos / 2 + 16 * half, lo);
+        tmem_st16(ts + c, hi);
+        if constexpr (kSplit) tmem_st16(ts + c + 16, lo);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -554,7 +590,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && which[2] != 0 && A.error != nullptr) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ETIMEOUT));
-  if (warp == 12) {
+  if (warp == kPromptThreads / 32 - 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::columns));
   }
