@@ -24,7 +24,7 @@ namespace ivb {
 namespace {
 
 constexpr int kRowsX = 128, kRowsCta = 256, kPos = 128;
-// 12 warps: with three on each of the SM's four parts a thread has 168 registers, enough for its 128 scores
+// 12 warps: with three on each of the SM's four parts a thread has 168 registers, enough to keep the loads of its 64 scores' terms ahead
 constexpr int kSoftmaxThreads = 256, kProducerWarps = 3, kProducers = 32 * kProducerWarps, kPromptThreads = kSoftmaxThreads + kProducers + 32;
 constexpr int kTermSets = 3;  // terms(it + 2) are written when S(it) is done, so when nobody reads terms(it - 1) any more
 constexpr unsigned long long kPromptTimeout = 2000000000ull;
@@ -91,7 +91,7 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
 }
 
 struct PromptBarriers {
-  unsigned long long k_full[2], k_free[2], v_full[2], v_free[2], terms_full[kTermSets], s_full[2], p_full[2], p_free[2], drain;
+  unsigned long long k_full[2], k_free[2], v_full[2], v_free[2], terms_full[kTermSets], s_full[2], p_full[2][2], p_free[2][2], drain;
 };
 
 // What a lane of a producer warp holds of the keys or values of one tile of 16 positions (D = 32: values in lanes 0..15), dealt
@@ -224,8 +224,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       mbar_init(&bar.v_full[i], kProducers);
       mbar_init(&bar.v_free[i], 1);
       mbar_init(&bar.s_full[i], 1);
-      mbar_init(&bar.p_full[i], kRowsX);
-      mbar_init(&bar.p_free[i], 1);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&bar.p_full[i][h], kRowsX);
+        mbar_init(&bar.p_free[i][h], 1);
+      }
     }
 #pragma unroll
     for (int i = 0; i < kTermSets; ++i) mbar_init(&bar.terms_full[i], kProducers);
@@ -414,16 +417,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
                         smem_desc(ka + kk * 256, D / 8 * 128), idesc_f16(kRowsX, kPos), kk + part > 0);
         umma_commit(&bar.s_full[xx]);
       };
-      auto issue_o = [&](int it, int xx) {
+      auto issue_o = [&](int it, int xx, int h) {
         const unsigned va = smem_addr(values_of(it));
         tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < kPos / 16; ++kk)
+        for (int k2 = 0; k2 < kPos / 32; ++k2) {
+          const int kk = h * (kPos / 32) + k2;
 #pragma unroll
           for (int part = 0; part < G::parts; ++part)
             umma_f16_ts(tmem + G::o_at + xx * D, tmem + G::s_at + xx * kPos + (kk >> 1) * 32 + part * 16 + (kk & 1) * 8,
-                        smem_desc_mn(va + kk * 2 * (D / 8) * 128, D / 8 * 128), idesc_f16_bt(kRowsX, D), it > 0 || kk + part > 0);
-        umma_commit(&bar.p_free[xx]);
+                        smem_desc_mn(va + kk * 2 * (D / 8) * 128, D / 8 * 128), idesc_f16_bt(kRowsX, D), it + h > 0 || k2 + part > 0);
+        }
+        umma_commit(&bar.p_free[xx][h]);
       };
       if (tiles > 0) {
         ok = mbar_wait_bounded(&bar.k_full[0], 0, kPromptTimeout);
@@ -435,13 +440,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       for (int it = 0; it < tiles && ok; ++it) {
         ok = mbar_wait_bounded(&bar.v_full[it % G::stages], turn_of(it), kPromptTimeout);
         for (int xx = 0; xx < row_tiles && ok; ++xx) {
-          ok = mbar_wait_bounded(&bar.p_full[xx], it & 1, kPromptTimeout);
+          for (int h = 0; h < 2 && ok; ++h) {
+            ok = mbar_wait_bounded(&bar.p_full[xx][h], it & 1, kPromptTimeout);
+            if (ok) issue_o(it, xx, h);
+          }
           if (!ok) break;
-          issue_o(it, xx);
           if (xx == row_tiles - 1) umma_commit(&bar.v_free[it % G::stages]);
           if (it + 1 < tiles) {
             ok = (xx > 0 || mbar_wait_bounded(&bar.k_full[(it + 1) % G::stages], turn_of(it + 1), kPromptTimeout)) &&
-                 mbar_wait_bounded(&bar.p_free[xx], it & 1, kPromptTimeout);  // S takes the place of P
+                 mbar_wait_bounded(&bar.p_free[xx][1], it & 1, kPromptTimeout);  // S takes the place of P
             if (!ok) break;
             issue_s(it + 1, xx);
             if (xx == row_tiles - 1) umma_commit(&bar.k_free[(it + 1) % G::stages]);
@@ -478,87 +485,97 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         for (int c = 0; c < kPos; c += 32) tmem_fill32(ts + c, 0u);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&bar.p_full[x]);
+        mbar_arrive(&bar.p_full[x][0]);
+        mbar_arrive(&bar.p_full[x][1]);
         continue;
       }
       const bool whole = __all_sync(0xFFFFFFFFu, all || !mine);
-      float xs[kPos];
-#pragma unroll
-      for (int c = 0; c < kPos; c += 32) {
-        uint32_t s[32];
-        tmem_ld32(ts + c, s);
-        const float4* t4 = reinterpret_cast<const float4*>(terms + 6 * c);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float4 k = t4[3 * i];
-          const float2 e = *reinterpret_cast<const float2*>(&t4[3 * i + 1]);
-          const float2 v = unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), pair(k.x, k.y),
-                                       fma2(q2, pair(k.z, k.w), pair(e.x, e.y))));
-          xs[c + 2 * i] = v.x;
-          xs[c + 2 * i + 1] = v.y;
-        }
-      }
-      if (!whole) {
-#pragma unroll
-        for (int j = 0; j < kPos; ++j) {
-          const int p = p0 + j;
-          if (!(p <= at && (A.window <= 0 || p > at - A.window || p < A.sinks))) xs[j] = -INFINITY;
-        }
-      }
-      float m[4] = {xs[0], xs[1], xs[2], xs[3]};
-#pragma unroll
-      for (int j = 4; j < kPos; j += 8) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m[i] = fmaxf(m[i], fmaxf(xs[j + i], j + 4 + i < kPos ? xs[j + 4 + i] : xs[j + i]));
-      }
-      const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-      if (__any_sync(0xFFFFFFFFu, top > ref + kRaise)) {  // the first seen position too: ref is -inf
-        const float next = fmaxf(ref, top);
-        const float corr = next > ref ? ex2(ref - next) : 1.0f;
-        ref = next;
-        sum2 = mul2(sum2, pair(corr, corr));
-        off2 = mul2(off2, pair(corr, corr));
-        if (it > 0) {
+      // 64 positions at a time, whose product is issued while the next are computed
 #pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            uint32_t o[32];
-            tmem_ld32(to + c0, o);
+      for (int h = 0; h < 2; ++h) {
+        const unsigned th = ts + h * (kPos / 2);
+        const float4* const t4 = reinterpret_cast<const float4*>(terms) + h * (kPos / 4 * 3);
+        float xs[kPos / 2];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-            tmem_st32(to + c0, o);
+        for (int c = 0; c < kPos / 2; c += 32) {
+          uint32_t s[32];
+          tmem_ld32(th + c, s);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float4 k = t4[3 * (c / 2 + i)];
+            const float2 e = *reinterpret_cast<const float2*>(&t4[3 * (c / 2 + i) + 1]);
+            const float2 v = unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), pair(k.x, k.y),
+                                         fma2(q2, pair(k.z, k.w), pair(e.x, e.y))));
+            xs[c + 2 * i] = v.x;
+            xs[c + 2 * i + 1] = v.y;
           }
         }
-      }
-      const float from = ref == -INFINITY ? 0.0f : -ref;  // a row that has seen nothing yet: its weights are 2^-inf
-      const f32x2 minus = pair(from, from);
+        if (!whole) {
 #pragma unroll
-      for (int c = 0; c < kPos; c += 32) {
-        uint32_t hi[16], lo[16];
-        const float4* t4 = reinterpret_cast<const float4*>(terms + 6 * c);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 mu = reinterpret_cast<const float2*>(t4)[6 * i + 3];
-          const float4 uo = t4[3 * i + 2];
-          const float2 d = unpair(add2(pair(xs[c + 2 * i], xs[c + 2 * i + 1]), minus));
-          const f32x2 pw = pair(ex2(d.x), ex2(d.y));
-          sum2 = fma2(pw, pair(uo.x, uo.y), sum2);
-          off2 = fma2(pw, pair(uo.z, uo.w), off2);
-          const float2 w = unpair(mul2(pw, pair(mu.x, mu.y)));
-          hi[i] = pack_f16(w.x, w.y);
-          if constexpr (kSplit) {
-            const float2 h = unpack_f16(hi[i]);
-            lo[i] = pack_f16(w.x - h.x, w.y - h.y);
+          for (int j = 0; j < kPos / 2; ++j) {
+            const int p = p0 + h * (kPos / 2) + j;
+            if (!(p <= at && (A.window <= 0 || p > at - A.window || p < A.sinks))) xs[j] = -INFINITY;
           }
         }
-        tmem_st16(ts + c, hi);
-        if constexpr (kSplit) tmem_st16(ts + c + 16, lo);
+        float m[4] = {xs[0], xs[1], xs[2], xs[3]};
+#pragma unroll
+        for (int j = 4; j < kPos / 2; ++j) m[j & 3] = fmaxf(m[j & 3], xs[j]);
+        const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        if (__any_sync(0xFFFFFFFFu, top > ref + kRaise)) {  // the first seen position too: ref is -inf
+          const float next = fmaxf(ref, top);
+          const float corr = next > ref ? ex2(ref - next) : 1.0f;
+          ref = next;
+          sum2 = mul2(sum2, pair(corr, corr));
+          off2 = mul2(off2, pair(corr, corr));
+          if (h == 1) {  // the product of the first 64 positions is under way
+            ok = mbar_wait_bounded(&bar.p_free[x][0], it & 1, kPromptTimeout);
+            tc_fence_after();
+          }
+          if (it + h > 0) {
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+              uint32_t o[32];
+              tmem_ld32(to + c0, o);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+              tmem_st32(to + c0, o);
+            }
+          }
+        }
+        const float from = ref == -INFINITY ? 0.0f : -ref;  // a row that has seen nothing yet: its weights are 2^-inf
+        const f32x2 minus = pair(from, from);
+#pragma unroll
+        for (int c = 0; c < kPos / 2; c += 32) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 mu = reinterpret_cast<const float2*>(t4)[6 * (c / 2 + i) + 3];
+            const float4 uo = t4[3 * (c / 2 + i) + 2];
+            const float2 d = unpair(add2(pair(xs[c + 2 * i], xs[c + 2 * i + 1]), minus));
+            const f32x2 pw = pair(ex2(d.x), ex2(d.y));
+            sum2 = fma2(pw, pair(uo.x, uo.y), sum2);
+            off2 = fma2(pw, pair(uo.z, uo.w), off2);
+            const float2 w = unpair(mul2(pw, pair(mu.x, mu.y)));
+            hi[i] = pack_f16(w.x, w.y);
+            if constexpr (kSplit) {
+              const float2 g = unpack_f16(hi[i]);
+              lo[i] = pack_f16(w.x - g.x, w.y - g.y);
+            }
+          }
+          tmem_st16(th + c, hi);
+          if constexpr (kSplit) tmem_st16(th + c + 16, lo);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bar.p_full[x][h]);
       }
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&bar.p_full[x]);
+      if (!__all_sync(0xFFFFFFFFu, ok)) {
+        ok = false;
+        break;
+      }
     }
     if (tiles > 0 && ok) {
-      ok = mbar_wait_bounded(&bar.p_free[x], (tiles - 1) & 1, kPromptTimeout);
+      ok = mbar_wait_bounded(&bar.p_free[x][1], (tiles - 1) & 1, kPromptTimeout);
       ok = __all_sync(0xFFFFFFFFu, ok);
     }
     tc_fence_after();
