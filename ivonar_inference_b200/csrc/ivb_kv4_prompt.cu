@@ -10,7 +10,9 @@
 //     reference raised only when the maximum passes it by 2^8, and O_X rescaled in tensor memory then. The weights P_X take
 //     S_X's place as the fp16 A operand, so S_X(it + 1) follows P_X(it)'s product; while one X waits for it the other computes.
 // fp32 queries and weights are hi + lo fp16 pairs: two products each. 128 positions because a product from shared memory takes
-// 70 cycles for 64 columns as for 128 (measured). What bounds it is the softmax's issue slots, then the tensor pipe (D = 128).
+// 70 cycles for 64 columns as for 128 (measured). With few CTAs a cluster of C shares the rows: each takes every C-th tile, and
+// they join what they found through one another's shared memory. What bounds it is the softmax's issue slots, then the tensor pipe (D = 128).
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -22,6 +24,8 @@
 
 namespace ivb {
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr int kRowsX = 128, kRowsCta = 256, kPos = 128;
 // 12 warps: with three on each of the SM's four parts a thread has 168 registers, enough to keep the loads of its 64 scores' terms ahead
@@ -88,6 +92,17 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   f32x2 r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void values_of_chunk(uint4 w, float (&v)[16 / sizeof(T)]) {
+  union {
+    uint4 w;
+    T t[16 / sizeof(T)];
+  } u;
+  u.w = w;
+#pragma unroll
+  for (int j = 0; j < static_cast<int>(16 / sizeof(T)); ++j) v[j] = to_f32<T>(u.t[j]);
 }
 
 struct PromptBarriers {
@@ -178,13 +193,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ PromptBarriers bar;
   __shared__ unsigned tmem_base;
-  __shared__ float largest[kSoftmaxThreads / 32];
+  __shared__ float largest[kSoftmaxThreads / 32], sums[kRowsCta];
   __shared__ int which[3];  // sequence, tile of its rows; and whether a wait ran out
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // which rows: the call's tiles of 256 items in the order of the sequences, the last ones (the longest rows) first
-  const int kvh = blockIdx.x % A.cache.kv_heads;
-  const int order = static_cast<int>(gridDim.x) / A.cache.kv_heads - 1 - blockIdx.x / A.cache.kv_heads;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int unit = static_cast<int>(blockIdx.x) / C, units = static_cast<int>(gridDim.x) / C;
+  const int kvh = unit % A.cache.kv_heads, order = units / A.cache.kv_heads - 1 - unit / A.cache.kv_heads;
   if (warp == 0) {
     int seen = 0, found = -1, tile = 0;
     for (int b0 = 0; b0 < A.cache.batch && found < 0; b0 += 32) {
@@ -254,40 +271,84 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };
   auto clamp_position = [&](int64_t p) { return static_cast<int>(max(static_cast<int64_t>(-1), min(p, static_cast<int64_t>(max_len)))); };
   const int first = clamp_position(base + token_of(i0)), last = clamp_position(base + token_of(i0 + live - 1));
-  if (last >= max_len && tid == 0 && A.error != nullptr) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
+  if (last >= max_len && tid == 0 && rank == 0 && A.error != nullptr) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
   // the tiles of 128 positions that some row sees: the sinks' below the window, then the window's
   const int high = min(last, max_len - 1);
   const int low = A.window > 0 ? max(0, max(first, 0) - A.window + 1) : 0;
   const int window_tile = low / kPos;
   const int sink_tiles = A.window > 0 ? min((min(A.sinks, low) + kPos - 1) / kPos, window_tile) : 0;
-  const int tiles = high < 0 ? 0 : sink_tiles + high / kPos - window_tile + 1;
-  auto tile_of = [&](int it) { return it < sink_tiles ? it : window_tile + it - sink_tiles; };
+  const int all_tiles = high < 0 ? 0 : sink_tiles + high / kPos - window_tile + 1;
+  const int tiles = all_tiles > rank ? (all_tiles - rank + C - 1) / C : 0;  // this CTA's
+  auto tile_of = [&](int it) {
+    const int i = rank + it * C;
+    return i < sink_tiles ? i : window_tile + i - sink_tiles;
+  };
 
-  // queries: the largest, then hi (and lo) parts as K-major operands, scaled by a power of two that brings it to 2^13
-  const int x = warp >> 2, row = tid & 127;  // row tile and row of a softmax thread
+  // queries: a warp takes its 32 rows in 16-byte chunks, 8 rows and 4 chunks at a time (64 contiguous bytes of a row, and no bank
+  // conflicts); the largest of all rows first, then hi (and lo) parts as K-major operands, scaled by a power of two that
+  // brings it to 2^13
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T)), L = D / kPer, kQuads = L / 4;  // values of a chunk, chunks of a row
+  const int row8 = lane & 7, chunk4 = lane >> 3;
+  const int x = warp >> 2;  // row tile of a softmax thread
   const int item = i0 + tid;
   const bool mine = tid < live;
-  const T* q = nullptr;
+  auto item_row = [&](const void* array, int i, int64_t row_stride, int64_t head_stride) {
+    const int t = token_of(i), h = kvh * A.group + i - t * A.group;
+    return static_cast<const T*>(array) + (row0 + t) * row_stride + h * head_stride;
+  };
   int at = -1;
-  float sum_q = 0.0f;
+  uint4 raw[4][kQuads];
   if (tid < kSoftmaxThreads) {
-    float most = 0.0f;
     if (mine) {
-      const int t = token_of(item), h = kvh * A.group + item - t * A.group;
-      q = static_cast<const T*>(A.q) + (row0 + t) * A.q_row + h * A.q_head;
-      const int p = clamp_position(base + t);
+      const int p = clamp_position(base + token_of(item));
       at = p < max_len ? p : -1;
+    }
+    const T* q[4];
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        float v[8];
-        load_values<T, 8>(q + 8 * c, A.q_vec, v);
+    for (int g = 0; g < 4; ++g) {
+      const int r = 32 * warp + 8 * g + row8;
+      q[g] = r < live ? item_row(A.q, i0 + r, A.q_row, A.q_head) + chunk4 * kPer : nullptr;
+    }
+    if (A.q_vec) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int k = 0; k < kQuads; ++k)
+          raw[g][k] = q[g] != nullptr ? __ldg(reinterpret_cast<const uint4*>(q[g]) + 4 * k) : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int k = 0; k < kQuads; ++k) {
+          union {
+            uint4 w;
+            T t[kPer];
+          } u;
+          u.w = make_uint4(0u, 0u, 0u, 0u);
+          if (q[g] != nullptr)
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) u.t[j] = q[g][4 * k * kPer + j];
+          raw[g][k] = u.w;
+        }
+    }
+    float most = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float total = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kQuads; ++k) {
+        float v[kPer];
+        values_of_chunk<T>(raw[g][k], v);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
           const float m = fabsf(v[j]);
           if (m <= 3.402823466e38f) most = fmaxf(most, m);
-          sum_q += v[j];
+          total += v[j];
         }
       }
+      total += __shfl_xor_sync(0xFFFFFFFFu, total, 8);
+      total += __shfl_xor_sync(0xFFFFFFFFu, total, 16);
+      if (chunk4 == 0) sums[32 * warp + 8 * g + row8] = total;
     }
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
@@ -305,24 +366,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     const float unit = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
     unsigned char* dst = smem + G::q_at + x * G::parts * G::q_bytes;
 #pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-      float v[8];
+    for (int g = 0; g < 4; ++g)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-      if (mine) load_values<T, 8>(q + 8 * c, A.q_vec, v);
-      uint32_t hi[4], lo[4];
+      for (int k = 0; k < kQuads; ++k) {
+        const int r = 32 * (warp & 3) + 8 * g + row8, i = 4 * k + chunk4;
+        float v[kPer];
+        values_of_chunk<T>(raw[g][k], v);
+        uint32_t hi[kPer / 2], lo[kPer / 2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a = v[2 * j] * unit, c2 = v[2 * j + 1] * unit;
-        hi[j] = pack_f16(a, c2);
-        if constexpr (kSplit) {
+        for (int j = 0; j < kPer / 2; ++j) {
+          const float a = v[2 * j] * unit, c = v[2 * j + 1] * unit;
+          hi[j] = pack_f16(a, c);
           const float2 h = unpack_f16(hi[j]);
-          lo[j] = pack_f16(a - h.x, c2 - h.y);
+          lo[j] = pack_f16(a - h.x, c - h.y);
+        }
+        if constexpr (kSplit) {
+          unsigned char* to = dst + chunk_at<D>(r, i / 2) + 8 * (i & 1);
+          *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+          *reinterpret_cast<uint2*>(to + G::q_bytes) = make_uint2(lo[0], lo[1]);
+        } else {
+          *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, i)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         }
       }
-      *reinterpret_cast<uint4*>(dst + chunk_at<D>(row, c)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      if constexpr (kSplit) *reinterpret_cast<uint4*>(dst + G::q_bytes + chunk_at<D>(row, c)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
   }
   fence_proxy_async();  // the tensor cores read what the threads wrote
   tc_fence_before();
@@ -334,6 +399,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   auto terms_of = [&](int it) { return reinterpret_cast<float*>(smem + G::terms_at + it % kTermSets * G::term_bytes); };
   auto turn_of = [&](int it) { return static_cast<unsigned>(it / G::stages) & 1u; };  // parity of a stage's use
   bool ok = true;
+  float ref = -INFINITY, total = 0.0f, offset = 0.0f;  // of a softmax thread's row
 
   if (warp >= kSoftmaxThreads / 32 && warp < kPromptThreads / 32 - 1) {
     // ---- producers: 16-position tiles in turn ----
@@ -464,8 +530,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     // ---- softmax: one row a thread ----
     const unsigned lanes = static_cast<unsigned>(32 * (warp & 3)) << 16;
     const unsigned ts = tmem + lanes + G::s_at + x * kPos, to = tmem + lanes + G::o_at + x * D;
-    const f32x2 q2 = pair(sum_q, sum_q);
-    float ref = -INFINITY;
+    const f32x2 q2 = pair(sums[tid], sums[tid]);
     f32x2 sum2 = pair(0.0f, 0.0f), off2 = pair(0.0f, 0.0f);
     for (int it = 0; it < tiles; ++it) {
       const int p0 = tile_of(it) * kPos;
@@ -578,30 +643,112 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       ok = mbar_wait_bounded(&bar.p_free[x][1], (tiles - 1) & 1, kPromptTimeout);
       ok = __all_sync(0xFFFFFFFFu, ok);
     }
-    tc_fence_after();
-    if (ok) {
-      const float2 s = unpair(sum2), f = unpair(off2);
-      const float total = s.x + s.y, inv = total == 0.0f ? 0.0f : 1.0f / total, offset = f.x + f.y;
-      T* out = nullptr;
-      if (mine) {
-        const int t = token_of(item), h = kvh * A.group + item - t * A.group;
-        out = static_cast<T*>(A.out) + (row0 + t) * A.o_row + h * A.o_head;
-      }
-#pragma unroll
+    const float2 s = unpair(sum2), f = unpair(off2);
+    total = s.x + s.y;
+    offset = f.x + f.y;
+  }
+  const unsigned to = tmem + (static_cast<unsigned>(32 * (warp & 3)) << 16) + G::o_at + x * D;
+  const bool softmax = tid < kSoftmaxThreads && x < row_tiles;
+  if (C == 1) {
+    if (softmax && ok) {
+      // the warp's rows go through its part of its tile's queries, which nobody reads any more, and leave in whole chunks
+      tc_fence_after();
+      const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+      unsigned char* const stage = smem + G::q_at + x * G::parts * G::q_bytes + 32 * (warp & 3) * D * static_cast<int>(sizeof(T));
+      auto chunk_of = [&](int r, int c) { return reinterpret_cast<uint4*>(stage + r * D * static_cast<int>(sizeof(T)) + ((c ^ (r & (L < 8 ? L - 1 : 7))) * 16)); };
+#pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 32) {
         uint32_t o[32];
         if (tiles > 0) tmem_ld32(to + c0, o);
-        if (mine) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float y[8];
+        for (int c = 0; c < 32 / kPer; ++c) {
+          union {
+            uint4 w;
+            T t[kPer];
+          } u;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = total == 0.0f ? 0.0f : fmaf(__uint_as_float(o[8 * c + j]), 1.0f / kWeightUnit, offset) * inv;
-            store_values<T, 8>(out + c0 + 8 * c, A.o_vec, y);
+          for (int j = 0; j < kPer; ++j)
+            u.t[j] = from_f32<T>(total == 0.0f ? 0.0f : fmaf(__uint_as_float(o[kPer * c + j]), 1.0f / kWeightUnit, offset) * inv);
+          *chunk_of(lane, c0 / kPer + c) = u.w;
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int r = 8 * g + row8;
+        if (32 * warp + r < live) {
+          T* out = const_cast<T*>(item_row(A.out, i0 + 32 * warp + r, A.o_row, A.o_head)) + chunk4 * kPer;
+#pragma unroll
+          for (int k = 0; k < kQuads; ++k) {
+            union {
+              uint4 w;
+              T t[kPer];
+            } u;
+            u.w = *chunk_of(r, 4 * k + chunk4);
+            if (A.o_vec) {
+              *reinterpret_cast<uint4*>(out + 4 * k * kPer) = u.w;
+            } else {
+#pragma unroll
+              for (int j = 0; j < kPer; ++j) out[4 * k * kPer + j] = u.t[j];
+            }
           }
         }
       }
     }
+  } else {
+    // every CTA leaves its O [channel][row] and (reference, sum, offset) [row], and finishes D / C channels of all rows
+    float* const part = reinterpret_cast<float*>(smem);
+    float* const stats = part + D * kRowsCta;
+    static_assert(D * kRowsCta * 4 + kRowsCta * 12 <= G::smem, "shared memory");
+    __syncthreads();  // all products are done: the operands' place is free
+    if (softmax) {
+      tc_fence_after();
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t o[32];
+        if (tiles > 0 && ok) tmem_ld32(to + c0, o);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) part[(c0 + j) * kRowsCta + tid] = tiles > 0 ? __uint_as_float(o[j]) : 0.0f;
+      }
+      stats[tid] = ref;
+      stats[kRowsCta + tid] = total;
+      stats[2 * kRowsCta + tid] = offset;
+    }
+    cluster.sync();
+    if (softmax && mine) {
+      T* out = const_cast<T*>(item_row(A.out, item, A.o_row, A.o_head));
+      float top = -INFINITY, l = 0.0f, off = 0.0f, scale[4];
+      for (int k = 0; k < C; ++k) top = fmaxf(top, cluster.map_shared_rank(stats, k)[tid]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        scale[k] = 0.0f;
+        if (k < C) {
+          const float* other = cluster.map_shared_rank(stats, k);
+          if (other[kRowsCta + tid] != 0.0f) {  // zero: the CTA saw nothing for this row
+            scale[k] = ex2(other[tid] - top);
+            l = fmaf(other[kRowsCta + tid], scale[k], l);
+            off = fmaf(other[2 * kRowsCta + tid], scale[k], off);
+          }
+        }
+      }
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      for (int c = rank * (D / C); c < (rank + 1) * (D / C); c += 8) {
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < C && scale[k] != 0.0f) {
+            const float* other = cluster.map_shared_rank(part, k) + c * kRowsCta + tid;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = fmaf(other[j * kRowsCta], scale[k], y[j]);
+          }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = l == 0.0f ? 0.0f : fmaf(y[j], 1.0f / kWeightUnit, off) * inv;
+        store_values<T, 8>(out + c, A.o_vec, y);
+      }
+    }
+    cluster.sync();  // no CTA leaves while another reads its shared memory
   }
   if (!ok) which[2] = 1;
   tc_fence_before();
@@ -629,9 +776,24 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   const int64_t sequences = std::min<int64_t>(A.cache.batch, items / (few + 1));
   const int64_t tiles = items / kRowsCta + sequences;
   if (sequences == 0) return IVB_OK;
-  if (tiles * A.cache.kv_heads > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(tiles));
-  kv4_prompt_kernel<D, T><<<static_cast<unsigned>(tiles * A.cache.kv_heads), kPromptThreads, G::smem, stream>>>(A, few);
-  IVB_CUDA(cudaGetLastError());
+  if (tiles * A.cache.kv_heads > 0x1fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(tiles));
+  // a cluster where one CTA each would leave SMs without work
+  int C = 1;
+  while (C < 4 && tiles * A.cache.kv_heads * C < 148 && A.cache.max_len > 2 * C * kPos) C *= 2;
+  if (getenv("KV4_P")) C = atoi(getenv("KV4_P"));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * A.cache.kv_heads * C));
+  cfg.blockDim = dim3(kPromptThreads);
+  cfg.dynamicSmemBytes = G::smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<D, T>, A, few));
   return IVB_OK;
 }
 
