@@ -6,7 +6,7 @@
 //     MN-major one: both are position rows of 16-byte channel chunks, so neither is transposed) and compute each
 //     position's terms (scales and offsets; ivb_kv4_attention.cuh);
 //   warp 11 (one thread) issues S_X = Q_X U^T and O_X += P_X U'^T, fp32 in tensor memory;
-//   warps 0..7 (a thread owns one row, which is its tensor-memory lane) turn S_X into weights: online softmax in 32 bits, the
+//   warps 0..7 (32 rows each, their tensor-memory lanes) turn S_X into weights: online softmax in 32 bits, the
 //     reference raised only when the maximum passes it by 2^8, and O_X rescaled in tensor memory then. The weights P_X take
 //     S_X's place as the fp16 A operand, so S_X(it + 1) follows P_X(it)'s product; while one X waits for it the other computes.
 // fp32 queries and weights are hi + lo fp16 pairs: two products each. 128 positions because a product from shared memory takes
@@ -44,7 +44,7 @@ struct PromptGeometry {
   static constexpr int term_bytes = kPos * 24;
   static constexpr int q_at = 0, k_at = 2 * parts * q_bytes, v_at = k_at + stages * kv_bytes, terms_at = v_at + stages * kv_bytes;
   static constexpr int smem = terms_at + kTermSets * term_bytes;
-  // tensor memory columns: S_X, then P_X in its place (of every 32 columns 16 hi, 16 lo), and O_X
+  // tensor memory columns: S_X, then P_X in its place (of every 64 columns 32 hi, 32 lo), and O_X
   static constexpr int s_at = 0, o_at = 2 * kPos, columns = 512;
   static_assert(o_at + 2 * D <= columns, "tensor memory");
 };
@@ -296,13 +296,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     const int t = token_of(i), h = kvh * A.group + i - t * A.group;
     return static_cast<const T*>(array) + (row0 + t) * row_stride + h * head_stride;
   };
-  int at = -1;
   uint4 raw[4][kQuads];
   if (tid < kSoftmaxThreads) {
-    if (mine) {
-      const int p = clamp_position(base + token_of(item));
-      at = p < max_len ? p : -1;
-    }
     const T* q[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -399,7 +394,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   auto terms_of = [&](int it) { return reinterpret_cast<float*>(smem + G::terms_at + it % kTermSets * G::term_bytes); };
   auto turn_of = [&](int it) { return static_cast<unsigned>(it / G::stages) & 1u; };  // parity of a stage's use
   bool ok = true;
-  float ref = -INFINITY, total = 0.0f, offset = 0.0f;  // of a softmax thread's row
+  float ref = -INFINITY, total = 0.0f, offset = 0.0f;  // in the end, of the row that is a softmax thread's lane
 
   if (warp >= kSoftmaxThreads / 32 && warp < kPromptThreads / 32 - 1) {
     // ---- producers: 16-position tiles in turn ----
@@ -491,7 +486,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           const int kk = h * (kPos / 32) + k2;
 #pragma unroll
           for (int part = 0; part < G::parts; ++part)
-            umma_f16_ts(tmem + G::o_at + xx * D, tmem + G::s_at + xx * kPos + (kk >> 1) * 32 + part * 16 + (kk & 1) * 8,
+            umma_f16_ts(tmem + G::o_at + xx * D, tmem + G::s_at + xx * kPos + h * (kPos / 2) + part * (kPos / 4) + k2 * 8,
                         smem_desc_mn(va + kk * 2 * (D / 8) * 128, D / 8 * 128), idesc_f16_bt(kRowsX, D), it + h > 0 || k2 + part > 0);
         }
         umma_commit(&bar.p_free[xx][h]);
@@ -527,11 +522,38 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       }
     }
   } else if (x < row_tiles) {
-    // ---- softmax: one row a thread ----
+    // ---- softmax: a warp has 32 rows, a thread in each 8-row set the row r and every fourth pair of positions, so that a
+    // position's terms are loaded once for four rows (loaded for each row they bound the kernel: 12 cycles of the SM's
+    // shared memory pipe for 64 scores)
     const unsigned lanes = static_cast<unsigned>(32 * (warp & 3)) << 16;
     const unsigned ts = tmem + lanes + G::s_at + x * kPos, to = tmem + lanes + G::o_at + x * D;
-    const f32x2 q2 = pair(sums[tid], sums[tid]);
-    f32x2 sum2 = pair(0.0f, 0.0f), off2 = pair(0.0f, 0.0f);
+    const int r = lane >> 2, c = lane & 3;
+    float sum_q[4], refs[4];
+    int at[4];
+    f32x2 sum2[4], off2[4];
+    bool live_rows = false;
+    int first_at = 0x7fffffff, last_at = -1;  // of the warp's rows
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = 32 * warp + 8 * i + r;
+      sum_q[i] = sums[n];
+      at[i] = -1;
+      if (n < live) {
+        const int p = clamp_position(base + token_of(i0 + n));
+        at[i] = p < max_len ? p : -1;
+        live_rows = true;
+        first_at = min(first_at, at[i]);
+        last_at = max(last_at, at[i]);
+      }
+      refs[i] = -INFINITY;
+      sum2[i] = off2[i] = pair(0.0f, 0.0f);
+    }
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) {
+      first_at = min(first_at, __shfl_xor_sync(0xFFFFFFFFu, first_at, d));
+      last_at = max(last_at, __shfl_xor_sync(0xFFFFFFFFu, last_at, d));
+    }
+    live_rows = __any_sync(0xFFFFFFFFu, live_rows);
     for (int it = 0; it < tiles; ++it) {
       const int p0 = tile_of(it) * kPos;
       const float* terms = terms_of(it);
@@ -543,92 +565,124 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         break;
       }
       tc_fence_after();
-      const bool all = at >= p0 + kPos - 1 && (A.window <= 0 || p0 > at - A.window || p0 <= A.sinks - kPos);
-      const bool none = at < p0 || (A.window > 0 && p0 + kPos - 1 <= at - A.window && p0 >= A.sinks);
-      if (__all_sync(0xFFFFFFFFu, none || !mine)) {  // nothing of the tile for this warp's rows
+      // what the warp's rows see of the tile: all of it, or nothing (first_at, last_at: the lowest and highest, -1 among them)
+      const bool whole = live_rows && first_at >= p0 + kPos - 1 && (A.window <= 0 || p0 > last_at - A.window || p0 <= A.sinks - kPos);
+      const bool none = last_at < p0 || (A.window > 0 && p0 + kPos - 1 <= first_at - A.window && p0 >= A.sinks);
+      if (none) {
 #pragma unroll
-        for (int c = 0; c < kPos; c += 32) tmem_fill32(ts + c, 0u);
+        for (int i = 0; i < kPos; i += 32) tmem_fill32(ts + i, 0u);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bar.p_full[x][0]);
         mbar_arrive(&bar.p_full[x][1]);
         continue;
       }
-      const bool whole = __all_sync(0xFFFFFFFFu, all || !mine);
       // 64 positions at a time, whose product is issued while the next are computed
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
         const unsigned th = ts + h * (kPos / 2);
-        const float4* const t4 = reinterpret_cast<const float4*>(terms) + h * (kPos / 4 * 3);
-        float xs[kPos / 2];
+        const float4* const t4 = reinterpret_cast<const float4*>(terms) + 3 * (32 * h + c);  // of the pair c; every fourth is ours
+        uint32_t s[2][32];  // [16 rows][4 pair + 2 (8 rows) + position], scores in place
 #pragma unroll
-        for (int c = 0; c < kPos / 2; c += 32) {
-          uint32_t s[32];
-          tmem_ld32(th + c, s);
+        for (int g = 0; g < 2; ++g) tmem_ld_16x256b_x8(th + (static_cast<unsigned>(16 * g) << 16), s[g]);
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float4 k = t4[3 * (c / 2 + i)];
-            const float2 e = *reinterpret_cast<const float2*>(&t4[3 * (c / 2 + i) + 1]);
-            const float2 v = unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), pair(k.x, k.y),
-                                         fma2(q2, pair(k.z, k.w), pair(e.x, e.y))));
-            xs[c + 2 * i] = v.x;
-            xs[c + 2 * i + 1] = v.y;
+        for (int i = 0; i < 8; ++i) {
+          const float4 k = t4[12 * i];
+          const float2 e = *reinterpret_cast<const float2*>(&t4[12 * i + 1]);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            uint32_t(&v)[32] = s[n >> 1];
+            const int j = 4 * i + 2 * (n & 1);
+            const float2 y = unpair(fma2(pair(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), pair(k.x, k.y),
+                                   fma2(pair(sum_q[n], sum_q[n]), pair(k.z, k.w), pair(e.x, e.y))));
+            v[j] = __float_as_uint(y.x);
+            v[j + 1] = __float_as_uint(y.y);
           }
         }
         if (!whole) {
 #pragma unroll
-          for (int j = 0; j < kPos / 2; ++j) {
-            const int p = p0 + h * (kPos / 2) + j;
-            if (!(p <= at && (A.window <= 0 || p > at - A.window || p < A.sinks))) xs[j] = -INFINITY;
+          for (int n = 0; n < 4; ++n) {
+            const int from = A.window > 0 ? at[n] - A.window : -1;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int p = p0 + h * (kPos / 2) + 8 * i + 2 * c + e;
+                if (p > at[n] || (p <= from && p >= A.sinks)) s[n >> 1][4 * i + 2 * (n & 1) + e] = 0xff800000u;
+              }
           }
         }
-        float m[4] = {xs[0], xs[1], xs[2], xs[3]};
 #pragma unroll
-        for (int j = 4; j < kPos / 2; ++j) m[j & 3] = fmaxf(m[j & 3], xs[j]);
-        const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-        if (__any_sync(0xFFFFFFFFu, top > ref + kRaise)) {  // the first seen position too: ref is -inf
-          const float next = fmaxf(ref, top);
-          const float corr = next > ref ? ex2(ref - next) : 1.0f;
-          ref = next;
-          sum2 = mul2(sum2, pair(corr, corr));
-          off2 = mul2(off2, pair(corr, corr));
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int j = 4 * i + 2 * (n & 1);
+            top[n] = fmaxf(top[n], fmaxf(__uint_as_float(s[n >> 1][j]), __uint_as_float(s[n >> 1][j + 1])));
+          }
+        bool raise = false;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          top[n] = fmaxf(top[n], __shfl_xor_sync(0xFFFFFFFFu, top[n], 1));
+          top[n] = fmaxf(top[n], __shfl_xor_sync(0xFFFFFFFFu, top[n], 2));
+          raise |= top[n] > refs[n] + kRaise;  // the first seen position too: the reference is -inf
+        }
+        if (__any_sync(0xFFFFFFFFu, raise)) {
+          float factor = 1.0f;  // of the row that is this thread's lane
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float next = fmaxf(refs[n], top[n]);
+            const float corr = next > refs[n] ? ex2(refs[n] - next) : 1.0f;
+            refs[n] = next;
+            sum2[n] = mul2(sum2[n], pair(corr, corr));
+            off2[n] = mul2(off2[n], pair(corr, corr));
+            const float theirs = __shfl_sync(0xFFFFFFFFu, corr, 4 * (lane & 7));
+            if (lane >> 3 == n) factor = theirs;
+          }
           if (h == 1) {  // the product of the first 64 positions is under way
             ok = mbar_wait_bounded(&bar.p_free[x][0], it & 1, kPromptTimeout);
             tc_fence_after();
           }
           if (it + h > 0) {
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-              uint32_t o[32];
-              tmem_ld32(to + c0, o);
+            for (int c0 = 0; c0 < D; c0 += 16) {
+              uint32_t o[16];
+              tmem_ld16(to + c0, o);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-              tmem_st32(to + c0, o);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
+              tmem_st16(to + c0, o);
             }
           }
         }
-        const float from = ref == -INFINITY ? 0.0f : -ref;  // a row that has seen nothing yet: its weights are 2^-inf
-        const f32x2 minus = pair(from, from);
+        f32x2 minus[4];  // a row that has seen nothing yet: its weights are 2^-inf
 #pragma unroll
-        for (int c = 0; c < kPos / 2; c += 32) {
-          uint32_t hi[16], lo[16];
+        for (int n = 0; n < 4; ++n) minus[n] = refs[n] == -INFINITY ? pair(0.0f, 0.0f) : pair(-refs[n], -refs[n]);
+        uint32_t hi[2][16], lo[2][16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 mu = reinterpret_cast<const float2*>(t4)[6 * (c / 2 + i) + 3];
-            const float4 uo = t4[3 * (c / 2 + i) + 2];
-            const float2 d = unpair(add2(pair(xs[c + 2 * i], xs[c + 2 * i + 1]), minus));
+        for (int i = 0; i < 8; ++i) {
+          const float2 mu = reinterpret_cast<const float2*>(t4)[24 * i + 3];
+          const float4 uo = t4[12 * i + 2];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const uint32_t(&v)[32] = s[n >> 1];
+            const int j = 4 * i + 2 * (n & 1);
+            const float2 d = unpair(add2(pair(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), minus[n]));
             const f32x2 pw = pair(ex2(d.x), ex2(d.y));
-            sum2 = fma2(pw, pair(uo.x, uo.y), sum2);
-            off2 = fma2(pw, pair(uo.z, uo.w), off2);
+            sum2[n] = fma2(pw, pair(uo.x, uo.y), sum2[n]);
+            off2[n] = fma2(pw, pair(uo.z, uo.w), off2[n]);
             const float2 w = unpair(mul2(pw, pair(mu.x, mu.y)));
-            hi[i] = pack_f16(w.x, w.y);
+            uint32_t& out = hi[n >> 1][2 * i + (n & 1)];
+            out = pack_f16(w.x, w.y);
             if constexpr (kSplit) {
-              const float2 g = unpack_f16(hi[i]);
-              lo[i] = pack_f16(w.x - g.x, w.y - g.y);
+              const float2 f = unpack_f16(out);
+              lo[n >> 1][2 * i + (n & 1)] = pack_f16(w.x - f.x, w.y - f.y);
             }
           }
-          tmem_st16(th + c, hi);
-          if constexpr (kSplit) tmem_st16(th + c + 16, lo);
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          tmem_st_16x128b_x8(th + (static_cast<unsigned>(16 * g) << 16), hi[g]);
+          if constexpr (kSplit) tmem_st_16x128b_x8(th + kPos / 4 + (static_cast<unsigned>(16 * g) << 16), lo[g]);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -643,9 +697,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       ok = mbar_wait_bounded(&bar.p_free[x][1], (tiles - 1) & 1, kPromptTimeout);
       ok = __all_sync(0xFFFFFFFFu, ok);
     }
-    const float2 s = unpair(sum2), f = unpair(off2);
-    total = s.x + s.y;
-    offset = f.x + f.y;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {  // a row's sums meet, and go to the thread that is its lane
+      const float2 s = unpair(sum2[n]), f = unpair(off2[n]);
+      float l = s.x + s.y, o = f.x + f.y;
+      l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+      l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+      o += __shfl_xor_sync(0xFFFFFFFFu, o, 1);
+      o += __shfl_xor_sync(0xFFFFFFFFu, o, 2);
+      const float lane_l = __shfl_sync(0xFFFFFFFFu, l, 4 * (lane & 7)), lane_o = __shfl_sync(0xFFFFFFFFu, o, 4 * (lane & 7));
+      const float lane_ref = __shfl_sync(0xFFFFFFFFu, refs[n], 4 * (lane & 7));
+      if (lane >> 3 == n) {
+        total = lane_l;
+        offset = lane_o;
+        ref = lane_ref;
+      }
+    }
   }
   const unsigned to = tmem + (static_cast<unsigned>(32 * (warp & 3)) << 16) + G::o_at + x * D;
   const bool softmax = tid < kSoftmaxThreads && x < row_tiles;
