@@ -12,7 +12,7 @@
 namespace ivb {
 namespace {
 
-constexpr int kKv4Threads = 256;  // 8 warps, one row of one head each
+constexpr int kKv4Threads = 256;  // 8 warps, a row of one or four heads each
 
 // The code of x by the real quotient (x - m) / s. The 32-bit product with the reciprocal is within 2^-18 of it; where that
 // could change the rounding (2e-4 of all values) the quotient is taken in 64 bits.
@@ -23,109 +23,131 @@ __device__ __forceinline__ int kv4_code(float x, float m, float s, float rs) {
   return static_cast<int>(fminf(fmaxf(u, 0.0f), 15.0f));
 }
 
-// One warp per (row, head): lanes 0..15 the key row, lanes 16..31 the value row, D / 16 channels each.
-template <int D, typename T>
+// fp16 of the real quotient d / 15, rounded to 32 bits and then to 16, with d = hi - m. The 32-bit product is within 2^-22 of it;
+// where that could change the rounding to 16 bits (1 of 250 rows, and scales below fp16's normal range) it is taken in 64.
+__device__ __forceinline__ __half kv4_scale(float hi, float m) {
+  float wide = (hi - m) * (1.0f / 15.0f);
+  const int to_border = static_cast<int>(__float_as_uint(wide) & 0x1fffu) - 0x1000;
+  if (!(wide >= 6.2e-5f) || abs(to_border) < 16) wide = static_cast<float>((static_cast<double>(hi) - static_cast<double>(m)) / 15.0);
+  return __float2half_rn(fminf(fmaxf(wide, 0.0f), 65504.0f));
+}
+
+// The row's sequence and position; false where there is nothing to do.
+__device__ __forceinline__ bool kv4_place(const IvbKv4Cache& C, const int32_t* starts, const int64_t* positions, int row, uint32_t* error,
+                                          int& b, int64_t& pos) {
+  b = kv4_sequence(starts, C.batch, row);
+  if (b >= C.batch) return false;
+  pos = __ldg(positions + b) + (starts == nullptr ? 0 : row - __ldg(starts + b));
+  if (pos >= C.max_len && (threadIdx.x & 31) == 0 && error != nullptr) atomicCAS(error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
+  return pos >= 0 && pos < C.max_len;
+}
+
+// One warp per row and kHeads heads: lanes 0..15 the key rows, lanes 16..31 the value rows, D / 16 channels each. Four heads a
+// warp share the look-up of the row and keep their loads in flight together; one is for calls too small to fill the GPU with
+// the others (2048 rows of 32 heads x 128 in bf16: 17 us with four, 24 with one; 256 rows of 16 x 64: 4.4 and 3.6 us).
+template <int D, typename T, int kHeads>
 __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(IvbKv4Cache C, const T* k, const T* v, int64_t k_row, int64_t k_head,
                                                                  int64_t v_row, int64_t v_head, const int32_t* starts,
                                                                  const int64_t* positions, int rows, bool vec, uint32_t* error) {
   constexpr int n = D / 16;
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kKv4Threads + threadIdx.x) >> 5;
-  if (item >= static_cast<int64_t>(rows) * C.kv_heads) return;
+  const int row = blockIdx.x * (kKv4Threads / 32) + (threadIdx.x >> 5), h0 = blockIdx.y * kHeads;
+  if (row >= rows) return;
   const int lane = threadIdx.x & 31, l = lane & 15;
-  const int row = static_cast<int>(item / C.kv_heads), h = static_cast<int>(item - static_cast<int64_t>(row) * C.kv_heads);
-  const int b = kv4_sequence(starts, C.batch, row);
-  if (b >= C.batch) return;
-  const int64_t pos = __ldg(positions + b) + (starts == nullptr ? 0 : row - __ldg(starts + b));
-  if (pos < 0) return;
-  if (pos >= C.max_len) {
-    if (lane == 0 && error != nullptr) atomicCAS(error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
-    return;
-  }
   const bool value = lane >= 16;
-  const T* src = value ? v + row * v_row + h * v_head : k + row * k_row + h * k_head;
-  float x[n];
-  load_values<T, n>(src + l * n, vec, x);
-  float lo = x[0], hi = x[0];
-  bool finite = fabsf(x[0]) <= 3.402823466e38f;
+  const T* src = (value ? v + row * v_row + h0 * v_head : k + row * k_row + h0 * k_head) + l * n;
+  float x[kHeads][n];
 #pragma unroll
-  for (int i = 1; i < n; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    finite = finite && fabsf(x[i]) <= 3.402823466e38f;
-  }
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, d));
-    hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, d));
-  }
-  const unsigned all = __ballot_sync(0xFFFFFFFFu, finite);
-  const bool row_finite = (value ? all >> 16 : all & 0xFFFFu) == 0xFFFFu;
-  const __half mh = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
-  const float m = __half2float(mh);
-  // to 32 bits first, then to 16
-  const float wide = static_cast<float>((static_cast<double>(hi) - static_cast<double>(m)) / 15.0);
-  const __half sh = __float2half_rn(fminf(fmaxf(wide, 0.0f), 65504.0f));
-  const float s = __half2float(sh);
-  const float rs = s > 0.0f ? 1.0f / s : 0.0f;
-  uint32_t word = 0;
-  if (s > 0.0f && row_finite) {
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const int ch = (l * n + i) & 7;
-      word |= static_cast<uint32_t>(kv4_code(x[i], m, s, rs)) << (4 * (ch >> 1) + 16 * (ch & 1));
-    }
-  }
-  // the D / 16 lanes' parts of each word meet in the first of them
-#pragma unroll
-  for (int d = 1; d < 8 / n; d <<= 1) word |= __shfl_xor_sync(0xFFFFFFFFu, word, d);
-  const int64_t tile = (static_cast<int64_t>(b) * C.kv_heads + h) * kv4_tiles(C.max_len) + (pos >> 4);
+  for (int h = 0; h < kHeads; ++h)
+    if (h0 + h < C.kv_heads) load_values<T, n>(src + h * (value ? v_head : k_head), vec, x[h]);
+  int b;
+  int64_t pos;
+  if (!kv4_place(C, starts, positions, row, error, b, pos)) return;
   const int p = static_cast<int>(pos & 15);
-  uint32_t* words = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(C.data) + tile * kv4_tile_bytes(D));
-  if (l % (8 / n) == 0) {
-    const int i = l / (8 / n);
-    words[value ? kv4_value_word<D>(p, i) : kv4_key_word<D>(p, i)] = word;
-  }
-  if (l == 0) {
-    // a row that holds an infinity or a NaN reads back as NaN
-    const uint32_t par = row_finite ? static_cast<uint32_t>(__half_as_ushort(sh)) | static_cast<uint32_t>(__half_as_ushort(mh)) << 16
-                                    : 0x7fff7fffu;
-    words[4 * D + 2 * p + (value ? 1 : 0)] = par;
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (h0 + h >= C.kv_heads) break;
+    float lo = x[h][0], hi = x[h][0];
+    bool finite = fabsf(x[h][0]) <= 3.402823466e38f;
+#pragma unroll
+    for (int i = 1; i < n; ++i) {
+      lo = fminf(lo, x[h][i]);
+      hi = fmaxf(hi, x[h][i]);
+      finite = finite && fabsf(x[h][i]) <= 3.402823466e38f;
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, d));
+      hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, d));
+    }
+    const unsigned all = __ballot_sync(0xFFFFFFFFu, finite);
+    const bool row_finite = (value ? all >> 16 : all & 0xFFFFu) == 0xFFFFu;
+    const __half mh = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
+    const float m = __half2float(mh);
+    const __half sh = kv4_scale(hi, m);
+    const float s = __half2float(sh);
+    const float rs = s > 0.0f ? 1.0f / s : 0.0f;
+    uint32_t word = 0;
+    if (s > 0.0f && row_finite) {
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const int ch = (l * n + i) & 7;
+        word |= static_cast<uint32_t>(kv4_code(x[h][i], m, s, rs)) << (4 * (ch >> 1) + 16 * (ch & 1));
+      }
+    }
+    // the D / 16 lanes' parts of each word meet in the first of them
+#pragma unroll
+    for (int d = 1; d < 8 / n; d <<= 1) word |= __shfl_xor_sync(0xFFFFFFFFu, word, d);
+    const int64_t tile = (static_cast<int64_t>(b) * C.kv_heads + h0 + h) * kv4_tiles(C.max_len) + (pos >> 4);
+    uint32_t* words = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(C.data) + tile * kv4_tile_bytes(D));
+    if (l % (8 / n) == 0) {
+      const int i = l / (8 / n);
+      words[value ? kv4_value_word<D>(p, i) : kv4_key_word<D>(p, i)] = word;
+    }
+    if (l == 0) {
+      // a row that holds an infinity or a NaN reads back as NaN
+      const uint32_t par = row_finite ? static_cast<uint32_t>(__half_as_ushort(sh)) | static_cast<uint32_t>(__half_as_ushort(mh)) << 16
+                                      : 0x7fff7fffu;
+      words[4 * D + 2 * p + (value ? 1 : 0)] = par;
+    }
   }
 }
 
-template <int D, typename T>
+template <int D, typename T, int kHeads>
 __global__ void __launch_bounds__(kKv4Threads) kv4_read_kernel(IvbKv4Cache C, T* k, T* v, int64_t k_row, int64_t k_head, int64_t v_row,
                                                                int64_t v_head, const int32_t* starts, const int64_t* positions, int rows,
                                                                bool vec, uint32_t* error) {
   constexpr int n = D / 16;
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kKv4Threads + threadIdx.x) >> 5;
-  if (item >= static_cast<int64_t>(rows) * C.kv_heads) return;
+  const int row = blockIdx.x * (kKv4Threads / 32) + (threadIdx.x >> 5), h0 = blockIdx.y * kHeads;
+  if (row >= rows) return;
   const int lane = threadIdx.x & 31, l = lane & 15;
-  const int row = static_cast<int>(item / C.kv_heads), h = static_cast<int>(item - static_cast<int64_t>(row) * C.kv_heads);
-  const int b = kv4_sequence(starts, C.batch, row);
-  if (b >= C.batch) return;
-  const int64_t pos = __ldg(positions + b) + (starts == nullptr ? 0 : row - __ldg(starts + b));
-  if (pos < 0) return;
-  if (pos >= C.max_len) {
-    if (lane == 0 && error != nullptr) atomicCAS(error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
-    return;
-  }
+  int b;
+  int64_t pos;
+  if (!kv4_place(C, starts, positions, row, error, b, pos)) return;
   const bool value = lane >= 16;
-  const int64_t tile = (static_cast<int64_t>(b) * C.kv_heads + h) * kv4_tiles(C.max_len) + (pos >> 4);
-  const int p = static_cast<int>(pos & 15);
-  const uint32_t* words = reinterpret_cast<const uint32_t*>(static_cast<const unsigned char*>(C.data) + tile * kv4_tile_bytes(D));
-  const int i = l * n / 8;
-  const uint32_t word = words[value ? kv4_value_word<D>(p, i) : kv4_key_word<D>(p, i)];
-  const uint32_t par = words[4 * D + 2 * p + (value ? 1 : 0)];
-  const float s = __half2float(__ushort_as_half(static_cast<uint16_t>(par))), m = __half2float(__ushort_as_half(static_cast<uint16_t>(par >> 16)));
-  float x[n];
+  const int p = static_cast<int>(pos & 15), i = l * n / 8;
+  const int64_t step = kv4_tiles(C.max_len) * kv4_tile_bytes(D);
+  const unsigned char* tile = static_cast<const unsigned char*>(C.data) + (static_cast<int64_t>(b) * C.kv_heads + h0) * step + (pos >> 4) * kv4_tile_bytes(D);
+  uint32_t word[kHeads], par[kHeads];
 #pragma unroll
-  for (int j = 0; j < n; ++j) {
-    const int ch = (l * n + j) & 7;
-    x[j] = fmaf(s, static_cast<float>((word >> (4 * (ch >> 1) + 16 * (ch & 1))) & 15u), m);
+  for (int h = 0; h < kHeads; ++h)
+    if (h0 + h < C.kv_heads) {
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(tile + h * step);
+      word[h] = words[value ? kv4_value_word<D>(p, i) : kv4_key_word<D>(p, i)];
+      par[h] = words[4 * D + 2 * p + (value ? 1 : 0)];
+    }
+  T* dst = (value ? v + row * v_row + h0 * v_head : k + row * k_row + h0 * k_head) + l * n;
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (h0 + h >= C.kv_heads) break;
+    const float s = __half2float(__ushort_as_half(static_cast<uint16_t>(par[h]))), m = __half2float(__ushort_as_half(static_cast<uint16_t>(par[h] >> 16)));
+    float x[n];
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const int ch = (l * n + j) & 7;
+      x[j] = fmaf(s, static_cast<float>((word[h] >> (4 * (ch >> 1) + 16 * (ch & 1))) & 15u), m);
+    }
+    store_values<T, n>(dst + h * (value ? v_head : k_head), vec, x);
   }
-  T* dst = value ? v + row * v_row + h * v_head : k + row * k_row + h * k_head;
-  store_values<T, n>(dst + l * n, vec, x);
 }
 
 // Whether rows at `p` with these strides (in values of `size` bytes) can be read in chunks of `chunk` bytes.
@@ -155,16 +177,22 @@ namespace {
 template <int D, typename T>
 int32_t launch_rows(bool append, const IvbKv4Cache& c, void* k, void* v, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
                     const int32_t* starts, const int64_t* positions, int32_t rows, uint32_t* error, cudaStream_t stream) {
-  const int64_t items = static_cast<int64_t>(rows) * c.kv_heads, blocks = (items + kKv4Threads / 32 - 1) / (kKv4Threads / 32);
-  if (blocks > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4: %lld rows of heads in one call", static_cast<long long>(items));
-  constexpr int size = sizeof(T), chunk = D / 16 * size >= 16 ? 16 : D / 16 * size;
+  constexpr int size = sizeof(T), chunk = D / 16 * size >= 16 ? 16 : D / 16 * size, kWarps = kKv4Threads / 32;
   const bool vec = aligned(k, k_row, k_head, size, chunk) && aligned(v, v_row, v_head, size, chunk);
-  if (append)
-    kv4_append_kernel<D, T><<<static_cast<unsigned>(blocks), kKv4Threads, 0, stream>>>(
-        c, static_cast<const T*>(k), static_cast<const T*>(v), k_row, k_head, v_row, v_head, starts, positions, rows, vec, error);
-  else
-    kv4_read_kernel<D, T><<<static_cast<unsigned>(blocks), kKv4Threads, 0, stream>>>(
-        c, static_cast<T*>(k), static_cast<T*>(v), k_row, k_head, v_row, v_head, starts, positions, rows, vec, error);
+  const int heads = static_cast<int64_t>(rows) * c.kv_heads > 148 * 64 ? 4 : 1;
+  const int by = (c.kv_heads + heads - 1) / heads;
+  if (by > 65535) return fail(IVB_EINVAL, "ivb_kv4: %d key/value heads", c.kv_heads);
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(rows) + kWarps - 1) / kWarps), static_cast<unsigned>(by));
+  auto go = [&](auto append_kernel, auto read_kernel) {
+    if (append)
+      append_kernel<<<grid, kKv4Threads, 0, stream>>>(c, static_cast<const T*>(k), static_cast<const T*>(v), k_row, k_head, v_row, v_head,
+                                                      starts, positions, rows, vec, error);
+    else
+      read_kernel<<<grid, kKv4Threads, 0, stream>>>(c, static_cast<T*>(k), static_cast<T*>(v), k_row, k_head, v_row, v_head, starts, positions,
+                                                    rows, vec, error);
+  };
+  if (heads == 4) go(kv4_append_kernel<D, T, 4>, kv4_read_kernel<D, T, 4>);
+  else go(kv4_append_kernel<D, T, 1>, kv4_read_kernel<D, T, 1>);
   IVB_CUDA(cudaGetLastError());
   return IVB_OK;
 }

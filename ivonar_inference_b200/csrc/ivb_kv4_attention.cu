@@ -4,7 +4,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cstdlib>
 #include <atomic>
 #include <type_traits>
 
@@ -510,8 +509,6 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   int W = 1, C = 1;
   while (W < kMostWarps && base * W < 2 * slots && A.cache.max_len > W * kKv4Group) W *= 2;
   while (C < 8 && W == kMostWarps && base * W * C * 2 <= slots && A.cache.max_len > 4 * C * W * kKv4Group) C *= 2;
-  if (getenv("KV4_W")) W = atoi(getenv("KV4_W"));
-  if (getenv("KV4_C")) C = atoi(getenv("KV4_C"));
   if (base * C > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(base));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(base * C));

@@ -5,7 +5,7 @@
 //   warps 8..10 (producers) read the codes, expand them to fp16 u - 8 in shared memory (keys as a K-major operand, values as an
 //     MN-major one: both are position rows of 16-byte channel chunks, so neither is transposed) and compute each
 //     position's terms (scales and offsets; ivb_kv4_attention.cuh);
-//   warp 11 (one thread) issues S_X = Q_X U^T and O_X += P_X U'^T, fp32 in tensor memory;
+//   warp 11 (one thread, whose instructions come slowly beside the softmax's: no more of them than needed) issues S_X = Q_X U^T and O_X += P_X U'^T, fp32 in tensor memory;
 //   warps 0..7 (32 rows each, their tensor-memory lanes) turn S_X into weights: online softmax in 32 bits, the
 //     reference raised only when the maximum passes it by 2^8, and O_X rescaled in tensor memory then. The weights P_X take
 //     S_X's place as the fp16 A operand, so S_X(it + 1) follows P_X(it)'s product; while one X waits for it the other computes.
@@ -28,8 +28,9 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kRowsX = 128, kRowsCta = 256, kPos = 128;
-// 12 warps: with three on each of the SM's four parts a thread has 168 registers, enough to keep the loads of its 64 scores' terms ahead
-constexpr int kSoftmaxThreads = 256, kProducerWarps = 3, kProducers = 32 * kProducerWarps, kPromptThreads = kSoftmaxThreads + kProducers + 32;
+// 12 warps: three on each of the SM's four parts have 168 registers a thread, for the scores of four rows at a time
+constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 32 * kSoftmaxWarps, kProducerWarps = 3, kProducers = 32 * kProducerWarps;
+constexpr int kIssueWarp = kSoftmaxWarps + kProducerWarps, kPromptThreads = 32 * (kIssueWarp + 1);
 constexpr int kTermSets = 3;  // terms(it + 2) are written when S(it) is done, so when nobody reads terms(it - 1) any more
 constexpr unsigned long long kPromptTimeout = 2000000000ull;
 constexpr float kWeightUnit = 64.0f;  // weights are at most 2 * 64 * 2^8 in fp16
@@ -106,7 +107,7 @@ __device__ __forceinline__ void values_of_chunk(uint4 w, float (&v)[16 / sizeof(
 }
 
 struct PromptBarriers {
-  unsigned long long k_full[2], k_free[2], v_full[2], v_free[2], terms_full[kTermSets], s_full[2], p_full[2][2], p_free[2][2], drain;
+  unsigned long long k_full[2], k_free[2], v_full[2], v_free[2], terms_full[kTermSets], s_full[2][2], p_full[2][2], p_free[2][2], drain;
 };
 
 // What a lane of a producer warp holds of the keys or values of one tile of 16 positions (D = 32: values in lanes 0..15), dealt
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ PromptBarriers bar;
   __shared__ unsigned tmem_base;
-  __shared__ float largest[kSoftmaxThreads / 32], sums[kRowsCta];
+  __shared__ float largest[kSoftmaxWarps], sums[kRowsCta], refs_of[kRowsCta], totals[kRowsCta], offsets[kRowsCta];
   __shared__ int which[3];  // sequence, tile of its rows; and whether a wait ran out
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -240,11 +241,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       mbar_init(&bar.k_free[i], 1);
       mbar_init(&bar.v_full[i], kProducers);
       mbar_init(&bar.v_free[i], 1);
-      mbar_init(&bar.s_full[i], 1);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        mbar_init(&bar.p_full[i][h], kRowsX);
+        mbar_init(&bar.p_full[i][h], kSoftmaxThreads / 2);
         mbar_init(&bar.p_free[i][h], 1);
+        mbar_init(&bar.s_full[i][h], 1);
       }
     }
 #pragma unroll
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   __syncthreads();
   const int b = which[0];
   if (b < 0) return;
-  if (warp == kPromptThreads / 32 - 1) {
+  if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)), "r"(G::columns));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -284,14 +285,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     return i < sink_tiles ? i : window_tile + i - sink_tiles;
   };
 
-  // queries: a warp takes its 32 rows in 16-byte chunks, 8 rows and 4 chunks at a time (64 contiguous bytes of a row, and no bank
+  // queries: a warp takes 32 rows in 16-byte chunks, 8 rows and 4 chunks at a time (64 contiguous bytes of a row, and no bank
   // conflicts); the largest of all rows first, then hi (and lo) parts as K-major operands, scaled by a power of two that
   // brings it to 2^13
   constexpr int kPer = 16 / static_cast<int>(sizeof(T)), L = D / kPer, kQuads = L / 4;  // values of a chunk, chunks of a row
   const int row8 = lane & 7, chunk4 = lane >> 3;
-  const int x = warp >> 2;  // row tile of a softmax thread
-  const int item = i0 + tid;
-  const bool mine = tid < live;
+  const int x = warp >> 2;  // row tile of a softmax warp
   auto item_row = [&](const void* array, int i, int64_t row_stride, int64_t head_stride) {
     const int t = token_of(i), h = kvh * A.group + i - t * A.group;
     return static_cast<const T*>(array) + (row0 + t) * row_stride + h * head_stride;
@@ -352,7 +351,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   __syncthreads();
   float most = 0.0f;
 #pragma unroll
-  for (int w = 0; w < kSoftmaxThreads / 32; ++w) most = fmaxf(most, largest[w]);
+  for (int w = 0; w < kSoftmaxWarps; ++w) most = fmaxf(most, largest[w]);
   int up = 13 - (static_cast<int>(__float_as_uint(most) >> 23) - 127);
   up = most == 0.0f ? 0 : min(max(up, -100), 100);
   const float offset_unit = A.scale * kLog2e;
@@ -394,9 +393,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   auto terms_of = [&](int it) { return reinterpret_cast<float*>(smem + G::terms_at + it % kTermSets * G::term_bytes); };
   auto turn_of = [&](int it) { return static_cast<unsigned>(it / G::stages) & 1u; };  // parity of a stage's use
   bool ok = true;
-  float ref = -INFINITY, total = 0.0f, offset = 0.0f;  // in the end, of the row that is a softmax thread's lane
 
-  if (warp >= kSoftmaxThreads / 32 && warp < kPromptThreads / 32 - 1) {
+  if (warp >= kSoftmaxWarps && warp < kIssueWarp) {
     // ---- producers: 16-position tiles in turn ----
     constexpr int kTile = kv4_tile_bytes(D), kUnits = kPos / 16, kMine = (kUnits + kProducerWarps - 1) / kProducerWarps;
     const int unit0 = warp - kSoftmaxThreads / 32;
@@ -463,58 +461,65 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       fence_proxy_async();
       mbar_arrive(&bar.v_full[it % G::stages]);
     }
-  } else if (warp == kPromptThreads / 32 - 1) {
+  } else if (warp >= kIssueWarp) {
     // ---- the thread that issues the products ----
     if (lane == 0) {
-      const unsigned q0 = smem_addr(smem + G::q_at);
-      auto issue_s = [&](int it, int xx) {
-        const unsigned ka = smem_addr(keys_of(it)), qa = q0 + xx * G::parts * G::q_bytes;
-        tc_fence_after();
+      const uint64_t q0 = smem_desc(smem_addr(smem + G::q_at), D / 8 * 128);
+      const uint64_t k0 = smem_desc(smem_addr(smem + G::k_at), D / 8 * 128), v0 = smem_desc_mn(smem_addr(smem + G::v_at), D / 8 * 128);
+      // Half h of tile it: its 64 columns of S_X, and with P_X in their place its 64 positions' part of O_X. Descriptors count
+      // in 16 bytes.
+      auto issue_s = [&](int it, int h) {
+        const uint64_t k = k0 + (it % G::stages * G::kv_bytes + h * (G::kv_bytes / 2)) / 16;
+        for (int xx = 0; xx < row_tiles; ++xx) {
+          if (it > 0) {  // S takes the place of P
+            ok = ok && mbar_wait_bounded(&bar.p_free[xx][h], (it - 1) & 1, kPromptTimeout);
+            if (!ok) return;
+          }
+          tc_fence_after();
+          const uint64_t q = q0 + xx * (G::parts * G::q_bytes / 16);
+          const unsigned t_s = tmem + G::s_at + xx * kPos + h * (kPos / 2);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
+          for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-          for (int part = 0; part < G::parts; ++part)
-            umma_f16_ss(tmem + G::s_at + xx * kPos, smem_desc(qa + part * G::q_bytes + kk * 256, D / 8 * 128),
-                        smem_desc(ka + kk * 256, D / 8 * 128), idesc_f16(kRowsX, kPos), kk + part > 0);
-        umma_commit(&bar.s_full[xx]);
-      };
-      auto issue_o = [&](int it, int xx, int h) {
-        const unsigned va = smem_addr(values_of(it));
-        tc_fence_after();
-#pragma unroll
-        for (int k2 = 0; k2 < kPos / 32; ++k2) {
-          const int kk = h * (kPos / 32) + k2;
-#pragma unroll
-          for (int part = 0; part < G::parts; ++part)
-            umma_f16_ts(tmem + G::o_at + xx * D, tmem + G::s_at + xx * kPos + h * (kPos / 2) + part * (kPos / 4) + k2 * 8,
-                        smem_desc_mn(va + kk * 2 * (D / 8) * 128, D / 8 * 128), idesc_f16_bt(kRowsX, D), it + h > 0 || k2 + part > 0);
+            for (int part = 0; part < G::parts; ++part)
+              umma_f16_ss(t_s, q + (part * G::q_bytes + kk * 256) / 16, k + kk * 16, idesc_f16(kRowsX, kPos / 2), kk + part > 0);
+          umma_commit(&bar.s_full[xx][h]);
         }
-        umma_commit(&bar.p_free[xx][h]);
+        if (h == 1) umma_commit(&bar.k_free[it % G::stages]);
+      };
+      auto issue_o = [&](int it, int h) {
+        const uint64_t v = v0 + (it % G::stages * G::kv_bytes + h * (G::kv_bytes / 2)) / 16;
+        for (int xx = 0; xx < row_tiles; ++xx) {
+          ok = ok && mbar_wait_bounded(&bar.p_full[xx][h], it & 1, kPromptTimeout);
+          if (!ok) return;
+          tc_fence_after();
+          const unsigned t_p = tmem + G::s_at + xx * kPos + h * (kPos / 2), t_o = tmem + G::o_at + xx * D;
+#pragma unroll
+          for (int kk = 0; kk < kPos / 32; ++kk)
+#pragma unroll
+            for (int part = 0; part < G::parts; ++part)
+              umma_f16_ts(t_o, t_p + part * (kPos / 4) + kk * 8, v + kk * 2 * (D / 8) * 8, idesc_f16_bt(kRowsX, D), kk + part > 0 || it + h > 0);
+          umma_commit(&bar.p_free[xx][h]);
+        }
+        if (h == 1) umma_commit(&bar.v_free[it % G::stages]);
       };
       if (tiles > 0) {
         ok = mbar_wait_bounded(&bar.k_full[0], 0, kPromptTimeout);
         if (ok) {
-          for (int xx = 0; xx < row_tiles; ++xx) issue_s(0, xx);
-          umma_commit(&bar.k_free[0]);
+          issue_s(0, 0);
+          issue_s(0, 1);
         }
       }
+      // both row tiles' weights of a half, then, while they are used up, their next scores in that half's place
       for (int it = 0; it < tiles && ok; ++it) {
         ok = mbar_wait_bounded(&bar.v_full[it % G::stages], turn_of(it), kPromptTimeout);
-        for (int xx = 0; xx < row_tiles && ok; ++xx) {
-          for (int h = 0; h < 2 && ok; ++h) {
-            ok = mbar_wait_bounded(&bar.p_full[xx][h], it & 1, kPromptTimeout);
-            if (ok) issue_o(it, xx, h);
-          }
-          if (!ok) break;
-          if (xx == row_tiles - 1) umma_commit(&bar.v_free[it % G::stages]);
-          if (it + 1 < tiles) {
-            ok = (xx > 0 || mbar_wait_bounded(&bar.k_full[(it + 1) % G::stages], turn_of(it + 1), kPromptTimeout)) &&
-                 mbar_wait_bounded(&bar.p_free[xx][1], it & 1, kPromptTimeout);  // S takes the place of P
-            if (!ok) break;
-            issue_s(it + 1, xx);
-            if (xx == row_tiles - 1) umma_commit(&bar.k_free[(it + 1) % G::stages]);
-          }
+        if (ok) issue_o(it, 0);
+        if (it + 1 < tiles) {
+          ok = ok && mbar_wait_bounded(&bar.k_full[(it + 1) % G::stages], turn_of(it + 1), kPromptTimeout);
+          if (ok) issue_s(it + 1, 0);
         }
+        if (ok) issue_o(it, 1);
+        if (ok && it + 1 < tiles) issue_s(it + 1, 1);
       }
       if (!ok) {  // let what was issued finish before shared and tensor memory go
         umma_commit(&bar.drain);
@@ -525,9 +530,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     // ---- softmax: a warp has 32 rows, a thread in each 8-row set the row r and every fourth pair of positions, so that a
     // position's terms are loaded once for four rows (loaded for each row they bound the kernel: 12 cycles of the SM's
     // shared memory pipe for 64 scores)
-    const unsigned lanes = static_cast<unsigned>(32 * (warp & 3)) << 16;
+    const int r = lane >> 2, c = lane & 3, row0x = 32 * (warp & 3);
+    const unsigned lanes = static_cast<unsigned>(row0x) << 16;
     const unsigned ts = tmem + lanes + G::s_at + x * kPos, to = tmem + lanes + G::o_at + x * D;
-    const int r = lane >> 2, c = lane & 3;
     float sum_q[4], refs[4];
     int at[4];
     f32x2 sum2[4], off2[4];
@@ -535,7 +540,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     int first_at = 0x7fffffff, last_at = -1;  // of the warp's rows
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int n = 32 * warp + 8 * i + r;
+      const int n = kRowsX * x + row0x + 8 * i + r;
       sum_q[i] = sums[n];
       at[i] = -1;
       if (n < live) {
@@ -557,31 +562,35 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     for (int it = 0; it < tiles; ++it) {
       const int p0 = tile_of(it) * kPos;
       const float* terms = terms_of(it);
-      // S is full: the last product with P is done too, so O and P are at rest
-      ok = mbar_wait_bounded(&bar.terms_full[it % kTermSets], static_cast<unsigned>(it / kTermSets) & 1u, kPromptTimeout) &&
-           mbar_wait_bounded(&bar.s_full[x], it & 1, kPromptTimeout);
-      if (!__all_sync(0xFFFFFFFFu, ok)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
+      ok = mbar_wait_bounded(&bar.terms_full[it % kTermSets], static_cast<unsigned>(it / kTermSets) & 1u, kPromptTimeout);
       // what the warp's rows see of the tile: all of it, or nothing (first_at, last_at: the lowest and highest, -1 among them)
       const bool whole = live_rows && first_at >= p0 + kPos - 1 && (A.window <= 0 || p0 > last_at - A.window || p0 <= A.sinks - kPos);
       const bool none = last_at < p0 || (A.window > 0 && p0 + kPos - 1 <= first_at - A.window && p0 >= A.sinks);
-      if (none) {
-#pragma unroll
-        for (int i = 0; i < kPos; i += 32) tmem_fill32(ts + i, 0u);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&bar.p_full[x][0]);
-        mbar_arrive(&bar.p_full[x][1]);
-        continue;
-      }
-      // 64 positions at a time, whose product is issued while the next are computed
+      // 64 positions at a time: the next ones' scores and the last ones' product are computed meanwhile
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
+        ok = ok && mbar_wait_bounded(&bar.s_full[x][h], it & 1, kPromptTimeout);
+        if (!__all_sync(0xFFFFFFFFu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
         const unsigned th = ts + h * (kPos / 2);
         const float4* const t4 = reinterpret_cast<const float4*>(terms) + 3 * (32 * h + c);  // of the pair c; every fourth is ours
+        if (none) {
+          uint32_t zero[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) zero[i] = 0u;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            tmem_st_16x128b_x8(th + (static_cast<unsigned>(16 * g) << 16), zero);
+            if constexpr (kSplit) tmem_st_16x128b_x8(th + kPos / 4 + (static_cast<unsigned>(16 * g) << 16), zero);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&bar.p_full[x][h]);
+          continue;
+        }
         uint32_t s[2][32];  // [16 rows][4 pair + 2 (8 rows) + position], scores in place
 #pragma unroll
         for (int g = 0; g < 2; ++g) tmem_ld_16x256b_x8(th + (static_cast<unsigned>(16 * g) << 16), s[g]);
@@ -592,12 +601,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           const float2 e = *reinterpret_cast<const float2*>(&t4[12 * i + 1]);
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            uint32_t(&v)[32] = s[n >> 1];
             const int j = 4 * i + 2 * (n & 1);
-            const float2 y = unpair(fma2(pair(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), pair(k.x, k.y),
-                                   fma2(pair(sum_q[n], sum_q[n]), pair(k.z, k.w), pair(e.x, e.y))));
-            v[j] = __float_as_uint(y.x);
-            v[j + 1] = __float_as_uint(y.y);
+            const float2 y = unpair(fma2(pair(__uint_as_float(s[n >> 1][j]), __uint_as_float(s[n >> 1][j + 1])), pair(k.x, k.y),
+                                         fma2(pair(sum_q[n], sum_q[n]), pair(k.z, k.w), pair(e.x, e.y))));
+            s[n >> 1][j] = __float_as_uint(y.x);
+            s[n >> 1][j + 1] = __float_as_uint(y.y);
           }
         }
         if (!whole) {
@@ -616,10 +624,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int j = 4 * i + 2 * (n & 1);
-            top[n] = fmaxf(top[n], fmaxf(__uint_as_float(s[n >> 1][j]), __uint_as_float(s[n >> 1][j + 1])));
-          }
+          for (int i = 0; i < 8; ++i)
+            top[n] = fmaxf(top[n], fmaxf(__uint_as_float(s[n >> 1][4 * i + 2 * (n & 1)]), __uint_as_float(s[n >> 1][4 * i + 2 * (n & 1) + 1])));
         bool raise = false;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
@@ -628,30 +634,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           raise |= top[n] > refs[n] + kRaise;  // the first seen position too: the reference is -inf
         }
         if (__any_sync(0xFFFFFFFFu, raise)) {
-          float factor = 1.0f;  // of the row that is this thread's lane
+          float corr[4];
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
             const float next = fmaxf(refs[n], top[n]);
-            const float corr = next > refs[n] ? ex2(refs[n] - next) : 1.0f;
+            corr[n] = next > refs[n] ? ex2(refs[n] - next) : 1.0f;
             refs[n] = next;
-            sum2[n] = mul2(sum2[n], pair(corr, corr));
-            off2[n] = mul2(off2[n], pair(corr, corr));
-            const float theirs = __shfl_sync(0xFFFFFFFFu, corr, 4 * (lane & 7));
-            if (lane >> 3 == n) factor = theirs;
+            sum2[n] = mul2(sum2[n], pair(corr[n], corr[n]));
+            off2[n] = mul2(off2[n], pair(corr[n], corr[n]));
           }
-          if (h == 1) {  // the product of the first 64 positions is under way
-            ok = mbar_wait_bounded(&bar.p_free[x][0], it & 1, kPromptTimeout);
+          if (it + h > 0) {  // the last 64 positions' product may be under way
+            ok = mbar_wait_bounded(&bar.p_free[x][h ^ 1], (it - (h ^ 1)) & 1, kPromptTimeout);
             tc_fence_after();
           }
           if (it + h > 0) {
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 16) {
-              uint32_t o[16];
-              tmem_ld16(to + c0, o);
+            for (int c0 = 0; c0 < D; c0 += 32)
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
-              tmem_st16(to + c0, o);
-            }
+              for (int g = 0; g < 2; ++g) {
+                uint32_t o[16];
+                const unsigned at_o = to + c0 + (static_cast<unsigned>(16 * g) << 16);
+                tmem_ld_16x256b_x4(at_o, o);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr[2 * g + ((j >> 1) & 1)]);
+                tmem_st_16x256b_x4(at_o, o);
+              }
           }
         }
         f32x2 minus[4];  // a row that has seen nothing yet: its weights are 2^-inf
@@ -664,17 +671,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           const float4 uo = t4[12 * i + 2];
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            const uint32_t(&v)[32] = s[n >> 1];
             const int j = 4 * i + 2 * (n & 1);
-            const float2 d = unpair(add2(pair(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), minus[n]));
+            const float2 d = unpair(add2(pair(__uint_as_float(s[n >> 1][j]), __uint_as_float(s[n >> 1][j + 1])), minus[n]));
             const f32x2 pw = pair(ex2(d.x), ex2(d.y));
             sum2[n] = fma2(pw, pair(uo.x, uo.y), sum2[n]);
             off2[n] = fma2(pw, pair(uo.z, uo.w), off2[n]);
             const float2 w = unpair(mul2(pw, pair(mu.x, mu.y)));
-            uint32_t& out = hi[n >> 1][2 * i + (n & 1)];
-            out = pack_f16(w.x, w.y);
+            hi[n >> 1][2 * i + (n & 1)] = pack_f16(w.x, w.y);
             if constexpr (kSplit) {
-              const float2 f = unpack_f16(out);
+              const float2 f = unpack_f16(hi[n >> 1][2 * i + (n & 1)]);
               lo[n >> 1][2 * i + (n & 1)] = pack_f16(w.x - f.x, w.y - f.y);
             }
           }
@@ -688,47 +693,47 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         tc_fence_before();
         mbar_arrive(&bar.p_full[x][h]);
       }
-      if (!__all_sync(0xFFFFFFFFu, ok)) {
-        ok = false;
-        break;
-      }
+      if (!ok) break;
     }
     if (tiles > 0 && ok) {
       ok = mbar_wait_bounded(&bar.p_free[x][1], (tiles - 1) & 1, kPromptTimeout);
       ok = __all_sync(0xFFFFFFFFu, ok);
     }
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {  // a row's sums meet, and go to the thread that is its lane
+    for (int n = 0; n < 4; ++n) {
       const float2 s = unpair(sum2[n]), f = unpair(off2[n]);
       float l = s.x + s.y, o = f.x + f.y;
       l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
       l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
       o += __shfl_xor_sync(0xFFFFFFFFu, o, 1);
       o += __shfl_xor_sync(0xFFFFFFFFu, o, 2);
-      const float lane_l = __shfl_sync(0xFFFFFFFFu, l, 4 * (lane & 7)), lane_o = __shfl_sync(0xFFFFFFFFu, o, 4 * (lane & 7));
-      const float lane_ref = __shfl_sync(0xFFFFFFFFu, refs[n], 4 * (lane & 7));
-      if (lane >> 3 == n) {
-        total = lane_l;
-        offset = lane_o;
-        ref = lane_ref;
+      if (c == 0) {
+        const int row = kRowsX * x + row0x + 8 * n + r;
+        refs_of[row] = refs[n];
+        totals[row] = l;
+        offsets[row] = o;
       }
     }
   }
+  tc_fence_before();
+  __syncthreads();  // all products are done: the operands' place is free
+  tc_fence_after();
+  // now a thread has a row of its own: tensor-memory lane tid % 128 of row tile x
+  const int row = tid & (kRowsCta - 1);
   const unsigned to = tmem + (static_cast<unsigned>(32 * (warp & 3)) << 16) + G::o_at + x * D;
-  const bool softmax = tid < kSoftmaxThreads && x < row_tiles;
+  const bool mine = tid < kSoftmaxThreads && x < row_tiles;
   if (C == 1) {
-    if (softmax && ok) {
-      // the warp's rows go through its part of its tile's queries, which nobody reads any more, and leave in whole chunks
-      tc_fence_after();
-      const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-      unsigned char* const stage = smem + G::q_at + x * G::parts * G::q_bytes + 32 * (warp & 3) * D * static_cast<int>(sizeof(T));
-      auto chunk_of = [&](int r, int c) { return reinterpret_cast<uint4*>(stage + r * D * static_cast<int>(sizeof(T)) + ((c ^ (r & (L < 8 ? L - 1 : 7))) * 16)); };
+    if (mine && ok) {
+      // through the place of its tile's queries, to leave in whole 16-byte chunks: 32 rows a warp
+      const float total = totals[row], offset = offsets[row], inv = total == 0.0f ? 0.0f : 1.0f / total;
+      uint4* const stage = reinterpret_cast<uint4*>(smem + G::q_at) + (32 * warp) * L;
+      auto chunk_of = [&](int r, int c) { return stage + r * L + (c ^ (r & (L < 8 ? L - 1 : 7))); };
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t o[32];
-        if (tiles > 0) tmem_ld32(to + c0, o);
+      for (int c0 = 0; c0 < D; c0 += 16) {
+        uint32_t o[16];
+        if (tiles > 0) tmem_ld16(to + c0, o);
 #pragma unroll
-        for (int c = 0; c < 32 / kPer; ++c) {
+        for (int c = 0; c < 16 / kPer; ++c) {
           union {
             uint4 w;
             T t[kPer];
@@ -741,60 +746,52 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       }
       __syncwarp();
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int r = 8 * g + row8;
-        if (32 * warp + r < live) {
-          T* out = const_cast<T*>(item_row(A.out, i0 + 32 * warp + r, A.o_row, A.o_head)) + chunk4 * kPer;
+      for (int k = 0; k < L; ++k) {
+        const int r = (32 / L) * k + lane / L, c = lane % L;
+        const int n = kRowsX * x + 32 * (warp & 3) + r;
+        if (n < live) {
+          T* out = const_cast<T*>(item_row(A.out, i0 + n, A.o_row, A.o_head)) + c * kPer;
+          union {
+            uint4 w;
+            T t[kPer];
+          } u;
+          u.w = *chunk_of(r, c);
+          if (A.o_vec) {
+            *reinterpret_cast<uint4*>(out) = u.w;
+          } else {
 #pragma unroll
-          for (int k = 0; k < kQuads; ++k) {
-            union {
-              uint4 w;
-              T t[kPer];
-            } u;
-            u.w = *chunk_of(r, 4 * k + chunk4);
-            if (A.o_vec) {
-              *reinterpret_cast<uint4*>(out + 4 * k * kPer) = u.w;
-            } else {
-#pragma unroll
-              for (int j = 0; j < kPer; ++j) out[4 * k * kPer + j] = u.t[j];
-            }
+            for (int j = 0; j < kPer; ++j) out[j] = u.t[j];
           }
         }
       }
     }
   } else {
-    // every CTA leaves its O [channel][row] and (reference, sum, offset) [row], and finishes D / C channels of all rows
+    // every CTA leaves its O [channel][row], and finishes D / C channels of all rows
     float* const part = reinterpret_cast<float*>(smem);
-    float* const stats = part + D * kRowsCta;
-    static_assert(D * kRowsCta * 4 + kRowsCta * 12 <= G::smem, "shared memory");
-    __syncthreads();  // all products are done: the operands' place is free
-    if (softmax) {
-      tc_fence_after();
+    static_assert(D * kRowsCta * 4 <= G::smem, "shared memory");
+    if (mine) {
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t o[32];
-        if (tiles > 0 && ok) tmem_ld32(to + c0, o);
+      for (int c0 = 0; c0 < D; c0 += 16) {
+        uint32_t o[16];
+        if (tiles > 0 && ok) tmem_ld16(to + c0, o);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) part[(c0 + j) * kRowsCta + tid] = tiles > 0 ? __uint_as_float(o[j]) : 0.0f;
+        for (int j = 0; j < 16; ++j) part[(c0 + j) * kRowsCta + row] = tiles > 0 ? __uint_as_float(o[j]) : 0.0f;
       }
-      stats[tid] = ref;
-      stats[kRowsCta + tid] = total;
-      stats[2 * kRowsCta + tid] = offset;
     }
     cluster.sync();
-    if (softmax && mine) {
-      T* out = const_cast<T*>(item_row(A.out, item, A.o_row, A.o_head));
+    if (mine && row < live) {
+      T* out = const_cast<T*>(item_row(A.out, i0 + row, A.o_row, A.o_head));
       float top = -INFINITY, l = 0.0f, off = 0.0f, scale[4];
-      for (int k = 0; k < C; ++k) top = fmaxf(top, cluster.map_shared_rank(stats, k)[tid]);
+      for (int k = 0; k < C; ++k) top = fmaxf(top, cluster.map_shared_rank(refs_of, k)[row]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         scale[k] = 0.0f;
         if (k < C) {
-          const float* other = cluster.map_shared_rank(stats, k);
-          if (other[kRowsCta + tid] != 0.0f) {  // zero: the CTA saw nothing for this row
-            scale[k] = ex2(other[tid] - top);
-            l = fmaf(other[kRowsCta + tid], scale[k], l);
-            off = fmaf(other[2 * kRowsCta + tid], scale[k], off);
+          const float theirs = cluster.map_shared_rank(totals, k)[row];
+          if (theirs != 0.0f) {  // zero: the CTA saw nothing for this row
+            scale[k] = ex2(cluster.map_shared_rank(refs_of, k)[row] - top);
+            l = fmaf(theirs, scale[k], l);
+            off = fmaf(cluster.map_shared_rank(offsets, k)[row], scale[k], off);
           }
         }
       }
@@ -806,7 +803,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (k < C && scale[k] != 0.0f) {
-            const float* other = cluster.map_shared_rank(part, k) + c * kRowsCta + tid;
+            const float* other = cluster.map_shared_rank(part, k) + c * kRowsCta + row;
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = fmaf(other[j * kRowsCta], scale[k], y[j]);
           }
@@ -821,7 +818,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && which[2] != 0 && A.error != nullptr) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ETIMEOUT));
-  if (warp == kPromptThreads / 32 - 1) {
+  if (warp == kIssueWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::columns));
   }
@@ -847,7 +844,6 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   // a cluster where one CTA each would leave SMs without work
   int C = 1;
   while (C < 4 && tiles * A.cache.kv_heads * C < 148 && A.cache.max_len > 2 * C * kPos) C *= 2;
-  if (getenv("KV4_P")) C = atoi(getenv("KV4_P"));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * A.cache.kv_heads * C));
   cfg.blockDim = dim3(kPromptThreads);
