@@ -14,13 +14,29 @@ namespace {
 
 constexpr int kKv4Threads = 256;  // 8 warps, a row of one or four heads each
 
-// The code of x by the real quotient (x - m) / s. The 32-bit product with the reciprocal is within 2^-18 of it; where that
-// could change the rounding (2e-4 of all values) the quotient is taken in 64 bits.
-__device__ __forceinline__ int kv4_code(float x, float m, float s, float rs) {
-  const float t = (x - m) * rs;
-  float u = rintf(t);
-  if (fabsf(t - u) > 0.4999f) u = static_cast<float>(rint((static_cast<double>(x) - static_cast<double>(m)) / static_cast<double>(s)));
-  return static_cast<int>(fminf(fmaxf(u, 0.0f), 15.0f));
+// The codes of n values by the real quotients (x - m) / s, value i at bit shift(i) of the result. The 32-bit products with the
+// reciprocal are within 2^-18 of them; where that could change a rounding (2e-4 of all values) the quotients are taken in 64
+// bits. Adding 1.5 2^23 rounds to an integer in the low bits; the constants' sum comes off at the end.
+template <int n, typename Shift>
+__device__ __forceinline__ uint32_t kv4_codes(const float (&x)[n], float m, float s, float rs, Shift shift) {
+  constexpr float kMagic = 12582912.0f;
+  uint32_t word = 0;
+  float off = 0.0f;
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    const float t = fminf(fmaxf((x[i] - m) * rs, 0.0f), 15.0f), u = t + kMagic;
+    off = fmaxf(off, fabsf(t - (u - kMagic)));
+    word += (__float_as_uint(u) - 0x4b400000u) << shift(i);
+  }
+  if (off > 0.4999f) {
+    word = 0;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const double u = rint((static_cast<double>(x[i]) - static_cast<double>(m)) / static_cast<double>(s));
+      word |= static_cast<uint32_t>(fmin(fmax(u, 0.0), 15.0)) << shift(i);
+    }
+  }
+  return word;
 }
 
 // fp16 of the real quotient d / 15, rounded to 32 bits and then to 16, with d = hi - m. The 32-bit product is within 2^-22 of it;
@@ -44,7 +60,8 @@ __device__ __forceinline__ bool kv4_place(const IvbKv4Cache& C, const int32_t* s
 
 // One warp per row and kHeads heads: lanes 0..15 the key rows, lanes 16..31 the value rows, D / 16 channels each. Four heads a
 // warp share the look-up of the row and keep their loads in flight together; one is for calls too small to fill the GPU with
-// the others (2048 rows of 32 heads x 128 in bf16: 17 us with four, 24 with one; 256 rows of 16 x 64: 4.4 and 3.6 us).
+// the others (2048 rows of 32 heads x 128 in bf16: written in 30 us and read in 11 with four, 32 and 18 with one; bound by
+// the instructions of the writing, 140 a row, and the latency of the reading).
 template <int D, typename T, int kHeads>
 __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(IvbKv4Cache C, const T* k, const T* v, int64_t k_row, int64_t k_head,
                                                                  int64_t v_row, int64_t v_head, const int32_t* starts,
@@ -66,34 +83,31 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(IvbKv4Cache C, 
 #pragma unroll
   for (int h = 0; h < kHeads; ++h) {
     if (h0 + h >= C.kv_heads) break;
-    float lo = x[h][0], hi = x[h][0];
-    bool finite = fabsf(x[h][0]) <= 3.402823466e38f;
+    float lo = x[h][0], hi = x[h][0], zero = 0.0f;
 #pragma unroll
-    for (int i = 1; i < n; ++i) {
+    for (int i = 0; i < n; ++i) {
       lo = fminf(lo, x[h][i]);
       hi = fmaxf(hi, x[h][i]);
-      finite = finite && fabsf(x[h][i]) <= 3.402823466e38f;
+      zero = fmaf(x[h][i], 0.0f, zero);  // NaN where a value is none or infinite
     }
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) {
       lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, d));
       hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, d));
     }
-    const unsigned all = __ballot_sync(0xFFFFFFFFu, finite);
+    const unsigned all = __ballot_sync(0xFFFFFFFFu, zero == 0.0f);
     const bool row_finite = (value ? all >> 16 : all & 0xFFFFu) == 0xFFFFu;
     const __half mh = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
     const float m = __half2float(mh);
     const __half sh = kv4_scale(hi, m);
     const float s = __half2float(sh);
-    const float rs = s > 0.0f ? 1.0f / s : 0.0f;
+    const float rs = __fdividef(1.0f, s);  // within 2 ulp; of no use where s is zero
     uint32_t word = 0;
-    if (s > 0.0f && row_finite) {
-#pragma unroll
-      for (int i = 0; i < n; ++i) {
+    if (s > 0.0f && row_finite)
+      word = kv4_codes<n>(x[h], m, s, rs, [&](int i) {
         const int ch = (l * n + i) & 7;
-        word |= static_cast<uint32_t>(kv4_code(x[h][i], m, s, rs)) << (4 * (ch >> 1) + 16 * (ch & 1));
-      }
-    }
+        return 4 * (ch >> 1) + 16 * (ch & 1);
+      });
     // the D / 16 lanes' parts of each word meet in the first of them
 #pragma unroll
     for (int d = 1; d < 8 / n; d <<= 1) word |= __shfl_xor_sync(0xFFFFFFFFu, word, d);

@@ -521,7 +521,7 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = C > 1 ? 1 : 0;
   IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_rows_kernel<D, T, kSplit, kTiles>, A, static_cast<int>(tiles)));
   return IVB_OK;
 }

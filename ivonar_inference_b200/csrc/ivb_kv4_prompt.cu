@@ -855,7 +855,7 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = C > 1 ? 1 : 0;
   IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<D, T>, A, few));
   return IVB_OK;
 }

@@ -58,6 +58,7 @@ class KV4Cache:
             raise ValueError("error must be an int32 tensor of one value on the cache's device")
         self.data, self.error, self.device = data, error, data.device
         self._error = 0 if error is None else error.data_ptr()
+        self._index = data.device.index
         self._desc = native.IvbKv4Cache(data.data_ptr(), self.batch, self.kv_heads, self.head_dim, self.max_len)
         self._ref = ctypes.byref(self._desc)
 
@@ -108,7 +109,7 @@ class KV4Cache:
             raise ValueError(f"{name} requires a gradient: the 4-bit cache has none")
 
     def _call(self, what: str, function, *args) -> None:
-        index = self.device.index
+        index = self._index
         if torch.cuda.current_device() == index:
             rc = function(*args, self._error, torch._C._cuda_getCurrentRawStream(index))
         else:
@@ -179,7 +180,7 @@ class KV4Cache:
         if window < 0 or sinks < 0 or window >= 2**31 or sinks >= 2**31:
             raise ValueError("window and sinks must not be negative")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q)
         else:
             self._values("out", out, heads, q.dtype)
             if out.shape[0] != q.shape[0]:
