@@ -246,6 +246,8 @@ int32_t ivb_batch_decode(IvbDecoder* dec, const IvbBatch* b, int32_t steps, void
  * ivb_batch_embed: resid[b] = embedding row of tokens[b] (advances *step_counter when not NULL);
  * ivb_batch_ssm: one SSM step per sequence (recurrent_step, ternary.cu:421-482);
  * ivb_batch_mla: latent-cache append at positions[b] and absorbed attention (ternary.cu:509-611);
+ * ivb_batch_qk: the token's queries and keys for an attention over keys and values ([batch][channels]): entry and
+ *   up-projected no-position channels (k_nope [batch][heads * nope], a GEMM of the quantised latent), rotated rest;
  * ivb_batch_sample: per-sequence sampler, then positions[b] += 1 (ternary.cu:1099-1337). */
 int32_t ivb_batch_embed(const IvbTernary* head, const int64_t* tokens, int32_t batch, int32_t hidden, float* resid,
                         int32_t* step_counter, void* stream);
@@ -255,6 +257,9 @@ int32_t ivb_batch_mla(const IvbLayerDesc* layer, const IvbBatchLayer* state, con
                       const int64_t* positions, int32_t batch, int32_t channels, int32_t latent, int32_t heads,
                       int32_t head_dim, int32_t rope, int32_t nope, int32_t max_len, float act_eps, uint32_t* error,
                       float* y, void* stream);
+int32_t ivb_batch_qk(const IvbLayerDesc* layer, const float* ent, int32_t ld, const float* k_nope, const int64_t* positions,
+                     int32_t batch, int32_t channels, int32_t latent, int32_t heads, int32_t head_dim, int32_t rope,
+                     int32_t nope, int32_t max_len, float* q, float* k, void* stream);
 int32_t ivb_batch_sample(const float* logits, uint8_t* seen, int32_t vocab, int32_t batch, const float* sampling,
                          const int64_t* top_k, int32_t max_top_k, uint64_t* rng, int64_t* tokens, int64_t* positions,
                          int64_t* history, int32_t history_len, const int32_t* step_counter, void* stream);

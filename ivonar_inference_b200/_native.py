@@ -184,6 +184,8 @@ SIGNATURES = {
                                 c_int32, c_int32, c_void_p, c_void_p]),
     "ivb_batch_mla": (c_int32, [POINTER(IvbLayerDesc), POINTER(IvbBatchLayer), c_void_p, c_int32, c_void_p, c_int32, c_int32,
                                 c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p]),
+    "ivb_batch_qk": (c_int32, [POINTER(IvbLayerDesc), c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
+                               c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
     "ivb_batch_sample": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p,
                                    c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
     "ivb_validate_buffers": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p]),

@@ -808,6 +808,35 @@ int32_t launch_batch_attention(const IvbLayerDesc& L, const IvbBatchLayer& BL, c
   return IVB_OK;
 }
 
+// Queries and keys of sequence blockIdx.x's token as the attention takes them, [heads][head_dim]: the no-position channels as
+// they are (queries from the entry row, keys from the up-projected latent), then the position channels rotated.
+__global__ void __launch_bounds__(kThreads) batch_qk_kernel(const float* rope_table, const float* ent, int ld, const float* k_nope,
+                                                            const int64_t* positions, int channels, int latent, int heads, int hd,
+                                                            int rope, int nope, int max_len, float* q, float* k) {
+  const int b = blockIdx.x;
+  const long long pos = min(max(positions[b], static_cast<int64_t>(0)), static_cast<int64_t>(max_len) - 1);  // idle: unused
+  const float* row = ent + static_cast<size_t>(b) * ld;
+  const float* table = rope_table + pos * rope;
+  for (int i = threadIdx.x; i < heads * hd; i += kThreads) {
+    const int h = i / hd, e = i - h * hd;
+    float qv, kv;
+    if (e < nope) {
+      qv = row[i];
+      kv = k_nope[static_cast<size_t>(b) * heads * nope + h * nope + e];
+    } else {
+      const int j = (e - nope) >> 1;
+      const bool odd = ((e - nope) & 1) != 0;
+      const float cs = __ldg(table + 2 * j), sn = __ldg(table + 2 * j + 1);
+      const float* q2 = row + h * hd + nope + 2 * j;
+      const float* k2 = row + channels + latent + h * rope + 2 * j;
+      qv = odd ? q2[0] * sn + q2[1] * cs : q2[0] * cs - q2[1] * sn;
+      kv = odd ? k2[0] * sn + k2[1] * cs : k2[0] * cs - k2[1] * sn;
+    }
+    q[static_cast<size_t>(b) * channels + i] = qv;
+    k[static_cast<size_t>(b) * channels + i] = kv;
+  }
+}
+
 struct BatchLayout {
   size_t resid, ent, y, h, q8, scale, partial, total;
   int ldq;
@@ -973,6 +1002,20 @@ int32_t ivb_batch_mla(const IvbLayerDesc* L, const IvbBatchLayer* B, const float
   if (int32_t rc = launch_batch_attention(*L, *B, ent, ld, positions, batch, channels, latent, heads, head_dim, rope, nope,
                                           max_len, lpad, rpad, y, s))
     return rc;
+  return IVB_OK;
+}
+
+int32_t ivb_batch_qk(const IvbLayerDesc* L, const float* ent, int32_t ld, const float* k_nope, const int64_t* positions, int32_t batch,
+                     int32_t channels, int32_t latent, int32_t heads, int32_t head_dim, int32_t rope, int32_t nope, int32_t max_len,
+                     float* q, float* k, void* stream) {
+  using namespace ivb;
+  if (L == nullptr || L->rope == nullptr || ent == nullptr || k_nope == nullptr || positions == nullptr || q == nullptr || k == nullptr ||
+      batch <= 0 || max_len <= 0 || channels != heads * head_dim || nope + rope != head_dim || (rope & 1) != 0 ||
+      ld < channels + latent + heads * rope)
+    return fail(IVB_EINVAL, "ivb_batch_qk: bad argument");
+  batch_qk_kernel<<<batch, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(L->rope, ent, ld, k_nope, positions, channels, latent, heads,
+                                                                             head_dim, rope, nope, max_len, q, k);
+  IVB_CUDA(cudaGetLastError());
   return IVB_OK;
 }
 

@@ -158,7 +158,8 @@ class KV4Cache:
                 rows = self.batch
             if dtype not in _TYPES:
                 raise ValueError(f"dtype {dtype}")
-            k, v = torch.empty((2, rows, self.kv_heads, self.head_dim), dtype=dtype, device=self.device).unbind(0)
+            k = torch.empty((rows, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
+            v = torch.empty_like(k)
         at = self._rows(rows, positions, starts)
         self._call("ivb_kv4_read", self.lib.ivb_kv4_read, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], k.stride(0), k.stride(1),
                    v.stride(0), v.stride(1), at, positions.data_ptr(), rows)

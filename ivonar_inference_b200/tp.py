@@ -20,6 +20,11 @@ candidates to every rank, and each rank runs the same merge and Philox draw (`iv
 so all ranks sample the token the unsharded sampler would (same seeds). The kernels are the batched
 decode's unit steps (`ivb_batch_*`, `ivb_ternary_gemm`, `ivb_quantize_rows[_amax]`). Prompts run through
 the same step teacher-forced, one token per step.
+
+With `cache="kv4"` the attention blocks keep keys and values in 4 bits (`KV4Cache`) instead of the compressed latent: the
+latent of each new token is up-projected once, its keys and values are quantised as they are written, and the
+attention reads them, over all positions or a `window` with the first `sinks` visible. No query is absorbed and no value
+projected per step, at twice the latent cache's bytes and with 4-bit rounding of what is attended to.
 """
 
 from __future__ import annotations
@@ -32,7 +37,8 @@ import torch.nn.functional as F
 from torch import Tensor
 
 from . import _native as native
-from .decoder import DeviceMatrix, rope_from_rotary
+from .kv4 import KV4Cache
+from .matrix import DeviceMatrix, rope_from_rotary
 
 
 def split_even(total: int, parts: int, unit: int = 1) -> list[tuple[int, int]]:
@@ -89,7 +95,14 @@ class B200TensorParallel:
 
     def __init__(self, model, rank: int, world: int, group=None, batch: int = 1, max_len: int = 1024,
                  device: str | torch.device | None = None, max_top_k: int = 256, history_len: int = 1024,
-                 graphs: bool = True) -> None:
+                 graphs: bool = True, cache: str = "latent", window: int = 0, sinks: int = 0) -> None:
+        if cache not in ("latent", "kv4"):
+            raise ValueError("cache must be 'latent' or 'kv4'")
+        if cache == "latent" and (window != 0 or sinks != 0):
+            raise ValueError("a window needs the kv4 cache")
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks must not be negative")
+        self.cache, self.window, self.sinks = cache, int(window), int(sinks)
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         self.device, self.rank, self.world, self.group = dev, int(rank), int(world), group
         self.batch, self.max_len, self.max_top_k = int(batch), int(max_len), int(max_top_k)
@@ -100,6 +113,8 @@ class B200TensorParallel:
         if H % world:
             raise ValueError(f"{H} heads do not split over {world} ranks")
         self.hidden, self.heads_local, self.head_dim = d, H // world, hd
+        self.latent = 0
+        self.error = torch.zeros(1, dtype=torch.int32, device=dev)
         h0, h1 = rank * self.heads_local, (rank + 1) * self.heads_local
         c0, c1 = h0 * hd, h1 * hd
         self.channels = c1 - c0
@@ -178,18 +193,23 @@ class B200TensorParallel:
                 vu = DeviceMatrix([row_slice(mixer.v_up_proj, c0, c1)], dev, scale_align=8)
                 table = rope_from_rotary(mixer.rope, self.max_len).to(dev)
                 lpad, rpad = (Lt + 15) // 16 * 16, (rope + 7) // 8 * 8
-                cache = (
-                    torch.zeros(B, self.max_len, lpad, dtype=torch.int8, device=dev),
-                    torch.zeros(B, self.max_len, dtype=torch.float32, device=dev),
-                    torch.zeros(B, self.heads_local, self.max_len, rpad, dtype=torch.float16, device=dev),
-                )
-                keep += [table, *cache]
+                if cache == "kv4":
+                    store = KV4Cache(B, self.heads_local, hd, self.max_len, device=dev, error=self.error)
+                    latents = ()
+                else:
+                    store = latents = (
+                        torch.zeros(B, self.max_len, lpad, dtype=torch.int8, device=dev),
+                        torch.zeros(B, self.max_len, dtype=torch.float32, device=dev),
+                        torch.zeros(B, self.heads_local, self.max_len, rpad, dtype=torch.float16, device=dev),
+                    )
+                keep += [table, *latents]
                 desc.k_nope_up, desc.v_up = kn.desc(), vu.desc()
                 desc.rope = table.data_ptr()
                 desc.attn_scale = 1.0 / math.sqrt(hd)
-                state.latent_q, state.latent_scale, state.k_rope_cache = (c.data_ptr() for c in cache)
+                if latents:
+                    state.latent_q, state.latent_scale, state.k_rope_cache = (c.data_ptr() for c in latents)
                 self.latent, self.rope, self.nope = Lt, rope, nope
-                layer = {"kind": "mla", "entry": entry, "k_nope_up": kn, "v_up": vu, "cache": cache}
+                layer = {"kind": "mla", "entry": entry, "k_nope_up": kn, "v_up": vu, "cache": store}
             else:
                 raise native.KernelError(f"unsupported mixer for the B200 kernels: {type(mixer).__name__}")
             out = DeviceMatrix([col_slice(mixer.out_proj, c0, c1, keep_bias=rank == 0)], dev)
@@ -201,12 +221,16 @@ class B200TensorParallel:
             ent_rows = max(ent_rows, layer["entry"].rows)
             self._keep.append(keep)
             self.layers.append(layer)
-        ldq = (max(d, self.ffn_local, self.channels) + 127) // 128 * 128
+        ldq = (max(d, self.ffn_local, self.channels, self.latent) + 127) // 128 * 128
         rows128 = (B + 127) // 128 * 128
         f32 = dict(dtype=torch.float32, device=dev)
         self.resid, self.partial = torch.zeros(B, d, **f32), torch.zeros(B, d, **f32)
         self.ent = torch.zeros(B, ent_rows, **f32)
         self.y = torch.zeros(B, self.channels, **f32)
+        if cache == "kv4" and self.latent:
+            # the new tokens' latents, up-projections and assembled queries and keys
+            self.latents, self.k_nope = torch.zeros(B, self.latent, **f32), torch.zeros(B, self.heads_local * self.nope, **f32)
+            self.q, self.k, self.v = (torch.zeros(B, self.heads_local, hd, **f32) for _ in range(3))
         self.h = torch.zeros(B, self.ffn_local, **f32)
         self.q8 = torch.zeros(rows128, ldq, dtype=torch.int8, device=dev)
         self.act_scale, self.amax = torch.zeros(B, **f32), torch.zeros(B, **f32)
@@ -225,7 +249,6 @@ class B200TensorParallel:
         self.step_counter = torch.zeros(1, dtype=torch.int32, device=dev)
         self.sampling = torch.ones(3, **f32)
         self.top_k = torch.ones(1, dtype=torch.int64, device=dev)
-        self.error = torch.zeros(1, dtype=torch.int32, device=dev)
         self.host_position = 0
         self.use_graphs = bool(graphs)
         self._graph: torch.cuda.CUDAGraph | None = None
@@ -290,6 +313,22 @@ class B200TensorParallel:
         self._all_reduce(self.partial, torch.distributed.ReduceOp.SUM if self.world > 1 else None)
         self.resid.add_(self.partial)
 
+    def _attend_kv4(self, desc, layer: dict, ld: int) -> None:
+        """The token's keys and values from its latent, into the 4-bit cache, and the attention over it into y."""
+
+        ent = self.ent.view(-1)[: self.batch * ld].view(self.batch, ld)
+        self.latents.copy_(ent[:, self.channels:self.channels + self.latent])
+        self._quant(self.latents, self.latent, None, 0.0)
+        self._gemm(layer["k_nope_up"], native.IVB_EPI_STORE, self.k_nope, self.k_nope.shape[1])
+        self._gemm(layer["v_up"], native.IVB_EPI_STORE, self.v, self.channels)
+        rc = self.lib.ivb_batch_qk(ctypes.byref(desc), ent.data_ptr(), ld, self.k_nope.data_ptr(), self.positions.data_ptr(), self.batch,
+                                   self.channels, self.latent, self.heads_local, self.head_dim, self.rope, self.nope, self.max_len,
+                                   self.q.data_ptr(), self.k.data_ptr(), self._stream())
+        native.check(rc, "ivb_batch_qk")
+        layer["cache"].append(self.k, self.v, self.positions)
+        layer["cache"].attention(self.q, self.positions, scale=desc.attn_scale, window=self.window, sinks=self.sinks,
+                                 out=self.y.view(self.batch, self.heads_local, self.head_dim))
+
     @torch.no_grad()
     def step(self, feed: Tensor | None = None, sample: bool = True) -> None:
         """One token for every sequence: `feed` [batch] teacher-forces the input tokens (no sampling)."""
@@ -313,6 +352,8 @@ class B200TensorParallel:
                                             self.batch, self.channels, self.heads_local, self.head_dim, self.state_dim,
                                             self.y.data_ptr(), st)
                 native.check(rc, "ivb_batch_ssm")
+            elif self.cache == "kv4":
+                self._attend_kv4(desc, layer, ld)
             else:
                 rc = self.lib.ivb_batch_mla(ctypes.byref(desc), ctypes.byref(self.batch_layers[index]), self.ent.data_ptr(), ld,
                                             self.positions.data_ptr(), self.batch, self.channels, self.latent,
