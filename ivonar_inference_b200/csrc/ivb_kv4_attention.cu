@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
     sum[s] = off[s] = 0.0f;
   }
 
+  const CodeMiddle key_middle = code_middle(8.0f, 8.0f), value_middle = code_middle(8.0f, 7.0f);  // halves: channels, positions
   int at_stage = 0, to_stage = G::stages - 1;
   for (int step = 0; step < steps; ++step) {
     cp_async_wait<G::stages - 2>();
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
     const int p0 = group_of(step) * kKv4Group;
     {
       const uint2 par = *reinterpret_cast<const uint2*>(stage + (lane >> 4) * kTile + 16 * D + (lane & 15) * 8);
-      const PositionTerms t = position_terms(par, score_unit, offset_unit, 16384.0f);
+      const PositionTerms t = position_terms(par, score_unit, offset_unit, 16384.0f, lane);
       terms4[lane] = make_float4(t.key_scale, t.key_offset, t.bias, t.mantissa);
       terms2[lane] = make_float2(t.unbias, t.value_offset);
     }
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const uint32_t v0 = s & 1 ? w[0][s >> 1] >> 8 : w[0][s >> 1], v1 = s & 1 ? w[1][s >> 1] >> 8 : w[1][s >> 1];
-        const uint32_t a0 = codes_low(v0), a1 = codes_low(v1), a2 = codes_high(v0), a3 = codes_high(v1);
+        const uint32_t a0 = codes_low(v0, key_middle), a1 = codes_low(v1, key_middle), a2 = codes_high(v0, key_middle), a3 = codes_high(v1, key_middle);
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) mma_f16(s2[n], a0, a1, a2, a3, qf[n][s][0], qf[n][s][1]);
       }
@@ -339,7 +340,8 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t y01 = i ? x01 >> 8 : x01, y23 = i ? x23 >> 8 : x23;
-          const uint32_t a0 = codes_low(y01), a1 = codes_high(y01), a2 = codes_low(y23), a3 = codes_high(y23);
+          const uint32_t a0 = codes_low(y01, value_middle), a1 = codes_high(y01, value_middle);
+          const uint32_t a2 = codes_low(y23, value_middle), a3 = codes_high(y23, value_middle);
 #pragma unroll
           for (int n = 0; n < kTiles; ++n) mma_f16(acc[n][i], a0, a1, a2, a3, bw[n][0], bw[n][1]);
         }
@@ -357,8 +359,8 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
               h01 >>= 8;
               h23 >>= 8;
             }
-            const uint32_t a0 = i & 1 ? codes_high(l01) : codes_low(l01), a1 = i & 1 ? codes_high(h01) : codes_low(h01);
-            const uint32_t a2 = i & 1 ? codes_high(l23) : codes_low(l23), a3 = i & 1 ? codes_high(h23) : codes_low(h23);
+            const uint32_t a0 = i & 1 ? codes_high(l01, value_middle) : codes_low(l01, value_middle), a1 = i & 1 ? codes_high(h01, value_middle) : codes_low(h01, value_middle);
+            const uint32_t a2 = i & 1 ? codes_high(l23, value_middle) : codes_low(l23, value_middle), a3 = i & 1 ? codes_high(h23, value_middle) : codes_low(h23, value_middle);
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) mma_f16(acc[n][4 * h + i], a0, a1, a2, a3, bw[n][0], bw[n][1]);
           }

@@ -2,10 +2,13 @@
 //
 // With k_j = m_j + s_j u_j (codes u_j) the score is  a q.k_j = a s_j (q.u_j) + a m_j sum(q), and with v_j = m'_j + s'_j u'_j the
 // output is  sum_j p_j v_j = sum_j (p_j s'_j) u'_j + sum_j p_j m'_j : both products run on the codes themselves, and scales and
-// offsets are applied to scores and weights in 32 bits, one multiply-add per score. The operands are u - 8, exact in
-// fp16, with m + 8 s in the offsets' place: the tensor cores cut their sums towards zero, which adds up over a long axis
-// where all terms have one sign (3e-6 of the output at 2000 positions with u, 5e-7 with u - 8). fp32 queries and weights are split in two fp16 (x = hi + lo, 22 bits); fp16 and bf16
-// queries are exact in fp16 after a common power of two, and weights are rounded once to fp16.
+// offsets are applied to scores and weights in 32 bits, one multiply-add per score. The operands are the codes less their
+// middle, exact in fp16, with m + 8 s in the offsets' place: the tensor cores cut their sums towards zero, which adds up over a
+// long axis where the terms have one sign (with u itself 3e-6 of the output at 2000 positions). Values take u - 8 at even
+// positions and u - 7 at odd ones, since the 0.5 that is left of either mean is what all of a long history has in
+// common (with u - 8 throughout 1.3e-5 at 100000 positions, where the values average out to little).
+// fp32 queries and weights are split in two fp16 (x = hi + lo, 22 bits); fp16 and bf16 queries are exact in fp16 after a common
+// power of two, and their weights are rounded once to fp16 where a tile has no place for a remainder.
 #pragma once
 
 #include "ivb_common.h"
@@ -48,17 +51,23 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   return y;
 }
 
-// Two nibbles of a word as fp16 values u - 8: the bits under 0x6400 give 1024 + u and 1024 + 16 u, the rest is exact. The
-// bare bits, fp16 subnormals u 2^-24, would save this instruction, but the tensor cores align products by the operands'
-// exponent fields and cut 7 to 10 bits more of a subnormal's: 5e-5 of the output, measured.
-__device__ __forceinline__ uint32_t codes_low(uint32_t w) {
+// Two nibbles of a word as fp16 values u - lo (low half) and u - hi: the bits under 0x6400 give 1024 + u and 1024 + 16 u, the rest
+// is exact. The bare bits, fp16 subnormals u 2^-24, would save this instruction, but the tensor cores align products by
+// the operands' exponent fields and cut 7 to 10 bits more of a subnormal's: 5e-5 of the output, measured.
+struct CodeMiddle {
+  __half2 low, high;  // to add to 1024 + u, and to 64 + u
+};
+__device__ __forceinline__ CodeMiddle code_middle(float lo, float hi) {
+  return {__floats2half2_rn(-1024.0f - lo, -1024.0f - hi), __floats2half2_rn(-64.0f - lo, -64.0f - hi)};
+}
+__device__ __forceinline__ uint32_t codes_low(uint32_t w, CodeMiddle m) {
   const uint32_t x = and_or(w, 0x000f000fu, 0x64006400u);
-  const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(-1032.0f, -1032.0f));
+  const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), m.low);
   return *reinterpret_cast<const uint32_t*>(&y);
 }
-__device__ __forceinline__ uint32_t codes_high(uint32_t w) {
+__device__ __forceinline__ uint32_t codes_high(uint32_t w, CodeMiddle m) {
   const uint32_t x = and_or(w, 0x00f000f0u, 0x64006400u);
-  const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-72.0f, -72.0f));
+  const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(0.0625f, 0.0625f), m.high);
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 
@@ -69,10 +78,10 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t w) {
 // value terms of zero: it makes the rows that see it NaN, and a masked one's weight of zero stays zero whatever it holds.
 struct PositionTerms {
   float key_scale, key_offset, bias, mantissa;  // mantissa of the value scale, times weight_unit
-  float unbias, value_offset;                   // 2^-bias, value offset times 2^-bias (offsets are of u - 8)
+  float unbias, value_offset;                   // 2^-bias, value offset times 2^-bias (offsets are of the middle)
 };
 
-__device__ __forceinline__ PositionTerms position_terms(uint2 par, float score_unit, float offset_unit, float weight_unit) {
+__device__ __forceinline__ PositionTerms position_terms(uint2 par, float score_unit, float offset_unit, float weight_unit, int position) {
   const float2 key = unpack_f16(par.x), value = unpack_f16(par.y);
   PositionTerms t;
   t.key_scale = key.x * score_unit;
@@ -82,7 +91,7 @@ __device__ __forceinline__ PositionTerms position_terms(uint2 par, float score_u
   t.bias = number ? static_cast<float>(static_cast<int>(e >> 23) - 127) : __uint_as_float(0x7fffffffu);
   t.unbias = number ? __uint_as_float(0x7f000000u - e) : 0.0f;
   t.mantissa = number ? value.x * t.unbias * weight_unit : 0.0f;
-  t.value_offset = number ? fmaf(8.0f, value.x, value.y) * t.unbias : 0.0f;
+  t.value_offset = number ? fmaf(position & 1 ? 7.0f : 8.0f, value.x, value.y) * t.unbias : 0.0f;
   return t;
 }
 

@@ -2,7 +2,7 @@
 //
 // One CTA per (sequence, key/value head, 256 rows), 12 warps. Row i of a sequence's head group is token i / group, query head
 // i % group; rows 0..127 and 128..255 are two tiles X of the tensor cores' 128 lanes. Per tile of 128 positions:
-//   warps 8..10 (producers) read the codes, expand them to fp16 u - 8 in shared memory (keys as a K-major operand, values as an
+//   warps 8..10 (producers) read the codes, expand them to fp16 in shared memory (keys as a K-major operand, values as an
 //     MN-major one: both are position rows of 16-byte channel chunks, so neither is transposed) and compute each
 //     position's terms (scales and offsets; ivb_kv4_attention.cuh);
 //   warp 11 (one thread, whose instructions come slowly beside the softmax's: no more of them than needed) issues S_X = Q_X U^T and O_X += P_X U'^T, fp32 in tensor memory;
@@ -35,6 +35,9 @@ constexpr int kTermSets = 3;  // terms(it + 2) are written when S(it) is done, s
 constexpr unsigned long long kPromptTimeout = 2000000000ull;
 constexpr float kWeightUnit = 64.0f;  // weights are at most 2 * 64 * 2^8 in fp16
 constexpr float kRaise = 8.0f;
+// The tensor cores cut what they add to an accumulator towards zero, a bias that grows with its length (1.6e-6 of the output after
+// 1024 positions). fp32 outputs keep a second one, to which the threads add the first every so many tiles, rounding to nearest.
+constexpr int kFoldTiles = 2;
 
 template <int D, bool kSplit>
 struct PromptGeometry {
@@ -43,11 +46,13 @@ struct PromptGeometry {
   static constexpr int q_bytes = kRowsX * D * 2;             // one part of one row tile
   static constexpr int kv_bytes = kPos * D * 2;              // keys or values of a stage
   static constexpr int term_bytes = kPos * 24;
-  static constexpr int q_at = 0, k_at = 2 * parts * q_bytes, v_at = k_at + stages * kv_bytes, terms_at = v_at + stages * kv_bytes;
+  static constexpr int q_at = 0, k_at = (kSplit && D == 128 ? 1 : 2) * parts * q_bytes, v_at = k_at + stages * kv_bytes, terms_at = v_at + stages * kv_bytes;
   static constexpr int smem = terms_at + kTermSets * term_bytes;
-  // tensor memory columns: S_X, then P_X in its place (of every 64 columns 32 hi, 32 lo), and O_X
-  static constexpr int s_at = 0, o_at = 2 * kPos, columns = 512;
-  static_assert(o_at + 2 * D <= columns, "tensor memory");
+  // row tiles of a CTA: at fp32 and D = 128 tensor memory holds the accumulators of one
+  static constexpr int row_tiles = kSplit && D == 128 ? 1 : 2, rows = row_tiles * kRowsX;
+  // tensor memory columns: S_X, then P_X in its place (of every 64 columns 32 hi, 32 lo), O_X, and O_X's sums (fp32)
+  static constexpr int s_at = 0, o_at = row_tiles * kPos, fold_at = o_at + row_tiles * D, columns = 512;
+  static_assert(fold_at + (kSplit ? row_tiles * D : 0) <= columns, "tensor memory");
 };
 
 // kind::f16, fp32 result, A K-major, B MN-major.
@@ -66,7 +71,9 @@ __device__ __forceinline__ int chunk_at(int p, int i) {
   return ((p >> 3) * (D / 8) + i) * 128 + (p & 7) * 16;
 }
 
-__device__ __forceinline__ uint4 expand(uint32_t w) { return make_uint4(codes_low(w), codes_high(w), codes_low(w >> 8), codes_high(w >> 8)); }
+__device__ __forceinline__ uint4 expand(uint32_t w, CodeMiddle m) {
+  return make_uint4(codes_low(w, m), codes_high(w, m), codes_low(w >> 8, m), codes_high(w >> 8, m));
+}
 
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair(float a, float b) {
@@ -147,6 +154,7 @@ __device__ __forceinline__ void load_codes_of_values(const unsigned char* tile, 
 // `keys`, `values`: the tile's 16 position rows.
 template <int D>
 __device__ __forceinline__ void store_keys(const RawChunks<D>& raw, int lane, unsigned char* keys) {
+  const CodeMiddle m = code_middle(8.0f, 8.0f);
   if constexpr (D == 128) {
     const int h = (lane >> 2) & 1, c = lane >> 3;
 #pragma unroll
@@ -154,7 +162,7 @@ __device__ __forceinline__ void store_keys(const RawChunks<D>& raw, int lane, un
       const int r = (lane & 3) + 4 * k, p = 4 * (r >> 1) + (r & 1) + 2 * h;
       const uint32_t w[4] = {raw.v[k].x, raw.v[k].y, raw.v[k].z, raw.v[k].w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(keys + chunk_at<D>(p, 4 * c + i)) = expand(w[i]);
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(keys + chunk_at<D>(p, 4 * c + i)) = expand(w[i], m);
     }
   } else {
     const int r = lane & 7, c = lane >> 3, other = r >> 2;  // the upper four rows' lanes take their two positions in the other order
@@ -162,19 +170,21 @@ __device__ __forceinline__ void store_keys(const RawChunks<D>& raw, int lane, un
     if constexpr (D == 64) {
       const uint2 a = other ? make_uint2(raw.v[0].z, raw.v[0].w) : make_uint2(raw.v[0].x, raw.v[0].y);
       const uint2 b = other ? make_uint2(raw.v[0].x, raw.v[0].y) : make_uint2(raw.v[0].z, raw.v[0].w);
-      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, 2 * c)) = expand(a.x);
-      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, 2 * c + 1)) = expand(a.y);
-      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, 2 * c)) = expand(b.x);
-      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, 2 * c + 1)) = expand(b.y);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, 2 * c)) = expand(a.x, m);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, 2 * c + 1)) = expand(a.y, m);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, 2 * c)) = expand(b.x, m);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, 2 * c + 1)) = expand(b.y, m);
     } else {
-      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, c)) = expand(other ? raw.v[0].y : raw.v[0].x);
-      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, c)) = expand(other ? raw.v[0].x : raw.v[0].y);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 * other, c)) = expand(other ? raw.v[0].y : raw.v[0].x, m);
+      *reinterpret_cast<uint4*>(keys + chunk_at<D>(p + 2 - 2 * other, c)) = expand(other ? raw.v[0].x : raw.v[0].y, m);
     }
   }
 }
 template <int D>
 __device__ __forceinline__ void store_codes_of_values(const RawChunks<D>& raw, int lane, unsigned char* values) {
   if (D == 32 && lane >= 16) return;
+  const float mine = lane & 1 ? 7.0f : 8.0f, other = 15.0f - mine;  // by the parity of the positions 4 c + (i + turn) % 4
+  const CodeMiddle middle[2] = {code_middle(mine, mine), code_middle(other, other)};
   const int turn = lane & 3, c = (lane >> 2) & 3, r = D == 32 ? lane & 3 : (lane & 3) + 4 * (lane >> 4);
 #pragma unroll
   for (int k = 0; k < RawChunks<D>::n; ++k) {
@@ -183,7 +193,7 @@ __device__ __forceinline__ void store_codes_of_values(const RawChunks<D>& raw, i
     if (turn & 2) v = make_uint4(v.z, v.w, v.x, v.y);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(values + chunk_at<D>(4 * c + ((i + turn) & 3), 8 * k + r)) = expand(w[i]);
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(values + chunk_at<D>(4 * c + ((i + turn) & 3), 8 * k + r)) = expand(w[i], middle[i & 1]);
   }
 }
 
@@ -212,7 +222,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         int count = 1;
         if (A.starts != nullptr) count = max(0, min(A.rows, __ldg(A.starts + b + 1)) - max(0, __ldg(A.starts + b)));
         const int items = count * A.group;
-        n = items > few ? (items + kRowsCta - 1) / kRowsCta : 0;
+        n = items > few ? (items + G::rows - 1) / G::rows : 0;
       }
       int upto = n;
 #pragma unroll
@@ -265,7 +275,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     row0 = max(0, __ldg(A.starts + b));
     count = min(A.rows, __ldg(A.starts + b + 1)) - row0;
   }
-  const int i0 = which[1] * kRowsCta, live = min(kRowsCta, count * A.group - i0), row_tiles = live > kRowsX ? 2 : 1;
+  const int i0 = which[1] * G::rows, live = min(G::rows, count * A.group - i0), row_tiles = live > kRowsX ? 2 : 1;
   const int64_t base = __ldg(A.positions + b);
   const int max_len = A.cache.max_len;
   const unsigned group_size = static_cast<unsigned>(A.group);
@@ -429,7 +439,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         for (int k = 0; k < kMine; ++k) {
           const int u = unit0 + k * kProducerWarps;
           if (u < kUnits) {
-            const PositionTerms p = position_terms(par[k], score_unit, offset_unit, kWeightUnit);
+            const PositionTerms p = position_terms(par[k], score_unit, offset_unit, kWeightUnit, lane);
             float* at_terms = terms_of(it) + 12 * (8 * u + (lane >> 1)) + (lane & 1);
             at_terms[0] = p.key_scale;
             at_terms[2] = p.key_offset;
@@ -498,7 +508,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           for (int kk = 0; kk < kPos / 32; ++kk)
 #pragma unroll
             for (int part = 0; part < G::parts; ++part)
-              umma_f16_ts(t_o, t_p + part * (kPos / 4) + kk * 8, v + kk * 2 * (D / 8) * 8, idesc_f16_bt(kRowsX, D), kk + part > 0 || it + h > 0);
+              umma_f16_ts(t_o, t_p + part * (kPos / 4) + kk * 8, v + kk * 2 * (D / 8) * 8, idesc_f16_bt(kRowsX, D), kk + part > 0 || h > 0 || (kSplit ? it % kFoldTiles != 0 : it > 0));
           umma_commit(&bar.p_free[xx][h]);
         }
         if (h == 1) umma_commit(&bar.v_free[it % G::stages]);
@@ -532,7 +542,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     // shared memory pipe for 64 scores)
     const int r = lane >> 2, c = lane & 3, row0x = 32 * (warp & 3);
     const unsigned lanes = static_cast<unsigned>(row0x) << 16;
-    const unsigned ts = tmem + lanes + G::s_at + x * kPos, to = tmem + lanes + G::o_at + x * D;
+    const unsigned ts = tmem + lanes + G::s_at + x * kPos, to = tmem + lanes + G::o_at + x * D, tf = tmem + lanes + G::fold_at + x * D;
     float sum_q[4], refs[4];
     int at[4];
     f32x2 sum2[4], off2[4];
@@ -576,6 +586,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         }
         tc_fence_after();
         const unsigned th = ts + h * (kPos / 2);
+        if (kSplit && h == 0 && it > 0 && it % kFoldTiles == 0) {  // the next product begins anew
+          ok = mbar_wait_bounded(&bar.p_free[x][1], (it - 1) & 1, kPromptTimeout);
+          tc_fence_after();
+#pragma unroll 1
+          for (int c0 = 0; c0 < 2 * D; c0 += 32) {
+            const unsigned at_c = static_cast<unsigned>(c0 / 64 * 32) + (static_cast<unsigned>(c0 / 32 % 2 * 16) << 16);  // 32 columns of 16 rows
+            uint32_t o[16], f[16];
+            tmem_ld_16x256b_x4(to + at_c, o);
+            if (it > kFoldTiles) {
+              tmem_ld_16x256b_x4(tf + at_c, f);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float(f[j]));
+            }
+            tmem_st_16x256b_x4(tf + at_c, o);
+          }
+        }
         const float4* const t4 = reinterpret_cast<const float4*>(terms) + 3 * (32 * h + c);  // of the pair c; every fourth is ours
         if (none) {
           uint32_t zero[16];
@@ -647,18 +673,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
             ok = mbar_wait_bounded(&bar.p_free[x][h ^ 1], (it - (h ^ 1)) & 1, kPromptTimeout);
             tc_fence_after();
           }
-          if (it + h > 0) {
+          auto rescale = [&](unsigned from) {
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32)
 #pragma unroll
               for (int g = 0; g < 2; ++g) {
                 uint32_t o[16];
-                const unsigned at_o = to + c0 + (static_cast<unsigned>(16 * g) << 16);
+                const unsigned at_o = from + c0 + (static_cast<unsigned>(16 * g) << 16);
                 tmem_ld_16x256b_x4(at_o, o);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr[2 * g + ((j >> 1) & 1)]);
                 tmem_st_16x256b_x4(at_o, o);
               }
+          };
+          if (h > 0 || (kSplit ? it % kFoldTiles != 0 : it > 0)) rescale(to);
+          if (kSplit && it >= kFoldTiles) {
+            tmem_wait_st();
+            rescale(tf);
           }
         }
         f32x2 minus[4];  // a row that has seen nothing yet: its weights are 2^-inf
@@ -722,6 +753,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   const int row = tid & (kRowsCta - 1);
   const unsigned to = tmem + (static_cast<unsigned>(32 * (warp & 3)) << 16) + G::o_at + x * D;
   const bool mine = tid < kSoftmaxThreads && x < row_tiles;
+  auto load_o = [&](int c0, uint32_t (&o)[16]) {  // 16 channels of the row
+    tmem_ld16(to + c0, o);
+    if (kSplit && tiles > kFoldTiles) {
+      uint32_t f[16];
+      tmem_ld16(to + (G::fold_at - G::o_at) + c0, f);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float(f[j]));
+    }
+  };
   if (C == 1) {
     if (mine && ok) {
       // through the place of its tile's queries, to leave in whole 16-byte chunks: 32 rows a warp
@@ -731,7 +771,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 16) {
         uint32_t o[16];
-        if (tiles > 0) tmem_ld16(to + c0, o);
+        if (tiles > 0) load_o(c0, o);
 #pragma unroll
         for (int c = 0; c < 16 / kPer; ++c) {
           union {
@@ -773,7 +813,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 16) {
         uint32_t o[16];
-        if (tiles > 0 && ok) tmem_ld16(to + c0, o);
+        if (tiles > 0 && ok) load_o(c0, o);
 #pragma unroll
         for (int j = 0; j < 16; ++j) part[(c0 + j) * kRowsCta + row] = tiles > 0 ? __uint_as_float(o[j]) : 0.0f;
       }
@@ -838,7 +878,7 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   // as many tiles as the rows can make: each sequence of the call may leave one unfilled
   const int64_t items = static_cast<int64_t>(A.rows) * A.group;
   const int64_t sequences = std::min<int64_t>(A.cache.batch, items / (few + 1));
-  const int64_t tiles = items / kRowsCta + sequences;
+  const int64_t tiles = items / G::rows + sequences;
   if (sequences == 0) return IVB_OK;
   if (tiles * A.cache.kv_heads > 0x1fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(tiles));
   // a cluster where one CTA each would leave SMs without work
