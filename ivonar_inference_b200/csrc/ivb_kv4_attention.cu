@@ -44,15 +44,21 @@ __device__ __forceinline__ void cp_async_wait() {
 // one to four rows half the products of the other order are needed, and half its accumulators. Scores leave the
 // first product as positions x rows in the C layout; an 8x8 transposition (movmatrix) makes them the second one's B.
 // Columns hold, per tile of 8: kSplit 4 rows, each as the fp16 of its values and next to it the remainder's; else 8 rows.
-template <int D, bool kSplit, int kTiles>
+// fp32 outputs: the tensor cores cut what they add to an accumulator towards zero, so every 16 groups (512 positions) it is added to
+// its sums in shared memory, rounding to nearest, and begins anew.
+constexpr int kFoldSteps = 16;
+
+template <int D, typename T, bool kSplit, int kTiles>
 struct RowsGeometry {
+  static constexpr bool fold = std::is_same<T, float>::value;
   static constexpr int rows = (kSplit ? 4 : 8) * kTiles;
   static constexpr int stages = D == 128 ? 2 : 3;
   static constexpr int group_bytes = kKv4Group * (D + 8);
   static constexpr int warp_bytes = stages * group_bytes;
   static constexpr int comb_floats = rows * D + 3 * rows;
   static constexpr int term_bytes = kKv4Group * 24;  // a float4 and a float2 for each position
-  static constexpr int smem(int warps) { return warps * (warp_bytes + term_bytes + rows * 12) + comb_floats * 4; }
+  static constexpr int fold_bytes = fold ? rows * D * 4 : 0;
+  static constexpr int smem(int warps) { return warps * (warp_bytes + term_bytes + rows * 12 + fold_bytes) + comb_floats * 4; }
 };
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -63,7 +69,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 
 template <int D, typename T, bool kSplit, int kTiles>
 __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int tiles_per_sequence) {
-  using G = RowsGeometry<D, kSplit, kTiles>;
+  using G = RowsGeometry<D, T, kSplit, kTiles>;
   constexpr int R = G::rows, kSteps = D / 16, kTile = kv4_tile_bytes(D);
   constexpr int kPer = kSplit ? 1 : 2;        // rows of a lane in a column tile
   constexpr int kSets = kPer * kTiles;        // rows of a lane
@@ -77,6 +83,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
   float2* const terms2 = reinterpret_cast<float2*>(terms4 + kKv4Group);
   float* const comb = reinterpret_cast<float*>(smem + W * (G::warp_bytes + G::term_bytes));  // [R][D], then ref, sum, offset [R]
   float* const stats = comb + G::comb_floats;                                               // [W][R][3]
+  float* const folded = stats + W * R * 3 + warp * R * D;                                    // [R][D], fp32 outputs only
 
   // which rows (rows x heads is below 2^31)
   const unsigned cluster_id = blockIdx.x / static_cast<unsigned>(C), group_size = static_cast<unsigned>(A.group);
@@ -199,6 +206,42 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
     ref[s] = -INFINITY;
     sum[s] = off[s] = 0.0f;
   }
+
+  constexpr int kPlanes = D == 128 ? 2 : 1, kRun = D == 32 ? 4 : 8;  // channels of a lane in a plane of 64 (or 32)
+  // channel of value j: D = 32: 8 (r / 2) + r % 2 + 2 j, else 64 plane + 8 r + j
+  auto channel = [&](int h, int j) { return D == 32 ? 8 * (r >> 1) + (r & 1) + 2 * j : 64 * h + 8 * r + j; };
+  float o[kSets][kPlanes][kRun];
+  float folded_ref[kSets];  // the reference that the sums in shared memory stand at, -inf: none yet
+#pragma unroll
+  for (int s = 0; s < kSets; ++s) folded_ref[s] = -INFINITY;
+  bool any_folded = false;
+  // the accumulators joined with what was folded before: into o at the end, into shared memory (each lane its own places) else
+  auto fold = [&](bool last) {
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) {
+      const float f = folded_ref[s] == -INFINITY ? 0.0f : ex2(folded_ref[s] - ref[s]);
+#pragma unroll
+      for (int h = 0; h < kPlanes; ++h)
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          const int i = 4 * h + (j >> 1), e = 2 * (j & 1);
+          float v;
+          if constexpr (kSplit) v = acc[s][i][e] + acc[s][i][e + 1];
+          else v = acc[s >> 1][i][e + (s & 1)];
+          v *= 0.00006103515625f;  // the weights' 2^14
+          if (any_folded) v = fmaf(folded[row_of(s) * D + channel(h, j)], f, v);
+          if (last) o[s][h][j] = v;
+          else folded[row_of(s) * D + channel(h, j)] = v;
+        }
+      folded_ref[s] = ref[s];
+    }
+    if (last) return;
+    any_folded = true;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int i = 0; i < kOut; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.0f;
+  };
 
   const CodeMiddle key_middle = code_middle(8.0f, 8.0f), value_middle = code_middle(8.0f, 7.0f);  // halves: channels, positions
   int at_stage = 0, to_stage = G::stages - 1;
@@ -368,6 +411,8 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
       }
     }
     __syncwarp();
+    if constexpr (G::fold)
+      if (step % kFoldSteps == kFoldSteps - 1 && step + 1 < steps) fold(false);
     issue(step + G::stages - 1, to_stage);
     at_stage = at_stage + 1 == G::stages ? 0 : at_stage + 1;
     to_stage = to_stage + 1 == G::stages ? 0 : to_stage + 1;
@@ -383,20 +428,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
       sum[s] += __shfl_xor_sync(0xFFFFFFFFu, sum[s], d);
       off[s] += __shfl_xor_sync(0xFFFFFFFFu, off[s], d);
     }
-  constexpr int kPlanes = D == 128 ? 2 : 1, kRun = D == 32 ? 4 : 8;  // channels of a lane in a plane
-  float o[kSets][kPlanes][kRun];
-#pragma unroll
-  for (int s = 0; s < kSets; ++s)
-#pragma unroll
-    for (int h = 0; h < kPlanes; ++h)
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        const int i = 4 * h + (j >> 1), e = 2 * (j & 1);
-        const float v = kSplit ? acc[s][i][e] + acc[s][i][e + 1] : acc[s >> 1][i][e + (s & 1)];
-        o[s][h][j] = v * 0.00006103515625f;  // the weights' 2^14
-      }
-  // channel of value j: D = 32: 8 (r / 2) + r % 2 + 2 j, else 64 plane + 8 r + j
-  auto channel = [&](int h, int j) { return D == 32 ? 8 * (r >> 1) + (r & 1) + 2 * j : 64 * h + 8 * r + j; };
+  fold(true);
   auto place = [&](int row) {
     const int t = token_of(i0 + row);
     return static_cast<T*>(A.out) + (row0 + t) * A.o_row + (kvh * A.group + i0 + row - t * A.group) * A.o_head;
@@ -500,7 +532,7 @@ int32_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
 
 template <int D, typename T, bool kSplit, int kTiles>
 int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
-  using G = RowsGeometry<D, kSplit, kTiles>;
+  using G = RowsGeometry<D, T, kSplit, kTiles>;
   constexpr int kMostWarps = 8;
   static std::atomic<uint64_t> done{0};
   if (int32_t rc = allow_smem(kv4_rows_kernel<D, T, kSplit, kTiles>, G::smem(kMostWarps), done)) return rc;
