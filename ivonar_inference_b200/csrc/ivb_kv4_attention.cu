@@ -18,7 +18,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kFewItems = 32;  // tokens x query heads of a group
+// Sequences of up to so many items (tokens x query heads of a group) are for the kernel of few rows, which splits a history over
+// more of the GPU; the others for the prompts' one, which reads it once for 256 items. Measured (rows / prompts): where the
+// prompts' clusters fill the GPU, 8 items 50 / 86 us and 16 items 92 / 89 (16 sequences, 16 heads x 64, 2000 positions, fp32), 32 items
+// 70 / 57 (8 sequences, 8 heads x 128, 4000 positions, bf16); where they do not, 32 items 119 / 151 and 64 items 194 / 152 (2
+// sequences, 8 heads x 128, 30000 positions, bf16), 32 items 87 / 177 and 64 items 199 / 178 (8 heads x 64, fp32).
+constexpr int kFewItems = 16, kFewItemsSparse = 48;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -146,7 +151,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
   // largest to 2^13
   uint32_t qf[kTiles][kSteps][2];
   float sum_q[kSets];
-  float score_unit, offset_unit;
+  float score_unit;
   {
     float qv[kTiles][D / 4];
     float amax = 0.0f, total[kTiles];
@@ -175,10 +180,11 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
     for (int s = 0; s < kSets; ++s)  // from the lanes that hold the row as a column
       sum_q[s] = __shfl_sync(0xFFFFFFFFu, total[kSplit ? s : s >> 1], kSplit ? 8 * c : 4 * (2 * c + (s & 1)));
     int up = 13 - (static_cast<int>(__float_as_uint(amax) >> 23) - 127);
-    up = amax == 0.0f ? 0 : min(max(up, -100), 100);
+    up = amax == 0.0f ? 0 : min(max(up, -114), 100);
     const float q_unit = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-    offset_unit = A.scale * kLog2e;
-    score_unit = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * offset_unit;
+    score_unit = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * (A.scale * kLog2e);
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) sum_q[s] *= q_unit;
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
@@ -252,7 +258,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
     const int p0 = group_of(step) * kKv4Group;
     {
       const uint2 par = *reinterpret_cast<const uint2*>(stage + (lane >> 4) * kTile + 16 * D + (lane & 15) * 8);
-      const PositionTerms t = position_terms(par, score_unit, offset_unit, 16384.0f, lane);
+      const PositionTerms t = position_terms(par, score_unit, 16384.0f, lane);
       terms4[lane] = make_float4(t.key_scale, t.key_offset, t.bias, t.mantissa);
       terms2[lane] = make_float2(t.unbias, t.value_offset);
     }
@@ -539,6 +545,10 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   const int64_t most = std::min<int64_t>(A.few, static_cast<int64_t>(A.starts == nullptr ? 1 : A.rows) * A.group);
   const int64_t tiles = (most + G::rows - 1) / G::rows;
   const int64_t base = tiles * A.cache.kv_heads * A.cache.batch;
+  // Warps a row tile by what fills the GPU twice over, then clusters where eight do not fill it once and leave each warp more than
+  // four groups at the cache's capacity (a cluster costs 1.4 us). Measured with 1, 2, 4, 8 warps: 4096 tiles at positions
+  // 128-640 51, 41, 49, 74 us; 1024 tiles at 300-1900 51, 36, 34, 38; 256 tiles of 1028 positions x 128 50, 30, 21, 17; 32 tiles
+  // of 30000 x 128 with 8 warps, clusters of 1 and 8: 203 and 42.
   const int64_t slots = 148 * 16;  // warps of this kernel that the GPU holds
   int W = 1, C = 1;
   while (W < kMostWarps && base * W < 2 * slots && A.cache.max_len > W * kKv4Group) W *= 2;
@@ -621,9 +631,11 @@ extern "C" int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_
   A.q_vec = aligned(q, q_row, q_head);
   A.o_vec = aligned(out, o_row, o_head);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // sequences of more than `few` items go to the prompt kernel; a lone sequence all of its rows, if it can have so many
   const int64_t items = static_cast<int64_t>(rows) * A.group;
-  A.few = starts == nullptr || items <= kFewItems ? 0x7fffffff : c->batch == 1 ? 0 : kFewItems;
+  const int64_t tiles = items / 256 + std::min<int64_t>(c->batch, items / (kFewItems + 1));
+  const int few = tiles * c->kv_heads * 4 >= 148 ? kFewItems : kFewItemsSparse;
+  // a lone sequence that can have more takes the prompts' kernel however many it has: one launch
+  A.few = starts == nullptr || items <= few ? 0x7fffffff : c->batch == 1 ? 0 : few;
   if (A.few != 0x7fffffff)
     if (int32_t rc = launch_kv4_prompts(A, dtype, A.few, s)) return rc;
   if (A.few == 0) return IVB_OK;

@@ -71,7 +71,8 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t w, CodeMiddle m) {
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 
-// What the softmax needs of one position: x = S key_scale + sum(q) key_offset + bias, with bias the exponent of the value
+// What the softmax needs of one position: x = S key_scale + sum(q) key_offset + bias (S and sum(q) of the queries as the operands hold
+// them, a power of two apart: score_unit undoes it), with bias the exponent of the value
 // scale, so that the running reference is the maximum of weight times value scale and neither overflows fp16, whatever the
 // scales; the weight is then 2^(x - ref) = p 2^bias, its product with the mantissa the A operand of the value product, and
 // p = weight * unbias enters the sum. A position whose value scale or offset is no number has a score that is none, and
@@ -81,11 +82,11 @@ struct PositionTerms {
   float unbias, value_offset;                   // 2^-bias, value offset times 2^-bias (offsets are of the middle)
 };
 
-__device__ __forceinline__ PositionTerms position_terms(uint2 par, float score_unit, float offset_unit, float weight_unit, int position) {
+__device__ __forceinline__ PositionTerms position_terms(uint2 par, float score_unit, float weight_unit, int position) {
   const float2 key = unpack_f16(par.x), value = unpack_f16(par.y);
   PositionTerms t;
   t.key_scale = key.x * score_unit;
-  t.key_offset = fmaf(8.0f, key.x, key.y) * offset_unit;
+  t.key_offset = fmaf(8.0f, key.x, key.y) * score_unit;
   const bool number = (par.y & 0x7c00u) != 0x7c00u && (par.y & 0x7c000000u) != 0x7c000000u;
   const uint32_t e = max(__float_as_uint(value.x) & 0x7f800000u, 0x33800000u);  // 2^-24 is the least scale above zero
   t.bias = number ? static_cast<float>(static_cast<int>(e >> 23) - 127) : __uint_as_float(0x7fffffffu);

@@ -363,11 +363,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll
   for (int w = 0; w < kSoftmaxWarps; ++w) most = fmaxf(most, largest[w]);
   int up = 13 - (static_cast<int>(__float_as_uint(most) >> 23) - 127);
-  up = most == 0.0f ? 0 : min(max(up, -100), 100);
-  const float offset_unit = A.scale * kLog2e;
-  const float score_unit = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * offset_unit;
+  up = most == 0.0f ? 0 : min(max(up, -114), 100);
+  const float q_unit = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+  const float score_unit = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * (A.scale * kLog2e);
   if (tid < kSoftmaxThreads && x < row_tiles) {
-    const float unit = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
     unsigned char* dst = smem + G::q_at + x * G::parts * G::q_bytes;
 #pragma unroll
     for (int g = 0; g < 4; ++g)
@@ -379,7 +378,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         uint32_t hi[kPer / 2], lo[kPer / 2];
 #pragma unroll
         for (int j = 0; j < kPer / 2; ++j) {
-          const float a = v[2 * j] * unit, c = v[2 * j + 1] * unit;
+          const float a = v[2 * j] * q_unit, c = v[2 * j + 1] * q_unit;
           hi[j] = pack_f16(a, c);
           const float2 h = unpack_f16(hi[j]);
           lo[j] = pack_f16(a - h.x, c - h.y);
@@ -439,7 +438,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         for (int k = 0; k < kMine; ++k) {
           const int u = unit0 + k * kProducerWarps;
           if (u < kUnits) {
-            const PositionTerms p = position_terms(par[k], score_unit, offset_unit, kWeightUnit, lane);
+            const PositionTerms p = position_terms(par[k], score_unit, kWeightUnit, lane);
             float* at_terms = terms_of(it) + 12 * (8 * u + (lane >> 1)) + (lane & 1);
             at_terms[0] = p.key_scale;
             at_terms[2] = p.key_offset;
@@ -551,7 +550,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = kRowsX * x + row0x + 8 * i + r;
-      sum_q[i] = sums[n];
+      sum_q[i] = sums[n] * q_unit;
       at[i] = -1;
       if (n < live) {
         const int p = clamp_position(base + token_of(i0 + n));
@@ -881,7 +880,8 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   const int64_t tiles = items / G::rows + sequences;
   if (sequences == 0) return IVB_OK;
   if (tiles * A.cache.kv_heads > 0x1fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(tiles));
-  // a cluster where one CTA each would leave SMs without work
+  // a cluster where one CTA each would leave SMs without work (128 CTAs of a 2048-row causal prompt: 72 us, in pairs 58; 256 CTAs
+  // of a chunk under a window: 262, in pairs 309)
   int C = 1;
   while (C < 4 && tiles * A.cache.kv_heads * C < 148 && A.cache.max_len > 2 * C * kPos) C *= 2;
   cudaLaunchConfig_t cfg = {};

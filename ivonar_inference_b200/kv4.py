@@ -74,12 +74,16 @@ class KV4Cache:
         return KV4Cache(1, self.kv_heads, self.head_dim, self.max_len, data=self.data[index:index + 1], error=self.error)
 
     def check(self) -> None:
-        """Wait for the device and raise ValueError if a call since the last check met a row beyond the capacity."""
+        """Wait for the device; raises ValueError if a call since the last check met a row beyond the capacity, and KernelError
+        if a wait inside a kernel ran out (its rows' outputs are then not to be used)."""
 
         if self.error is None:
             raise RuntimeError("this cache was made without an error word")
-        if int(self.error.item()) != 0:
+        code = int(self.error.item())
+        if code != native.IVB_OK:
             self.error.zero_()
+            if code != native.IVB_ECAPACITY:
+                raise native.KernelError(f"the 4-bit attention reported error {code}")
             raise ValueError(f"a row lies beyond the cache's capacity of {self.max_len} positions")
 
     # ------------------------------------------------------------------------------------------

@@ -425,6 +425,121 @@ def test_offsets_beyond_32_bits() -> None:
     cache.check()
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim,batch,first,counts,group,window,sinks", [
+    (64, 1, 600, [700], 2, 0, 0),          # one sequence, few tiles: clusters of four
+    (128, 1, 0, [530], 1, 0, 0),
+    (32, 1, 1000, [290], 4, 300, 70),
+    (64, 4, 3, [513, 16, 17, 129], 1, 0, 0),
+    (128, 3, 290, [257, 49, 1], 1, 100, 5),
+    (64, 24, 0, [130, 3] * 12, 2, 33, 0),  # many tiles: one CTA each
+])
+def test_long_prompts(dim, batch, first, counts, group, window, sinks, dtype) -> None:
+    """Prompts over more than one tile of rows and many of positions, with accumulators that are folded, against 64 bits."""
+    from ivonar_inference_b200 import KV4Cache
+
+    T, Hkv = TYPES[dtype], 2
+    cache = KV4Cache(batch, Hkv, dim, first + max(counts) + 3)
+    total = [first + n for n in counts]
+    filled(cache, total, seed=dim + batch)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    q = (torch.randn(sum(counts), Hkv * group, dim, generator=gen, device="cuda") * 1.5).to(T)
+    at, starts = rows_of(batch, [first] * batch, counts)
+    got = cache.attention(q, at, starts, window=window, sinks=sinks)
+    cache.check()
+    k, v, par = contents(cache.data, dim)
+    bounds = starts.tolist()
+    for b in sorted({0, batch // 2, batch - 1}):
+        n, L = counts[b], total[b]
+        where, mine = torch.arange(L), torch.arange(first, L)[:, None]
+        hidden = where > mine
+        if window:
+            hidden |= (where <= mine - window) & (where >= sinks)
+        x = q[bounds[b]:bounds[b + 1]].double().cpu().unflatten(1, (Hkv, group))
+        score = torch.einsum("nhgd,hjd->hgnj", x, k[b, :, :L]) * dim**-0.5
+        weight = torch.softmax(score.masked_fill(hidden, -math.inf), -1)
+        want = torch.einsum("hgnj,hjd->nhgd", weight, v[b, :, :L]).flatten(1, 2)
+        most = float((par[b, :, :L, 1].abs() + 15 * par[b, :, :L, 0]).max())
+        tol = tolerance(q[bounds[b]:bounds[b + 1]], most, float(v[b, :, :L].abs().max()), dim**-0.5, want, T)
+        diff = (got[bounds[b]:bounds[b + 1]].double().cpu() - want).abs()
+        assert bool((diff <= tol).all()), (b, float(diff.max()))
+        if T == torch.float32:
+            # what folding is for: without it the error of the whole grows with the history, with it it stays near that of
+            # 32-bit products (2^-24 a rounding, a chain of 2^5 products before each fold, cut towards zero: 2^-20)
+            assert float(diff.norm() / want.norm()) < 2.0**-18
+
+
+def test_long_histories_keep_fp32() -> None:
+    """Many sequences, so that one warp walks many groups and folds its accumulators: the error stays that of 32-bit sums."""
+    from ivonar_inference_b200 import KV4Cache
+
+    for batch, heads, dim, length in ((600, 4, 64, 1500), (300, 8, 32, 1700), (300, 8, 128, 1300)):
+        cache = KV4Cache(batch, heads, dim, length)
+        filled(cache, [length] * batch, seed=dim)
+        gen = torch.Generator(device="cuda").manual_seed(9)
+        for group in (1, 6):
+            q = torch.randn(batch, heads * group, dim, generator=gen, device="cuda")
+            got = cache.attention(q, torch.full((batch,), length - 1, device="cuda"))
+            for b in (0, batch - 1):
+                k, v, _ = contents(cache.data[b:b + 1], dim)
+                x = q[b].double().cpu().unflatten(0, (heads, group))
+                weight = torch.softmax(torch.einsum("hgd,hjd->hgj", x, k[0, :, :length]) * dim**-0.5, -1)
+                want = torch.einsum("hgj,hjd->hgd", weight, v[0, :, :length]).flatten(0, 1)
+                assert float((got[b].double().cpu() - want).norm() / want.norm()) < 2.0**-18
+
+
+def test_a_visible_nan_reaches_its_rows_only_in_prompts() -> None:
+    from ivonar_inference_b200 import KV4Cache
+
+    for dtype in TYPES.values():
+        cache = KV4Cache(2, 2, 64, 400)
+        filled(cache, [400, 400])
+        x = torch.randn(2, 2, 64, device="cuda")
+        x[0, 1, 5] = math.nan                       # the key of sequence 0, head 1, and the value of sequence 1, head 0
+        y = torch.randn(2, 2, 64, device="cuda")
+        y[1, 0, 7] = math.inf
+        cache.append(x, y, torch.tensor([200, 200], device="cuda"))
+        q = torch.randn(400, 4, 64, device="cuda").to(dtype)
+        q[350, 3, 0] = math.inf
+        at, starts = rows_of(2, [100, 100], [200, 200])
+        got = cache.attention(q, at, starts)
+        bad = torch.zeros(400, 4, dtype=torch.bool)
+        bad[100:200, 2:] = True                     # rows at positions 200 .. 299 of sequence 0
+        bad[300:400, :2] = True
+        bad[350, 3] = True
+        assert torch.equal(got.isnan().all(-1).cpu(), bad) and torch.equal(got.isnan().any(-1).cpu(), bad)
+        got = cache.attention(q, at, starts, window=50)
+        assert bool(torch.isfinite(got[160:200]).all()) and bool(got[100:150, 2:].isnan().all()) and bool(torch.isfinite(got[100:150, :2]).all())
+
+
+def test_large_and_small_queries() -> None:
+    from ivonar_inference_b200 import KV4Cache
+
+    cache = KV4Cache(1, 1, 64, 300)
+    filled(cache, [300])
+    q = torch.randn(40, 1, 64, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    at, starts = rows_of(1, [260], [40])
+    want = cache.attention(q, at, starts, scale=0.125)
+    for size in (2.0**120, 2.0**-60):
+        # the queries' power of two comes off exactly, and the scale's product with log2 e is rounded alike
+        assert torch.equal(cache.attention(q * size, at, starts, scale=0.125 / size), want)
+        one = cache.attention(q[39:], at + 39, scale=0.125)
+        assert torch.equal(cache.attention(q[39:] * size, at + 39, scale=0.125 / size), one)
+
+
+def test_expanded_inputs() -> None:
+    from ivonar_inference_b200 import KV4Cache
+
+    cache = KV4Cache(3, 2, 64, 40)
+    x = torch.randn(1, 1, 64, device="cuda").expand(3, 2, 64)
+    at = torch.tensor([3, 3, 3], device="cuda")
+    cache.append(x, x, at)
+    k, v = cache.read(at)
+    assert torch.equal(k.cpu(), held(x).float()) and torch.equal(v, k)
+    q = torch.randn(1, 4, 64, device="cuda")
+    assert torch.equal(cache.attention(q.expand(3, 4, 64), at), cache.attention(q.repeat(3, 1, 1), at))
+
+
 # ---- as they are used ---------------------------------------------------------------------------
 def test_a_prompt_and_steps_together() -> None:
     """Prompts of several sequences written and attended to in one call, then single tokens: every output against 64 bits over
