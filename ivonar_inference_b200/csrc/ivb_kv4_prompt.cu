@@ -47,7 +47,8 @@ struct PromptGeometry {
   static constexpr int kv_bytes = kPos * D * 2;              // keys or values of a stage
   static constexpr int term_bytes = kPos * 24;
   static constexpr int q_at = 0, k_at = (kSplit && D == 128 ? 1 : 2) * parts * q_bytes, v_at = k_at + stages * kv_bytes, terms_at = v_at + stages * kv_bytes;
-  static constexpr int smem = terms_at + kTermSets * term_bytes;
+  // over half of an SM's at least: of two clusters sharing two SMs each could hold the tensor memory that the other waits for
+  static constexpr int used = terms_at + kTermSets * term_bytes, smem = used < 118 * 1024 ? 118 * 1024 : used;
   // row tiles of a CTA: at fp32 and D = 128 tensor memory holds the accumulators of one
   static constexpr int row_tiles = kSplit && D == 128 ? 1 : 2, rows = row_tiles * kRowsX;
   // tensor memory columns: S_X, then P_X in its place (of every 64 columns 32 hi, 32 lo), O_X, and O_X's sums (fp32)

@@ -59,6 +59,7 @@ class KV4Cache:
         self.data, self.error, self.device = data, error, data.device
         self._error = 0 if error is None else error.data_ptr()
         self._index = data.device.index
+        self._sequences = (self.batch,)
         self._desc = native.IvbKv4Cache(data.data_ptr(), self.batch, self.kv_heads, self.head_dim, self.max_len)
         self._ref = ctypes.byref(self._desc)
 
@@ -90,27 +91,34 @@ class KV4Cache:
     def _rows(self, rows: int, positions: Tensor, starts: Tensor | None) -> int:
         """Checks of what names the rows; the device address of `starts`."""
 
-        if positions.dtype != torch.int64 or positions.shape != (self.batch,) or positions.device != self.device or not positions.is_contiguous():
+        if (positions.dtype is not torch.int64 or positions.shape != self._sequences or positions.device != self.device
+                or not positions.is_contiguous()):
             raise ValueError(f"positions must be an int64 tensor [{self.batch}] on {self.device}")
         if starts is None:
             if rows != self.batch:
                 raise ValueError(f"{rows} rows for {self.batch} sequences need starts")
             return 0
-        if starts.dtype != torch.int32 or starts.shape != (self.batch + 1,) or starts.device != self.device or not starts.is_contiguous():
+        if (starts.dtype is not torch.int32 or starts.shape != (self.batch + 1,) or starts.device != self.device
+                or not starts.is_contiguous()):
             raise ValueError(f"starts must be an int32 tensor [{self.batch + 1}] on {self.device}")
         return starts.data_ptr()
 
-    def _values(self, name: str, x: Tensor, heads: int, dtype: torch.dtype | None = None) -> None:
-        if x.ndim != 3 or x.shape[1] != heads or x.shape[2] != self.head_dim:
-            raise ValueError(f"{name} must have shape [rows, {heads}, {self.head_dim}], not {list(x.shape)}")
-        if x.dtype not in _TYPES or (dtype is not None and x.dtype != dtype):
+    def _values(self, name: str, x: Tensor, heads: int, dtype: torch.dtype | None = None) -> tuple[int, int]:
+        """Checks of rows of values; their strides (row, head)."""
+
+        shape = x.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim:
+            raise ValueError(f"{name} must have shape [rows, {heads}, {self.head_dim}], not {list(shape)}")
+        if x.dtype not in _TYPES or (dtype is not None and x.dtype is not dtype):
             raise ValueError(f"{name} has type {x.dtype}" + ("" if dtype is None else f", not {dtype}"))
         if x.device != self.device:
             raise ValueError(f"{name} lies on {x.device}, the cache on {self.device}")
-        if x.stride(2) != 1:
+        row, head, channel = x.stride()
+        if channel != 1:
             raise ValueError(f"the channels of {name} must be contiguous")
         if x.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires a gradient: the 4-bit cache has none")
+        return row, head
 
     def _call(self, what: str, function, *args) -> None:
         index = self._index
@@ -128,14 +136,14 @@ class KV4Cache:
         A row that holds an infinity or a NaN reads back as NaN; values beyond +-65504 are clipped.
         """
 
-        self._values("k", k, self.kv_heads)
-        self._values("v", v, self.kv_heads, k.dtype)
+        k_row, k_head = self._values("k", k, self.kv_heads)
+        v_row, v_head = self._values("v", v, self.kv_heads, k.dtype)
         rows = k.shape[0]
         if v.shape[0] != rows:
             raise ValueError(f"{rows} rows of keys and {v.shape[0]} of values")
         at = self._rows(rows, positions, starts)
-        self._call("ivb_kv4_append", self.lib.ivb_kv4_append, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], k.stride(0),
-                   k.stride(1), v.stride(0), v.stride(1), at, positions.data_ptr(), rows)
+        self._call("ivb_kv4_append", self.lib.ivb_kv4_append, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], k_row, k_head, v_row,
+                   v_head, at, positions.data_ptr(), rows)
 
     def read(self, positions: Tensor, starts: Tensor | None = None, rows: int | None = None, dtype: torch.dtype = torch.float32,
              out: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
@@ -181,21 +189,22 @@ class KV4Cache:
         heads = q.shape[1] if q.ndim == 3 else 0
         if heads == 0 or heads % self.kv_heads != 0:
             raise ValueError(f"q must have shape [rows, a multiple of {self.kv_heads}, {self.head_dim}]")
-        self._values("q", q, heads)
+        q_row, q_head = self._values("q", q, heads)
+        rows = q.shape[0]
         if window < 0 or sinks < 0 or window >= 2**31 or sinks >= 2**31:
             raise ValueError("window and sinks must not be negative")
         if out is None:
             out = torch.empty_like(q)
+            o_row, o_head, _ = out.stride()
         else:
-            self._values("out", out, heads, q.dtype)
-            if out.shape[0] != q.shape[0]:
+            o_row, o_head = self._values("out", out, heads, q.dtype)
+            if out.shape[0] != rows:
                 raise ValueError("out and q disagree")
             _writable(out)
-        rows = q.shape[0]
         at = self._rows(rows, positions, starts)
-        self._call("ivb_kv4_attention", self.lib.ivb_kv4_attention, self._ref, q.data_ptr(), _TYPES[q.dtype], q.stride(0), q.stride(1),
-                   heads, at, positions.data_ptr(), rows, self.head_dim**-0.5 if scale is None else scale, window, sinks,
-                   out.data_ptr(), out.stride(0), out.stride(1))
+        self._call("ivb_kv4_attention", self.lib.ivb_kv4_attention, self._ref, q.data_ptr(), _TYPES[q.dtype], q_row, q_head, heads,
+                   at, positions.data_ptr(), rows, self.head_dim**-0.5 if scale is None else scale, window, sinks, out.data_ptr(), o_row,
+                   o_head)
         return out
 
 

@@ -49,6 +49,15 @@ def test_the_c_entry_points_refuse_bad_arguments() -> None:
         assert rc == native.IVB_OK, name
 
 
+def test_the_struct_matches_the_c_layout() -> None:
+    from ivonar_inference_b200 import _native as native
+
+    # pointer, then four int32 (include/ivonar_b200.h)
+    assert ctypes.sizeof(native.IvbKv4Cache) == 24
+    assert [getattr(native.IvbKv4Cache, f).offset for f, _ in native.IvbKv4Cache._fields_] == [0, 8, 12, 16, 20]
+    assert [f for f, _ in native.IvbKv4Cache._fields_] == ["data", "batch", "kv_heads", "head_dim", "max_len"]
+
+
 def test_sizes() -> None:
     from ivonar_inference_b200 import _native as native
 
