@@ -76,32 +76,13 @@ __device__ __forceinline__ uint4 expand(uint32_t w, CodeMiddle m) {
   return make_uint4(codes_low(w, m), codes_high(w, m), codes_low(w >> 8, m), codes_high(w >> 8, m));
 }
 
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pair(float a, float b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(f32x2 a) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
+// Two fp32 operations in one instruction.
+typedef float2 f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) { return make_float2(a, b); }
+__device__ __forceinline__ float2 unpair(f32x2 a) { return a; }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { return __fadd2_rn(a, b); }
 
 template <typename T>
 __device__ __forceinline__ void values_of_chunk(uint4 w, float (&v)[16 / sizeof(T)]) {
