@@ -5,7 +5,8 @@
 //   warps 8..10 (producers) read the codes, expand them to fp16 in shared memory (keys as a K-major operand, values as an
 //     MN-major one: both are position rows of 16-byte channel chunks, so neither is transposed) and compute each
 //     position's terms (scales and offsets; ivb_kv4_attention.cuh);
-//   warp 11 (one thread, whose instructions come slowly beside the softmax's: no more of them than needed) issues S_X = Q_X U^T and O_X += P_X U'^T, fp32 in tensor memory;
+//   warp 11 (whose instructions come slowly beside the softmax's: no more of them than needed) issues S_X = Q_X U^T and
+//     O_X += P_X U'^T, fp32 in tensor memory;
 //   warps 0..7 (32 rows each, their tensor-memory lanes) turn S_X into weights: online softmax in 32 bits, the
 //     reference raised only when the maximum passes it by 2^8, and O_X rescaled in tensor memory then. The weights P_X take
 //     S_X's place as the fp16 A operand, so S_X(it + 1) follows P_X(it)'s product; while one X waits for it the other computes.
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   __shared__ unsigned tmem_base;
   __shared__ float largest[kSoftmaxWarps], sums[kRowsCta], refs_of[kRowsCta], totals[kRowsCta], offsets[kRowsCta];
   __shared__ int which[3];  // sequence, tile of its rows; and whether a wait ran out
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
   // which rows: the call's tiles of 256 items in the order of the sequences, the last ones (the longest rows) first
   cg::cluster_group cluster = cg::this_cluster();
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const unsigned tmem = tmem_base;
+  const unsigned tmem = __shfl_sync(0xFFFFFFFFu, tmem_base, 0);
   auto keys_of = [&](int it) { return smem + G::k_at + it % G::stages * G::kv_bytes; };
   auto values_of = [&](int it) { return smem + G::v_at + it % G::stages * G::kv_bytes; };
   auto terms_of = [&](int it) { return reinterpret_cast<float*>(smem + G::terms_at + it % kTermSets * G::term_bytes); };
@@ -453,69 +454,68 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       mbar_arrive(&bar.v_full[it % G::stages]);
     }
   } else if (warp >= kIssueWarp) {
-    // ---- the thread that issues the products ----
-    if (lane == 0) {
-      const uint64_t q0 = smem_desc(smem_addr(smem + G::q_at), D / 8 * 128);
-      const uint64_t k0 = smem_desc(smem_addr(smem + G::k_at), D / 8 * 128), v0 = smem_desc_mn(smem_addr(smem + G::v_at), D / 8 * 128);
-      // Half h of tile it: its 64 columns of S_X, and with P_X in their place its 64 positions' part of O_X. Descriptors count
-      // in 16 bytes.
-      auto issue_s = [&](int it, int h) {
-        const uint64_t k = k0 + (it % G::stages * G::kv_bytes + h * (G::kv_bytes / 2)) / 16;
-        for (int xx = 0; xx < row_tiles; ++xx) {
-          if (it > 0) {  // S takes the place of P
-            ok = ok && mbar_wait_bounded(&bar.p_free[xx][h], (it - 1) & 1, kPromptTimeout);
-            if (!ok) return;
-          }
-          tc_fence_after();
-          const uint64_t q = q0 + xx * (G::parts * G::q_bytes / 16);
-          const unsigned t_s = tmem + G::s_at + xx * kPos + h * (kPos / 2);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-#pragma unroll
-            for (int part = 0; part < G::parts; ++part)
-              umma_f16_ss(t_s, q + (part * G::q_bytes + kk * 256) / 16, k + kk * 16, idesc_f16(kRowsX, kPos / 2), kk + part > 0);
-          umma_commit(&bar.s_full[xx][h]);
-        }
-        if (h == 1) umma_commit(&bar.k_free[it % G::stages]);
-      };
-      auto issue_o = [&](int it, int h) {
-        const uint64_t v = v0 + (it % G::stages * G::kv_bytes + h * (G::kv_bytes / 2)) / 16;
-        for (int xx = 0; xx < row_tiles; ++xx) {
-          ok = ok && mbar_wait_bounded(&bar.p_full[xx][h], it & 1, kPromptTimeout);
+    // ---- the warp that issues the products: all its lanes take the same way (ok is the same in each) ----
+    auto wait = [&](unsigned long long* at, unsigned turn) { return __all_sync(0xFFFFFFFFu, mbar_wait_bounded(at, turn, kPromptTimeout)) != 0; };
+    const uint64_t q0 = smem_desc(smem_addr(smem + G::q_at), D / 8 * 128);
+    const uint64_t k0 = smem_desc(smem_addr(smem + G::k_at), D / 8 * 128), v0 = smem_desc_mn(smem_addr(smem + G::v_at), D / 8 * 128);
+    // Half h of tile it: its 64 columns of S_X, and with P_X in their place its 64 positions' part of O_X. Descriptors count
+    // in 16 bytes.
+    auto issue_s = [&](int it, int h) {
+      const uint64_t k = k0 + (it % G::stages * G::kv_bytes + h * (G::kv_bytes / 2)) / 16;
+      for (int xx = 0; xx < row_tiles; ++xx) {
+        if (it > 0) {  // S takes the place of P
+          ok = ok && wait(&bar.p_free[xx][h], (it - 1) & 1);
           if (!ok) return;
-          tc_fence_after();
-          const unsigned t_p = tmem + G::s_at + xx * kPos + h * (kPos / 2), t_o = tmem + G::o_at + xx * D;
+        }
+        tc_fence_after();
+        const uint64_t q = q0 + xx * (G::parts * G::q_bytes / 16);
+        const unsigned t_s = tmem + G::s_at + xx * kPos + h * (kPos / 2);
 #pragma unroll
-          for (int kk = 0; kk < kPos / 32; ++kk)
+        for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-            for (int part = 0; part < G::parts; ++part)
-              umma_f16_ts(t_o, t_p + part * (kPos / 4) + kk * 8, v + kk * 2 * (D / 8) * 8, idesc_f16_bt(kRowsX, D), kk + part > 0 || h > 0 || (kSplit ? it % kFoldTiles != 0 : it > 0));
-          umma_commit(&bar.p_free[xx][h]);
-        }
-        if (h == 1) umma_commit(&bar.v_free[it % G::stages]);
-      };
-      if (tiles > 0) {
-        ok = mbar_wait_bounded(&bar.k_full[0], 0, kPromptTimeout);
-        if (ok) {
-          issue_s(0, 0);
-          issue_s(0, 1);
-        }
+          for (int part = 0; part < G::parts; ++part)
+            umma_f16_ss_warp(t_s, q + (part * G::q_bytes + kk * 256) / 16, k + kk * 16, idesc_f16(kRowsX, kPos / 2), kk + part > 0);
+        umma_commit_warp(&bar.s_full[xx][h]);
       }
-      // both row tiles' weights of a half, then, while they are used up, their next scores in that half's place
-      for (int it = 0; it < tiles && ok; ++it) {
-        ok = mbar_wait_bounded(&bar.v_full[it % G::stages], turn_of(it), kPromptTimeout);
-        if (ok) issue_o(it, 0);
-        if (it + 1 < tiles) {
-          ok = ok && mbar_wait_bounded(&bar.k_full[(it + 1) % G::stages], turn_of(it + 1), kPromptTimeout);
-          if (ok) issue_s(it + 1, 0);
-        }
-        if (ok) issue_o(it, 1);
-        if (ok && it + 1 < tiles) issue_s(it + 1, 1);
+      if (h == 1) umma_commit_warp(&bar.k_free[it % G::stages]);
+    };
+    auto issue_o = [&](int it, int h) {
+      const uint64_t v = v0 + (it % G::stages * G::kv_bytes + h * (G::kv_bytes / 2)) / 16;
+      for (int xx = 0; xx < row_tiles; ++xx) {
+        ok = ok && wait(&bar.p_full[xx][h], it & 1);
+        if (!ok) return;
+        tc_fence_after();
+        const unsigned t_p = tmem + G::s_at + xx * kPos + h * (kPos / 2), t_o = tmem + G::o_at + xx * D;
+#pragma unroll
+        for (int kk = 0; kk < kPos / 32; ++kk)
+#pragma unroll
+          for (int part = 0; part < G::parts; ++part)
+            umma_f16_ts_warp(t_o, t_p + part * (kPos / 4) + kk * 8, v + kk * 2 * (D / 8) * 8, idesc_f16_bt(kRowsX, D), kk + part > 0 || h > 0 || (kSplit ? it % kFoldTiles != 0 : it > 0));
+        umma_commit_warp(&bar.p_free[xx][h]);
       }
-      if (!ok) {  // let what was issued finish before shared and tensor memory go
-        umma_commit(&bar.drain);
-        mbar_wait_bounded(&bar.drain, 0, kPromptTimeout);
+      if (h == 1) umma_commit_warp(&bar.v_free[it % G::stages]);
+    };
+    if (tiles > 0) {
+      ok = wait(&bar.k_full[0], 0);
+      if (ok) {
+        issue_s(0, 0);
+        issue_s(0, 1);
       }
+    }
+    // both row tiles' weights of a half, then, while they are used up, their next scores in that half's place
+    for (int it = 0; it < tiles && ok; ++it) {
+      ok = wait(&bar.v_full[it % G::stages], turn_of(it));
+      if (ok) issue_o(it, 0);
+      if (it + 1 < tiles) {
+        ok = ok && wait(&bar.k_full[(it + 1) % G::stages], turn_of(it + 1));
+        if (ok) issue_s(it + 1, 0);
+      }
+      if (ok) issue_o(it, 1);
+      if (ok && it + 1 < tiles) issue_s(it + 1, 1);
+    }
+    if (!ok) {  // let what was issued finish before shared and tensor memory go
+      umma_commit_warp(&bar.drain);
+      wait(&bar.drain, 0);
     }
   } else if (x < row_tiles) {
     // ---- softmax: a warp has 32 rows, a thread in each 8-row set the row r and every fourth pair of positions, so that a
