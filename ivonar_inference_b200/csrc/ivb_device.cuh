@@ -83,11 +83,14 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, unsigned b
       "l"(src), "r"(bytes), "r"(smem_addr(bar))
       : "memory");
 }
-// First statement of a kernel launched with launch_pdl: wait until the previous grid on the stream has
-// completed and its writes are visible, then let the next grid be scheduled (it waits the same way).
+// Wait until the previous grid on the stream has completed and its writes are visible (not to read-only loads).
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Let the next grid be scheduled (it waits the same way).
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// First statement of a kernel launched with launch_pdl.
 __device__ __forceinline__ void pdl_enter() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  pdl_wait();
+  pdl_trigger();
 }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ bool mbar_try_wait(unsigned long long* bar, unsigned parity) {

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include "ivb_common.h"
+#include "ivb_device.cuh"
 #include "ivb_kv4.cuh"
 
 namespace ivb {
@@ -53,7 +54,7 @@ __device__ __forceinline__ bool kv4_place(const IvbKv4Cache& C, const int32_t* s
                                           int& b, int64_t& pos) {
   b = kv4_sequence(starts, C.batch, row);
   if (b >= C.batch) return false;
-  pos = __ldg(positions + b) + (starts == nullptr ? 0 : row - __ldg(starts + b));
+  pos = positions[b] + (starts == nullptr ? 0 : row - starts[b]);
   if (pos >= C.max_len && (threadIdx.x & 31) == 0 && error != nullptr) atomicCAS(error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
   return pos >= 0 && pos < C.max_len;
 }
@@ -66,6 +67,7 @@ template <int D, typename T, int kHeads>
 __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(IvbKv4Cache C, const T* k, const T* v, int64_t k_row, int64_t k_head,
                                                                  int64_t v_row, int64_t v_head, const int32_t* starts,
                                                                  const int64_t* positions, int rows, bool vec, uint32_t* error) {
+  pdl_enter();
   constexpr int n = D / 16;
   const int row = blockIdx.x * (kKv4Threads / 32) + (threadIdx.x >> 5), h0 = blockIdx.y * kHeads;
   if (row >= rows) return;
@@ -130,6 +132,7 @@ template <int D, typename T, int kHeads>
 __global__ void __launch_bounds__(kKv4Threads) kv4_read_kernel(IvbKv4Cache C, T* k, T* v, int64_t k_row, int64_t k_head, int64_t v_row,
                                                                int64_t v_head, const int32_t* starts, const int64_t* positions, int rows,
                                                                bool vec, uint32_t* error) {
+  pdl_enter();
   constexpr int n = D / 16;
   const int row = blockIdx.x * (kKv4Threads / 32) + (threadIdx.x >> 5), h0 = blockIdx.y * kHeads;
   if (row >= rows) return;
@@ -198,16 +201,13 @@ int32_t launch_rows(bool append, const IvbKv4Cache& c, void* k, void* v, int64_t
   if (by > 65535) return fail(IVB_EINVAL, "ivb_kv4: %d key/value heads", c.kv_heads);
   const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(rows) + kWarps - 1) / kWarps), static_cast<unsigned>(by));
   auto go = [&](auto append_kernel, auto read_kernel) {
-    if (append)
-      append_kernel<<<grid, kKv4Threads, 0, stream>>>(c, static_cast<const T*>(k), static_cast<const T*>(v), k_row, k_head, v_row, v_head,
-                                                      starts, positions, rows, vec, error);
-    else
-      read_kernel<<<grid, kKv4Threads, 0, stream>>>(c, static_cast<T*>(k), static_cast<T*>(v), k_row, k_head, v_row, v_head, starts, positions,
-                                                    rows, vec, error);
+    return append ? launch_pdl(append_kernel, grid, dim3(kKv4Threads), 0, stream, c, static_cast<const T*>(k), static_cast<const T*>(v), k_row,
+                               k_head, v_row, v_head, starts, positions, static_cast<int>(rows), vec, error)
+                  : launch_pdl(read_kernel, grid, dim3(kKv4Threads), 0, stream, c, static_cast<T*>(k), static_cast<T*>(v), k_row, k_head, v_row,
+                               v_head, starts, positions, static_cast<int>(rows), vec, error);
   };
-  if (heads == 4) go(kv4_append_kernel<D, T, 4>, kv4_read_kernel<D, T, 4>);
-  else go(kv4_append_kernel<D, T, 1>, kv4_read_kernel<D, T, 1>);
-  IVB_CUDA(cudaGetLastError());
+  if (heads == 4) IVB_CUDA(go(kv4_append_kernel<D, T, 4>, kv4_read_kernel<D, T, 4>));
+  else IVB_CUDA(go(kv4_append_kernel<D, T, 1>, kv4_read_kernel<D, T, 1>));
   return IVB_OK;
 }
 

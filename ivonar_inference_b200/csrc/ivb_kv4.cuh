@@ -44,9 +44,9 @@ __device__ __forceinline__ int kv4_sequence(const int32_t* starts, int batch, in
   int before = 0;
   for (int b0 = 0; b0 < batch; b0 += 32) {
     const int b = b0 + lane;
-    before += __popc(__ballot_sync(0xFFFFFFFFu, b < batch && __ldg(starts + b + 1) <= row));
+    before += __popc(__ballot_sync(0xFFFFFFFFu, b < batch && starts[b + 1] <= row));
   }
-  return row < __ldg(starts) ? batch : before;
+  return row < *starts ? batch : before;
 }
 
 template <typename T>
@@ -81,9 +81,9 @@ __device__ __forceinline__ void load_values(const T* p, bool vec, float (&v)[n])
         T t[step / sizeof(T)];
       } u;
       const char* at = reinterpret_cast<const char*>(p) + i * step;
-      if constexpr (step == 16) u.q = __ldg(reinterpret_cast<const uint4*>(at));
-      else if constexpr (step == 8) u.d = __ldg(reinterpret_cast<const uint2*>(at));
-      else u.w = __ldg(reinterpret_cast<const uint32_t*>(at));
+      if constexpr (step == 16) u.q = *reinterpret_cast<const uint4*>(at);
+      else if constexpr (step == 8) u.d = *reinterpret_cast<const uint2*>(at);
+      else u.w = *reinterpret_cast<const uint32_t*>(at);
 #pragma unroll
       for (int j = 0; j < step / static_cast<int>(sizeof(T)); ++j) v[i * (step / static_cast<int>(sizeof(T))) + j] = to_f32<T>(u.t[j]);
     }

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
   extern __shared__ __align__(128) unsigned char smem[];
   cg::cluster_group cluster = cg::this_cluster();
   const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank()), W = blockDim.x >> 5;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   unsigned char* const ring = smem + warp * G::warp_bytes;
   float4* const terms4 = reinterpret_cast<float4*>(smem + W * G::warp_bytes + warp * G::term_bytes);
   float2* const terms2 = reinterpret_cast<float2*>(terms4 + kKv4Group);
@@ -90,6 +90,8 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
   float* const stats = comb + G::comb_floats;                                               // [W][R][3]
   float* const folded = stats + W * R * 3 + warp * R * D;                                    // [R][D], fp32 outputs only
 
+  if (!A.beside_prompts) pdl_wait();
+  pdl_trigger();
   // which rows (rows x heads is below 2^31)
   const unsigned cluster_id = blockIdx.x / static_cast<unsigned>(C), group_size = static_cast<unsigned>(A.group);
   const int tile = static_cast<int>(cluster_id % static_cast<unsigned>(tiles_per_sequence));
@@ -97,13 +99,16 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
   const int b = static_cast<int>(sh / static_cast<unsigned>(A.cache.kv_heads)), kvh = static_cast<int>(sh) - b * A.cache.kv_heads;
   int row0 = b, count = 1;
   if (A.starts != nullptr) {
-    row0 = max(0, __ldg(A.starts + b));
-    count = min(A.rows, __ldg(A.starts + b + 1)) - row0;
+    row0 = max(0, A.starts[b]);
+    count = min(A.rows, A.starts[b + 1]) - row0;
   }
   const int items = max(count, 0) * A.group, i0 = tile * R;
-  if (i0 >= items || items > A.few) return;  // the whole cluster
+  if (i0 >= items || items > A.few) {  // the whole cluster
+    if (A.beside_prompts && blockIdx.x == 0) pdl_wait();
+    return;
+  }
   const int live = min(R, items - i0);
-  const int64_t base = __ldg(A.positions + b);
+  const int64_t base = A.positions[b];
   const int max_len = A.cache.max_len;
   // token and query head of an item of the sequence's head group
   auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };
@@ -502,7 +507,10 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
       }
     }
   }
-  if (C == 1) return;
+  if (C == 1) {
+    if (A.beside_prompts && blockIdx.x == 0) pdl_wait();
+    return;
+  }
   cluster.sync();
   // the cluster's parts: every CTA writes its share of the rows' values
   for (int i = rank * 32 * W + threadIdx.x; i < live * D; i += C * 32 * W) {
@@ -522,6 +530,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
     place(row)[i - row * D] = from_f32<T>(l == 0.0f ? 0.0f : v / l);
   }
   cluster.sync();  // no CTA leaves while another reads its shared memory
+  if (A.beside_prompts && blockIdx.x == 0) pdl_wait();
 }
 
 // Opt-in shared memory, once per device and kernel.
@@ -559,13 +568,9 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   cfg.blockDim = dim3(32 * W);
   cfg.dynamicSmemBytes = G::smem(W);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = C;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  cfg.numAttrs = C > 1 ? 1 : 0;
+  cfg.numAttrs = kv4_attributes(C, attr);
   IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_rows_kernel<D, T, kSplit, kTiles>, A, static_cast<int>(tiles)));
   return IVB_OK;
 }
@@ -636,6 +641,7 @@ extern "C" int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_
   const int few = tiles * c->kv_heads * 4 >= 148 ? kFewItems : kFewItemsSparse;
   // a lone sequence that can have more takes the prompts' kernel however many it has: one launch
   A.few = starts == nullptr || items <= few ? 0x7fffffff : c->batch == 1 ? 0 : few;
+  A.beside_prompts = A.few != 0x7fffffff;
   if (A.few != 0x7fffffff)
     if (int32_t rc = launch_kv4_prompts(A, dtype, A.few, s)) return rc;
   if (A.few == 0) return IVB_OK;

@@ -12,6 +12,7 @@
 #pragma once
 
 #include "ivb_common.h"
+#include "ivb_device.cuh"
 #include "ivb_kv4.cuh"
 
 namespace ivb {
@@ -31,7 +32,22 @@ struct Kv4Attention {
   int rows, window, sinks;
   int few;             // sequences with more items (tokens x group) are prompts
   bool q_vec, o_vec;   // rows begin on 16 bytes
+  // The few rows' kernel runs beside the prompts', which is the grid before it: what both read was complete when every CTA of
+  // that one had passed its own wait, and they write different rows. Its first CTA waits at its end instead, so that who
+  // waits for this grid has waited for both.
+  bool beside_prompts;
 };
+
+// Launch attributes: beside the end of the grid before, and clusters of C CTAs.
+inline int kv4_attributes(int C, cudaLaunchAttribute (&attr)[2]) {
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = C;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  return C > 1 ? 2 : 1;
+}
 
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);

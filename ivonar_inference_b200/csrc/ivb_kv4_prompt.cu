@@ -114,13 +114,13 @@ __device__ __forceinline__ void load_keys(const unsigned char* tile, bool in, in
   if constexpr (D == 128) {
     const int h = (lane >> 2) & 1, c = lane >> 3;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) raw.v[k] = in ? __ldg(reinterpret_cast<const uint4*>(tile + 512 * h + (((lane & 3) + 4 * k) * 4 + c) * 16)) : zero;
+    for (int k = 0; k < 2; ++k) raw.v[k] = in ? *reinterpret_cast<const uint4*>(tile + 512 * h + (((lane & 3) + 4 * k) * 4 + c) * 16) : zero;
   } else {
     const int r = lane & 7, c = lane >> 3;
     if constexpr (D == 64) {
-      raw.v[0] = in ? __ldg(reinterpret_cast<const uint4*>(tile + (r * 4 + c) * 16)) : zero;
+      raw.v[0] = in ? *reinterpret_cast<const uint4*>(tile + (r * 4 + c) * 16) : zero;
     } else {
-      const uint2 v = in ? __ldg(reinterpret_cast<const uint2*>(tile + (r * 4 + c) * 8)) : make_uint2(0u, 0u);
+      const uint2 v = in ? *reinterpret_cast<const uint2*>(tile + (r * 4 + c) * 8) : make_uint2(0u, 0u);
       raw.v[0] = make_uint4(v.x, v.y, 0u, 0u);
     }
   }
@@ -131,7 +131,7 @@ __device__ __forceinline__ void load_codes_of_values(const unsigned char* tile, 
   in = in && (D != 32 || lane < 16);
 #pragma unroll
   for (int k = 0; k < RawChunks<D>::n; ++k)
-    raw.v[k] = in ? __ldg(reinterpret_cast<const uint4*>(tile + 8 * D + 512 * k + (r * 4 + c) * 16)) : make_uint4(0u, 0u, 0u, 0u);
+    raw.v[k] = in ? *reinterpret_cast<const uint4*>(tile + 8 * D + 512 * k + (r * 4 + c) * 16) : make_uint4(0u, 0u, 0u, 0u);
 }
 
 // `keys`, `values`: the tile's 16 position rows.
@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   __shared__ int which[3];  // sequence, tile of its rows; and whether a wait ran out
   const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
+  pdl_wait();
   // which rows: the call's tiles of 256 items in the order of the sequences, the last ones (the longest rows) first
   cg::cluster_group cluster = cg::this_cluster();
   const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       int n = 0;
       if (b < A.cache.batch) {
         int count = 1;
-        if (A.starts != nullptr) count = max(0, min(A.rows, __ldg(A.starts + b + 1)) - max(0, __ldg(A.starts + b)));
+        if (A.starts != nullptr) count = max(0, min(A.rows, A.starts[b + 1]) - max(0, A.starts[b]));
         const int items = count * A.group;
         n = items > few ? (items + G::rows - 1) / G::rows : 0;
       }
@@ -252,14 +253,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)), "r"(G::columns));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    pdl_trigger();  // not before this CTA has its tensor memory: the next grid may take some too, and waits for this one
   }
   int row0 = b, count = 1;
   if (A.starts != nullptr) {
-    row0 = max(0, __ldg(A.starts + b));
-    count = min(A.rows, __ldg(A.starts + b + 1)) - row0;
+    row0 = max(0, A.starts[b]);
+    count = min(A.rows, A.starts[b + 1]) - row0;
   }
   const int i0 = which[1] * G::rows, live = min(G::rows, count * A.group - i0), row_tiles = live > kRowsX ? 2 : 1;
-  const int64_t base = __ldg(A.positions + b);
+  const int64_t base = A.positions[b];
   const int max_len = A.cache.max_len;
   const unsigned group_size = static_cast<unsigned>(A.group);
   auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };
@@ -301,7 +303,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       for (int g = 0; g < 4; ++g)
 #pragma unroll
         for (int k = 0; k < kQuads; ++k)
-          raw[g][k] = q[g] != nullptr ? __ldg(reinterpret_cast<const uint4*>(q[g]) + 4 * k) : make_uint4(0u, 0u, 0u, 0u);
+          raw[g][k] = q[g] != nullptr ? reinterpret_cast<const uint4*>(q[g])[4 * k] : make_uint4(0u, 0u, 0u, 0u);
     } else {
 #pragma unroll
       for (int g = 0; g < 4; ++g)
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         const unsigned char* tile = codes + (in ? t : 0) * kTile;
         if (keys) {
           load_keys<D>(tile, in, lane, key[k]);
-          par[k] = in && lane < 16 ? __ldg(reinterpret_cast<const uint2*>(tile + 16 * D + lane * 8)) : make_uint2(0u, 0u);
+          par[k] = in && lane < 16 ? *reinterpret_cast<const uint2*>(tile + 16 * D + lane * 8) : make_uint2(0u, 0u);
         } else {
           load_codes_of_values<D>(tile, in, lane, value[k]);
         }
@@ -860,7 +862,6 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   const int64_t items = static_cast<int64_t>(A.rows) * A.group;
   const int64_t sequences = std::min<int64_t>(A.cache.batch, items / (few + 1));
   const int64_t tiles = items / G::rows + sequences;
-  if (sequences == 0) return IVB_OK;
   if (tiles * A.cache.kv_heads > 0x1fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(tiles));
   // a cluster where one CTA each would leave SMs without work (128 CTAs of a 2048-row causal prompt: 72 us, in pairs 58; 256 CTAs
   // of a chunk under a window: 262, in pairs 309)
@@ -871,13 +872,9 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   cfg.blockDim = dim3(kPromptThreads);
   cfg.dynamicSmemBytes = G::smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = C;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  cfg.numAttrs = C > 1 ? 1 : 0;
+  cfg.numAttrs = kv4_attributes(C, attr);
   IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<D, T>, A, few));
   return IVB_OK;
 }
