@@ -77,6 +77,11 @@ __device__ __forceinline__ uint4 expand(uint32_t w, CodeMiddle m) {
   return make_uint4(codes_low(w, m), codes_high(w, m), codes_low(w >> 8, m), codes_high(w >> 8, m));
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 // Two fp32 operations in one instruction.
 typedef float2 f32x2;
 __device__ __forceinline__ f32x2 pair(float a, float b) { return make_float2(a, b); }
@@ -634,18 +639,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         for (int n = 0; n < 4; ++n)
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            top[n] = fmaxf(top[n], fmaxf(__uint_as_float(s[n >> 1][4 * i + 2 * (n & 1)]), __uint_as_float(s[n >> 1][4 * i + 2 * (n & 1) + 1])));
+            top[n] = max3(top[n], __uint_as_float(s[n >> 1][4 * i + 2 * (n & 1)]), __uint_as_float(s[n >> 1][4 * i + 2 * (n & 1) + 1]));
         bool raise = false;
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          top[n] = fmaxf(top[n], __shfl_xor_sync(0xFFFFFFFFu, top[n], 1));
-          top[n] = fmaxf(top[n], __shfl_xor_sync(0xFFFFFFFFu, top[n], 2));
-          raise |= top[n] > refs[n] + kRaise;  // the first seen position too: the reference is -inf
-        }
+        for (int n = 0; n < 4; ++n) raise |= top[n] > refs[n] + kRaise;  // the first seen position too: the reference is -inf
         if (__any_sync(0xFFFFFFFFu, raise)) {
           float corr[4];
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
+            top[n] = fmaxf(top[n], __shfl_xor_sync(0xFFFFFFFFu, top[n], 1));
+            top[n] = fmaxf(top[n], __shfl_xor_sync(0xFFFFFFFFu, top[n], 2));
             const float next = fmaxf(refs[n], top[n]);
             corr[n] = next > refs[n] ? ex2(refs[n] - next) : 1.0f;
             refs[n] = next;
