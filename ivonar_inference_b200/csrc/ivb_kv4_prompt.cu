@@ -607,7 +607,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         }
         uint32_t s[2][32];  // [16 rows][4 pair + 2 (8 rows) + position], scores in place
 #pragma unroll
-        for (int g = 0; g < 2; ++g) tmem_ld_16x256b_x8(th + (static_cast<unsigned>(16 * g) << 16), s[g]);
+        for (int g = 0; g < 2; ++g) tmem_ld_16x256b_x8_begin(th + (static_cast<unsigned>(16 * g) << 16), s[g]);
+        tmem_ld_end(s[0], s[1]);
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
