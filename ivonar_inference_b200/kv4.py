@@ -156,8 +156,8 @@ class KV4Cache:
 
         if out is not None:
             k, v = out
-            self._values("out[0]", k, self.kv_heads)
-            self._values("out[1]", v, self.kv_heads, k.dtype)
+            k_row, k_head = self._values("out[0]", k, self.kv_heads)
+            v_row, v_head = self._values("out[1]", v, self.kv_heads, k.dtype)
             if v.shape[0] != k.shape[0] or rows not in (None, k.shape[0]):
                 raise ValueError("out and rows disagree")
             for x in out:
@@ -170,11 +170,13 @@ class KV4Cache:
                 rows = self.batch
             if dtype not in _TYPES:
                 raise ValueError(f"dtype {dtype}")
-            k = torch.empty((rows, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
+            k = self.data.new_empty((rows, self.kv_heads, self.head_dim), dtype=dtype)
             v = torch.empty_like(k)
+            k_row = v_row = self.kv_heads * self.head_dim
+            k_head = v_head = self.head_dim
         at = self._rows(rows, positions, starts)
-        self._call("ivb_kv4_read", self.lib.ivb_kv4_read, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], k.stride(0), k.stride(1),
-                   v.stride(0), v.stride(1), at, positions.data_ptr(), rows)
+        self._call("ivb_kv4_read", self.lib.ivb_kv4_read, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], k_row, k_head, v_row, v_head, at,
+                   positions.data_ptr(), rows)
         return k, v
 
     def attention(self, q: Tensor, positions: Tensor, starts: Tensor | None = None, scale: float | None = None, window: int = 0,
