@@ -20,10 +20,11 @@ namespace cg = cooperative_groups;
 
 // Sequences of up to so many items (tokens x query heads of a group) are for the kernel of few rows, which splits a history over
 // more of the GPU; the others for the prompts' one, which reads it once for 256 items. Measured (rows / prompts): where the
-// prompts' clusters fill the GPU, 8 items 50 / 86 us and 16 items 92 / 89 (16 sequences, 16 heads x 64, 2000 positions, fp32), 32 items
-// 70 / 57 (8 sequences, 8 heads x 128, 4000 positions, bf16); where they do not, 32 items 119 / 151 and 64 items 194 / 152 (2
-// sequences, 8 heads x 128, 30000 positions, bf16), 32 items 87 / 177 and 64 items 199 / 178 (8 heads x 64, fp32).
-constexpr int kFewItems = 16, kFewItemsSparse = 48;
+// prompts' tiles are many, 32 items 57 / 84 us and 42 / 67 (16 sequences, 16 heads x 64, 2000 positions, fp32 and fp16), 44 / 53 (8
+// sequences, 8 heads x 128, 4000 positions, bf16), 48 items 60 / 67 and 64 / 54 (those two in 16 bits), 116 / 101 (64 sequences, 8 heads
+// x 128, 1000 positions); where they are few, 64 items 111 / 138 and 96 items 177 / 138 (2 sequences, 8 heads x 128, 30000 positions,
+// bf16), 64 items 86 / 163 and 100 items 195 / 165 (8 heads x 64, fp32).
+constexpr int kFewItems = 32, kFewItemsSparse = 64;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -553,7 +554,10 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   if (int32_t rc = allow_smem(kv4_rows_kernel<D, T, kSplit, kTiles>, G::smem(kMostWarps), done)) return rc;
   const int64_t most = std::min<int64_t>(A.few, static_cast<int64_t>(A.starts == nullptr ? 1 : A.rows) * A.group);
   const int64_t tiles = (most + G::rows - 1) / G::rows;
-  const int64_t base = tiles * A.cache.kv_heads * A.cache.batch;
+  const int64_t grid = tiles * A.cache.kv_heads * A.cache.batch;
+  // the tiles with rows in them, if the call's rows are spread evenly: the grid has places for each sequence's most
+  const int64_t even = (static_cast<int64_t>(A.rows) * A.group + G::rows - 1) / G::rows;
+  const int64_t base = std::min(tiles * A.cache.batch, std::max<int64_t>(std::min(A.rows, A.cache.batch), even)) * A.cache.kv_heads;
   // Warps a row tile by what fills the GPU twice over, then clusters where eight do not fill it once and leave each warp more than
   // four groups at the cache's capacity (a cluster costs 1.4 us). Measured with 1, 2, 4, 8 warps: 4096 tiles at positions
   // 128-640 51, 41, 49, 74 us; 1024 tiles at 300-1900 51, 36, 34, 38; 256 tiles of 1028 positions x 128 50, 30, 21, 17; 32 tiles
@@ -562,9 +566,9 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   int W = 1, C = 1;
   while (W < kMostWarps && base * W < 2 * slots && A.cache.max_len > W * kKv4Group) W *= 2;
   while (C < 8 && W == kMostWarps && base * W * C * 2 <= slots && A.cache.max_len > 4 * C * W * kKv4Group) C *= 2;
-  if (base * C > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(base));
+  if (grid * C > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(grid));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(base * C));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid * C));
   cfg.blockDim = dim3(32 * W);
   cfg.dynamicSmemBytes = G::smem(W);
   cfg.stream = stream;
