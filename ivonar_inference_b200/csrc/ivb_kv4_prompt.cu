@@ -10,9 +10,11 @@
 //   warps 0..7 (32 rows each, their tensor-memory lanes) turn S_X into weights: online softmax in 32 bits, the
 //     reference raised only when the maximum passes it by 2^8, and O_X rescaled in tensor memory then. The weights P_X take
 //     S_X's place as the fp16 A operand, so S_X(it + 1) follows P_X(it)'s product; while one X waits for it the other computes.
-// fp32 queries and weights are hi + lo fp16 pairs: two products each. 128 positions because a product from shared memory takes
-// 70 cycles for 64 columns as for 128 (measured). With few CTAs a cluster of C shares the rows: each takes every C-th tile, and
-// they join what they found through one another's shared memory. What bounds it is the softmax's issue slots, then the tensor pipe (D = 128).
+// fp32 queries and weights are hi + lo fp16 pairs: two products each. The scores come 64 positions at a time (48 cycles a product
+// where 128 columns take 65), so that the next half's are there when a half's weights are done. With few CTAs a cluster of C shares the rows: each takes every C-th tile, and
+// they join what they found through one another's shared memory. What bounds it is the latency of the
+// softmax's instructions: 2048 rows at 6144 under a window of 4096, 32 heads x 128 in bf16, take 228 us (0.60 PFLOP/s) with 47 % of
+// the issue slots used; without its exponentials 203, with an eighth of the products 222, without the producers' stores 226.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -867,8 +869,8 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   const int64_t sequences = std::min<int64_t>(A.cache.batch, items / (few + 1));
   const int64_t tiles = items / G::rows + sequences;
   if (tiles * A.cache.kv_heads > 0x1fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(tiles));
-  // a cluster where one CTA each would leave SMs without work (128 CTAs of a 2048-row causal prompt: 72 us, in pairs 58; 256 CTAs
-  // of a chunk under a window: 262, in pairs 309)
+  // a cluster where one CTA each would leave SMs without work (128 CTAs of a 2048-row causal prompt: 68 us, in pairs 56, in fours
+  // 88; 256 CTAs of a chunk under a window: 228, in pairs 275)
   int C = 1;
   while (C < 4 && tiles * A.cache.kv_heads * C < 148 && A.cache.max_len > 2 * C * kPos) C *= 2;
   cudaLaunchConfig_t cfg = {};

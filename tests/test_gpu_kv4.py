@@ -627,6 +627,69 @@ def test_results_are_the_same_every_time_on_any_stream_and_in_graphs() -> None:
     assert torch.equal(moved, caches[0].attention(q, at)) and not torch.equal(moved, expected[0])
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("counts", [[65], [64, 65], [33, 32, 64, 65, 1, 31, 66]])
+def test_between_few_rows_and_prompts(counts, dtype) -> None:
+    """Sequences on either side of where the kernels change, with few sequences in a call and with many."""
+
+    from ivonar_inference_b200 import KV4Cache
+
+    lengths = [90 - 11 * i for i in range(len(counts))]
+    cache = KV4Cache(len(counts), 6, 64, 300)
+    filled(cache, [n + c for n, c in zip(lengths, counts)], seed=3)
+    at, starts = rows_of(len(counts), lengths, counts)
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    q = torch.randn(sum(counts), 6, 64, generator=gen, device="cuda").to(TYPES[dtype])
+    check_attention(cache, q, at, starts, TYPES[dtype])
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_that_follow_one_another_need_no_wait_between_them(captured) -> None:
+    """Each call's inputs are the last one's outputs, prompts and few rows in one call: as with a wait after every call."""
+
+    from ivonar_inference_b200 import KV4Cache
+
+    counts, lengths = [1, 100, 3, 40, 1, 70, 2], [400, 0, 250, 130, 7, 300, 511]
+    at, starts = rows_of(7, lengths, counts)
+    rows = sum(counts)
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    start = torch.randn(rows, 8, 64, generator=gen, device="cuda")
+    results = []
+    for wait in (True, False):
+        cache = KV4Cache(7, 4, 64, 1100)
+        filled(cache, lengths, seed=4)
+        x, where, history = start.clone(), at.clone(), []
+        moves = torch.tensor(counts, device="cuda")
+
+        def step():
+            cache.append(x[:, :4], x[:, 4:], where, starts)
+            y = cache.attention(x, where, starts)
+            if wait:
+                torch.cuda.synchronize()
+            cache.attention(y, where, starts, out=x)
+            where.add_(moves)
+            k, v = cache.read(where - moves, starts, rows)
+            if wait:
+                torch.cuda.synchronize()
+            return y, k, v
+
+        if captured and not wait:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = step()
+            for _ in range(5):
+                graph.replay()
+                history.append([t.clone() for t in (*out, x)])
+        else:
+            for _ in range(5):
+                history.append([t.clone() for t in (*step(), x)])
+        torch.cuda.synchronize()
+        results.append(history)
+    for waited, free in zip(*results):
+        for a, b in zip(waited, free):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
 def test_one_sequence_of_a_cache() -> None:
     from ivonar_inference_b200 import KV4Cache
 
