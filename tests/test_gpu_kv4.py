@@ -690,6 +690,49 @@ def test_calls_that_follow_one_another_need_no_wait_between_them(captured) -> No
             assert torch.isfinite(a).all() and torch.equal(a, b)
 
 
+def test_a_graph_that_joins_streams_before_each_call() -> None:
+    from ivonar_inference_b200 import KV4Cache
+
+    counts, lengths = [1, 90, 2], [300, 10, 77]
+    at, starts = rows_of(3, lengths, counts)
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    base = torch.randn(sum(counts), 4, 64, generator=gen, device="cuda")
+    side = torch.cuda.Stream()
+
+    def step(cache, x):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        k = x[:, :2] * 2
+        with torch.cuda.stream(side):
+            v = x[:, 2:] + 1
+            q = torch.zeros_like(x)
+        main.wait_stream(side)
+        cache.append(k, v, at, starts)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            q.add_(x)
+            held = cache.read(at, starts, sum(counts))
+        q2 = x * 0.5
+        main.wait_stream(side)
+        out = cache.attention(q, at, starts) + cache.attention(q2, at, starts)
+        return out, *held
+
+    caches = [KV4Cache(3, 2, 64, 400) for _ in range(2)]
+    for cache in caches:
+        filled(cache, lengths, seed=5)
+    x = base.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(caches[0], x)
+    for i in range(3):
+        x.copy_(base * (i + 1))
+        graph.replay()
+        want = step(caches[1], x)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 def test_one_sequence_of_a_cache() -> None:
     from ivonar_inference_b200 import KV4Cache
 
