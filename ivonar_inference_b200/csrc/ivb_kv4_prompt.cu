@@ -11,10 +11,11 @@
 //     reference raised only when the maximum passes it by 2^8, and O_X rescaled in tensor memory then. The weights P_X take
 //     S_X's place as the fp16 A operand, so S_X(it + 1) follows P_X(it)'s product; while one X waits for it the other computes.
 // fp32 queries and weights are hi + lo fp16 pairs: two products each. The scores come 64 positions at a time (48 cycles a product
-// where 128 columns take 65), so that the next half's are there when a half's weights are done. With few CTAs a cluster of C shares the rows: each takes every C-th tile, and
-// they join what they found through one another's shared memory. What bounds it is the latency of the
-// softmax's instructions: 2048 rows at 6144 under a window of 4096, 32 heads x 128 in bf16, take 228 us (0.60 PFLOP/s) with 47 % of
-// the issue slots used; without its exponentials 203, with an eighth of the products 222, without the producers' stores 226.
+// where 128 columns take 65), so that the next half's are there when a half's weights are done. With few CTAs a cluster of C shares
+// the rows: each takes every C-th tile, and they join what they found through one another's shared memory.
+// What bounds it is the latency of the softmax's instructions: 2048 rows at 6144 under a window of 4096, 32 heads x 128 in bf16, take
+// 228 us (0.60 PFLOP/s) with 47 % of the issue slots used; without its exponentials 203, with a sixth of the products 222, without the
+// producers' stores 226.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
