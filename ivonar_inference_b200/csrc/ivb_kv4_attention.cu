@@ -74,7 +74,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 }
 
 template <int D, typename T, bool kSplit, int kTiles>
-__global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int tiles_per_sequence) {
+__device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_sequence) {
   using G = RowsGeometry<D, T, kSplit, kTiles>;
   constexpr int R = G::rows, kSteps = D / 16, kTile = kv4_tile_bytes(D);
   constexpr int kPer = kSplit ? 1 : 2;        // rows of a lane in a column tile
@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
   float* const stats = comb + G::comb_floats;                                               // [W][R][3]
   float* const folded = stats + W * R * 3 + warp * R * D;                                    // [R][D], fp32 outputs only
 
-  if (!A.beside_prompts) pdl_wait();
+  if (A.beside_prompts) __threadfence();
+  else pdl_wait();
   pdl_trigger();
   // which rows (rows x heads is below 2^31)
   const unsigned cluster_id = blockIdx.x / static_cast<unsigned>(C), group_size = static_cast<unsigned>(A.group);
@@ -104,10 +105,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
     count = min(A.rows, A.starts[b + 1]) - row0;
   }
   const int items = max(count, 0) * A.group, i0 = tile * R;
-  if (i0 >= items || items > A.few) {  // the whole cluster
-    if (A.beside_prompts && blockIdx.x == 0) pdl_wait();
-    return;
-  }
+  if (i0 >= items || items > A.few) return;  // the whole cluster
   const int live = min(R, items - i0);
   const int64_t base = A.positions[b];
   const int max_len = A.cache.max_len;
@@ -508,10 +506,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
       }
     }
   }
-  if (C == 1) {
-    if (A.beside_prompts && blockIdx.x == 0) pdl_wait();
-    return;
-  }
+  if (C == 1) return;
   cluster.sync();
   // the cluster's parts: every CTA writes its share of the rows' values
   for (int i = rank * 32 * W + threadIdx.x; i < live * D; i += C * 32 * W) {
@@ -531,6 +526,12 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int ti
     place(row)[i - row * D] = from_f32<T>(l == 0.0f ? 0.0f : v / l);
   }
   cluster.sync();  // no CTA leaves while another reads its shared memory
+}
+
+template <int D, typename T, bool kSplit, int kTiles>
+__global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int tiles_per_sequence) {
+  kv4_rows<D, T, kSplit, kTiles>(A, tiles_per_sequence);
+  // whichever way the rows took: this grid does not end before the prompts' that it runs beside
   if (A.beside_prompts && blockIdx.x == 0) pdl_wait();
 }
 

@@ -32,9 +32,10 @@ struct Kv4Attention {
   int rows, window, sinks;
   int few;             // sequences with more items (tokens x group) are prompts
   bool q_vec, o_vec;   // rows begin on 16 bytes
-  // The few rows' kernel runs beside the prompts', which is the grid before it: what both read was complete when every CTA of
-  // that one had passed its own wait, and they write different rows. Its first CTA waits at its end instead, so that who
-  // waits for this grid has waited for both.
+  // The few rows' kernel runs beside the prompts', which is the grid before it, and does not wait before it reads. It is launched
+  // once every CTA of that one has triggered or ended, which each does only after its own wait for the grids before both: these
+  // had ended then, with their writes in device memory, and a fence at its start keeps it from what an SM's cache may have from before.
+  // The two write different rows. The first CTA waits at its end instead, so that who waits for this grid has waited for both.
   bool beside_prompts;
 };
 
