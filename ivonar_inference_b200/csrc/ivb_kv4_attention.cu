@@ -151,51 +151,38 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
 #pragma unroll
   for (int s = 0; s < G::stages - 1; ++s) issue(s, s);
 
-  // queries as B fragments (this lane: column r, channels D/4 c .. of its row), scaled by a power of two that brings the
-  // largest to 2^13
+  // queries as B fragments (this lane: column r, channels D/4 c .. of its row), each row scaled by the power of two that brings its
+  // largest to 2^13, so that no row's bits depend on its neighbours; row_unit undoes it. Idle rows' queries are not read.
   uint32_t qf[kTiles][kSteps][2];
-  float sum_q[kSets];
-  float score_unit;
+  float sum_q[kSets], row_unit[kSets];
   {
-    float qv[kTiles][D / 4];
-    float amax = 0.0f, total[kTiles];
+    float total[kTiles], unit[kTiles];
+    const float scale = A.scale * kLog2e;
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
       const int row = kSplit ? 4 * n + (r >> 1) : 8 * n + r;
+      float qv[D / 4];
 #pragma unroll
-      for (int j = 0; j < D / 4; ++j) qv[n][j] = 0.0f;
-      if (row < live) {
-        const int t = token_of(i0 + row), h = kvh * A.group + i0 + row - t * A.group;
-        load_values<T, D / 4>(static_cast<const T*>(A.q) + (row0 + t) * A.q_row + h * A.q_head + D / 4 * c, A.q_vec, qv[n]);
-      }
+      for (int j = 0; j < D / 4; ++j) qv[j] = 0.0f;
+      const int t = token_of(i0 + row), p = clamp_position(base + t);
+      if (row < live && p >= 0 && p < max_len)
+        load_values<T, D / 4>(static_cast<const T*>(A.q) + (row0 + t) * A.q_row + (kvh * A.group + i0 + row - t * A.group) * A.q_head + D / 4 * c,
+                              A.q_vec, qv);
+      float amax = 0.0f;
+#pragma unroll
+      for (int j = 0; j < D / 4; ++j) amax = fmaxf(amax, finite_size(qv[j]));
+      amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
+      const int up = query_power(amax);
+      const float q_unit = power_of_two(up);
+      unit[n] = power_of_two(-up) * scale;
       total[n] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < D / 4; ++j) {
-        total[n] += qv[n][j];
-        const float m = fabsf(qv[n][j]);
-        if (m <= 3.402823466e38f) amax = fmaxf(amax, m);
-      }
-      total[n] += __shfl_xor_sync(0xFFFFFFFFu, total[n], 1);
-      total[n] += __shfl_xor_sync(0xFFFFFFFFu, total[n], 2);
-    }
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
-#pragma unroll
-    for (int s = 0; s < kSets; ++s)  // from the lanes that hold the row as a column
-      sum_q[s] = __shfl_sync(0xFFFFFFFFu, total[kSplit ? s : s >> 1], kSplit ? 8 * c : 4 * (2 * c + (s & 1)));
-    int up = 13 - (static_cast<int>(__float_as_uint(amax) >> 23) - 127);
-    up = amax == 0.0f ? 0 : min(max(up, -114), 100);
-    const float q_unit = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-    score_unit = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * (A.scale * kLog2e);
-#pragma unroll
-    for (int s = 0; s < kSets; ++s) sum_q[s] *= q_unit;
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n)
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float x0 = qv[n][4 * s + 2 * e] * q_unit, x1 = qv[n][4 * s + 2 * e + 1] * q_unit;
+          const float x0 = qv[4 * s + 2 * e] * q_unit, x1 = qv[4 * s + 2 * e + 1] * q_unit;
+          total[n] = total[n] + x0 + x1;
           uint32_t w = pack_f16(x0, x1);
           if (kSplit && (r & 1)) {
             const float2 hi = unpack_f16(w);
@@ -203,6 +190,15 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
           }
           qf[n][s][e] = w;
         }
+      total[n] += __shfl_xor_sync(0xFFFFFFFFu, total[n], 1);
+      total[n] += __shfl_xor_sync(0xFFFFFFFFu, total[n], 2);
+    }
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) {  // from the lanes that hold the row as a column
+      const int from = kSplit ? 8 * c : 4 * (2 * c + (s & 1));
+      row_unit[s] = __shfl_sync(0xFFFFFFFFu, unit[kSplit ? s : s >> 1], from);
+      sum_q[s] = __shfl_sync(0xFFFFFFFFu, total[kSplit ? s : s >> 1], from) * row_unit[s];
+    }
   }
 
   float acc[kTiles][kOut][4];
@@ -262,7 +258,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
     const int p0 = group_of(step) * kKv4Group;
     {
       const uint2 par = *reinterpret_cast<const uint2*>(stage + (lane >> 4) * kTile + 16 * D + (lane & 15) * 8);
-      const PositionTerms t = position_terms(par, score_unit, 16384.0f, lane);
+      const PositionTerms t = position_terms(par, 1.0f, 16384.0f, lane);
       terms4[lane] = make_float4(t.key_scale, t.key_offset, t.bias, t.mantissa);
       terms2[lane] = make_float2(t.unbias, t.value_offset);
     }
@@ -311,7 +307,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
 #pragma unroll
         for (int s = 0; s < kSets; ++s) {
           const float dot = kSplit ? s2[s][2 * h] + s2[s][2 * h + 1] : s2[s >> 1][2 * h + (s & 1)];
-          x[s][2 * t + h] = fmaf(dot, pt.x, fmaf(sum_q[s], pt.y, pt.z));
+          x[s][2 * t + h] = fmaf(dot * row_unit[s], pt.x, fmaf(sum_q[s], pt.y, pt.z));
         }
       }
     }

@@ -7,8 +7,9 @@
 // long axis where the terms have one sign (with u itself 3e-6 of the output at 2000 positions). Values take u - 8 at even
 // positions and u - 7 at odd ones, since the 0.5 that is left of either mean is what all of a long history has in
 // common (with u - 8 throughout 1.3e-5 at 100000 positions, where the values average out to little).
-// fp32 queries and weights are split in two fp16 (x = hi + lo, 22 bits); fp16 and bf16 queries are exact in fp16 after a common
-// power of two, and their weights are rounded once to fp16 where a tile has no place for a remainder.
+// fp32 queries and weights are split in two fp16 (x = hi + lo, 22 bits). fp16 and bf16 queries have no more bits than fp16 after their
+// row's power of two (what lies 2^27 and more below the row's largest is cut at that), and their weights are rounded once to fp16 where
+// a tile has no place for a remainder.
 #pragma once
 
 #include "ivb_common.h"
@@ -61,6 +62,17 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Queries become fp16 by a power of two that brings the largest finite value of their row to 2^13 (a row's values below 2^-87 stay small).
+__device__ __forceinline__ float finite_size(float x) {
+  const float m = fabsf(x);
+  return m <= 3.402823466e38f ? m : 0.0f;
+}
+__device__ __forceinline__ int query_power(float largest) {
+  const int up = 13 - (static_cast<int>(__float_as_uint(largest) >> 23) - 127);
+  return largest == 0.0f ? 0 : min(max(up, -114), 100);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+
 // (a & b) | c in one instruction (two constants keep the compiler from it).
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t y;
@@ -89,7 +101,7 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t w, CodeMiddle m) {
 }
 
 // What the softmax needs of one position: x = S key_scale + sum(q) key_offset + bias (S and sum(q) of the queries as the operands hold
-// them, a power of two apart: score_unit undoes it), with bias the exponent of the value
+// them, a power of two apart, which score_unit undoes together with the scale, or 1 where the rows have units of their own), with bias the exponent of the value
 // scale, so that the running reference is the maximum of weight times value scale and neither overflows fp16, whatever the
 // scales; the weight is then 2^(x - ref) = p 2^bias, its product with the mantissa the A operand of the value product, and
 // p = weight * unbias enters the sum. A position whose value scale or offset is no number has a score that is none, and

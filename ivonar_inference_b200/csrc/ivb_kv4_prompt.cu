@@ -39,6 +39,9 @@ constexpr int kTermSets = 3;  // terms(it + 2) are written when S(it) is done, s
 constexpr unsigned long long kPromptTimeout = 2000000000ull;
 constexpr float kWeightUnit = 64.0f;  // weights are at most 2 * 64 * 2^8 in fp16
 constexpr float kRaise = 8.0f;
+// A tile's rows share the queries' power of two (no multiplication of the scores by a row's own) unless one's largest is so far below
+// another's: to there hi + lo keep 2^-23 of a row's largest, and fp16 as many bits as bf16 or fp16 queries have.
+constexpr float kEven = 0.000244140625f;
 // The tensor cores cut what they add to an accumulator towards zero, a bias that grows with its length (1.6e-6 of the output after
 // 1024 positions). fp32 outputs keep a second one, to which the threads add the first every so many tiles, rounding to nearest.
 constexpr int kFoldTiles = 2;
@@ -195,7 +198,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ PromptBarriers bar;
   __shared__ unsigned tmem_base;
-  __shared__ float largest[kSoftmaxWarps], sums[kRowsCta], refs_of[kRowsCta], totals[kRowsCta], offsets[kRowsCta];
+  __shared__ float largest[kSoftmaxWarps], smallest[kSoftmaxWarps], sums[kRowsCta], row_units[kRowsCta], refs_of[kRowsCta], totals[kRowsCta], offsets[kRowsCta];
   __shared__ int which[3];  // sequence, tile of its rows; and whether a wait ran out
   const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
@@ -289,8 +292,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   };
 
   // queries: a warp takes 32 rows in 16-byte chunks, 8 rows and 4 chunks at a time (64 contiguous bytes of a row, and no bank
-  // conflicts); the largest of all rows first, then hi (and lo) parts as K-major operands, scaled by a power of two that
-  // brings it to 2^13
+  // conflicts); the rows' largest first, then hi (and lo) parts as K-major operands, scaled by a power of two that brings the largest of
+  // all rows to 2^13, or each row's own where they are uneven. Idle rows' queries are not read.
   constexpr int kPer = 16 / static_cast<int>(sizeof(T)), L = D / kPer, kQuads = L / 4;  // values of a chunk, chunks of a row
   const int row8 = lane & 7, chunk4 = lane >> 3;
   const int x = warp >> 2;  // row tile of a softmax warp
@@ -304,7 +307,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int r = 32 * warp + 8 * g + row8;
-      q[g] = r < live ? item_row(A.q, i0 + r, A.q_row, A.q_head) + chunk4 * kPer : nullptr;
+      const int p = clamp_position(base + token_of(i0 + r));
+      q[g] = r < live && p >= 0 && p < max_len ? item_row(A.q, i0 + r, A.q_row, A.q_head) + chunk4 * kPer : nullptr;
     }
     if (A.q_vec) {
 #pragma unroll
@@ -328,41 +332,51 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           raw[g][k] = u.w;
         }
     }
-    float most = 0.0f;
+    float most = 0.0f, least = INFINITY;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      float total = 0.0f;
+      float top = 0.0f;
 #pragma unroll
       for (int k = 0; k < kQuads; ++k) {
         float v[kPer];
         values_of_chunk<T>(raw[g][k], v);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const float m = fabsf(v[j]);
-          if (m <= 3.402823466e38f) most = fmaxf(most, m);
-          total += v[j];
-        }
+        for (int j = 0; j < kPer; ++j) top = fmaxf(top, finite_size(v[j]));
       }
-      total += __shfl_xor_sync(0xFFFFFFFFu, total, 8);
-      total += __shfl_xor_sync(0xFFFFFFFFu, total, 16);
-      if (chunk4 == 0) sums[32 * warp + 8 * g + row8] = total;
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+      if (chunk4 == 0) row_units[32 * warp + 8 * g + row8] = top;
+      most = fmaxf(most, top);
+      if (top > 0.0f) least = fminf(least, top);
     }
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
-    if (lane == 0) largest[warp] = most;
+    for (int d = 1; d < 8; d <<= 1) {
+      most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+      least = fminf(least, __shfl_xor_sync(0xFFFFFFFFu, least, d));
+    }
+    if (lane == 0) {
+      largest[warp] = most;
+      smallest[warp] = least;
+    }
   }
   __syncthreads();
-  float most = 0.0f;
+  float most = 0.0f, least = INFINITY;
 #pragma unroll
-  for (int w = 0; w < kSoftmaxWarps; ++w) most = fmaxf(most, largest[w]);
-  int up = 13 - (static_cast<int>(__float_as_uint(most) >> 23) - 127);
-  up = most == 0.0f ? 0 : min(max(up, -114), 100);
-  const float q_unit = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-  const float score_unit = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * (A.scale * kLog2e);
+  for (int w = 0; w < kSoftmaxWarps; ++w) {
+    most = fmaxf(most, largest[w]);
+    least = fminf(least, smallest[w]);
+  }
+  const bool even = least >= most * kEven;
+  const int up = query_power(most);
+  // of the scores, in the positions' terms or (uneven) for each row
+  const float score_unit = even ? power_of_two(-up) * (A.scale * kLog2e) : 1.0f;
   if (tid < kSoftmaxThreads && x < row_tiles) {
     unsigned char* dst = smem + G::q_at + x * G::parts * G::q_bytes;
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
+    for (int g = 0; g < 4; ++g) {
+      const int row = 32 * warp + 8 * g + row8, own = even ? up : query_power(row_units[row]);
+      const float q_unit = power_of_two(own);
+      float total = 0.0f;
 #pragma unroll
       for (int k = 0; k < kQuads; ++k) {
         const int r = 32 * (warp & 3) + 8 * g + row8, i = 4 * k + chunk4;
@@ -372,6 +386,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll
         for (int j = 0; j < kPer / 2; ++j) {
           const float a = v[2 * j] * q_unit, c = v[2 * j + 1] * q_unit;
+          total = total + a + c;
           hi[j] = pack_f16(a, c);
           const float2 h = unpack_f16(hi[j]);
           lo[j] = pack_f16(a - h.x, c - h.y);
@@ -384,6 +399,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, i)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         }
       }
+      total += __shfl_xor_sync(0xFFFFFFFFu, total, 8);
+      total += __shfl_xor_sync(0xFFFFFFFFu, total, 16);  // the lanes of the row have read row_units[row]
+      const float unit = even ? 1.0f : power_of_two(-own) * (A.scale * kLog2e);
+      if (chunk4 == 0) {
+        row_units[row] = unit;
+        sums[row] = total * unit;
+      }
+    }
   }
   fence_proxy_async();  // the tensor cores read what the threads wrote
   tc_fence_before();
@@ -542,7 +565,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = kRowsX * x + row0x + 8 * i + r;
-      sum_q[i] = sums[n] * q_unit;
+      sum_q[i] = sums[n];
       at[i] = -1;
       if (n < live) {
         const int p = clamp_position(base + token_of(i0 + n));
@@ -612,6 +635,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll
         for (int g = 0; g < 2; ++g) tmem_ld_16x256b_x8_begin(th + (static_cast<unsigned>(16 * g) << 16), s[g]);
         tmem_ld_end(s[0], s[1]);
+        if (!even) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float unit = row_units[kRowsX * x + row0x + 8 * n + r];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int j = 4 * i + 2 * (n & 1) + e;
+                s[n >> 1][j] = __float_as_uint(__uint_as_float(s[n >> 1][j]) * unit);
+              }
+          }
+        }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {

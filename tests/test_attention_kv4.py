@@ -79,3 +79,87 @@ def test_calls_that_follow_a_mixed_call_of_one_warp_a_tile(dtype, dim, kv_heads,
     for waited, free in zip(*results):
         for a, b in zip(waited, free):
             assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+# ---- rows beside rows of another size -----------------------------------------------------------
+SHAPES = [  # dim, kv_heads, group, batch, first position, counts (None: one row each)
+    (64, 2, 4, 3, 39, None),
+    (128, 1, 8, 2, 50, None),
+    (32, 1, 16, 2, 33, None),
+    (64, 1, 2, 2, 30, [7, 3]),
+    (128, 2, 1, 1, 20, [150]),
+    (64, 2, 2, 2, 10, [200, 5]),
+    (32, 1, 4, 1, 40, [100]),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim,kv_heads,group,batch,first,counts", SHAPES)
+def test_rows_do_not_depend_on_the_size_of_others(dim, kv_heads, group, batch, first, counts, dtype) -> None:
+    """Queries of a call 2^33 (fp16: 2^12) apart, the scale for the small ones, so that the large ones see the key of their largest
+    score only: small rows within the bound of their own size, large rows that value."""
+    from ivonar_inference_b200 import KV4Cache
+
+    T, k = TYPES[dtype], 12 if dtype == "fp16" else 33
+    counts_ = [1] * batch if counts is None else counts
+    total = [first + n for n in counts_]
+    cache = KV4Cache(batch, kv_heads, dim, max(total))
+    filled(cache, total, seed=dim + batch)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    rows, H = sum(counts_), kv_heads * group
+    q = torch.randn(rows, H, dim, generator=gen, device="cuda") * 1.5
+    # every third head of a group, or every third token
+    large = (torch.arange(rows)[:, None] + torch.arange(H)[None]) % 3 == 1
+    q = torch.where(large[..., None].cuda(), q, q * 2.0**-k).to(T)
+    scale = 2.0**k * dim**-0.5
+    at, starts = rows_of(batch, [first] * batch, counts_)
+    got = cache.attention(q, at, None if counts is None else starts, scale=scale).double().cpu()
+    kk, vv, par = contents(cache.data, dim)
+    tested, r0 = 0, 0
+    for b in range(batch):
+        n = counts_[b]
+        x = q[r0:r0 + n].double().cpu().unflatten(1, (kv_heads, group))
+        score = torch.einsum("nhgd,hjd->nhgj", x, kk[b, :, :total[b]]) * scale
+        hidden = torch.arange(total[b])[None] > first + torch.arange(n)[:, None]
+        score = score.masked_fill(hidden[:, None, None], -math.inf).flatten(1, 2)
+        weight = torch.softmax(score, -1).unflatten(1, (kv_heads, group))
+        want = torch.einsum("nhgj,hjd->nhgd", weight, vv[b, :, :total[b]]).flatten(1, 2)
+        most = float((par[b, :, :total[b], 1].abs() + 15 * par[b, :, :total[b], 0]).max())
+        vmax = float(vv[b, :, :total[b]].abs().max())
+        small = ~large[r0:r0 + n]
+        tol = tolerance(q[r0:r0 + n][small.cuda()], most, vmax, scale, want, T)
+        diff = (got[r0:r0 + n] - want).abs()
+        assert bool((diff[small] <= tol[small]).all()), (b, float(diff[small].max()))
+        # a large row: scores are off by A 2^-18 at most, so a gap of twice that and 40 leaves the others weights below e^-40
+        A = scale * float(q[r0:r0 + n].double().abs().sum(-1).max()) * most
+        two = score.topk(2, -1).values
+        clear = ~small & (two[..., 0] - two[..., 1] > 2 * A * 2.0**-18 + 40)
+        tested += int(clear.sum())
+        tol = 2 * vmax * (2.0**-17 + (0 if T == torch.float32 else 2.0**-11)) + (0 if T == torch.float32 else torch.finfo(T).eps / 2) * want.abs()
+        assert bool((diff[clear] <= tol[clear]).all()), (b, float(diff[clear].max()))
+        r0 += n
+    assert tested >= int(large.sum()) // 2
+    cache.check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim,group,counts,idle", [(64, 1, [9], 4), (64, 4, [3, 6], 2), (128, 2, [150], 40), (32, 1, [300, 5], 3), (64, 3, [100, 1], 30)])
+def test_idle_rows_may_hold_any_query(dim, group, counts, idle, dtype) -> None:
+    """Rows before position 0 and beyond the capacity: the others' results to the last bit whatever they hold."""
+    from ivonar_inference_b200 import KV4Cache
+
+    T, batch = TYPES[dtype], len(counts)
+    length = max(counts)
+    cache = KV4Cache(batch, 2, dim, length - idle - 1)    # the longest sequence's last row is beyond it
+    filled(cache, [length - idle - 1] * batch, seed=dim)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    at, starts = rows_of(batch, [-idle] * batch, counts)
+    q = (torch.randn(sum(counts), 2 * group, dim, generator=gen, device="cuda") * 1.5).to(T)
+    live = torch.cat([(torch.arange(n) >= idle) & (torch.arange(n) - idle < cache.max_len) for n in counts]).cuda()
+    want = cache.attention(q, at, starts)
+    assert bool((want[~live] == 0).all()) and bool((want[live] != 0).any()) and 0 < int(live.sum()) < sum(counts)
+    for value in (0.0, 1e30, torch.finfo(T).max, math.inf, math.nan):
+        q[~live] = torch.tensor(value).to(T).cuda()
+        assert torch.equal(cache.attention(q, at, starts), want)
