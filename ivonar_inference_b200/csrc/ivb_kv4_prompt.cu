@@ -583,175 +583,180 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       last_at = max(last_at, __shfl_xor_sync(0xFFFFFFFFu, last_at, d));
     }
     live_rows = __any_sync(0xFFFFFFFFu, live_rows);
-    for (int it = 0; it < tiles; ++it) {
-      const int p0 = tile_of(it) * kPos;
-      const float* terms = terms_of(it);
-      ok = mbar_wait_bounded(&bar.terms_full[it % kTermSets], static_cast<unsigned>(it / kTermSets) & 1u, kPromptTimeout);
-      // what the warp's rows see of the tile: all of it, or nothing (first_at, last_at: the lowest and highest, -1 among them)
-      const bool whole = live_rows && first_at >= p0 + kPos - 1 && (A.window <= 0 || p0 > last_at - A.window || p0 <= A.sinks - kPos);
-      const bool none = last_at < p0 || (A.window > 0 && p0 + kPos - 1 <= first_at - A.window && p0 >= A.sinks);
-      // 64 positions at a time: the next ones' scores and the last ones' product are computed meanwhile
+    // a copy for each kind of rows: the test within costs a chunk 235 us in place of 230
+    auto walk = [&](auto evenly) {
+      for (int it = 0; it < tiles; ++it) {
+        const int p0 = tile_of(it) * kPos;
+        const float* terms = terms_of(it);
+        ok = mbar_wait_bounded(&bar.terms_full[it % kTermSets], static_cast<unsigned>(it / kTermSets) & 1u, kPromptTimeout);
+        // what the warp's rows see of the tile: all of it, or nothing (first_at, last_at: the lowest and highest, -1 among them)
+        const bool whole = live_rows && first_at >= p0 + kPos - 1 && (A.window <= 0 || p0 > last_at - A.window || p0 <= A.sinks - kPos);
+        const bool none = last_at < p0 || (A.window > 0 && p0 + kPos - 1 <= first_at - A.window && p0 >= A.sinks);
+        // 64 positions at a time: the next ones' scores and the last ones' product are computed meanwhile
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        ok = ok && mbar_wait_bounded(&bar.s_full[x][h], it & 1, kPromptTimeout);
-        if (!__all_sync(0xFFFFFFFFu, ok)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const unsigned th = ts + h * (kPos / 2);
-        if (kSplit && h == 0 && it > 0 && it % kFoldTiles == 0) {  // the next product begins anew
-          ok = mbar_wait_bounded(&bar.p_free[x][1], (it - 1) & 1, kPromptTimeout);
-          tc_fence_after();
-#pragma unroll 1
-          for (int c0 = 0; c0 < 2 * D; c0 += 32) {
-            const unsigned at_c = static_cast<unsigned>(c0 / 64 * 32) + (static_cast<unsigned>(c0 / 32 % 2 * 16) << 16);  // 32 columns of 16 rows
-            uint32_t o[16], f[16];
-            tmem_ld_16x256b_x4(to + at_c, o);
-            if (it > kFoldTiles) {
-              tmem_ld_16x256b_x4(tf + at_c, f);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float(f[j]));
-            }
-            tmem_st_16x256b_x4(tf + at_c, o);
+        for (int h = 0; h < 2; ++h) {
+          ok = ok && mbar_wait_bounded(&bar.s_full[x][h], it & 1, kPromptTimeout);
+          if (!__all_sync(0xFFFFFFFFu, ok)) {
+            ok = false;
+            break;
           }
-        }
-        const float4* const t4 = reinterpret_cast<const float4*>(terms) + 3 * (32 * h + c);  // of the pair c; every fourth is ours
-        if (none) {
-          uint32_t zero[16];
+          tc_fence_after();
+          const unsigned th = ts + h * (kPos / 2);
+          if (kSplit && h == 0 && it > 0 && it % kFoldTiles == 0) {  // the next product begins anew
+            ok = mbar_wait_bounded(&bar.p_free[x][1], (it - 1) & 1, kPromptTimeout);
+            tc_fence_after();
+#pragma unroll 1
+            for (int c0 = 0; c0 < 2 * D; c0 += 32) {
+              const unsigned at_c = static_cast<unsigned>(c0 / 64 * 32) + (static_cast<unsigned>(c0 / 32 % 2 * 16) << 16);  // 32 columns of 16 rows
+              uint32_t o[16], f[16];
+              tmem_ld_16x256b_x4(to + at_c, o);
+              if (it > kFoldTiles) {
+                tmem_ld_16x256b_x4(tf + at_c, f);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) zero[i] = 0u;
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float(f[j]));
+              }
+              tmem_st_16x256b_x4(tf + at_c, o);
+            }
+          }
+          const float4* const t4 = reinterpret_cast<const float4*>(terms) + 3 * (32 * h + c);  // of the pair c; every fourth is ours
+          if (none) {
+            uint32_t zero[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) zero[i] = 0u;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              tmem_st_16x128b_x8(th + (static_cast<unsigned>(16 * g) << 16), zero);
+              if constexpr (kSplit) tmem_st_16x128b_x8(th + kPos / 4 + (static_cast<unsigned>(16 * g) << 16), zero);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&bar.p_full[x][h]);
+            continue;
+          }
+          uint32_t s[2][32];  // [16 rows][4 pair + 2 (8 rows) + position], scores in place
+#pragma unroll
+          for (int g = 0; g < 2; ++g) tmem_ld_16x256b_x8_begin(th + (static_cast<unsigned>(16 * g) << 16), s[g]);
+          tmem_ld_end(s[0], s[1]);
+          if constexpr (!decltype(evenly)::value) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const float unit = row_units[kRowsX * x + row0x + 8 * n + r];
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int j = 4 * i + 2 * (n & 1) + e;
+                  s[n >> 1][j] = __float_as_uint(__uint_as_float(s[n >> 1][j]) * unit);
+                }
+            }
+          }
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 k = t4[12 * i];
+            const float2 e = *reinterpret_cast<const float2*>(&t4[12 * i + 1]);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const int j = 4 * i + 2 * (n & 1);
+              const float2 y = unpair(fma2(pair(__uint_as_float(s[n >> 1][j]), __uint_as_float(s[n >> 1][j + 1])), pair(k.x, k.y),
+                                           fma2(pair(sum_q[n], sum_q[n]), pair(k.z, k.w), pair(e.x, e.y))));
+              s[n >> 1][j] = __float_as_uint(y.x);
+              s[n >> 1][j + 1] = __float_as_uint(y.y);
+            }
+          }
+          if (!whole) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const int from = A.window > 0 ? at[n] - A.window : -1;
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int p = p0 + h * (kPos / 2) + 8 * i + 2 * c + e;
+                  if (p > at[n] || (p <= from && p >= A.sinks)) s[n >> 1][4 * i + 2 * (n & 1) + e] = 0xff800000u;
+                }
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              top[n] = max3(top[n], __uint_as_float(s[n >> 1][4 * i + 2 * (n & 1)]), __uint_as_float(s[n >> 1][4 * i + 2 * (n & 1) + 1]));
+          bool raise = false;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) raise |= top[n] > refs[n] + kRaise;  // the first seen position too: the reference is -inf
+          if (__any_sync(0xFFFFFFFFu, raise)) {
+            float corr[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              top[n] = fmaxf(top[n], __shfl_xor_sync(0xFFFFFFFFu, top[n], 1));
+              top[n] = fmaxf(top[n], __shfl_xor_sync(0xFFFFFFFFu, top[n], 2));
+              const float next = fmaxf(refs[n], top[n]);
+              corr[n] = next > refs[n] ? ex2(refs[n] - next) : 1.0f;
+              refs[n] = next;
+              sum2[n] = mul2(sum2[n], pair(corr[n], corr[n]));
+              off2[n] = mul2(off2[n], pair(corr[n], corr[n]));
+            }
+            if (it + h > 0) {  // the last 64 positions' product may be under way
+              ok = mbar_wait_bounded(&bar.p_free[x][h ^ 1], (it - (h ^ 1)) & 1, kPromptTimeout);
+              tc_fence_after();
+            }
+            auto rescale = [&](unsigned from) {
+#pragma unroll 1
+              for (int c0 = 0; c0 < D; c0 += 32)
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                  uint32_t o[16];
+                  const unsigned at_o = from + c0 + (static_cast<unsigned>(16 * g) << 16);
+                  tmem_ld_16x256b_x4(at_o, o);
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr[2 * g + ((j >> 1) & 1)]);
+                  tmem_st_16x256b_x4(at_o, o);
+                }
+            };
+            if (h > 0 || (kSplit ? it % kFoldTiles != 0 : it > 0)) rescale(to);
+            if (kSplit && it >= kFoldTiles) {
+              tmem_wait_st();
+              rescale(tf);
+            }
+          }
+          f32x2 minus[4];  // a row that has seen nothing yet: its weights are 2^-inf
+#pragma unroll
+          for (int n = 0; n < 4; ++n) minus[n] = refs[n] == -INFINITY ? pair(0.0f, 0.0f) : pair(-refs[n], -refs[n]);
+          uint32_t hi[2][16], lo[2][16];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 mu = reinterpret_cast<const float2*>(t4)[24 * i + 3];
+            const float4 uo = t4[12 * i + 2];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const int j = 4 * i + 2 * (n & 1);
+              const float2 d = unpair(add2(pair(__uint_as_float(s[n >> 1][j]), __uint_as_float(s[n >> 1][j + 1])), minus[n]));
+              const f32x2 pw = pair(ex2(d.x), ex2(d.y));
+              sum2[n] = fma2(pw, pair(uo.x, uo.y), sum2[n]);
+              off2[n] = fma2(pw, pair(uo.z, uo.w), off2[n]);
+              const float2 w = unpair(mul2(pw, pair(mu.x, mu.y)));
+              hi[n >> 1][2 * i + (n & 1)] = pack_f16(w.x, w.y);
+              if constexpr (kSplit) {
+                const float2 f = unpack_f16(hi[n >> 1][2 * i + (n & 1)]);
+                lo[n >> 1][2 * i + (n & 1)] = pack_f16(w.x - f.x, w.y - f.y);
+              }
+            }
+          }
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
-            tmem_st_16x128b_x8(th + (static_cast<unsigned>(16 * g) << 16), zero);
-            if constexpr (kSplit) tmem_st_16x128b_x8(th + kPos / 4 + (static_cast<unsigned>(16 * g) << 16), zero);
+            tmem_st_16x128b_x8(th + (static_cast<unsigned>(16 * g) << 16), hi[g]);
+            if constexpr (kSplit) tmem_st_16x128b_x8(th + kPos / 4 + (static_cast<unsigned>(16 * g) << 16), lo[g]);
           }
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&bar.p_full[x][h]);
-          continue;
         }
-        uint32_t s[2][32];  // [16 rows][4 pair + 2 (8 rows) + position], scores in place
-#pragma unroll
-        for (int g = 0; g < 2; ++g) tmem_ld_16x256b_x8_begin(th + (static_cast<unsigned>(16 * g) << 16), s[g]);
-        tmem_ld_end(s[0], s[1]);
-        if (!even) {
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const float unit = row_units[kRowsX * x + row0x + 8 * n + r];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int j = 4 * i + 2 * (n & 1) + e;
-                s[n >> 1][j] = __float_as_uint(__uint_as_float(s[n >> 1][j]) * unit);
-              }
-          }
-        }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 k = t4[12 * i];
-          const float2 e = *reinterpret_cast<const float2*>(&t4[12 * i + 1]);
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int j = 4 * i + 2 * (n & 1);
-            const float2 y = unpair(fma2(pair(__uint_as_float(s[n >> 1][j]), __uint_as_float(s[n >> 1][j + 1])), pair(k.x, k.y),
-                                         fma2(pair(sum_q[n], sum_q[n]), pair(k.z, k.w), pair(e.x, e.y))));
-            s[n >> 1][j] = __float_as_uint(y.x);
-            s[n >> 1][j + 1] = __float_as_uint(y.y);
-          }
-        }
-        if (!whole) {
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int from = A.window > 0 ? at[n] - A.window : -1;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int p = p0 + h * (kPos / 2) + 8 * i + 2 * c + e;
-                if (p > at[n] || (p <= from && p >= A.sinks)) s[n >> 1][4 * i + 2 * (n & 1) + e] = 0xff800000u;
-              }
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            top[n] = max3(top[n], __uint_as_float(s[n >> 1][4 * i + 2 * (n & 1)]), __uint_as_float(s[n >> 1][4 * i + 2 * (n & 1) + 1]));
-        bool raise = false;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) raise |= top[n] > refs[n] + kRaise;  // the first seen position too: the reference is -inf
-        if (__any_sync(0xFFFFFFFFu, raise)) {
-          float corr[4];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            top[n] = fmaxf(top[n], __shfl_xor_sync(0xFFFFFFFFu, top[n], 1));
-            top[n] = fmaxf(top[n], __shfl_xor_sync(0xFFFFFFFFu, top[n], 2));
-            const float next = fmaxf(refs[n], top[n]);
-            corr[n] = next > refs[n] ? ex2(refs[n] - next) : 1.0f;
-            refs[n] = next;
-            sum2[n] = mul2(sum2[n], pair(corr[n], corr[n]));
-            off2[n] = mul2(off2[n], pair(corr[n], corr[n]));
-          }
-          if (it + h > 0) {  // the last 64 positions' product may be under way
-            ok = mbar_wait_bounded(&bar.p_free[x][h ^ 1], (it - (h ^ 1)) & 1, kPromptTimeout);
-            tc_fence_after();
-          }
-          auto rescale = [&](unsigned from) {
-#pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32)
-#pragma unroll
-              for (int g = 0; g < 2; ++g) {
-                uint32_t o[16];
-                const unsigned at_o = from + c0 + (static_cast<unsigned>(16 * g) << 16);
-                tmem_ld_16x256b_x4(at_o, o);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr[2 * g + ((j >> 1) & 1)]);
-                tmem_st_16x256b_x4(at_o, o);
-              }
-          };
-          if (h > 0 || (kSplit ? it % kFoldTiles != 0 : it > 0)) rescale(to);
-          if (kSplit && it >= kFoldTiles) {
-            tmem_wait_st();
-            rescale(tf);
-          }
-        }
-        f32x2 minus[4];  // a row that has seen nothing yet: its weights are 2^-inf
-#pragma unroll
-        for (int n = 0; n < 4; ++n) minus[n] = refs[n] == -INFINITY ? pair(0.0f, 0.0f) : pair(-refs[n], -refs[n]);
-        uint32_t hi[2][16], lo[2][16];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 mu = reinterpret_cast<const float2*>(t4)[24 * i + 3];
-          const float4 uo = t4[12 * i + 2];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int j = 4 * i + 2 * (n & 1);
-            const float2 d = unpair(add2(pair(__uint_as_float(s[n >> 1][j]), __uint_as_float(s[n >> 1][j + 1])), minus[n]));
-            const f32x2 pw = pair(ex2(d.x), ex2(d.y));
-            sum2[n] = fma2(pw, pair(uo.x, uo.y), sum2[n]);
-            off2[n] = fma2(pw, pair(uo.z, uo.w), off2[n]);
-            const float2 w = unpair(mul2(pw, pair(mu.x, mu.y)));
-            hi[n >> 1][2 * i + (n & 1)] = pack_f16(w.x, w.y);
-            if constexpr (kSplit) {
-              const float2 f = unpack_f16(hi[n >> 1][2 * i + (n & 1)]);
-              lo[n >> 1][2 * i + (n & 1)] = pack_f16(w.x - f.x, w.y - f.y);
-            }
-          }
-        }
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          tmem_st_16x128b_x8(th + (static_cast<unsigned>(16 * g) << 16), hi[g]);
-          if constexpr (kSplit) tmem_st_16x128b_x8(th + kPos / 4 + (static_cast<unsigned>(16 * g) << 16), lo[g]);
-        }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&bar.p_full[x][h]);
+        if (!ok) break;
       }
-      if (!ok) break;
-    }
+    };
+    if (even) walk(std::true_type{});
+    else walk(std::false_type{});
     if (tiles > 0 && ok) {
       ok = mbar_wait_bounded(&bar.p_free[x][1], (tiles - 1) & 1, kPromptTimeout);
       ok = __all_sync(0xFFFFFFFFu, ok);
