@@ -333,10 +333,16 @@ int32_t ivb_kv4_read(const IvbKv4Cache* c, void* k, void* v, int32_t dtype, int6
                      void* stream);
 /* Attention of the rows' queries q [rows][heads][head_dim] over their sequences' caches into out (same shape
  * and type); query head h reads key/value head h / (heads / kv_heads). The row at position p sees positions
- * j <= p with j > p - window or j < sinks (window 0: all j <= p). out = sum_j softmax_j(scale q.k_j) v_j. */
+ * j <= p with j > p - window or j < sinks (window 0: all j <= p). out = sum_j softmax_j(scale q.k_j) v_j.
+ * A wait inside the prompts' kernel that runs out (2 s of wall time, in which the context may not have been scheduled) sets *error to
+ * IVB_ETIMEOUT; the rows that it concerns are then NaN. */
 int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
                           const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,
                           int32_t sinks, void* out, int64_t o_row, int64_t o_head, uint32_t* error, void* stream);
+/* Failure-detection probe: the same call, but the prompts' kernel issues no products and its waits run out after 1 ms. */
+int32_t ivb_probe_kv4_timeout(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
+                              const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,
+                              int32_t sinks, void* out, int64_t o_row, int64_t o_head, uint32_t* error, void* stream);
 
 /* Per-row max |x| (rows x n fp32) into amax [rows]; with ivb_quantize_rows_amax the quantisation of a
  * row-parallel shard uses the amax of the whole row (after an all-reduce MAX), so every shard's codes

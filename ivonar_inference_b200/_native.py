@@ -204,6 +204,7 @@ SIGNATURES = {
                                     c_float, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
     "ivb_decoder_check": (c_int32, [c_void_p, c_void_p]),
 }
+SIGNATURES["ivb_probe_kv4_timeout"] = SIGNATURES["ivb_kv4_attention"]
 
 _lib: ctypes.CDLL | None = None
 

@@ -599,13 +599,9 @@ int32_t launch_attention(const Kv4Attention& A, cudaStream_t stream) {
   }
 }
 
-}  // namespace
-}  // namespace ivb
-
-extern "C" int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
-                                     const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,
-                                     int32_t sinks, void* out, int64_t o_row, int64_t o_head, uint32_t* error, void* stream) {
-  using namespace ivb;
+int32_t attention_call(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads, const int32_t* starts,
+                       const int64_t* positions, int32_t rows, float scale, int32_t window, int32_t sinks, void* out, int64_t o_row,
+                       int64_t o_head, uint32_t* error, void* stream, bool withhold) {
   if (int32_t rc = check_kv4(c, "ivb_kv4_attention")) return rc;
   if (int32_t rc = check_kv4_rows(c, starts, positions, rows, dtype, "ivb_kv4_attention")) return rc;
   if (heads <= 0 || heads % c->kv_heads != 0) return fail(IVB_EINVAL, "ivb_kv4_attention: %d query heads over %d key/value heads", heads, c->kv_heads);
@@ -630,6 +626,8 @@ extern "C" int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_
   A.rows = rows;
   A.window = window;
   A.sinks = sinks;
+  A.wait_ns = withhold ? kKv4ProbeNs : kKv4WaitNs;
+  A.withhold = withhold;
   const int size = dtype == IVB_F32 ? 4 : 2;
   auto aligned = [&](const void* p, int64_t row, int64_t head) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row * size % 16 == 0 && head * size % 16 == 0;
@@ -650,3 +648,23 @@ extern "C" int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_
   if (dtype == IVB_F16) return launch_attention<__half>(A, s);
   return launch_attention<__nv_bfloat16>(A, s);
 }
+
+}  // namespace
+}  // namespace ivb
+
+extern "C" {
+
+int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
+                          const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window, int32_t sinks, void* out,
+                          int64_t o_row, int64_t o_head, uint32_t* error, void* stream) {
+  return ivb::attention_call(c, q, dtype, q_row, q_head, heads, starts, positions, rows, scale, window, sinks, out, o_row, o_head, error, stream,
+                             false);
+}
+
+int32_t ivb_probe_kv4_timeout(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
+                              const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window, int32_t sinks,
+                              void* out, int64_t o_row, int64_t o_head, uint32_t* error, void* stream) {
+  return ivb::attention_call(c, q, dtype, q_row, q_head, heads, starts, positions, rows, scale, window, sinks, out, o_row, o_head, error, stream, true);
+}
+
+}  // extern "C"

@@ -19,6 +19,7 @@
 namespace ivb {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr unsigned long long kKv4WaitNs = 2000000000ull, kKv4ProbeNs = 1000000ull;
 
 struct Kv4Attention {
   IvbKv4Cache cache;
@@ -38,6 +39,8 @@ struct Kv4Attention {
   // had ended then, with their writes in device memory, and a fence at its start keeps it from what an SM's cache may have from before.
   // The two write different rows. The first CTA waits at its end instead, so that who waits for this grid has waited for both.
   bool beside_prompts;
+  unsigned long long wait_ns;  // the longest wait within the prompts' kernel
+  bool withhold;               // issue no products, so that the waits for them run out (ivb_probe_kv4_timeout)
 };
 
 // Launch attributes: beside the end of the grid before, and clusters of C CTAs.

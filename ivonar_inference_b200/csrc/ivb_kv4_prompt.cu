@@ -36,7 +36,6 @@ constexpr int kRowsX = 128, kRowsCta = 256, kPos = 128;
 constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 32 * kSoftmaxWarps, kProducerWarps = 3, kProducers = 32 * kProducerWarps;
 constexpr int kIssueWarp = kSoftmaxWarps + kProducerWarps, kPromptThreads = 32 * (kIssueWarp + 1);
 constexpr int kTermSets = 3;  // terms(it + 2) are written when S(it) is done, so when nobody reads terms(it - 1) any more
-constexpr unsigned long long kPromptTimeout = 2000000000ull;
 constexpr float kWeightUnit = 64.0f;  // weights are at most 2 * 64 * 2^8 in fp16
 constexpr float kRaise = 8.0f;
 // A tile's rows share the queries' power of two (no multiplication of the scores by a row's own) unless one's largest is so far below
@@ -418,6 +417,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   auto terms_of = [&](int it) { return reinterpret_cast<float*>(smem + G::terms_at + it % kTermSets * G::term_bytes); };
   auto turn_of = [&](int it) { return static_cast<unsigned>(it / G::stages) & 1u; };  // parity of a stage's use
   bool ok = true;
+  auto wait_for = [&](unsigned long long* at, unsigned turn) { return mbar_wait_bounded(at, turn, A.wait_ns); };
 
   if (warp >= kSoftmaxWarps && warp < kIssueWarp) {
     // ---- producers: 16-position tiles in turn ----
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     if (tiles > 0) fetch(0, true);
     for (int it = 0; it < tiles; ++it) {
       fetch(it, false);
-      if (it >= G::stages && !mbar_wait_bounded(&bar.k_free[it % G::stages], turn_of(it) ^ 1u, kPromptTimeout)) {
+      if (it >= G::stages && !wait_for(&bar.k_free[it % G::stages], turn_of(it) ^ 1u)) {
         ok = false;
         break;
       }
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       fence_proxy_async();
       mbar_arrive(&bar.k_full[it % G::stages]);
       if (it + 1 < tiles) fetch(it + 1, true);
-      if (it >= G::stages && !mbar_wait_bounded(&bar.v_free[it % G::stages], turn_of(it) ^ 1u, kPromptTimeout)) {
+      if (it >= G::stages && !wait_for(&bar.v_free[it % G::stages], turn_of(it) ^ 1u)) {
         ok = false;
         break;
       }
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     }
   } else if (warp >= kIssueWarp) {
     // ---- the warp that issues the products: all its lanes take the same way (ok is the same in each) ----
-    auto wait = [&](unsigned long long* at, unsigned turn) { return __all_sync(0xFFFFFFFFu, mbar_wait_bounded(at, turn, kPromptTimeout)) != 0; };
+    auto wait = [&](unsigned long long* at, unsigned turn) { return __all_sync(0xFFFFFFFFu, wait_for(at, turn)) != 0; };
     const uint64_t q0 = smem_desc(smem_addr(smem + G::q_at), D / 8 * 128);
     const uint64_t k0 = smem_desc(smem_addr(smem + G::k_at), D / 8 * 128), v0 = smem_desc_mn(smem_addr(smem + G::v_at), D / 8 * 128);
     // Half h of tile it: its 64 columns of S_X, and with P_X in their place its 64 positions' part of O_X. Descriptors count
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       if (h == 1) umma_commit_warp(&bar.v_free[it % G::stages]);
     };
     if (tiles > 0) {
-      ok = wait(&bar.k_full[0], 0);
+      ok = wait(&bar.k_full[0], 0) && !A.withhold;
       if (ok) {
         issue_s(0, 0);
         issue_s(0, 1);
@@ -546,10 +546,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       if (ok) issue_o(it, 1);
       if (ok && it + 1 < tiles) issue_s(it + 1, 1);
     }
-    if (!ok) {  // let what was issued finish before shared and tensor memory go
-      umma_commit_warp(&bar.drain);
-      wait(&bar.drain, 0);
-    }
+    // what was issued ends before shared and tensor memory go, also where another warp's wait ran out
+    umma_commit_warp(&bar.drain);
+    ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&bar.drain, 0, kKv4WaitNs)) != 0 && ok;
   } else if (x < row_tiles) {
     // ---- softmax: a warp has 32 rows, a thread in each 8-row set the row r and every fourth pair of positions, so that a
     // position's terms are loaded once for four rows (loaded for each row they bound the kernel: 12 cycles of the SM's
@@ -585,25 +584,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     live_rows = __any_sync(0xFFFFFFFFu, live_rows);
     // a copy for each kind of rows: the test within costs a chunk 235 us in place of 230
     auto walk = [&](auto evenly) {
-      for (int it = 0; it < tiles; ++it) {
+      bool stop = false;  // the same in all lanes, where `ok` is each lane's own between two votes
+      for (int it = 0; it < tiles && !stop; ++it) {
         const int p0 = tile_of(it) * kPos;
         const float* terms = terms_of(it);
-        ok = mbar_wait_bounded(&bar.terms_full[it % kTermSets], static_cast<unsigned>(it / kTermSets) & 1u, kPromptTimeout);
+        ok = ok && wait_for(&bar.terms_full[it % kTermSets], static_cast<unsigned>(it / kTermSets) & 1u);
         // what the warp's rows see of the tile: all of it, or nothing (first_at, last_at: the lowest and highest, -1 among them)
         const bool whole = live_rows && first_at >= p0 + kPos - 1 && (A.window <= 0 || p0 > last_at - A.window || p0 <= A.sinks - kPos);
         const bool none = last_at < p0 || (A.window > 0 && p0 + kPos - 1 <= first_at - A.window && p0 >= A.sinks);
         // 64 positions at a time: the next ones' scores and the last ones' product are computed meanwhile
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
-          ok = ok && mbar_wait_bounded(&bar.s_full[x][h], it & 1, kPromptTimeout);
+          ok = ok && wait_for(&bar.s_full[x][h], it & 1);
           if (!__all_sync(0xFFFFFFFFu, ok)) {
             ok = false;
+            stop = true;
             break;
           }
           tc_fence_after();
           const unsigned th = ts + h * (kPos / 2);
           if (kSplit && h == 0 && it > 0 && it % kFoldTiles == 0) {  // the next product begins anew
-            ok = mbar_wait_bounded(&bar.p_free[x][1], (it - 1) & 1, kPromptTimeout);
+            ok = wait_for(&bar.p_free[x][1], (it - 1) & 1);
             tc_fence_after();
 #pragma unroll 1
             for (int c0 = 0; c0 < 2 * D; c0 += 32) {
@@ -698,7 +699,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
               off2[n] = mul2(off2[n], pair(corr[n], corr[n]));
             }
             if (it + h > 0) {  // the last 64 positions' product may be under way
-              ok = mbar_wait_bounded(&bar.p_free[x][h ^ 1], (it - (h ^ 1)) & 1, kPromptTimeout);
+              ok = ok && wait_for(&bar.p_free[x][h ^ 1], (it - (h ^ 1)) & 1);
               tc_fence_after();
             }
             auto rescale = [&](unsigned from) {
@@ -752,15 +753,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           tc_fence_before();
           mbar_arrive(&bar.p_full[x][h]);
         }
-        if (!ok) break;
       }
     };
     if (even) walk(std::true_type{});
     else walk(std::false_type{});
-    if (tiles > 0 && ok) {
-      ok = mbar_wait_bounded(&bar.p_free[x][1], (tiles - 1) & 1, kPromptTimeout);
-      ok = __all_sync(0xFFFFFFFFu, ok);
-    }
+    if (tiles > 0) ok = __all_sync(0xFFFFFFFFu, ok && wait_for(&bar.p_free[x][1], (tiles - 1) & 1)) != 0;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const float2 s = unpair(sum2[n]), f = unpair(off2[n]);
@@ -772,7 +769,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       if (c == 0) {
         const int row = kRowsX * x + row0x + 8 * n + r;
         refs_of[row] = refs[n];
-        totals[row] = l;
+        totals[row] = ok ? l : __uint_as_float(0x7fffffffu);  // a row whose wait ran out becomes NaN, in all of a cluster
         offsets[row] = o;
       }
     }
@@ -794,7 +791,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     }
   };
   if (C == 1) {
-    if (mine && ok) {
+    if (mine) {
       // through the place of its tile's queries, to leave in whole 16-byte chunks: 32 rows a warp
       const float total = totals[row], offset = offsets[row], inv = total == 0.0f ? 0.0f : 1.0f / total;
       uint4* const stage = reinterpret_cast<uint4*>(smem + G::q_at) + (32 * warp) * L;
@@ -802,7 +799,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 16) {
         uint32_t o[16];
-        if (tiles > 0) load_o(c0, o);
+        if (tiles > 0 && ok) load_o(c0, o);
+        else
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = 0u;
 #pragma unroll
         for (int c = 0; c < 16 / kPer; ++c) {
           union {
@@ -846,7 +846,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         uint32_t o[16];
         if (tiles > 0 && ok) load_o(c0, o);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) part[(c0 + j) * kRowsCta + row] = tiles > 0 ? __uint_as_float(o[j]) : 0.0f;
+        for (int j = 0; j < 16; ++j) part[(c0 + j) * kRowsCta + row] = tiles > 0 && ok ? __uint_as_float(o[j]) : 0.0f;
       }
     }
     cluster.sync();

@@ -76,7 +76,7 @@ class KV4Cache:
 
     def check(self) -> None:
         """Wait for the device; raises ValueError if a call since the last check met a row beyond the capacity, and KernelError
-        if a wait inside a kernel ran out (its rows' outputs are then not to be used)."""
+        if a wait inside a kernel ran out (the rows that it concerns are then NaN)."""
 
         if self.error is None:
             raise RuntimeError("this cache was made without an error word")

@@ -163,3 +163,39 @@ def test_idle_rows_may_hold_any_query(dim, group, counts, idle, dtype) -> None:
     for value in (0.0, 1e30, torch.finfo(T).max, math.inf, math.nan):
         q[~live] = torch.tensor(value).to(T).cuda()
         assert torch.equal(cache.attention(q, at, starts), want)
+
+
+# ---- waits that run out -------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim,kv_heads,counts", [(64, 2, [300, 1, 5]), (128, 40, [90] * 5 + [2]), (32, 1, [400]), (128, 1, [1, 1, 500])])
+def test_rows_whose_wait_ran_out_are_nan_and_reported(dim, kv_heads, counts, dtype) -> None:
+    """One CTA a tile of rows and clusters: no row of a prompt looks like a result, few rows are what they were, and the next call is."""
+    import ctypes
+
+    from ivonar_inference_b200 import KernelError, KV4Cache
+    from ivonar_inference_b200 import _native as native
+
+    T, batch = TYPES[dtype], len(counts)
+    cache = KV4Cache(batch, kv_heads, dim, 700)
+    filled(cache, [100 + n for n in counts], seed=dim)
+    at, starts = rows_of(batch, [100] * batch, counts)
+    q = torch.randn(sum(counts), kv_heads, dim, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(T)
+    want = cache.attention(q, at, starts)
+    out = torch.full_like(q, 3.0)
+    rc = native.library().ivb_probe_kv4_timeout(
+        ctypes.byref(native.IvbKv4Cache(cache.data.data_ptr(), batch, kv_heads, dim, 700)), q.data_ptr(), list(TYPES).index(dtype), *q.stride()[:2],
+        kv_heads, starts.data_ptr(), at.data_ptr(), q.shape[0], dim**-0.5, 0, 0, out.data_ptr(), *out.stride()[:2], cache.error.data_ptr(),
+        torch.cuda.current_stream().cuda_stream)
+    assert rc == native.IVB_OK
+    with pytest.raises(KernelError, match=str(native.IVB_ETIMEOUT)):
+        cache.check()
+    r0 = 0
+    for n in counts:
+        if n > 64:
+            assert bool(out[r0:r0 + n].isnan().all())
+        else:
+            assert torch.equal(out[r0:r0 + n], want[r0:r0 + n])
+        r0 += n
+    assert torch.equal(cache.attention(q, at, starts), want)
+    cache.check()
