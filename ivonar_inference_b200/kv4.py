@@ -160,8 +160,9 @@ class KV4Cache:
             v_row, v_head = self._values("out[1]", v, self.kv_heads, k.dtype)
             if v.shape[0] != k.shape[0] or rows not in (None, k.shape[0]):
                 raise ValueError("out and rows disagree")
-            for x in out:
-                _writable(x)
+            _writable(k)
+            _writable(v)
+            _apart(k, v)
             rows = k.shape[0]
         else:
             if rows is None:
@@ -210,7 +211,47 @@ class KV4Cache:
         return out
 
 
+def _places(x: Tensor) -> Tensor:
+    """The addresses of the rows of x [rows, heads, head_dim], ascending (int64 on the host)."""
+
+    rows, heads, _ = x.shape
+    row, head, _ = x.stride()
+    at = torch.arange(rows).mul_(row)[:, None] + torch.arange(heads).mul_(head)
+    return at.flatten().mul_(x.element_size()).add_(x.data_ptr()).sort().values
+
+
 def _writable(x: Tensor) -> None:
-    for axis in (0, 1):
-        if x.shape[axis] > 1 and x.stride(axis) < x.shape[2]:
-            raise ValueError("the rows of an output must not overlap")
+    """Refuses an output whose rows share memory."""
+
+    rows, heads, dim = x.shape
+    if rows == 0:
+        return
+    row, head, _ = x.stride()
+    # one axis within the other's step, as nearly every layout has it; else the rows one by one
+    if (heads == 1 or head >= dim) and (rows == 1 or row >= (heads - 1) * head + dim):
+        return
+    if (rows == 1 or row >= dim) and (heads == 1 or head >= (rows - 1) * row + dim):
+        return
+    at = _places(x)
+    if bool((at.diff() < dim * x.element_size()).any()):
+        raise ValueError("the rows of an output must not overlap")
+
+
+def _apart(a: Tensor, b: Tensor) -> None:
+    """Refuses two outputs of one shape and type that share memory."""
+
+    rows, heads, dim = a.shape
+    if rows == 0:
+        return
+    size = a.element_size()
+    first, second = (a, b) if a.data_ptr() <= b.data_ptr() else (b, a)
+    gap = second.data_ptr() - first.data_ptr()
+    row, head, _ = first.stride()
+    if gap >= ((rows - 1) * row + (heads - 1) * head + dim) * size:
+        return
+    # side by side in each row, as a fused projection has them
+    if first.stride() == second.stride() and ((heads - 1) * head + dim) * size <= gap <= (row - (heads - 1) * head - dim) * size:
+        return
+    at = torch.cat([_places(a), _places(b)]).sort().values
+    if bool((at.diff() < dim * size).any()):
+        raise ValueError("the outputs must not overlap")

@@ -199,3 +199,73 @@ def test_rows_whose_wait_ran_out_are_nan_and_reported(dim, kv_heads, counts, dty
         r0 += n
     assert torch.equal(cache.attention(q, at, starts), want)
     cache.check()
+
+
+# ---- outputs whose rows share memory ------------------------------------------------------------
+def _shared(x: torch.Tensor) -> bool:
+    """By the places of every value."""
+    rows, heads, dim = x.shape
+    row, head, channel = x.stride()
+    at = (torch.arange(rows)[:, None, None] * row + torch.arange(heads)[:, None] * head + torch.arange(dim) * channel).flatten()
+    return at.unique().numel() < at.numel()
+
+
+def test_overlapping_outputs_are_found() -> None:
+    """Every pair of strides of small outputs, and pairs of outputs, against the places of every value."""
+    from ivonar_inference_b200.kv4 import _apart, _writable
+
+    memory = torch.zeros(4096)
+    for rows, heads in ((1, 1), (1, 3), (3, 1), (2, 2), (3, 4), (4, 3)):
+        for row in (0, 1, 4, 7, 8, 9, 16, 24, 25, 32, 40, 64):
+            for head in (0, 1, 4, 7, 8, 9, 16, 24, 25, 32, 40, 64):
+                x = memory.as_strided((rows, heads, 8), (row, head, 1))
+                if _shared(x):
+                    with pytest.raises(ValueError, match="overlap"):
+                        _writable(x)
+                else:
+                    _writable(x)
+    for rows, heads in ((1, 1), (3, 2), (2, 3)):
+        for strides in ((8 * heads, 8), (16 * heads, 8), (8, 8 * rows), (16, 16 * rows), (24 * heads, 24)):
+            for other in (strides, (8 * heads, 8), (32 * heads, 16)):
+                for gap in (0, 1, 7, 8, 9, 16, 8 * heads, 8 * rows, 8 * rows * heads, 1000):
+                    a = memory.as_strided((rows, heads, 8), (*strides, 1))
+                    b = memory.as_strided((rows, heads, 8), (*other, 1), gap)
+                    places = torch.cat([torch.arange(4096).as_strided(t.shape, t.stride(), t.storage_offset()).flatten() for t in (a, b)])
+                    for pair in ((a, b), (b, a)):
+                        if places.unique().numel() < places.numel():
+                            with pytest.raises(ValueError, match="overlap"):
+                                _apart(*pair)
+                        else:
+                            _apart(*pair)
+    _writable(memory[:0].view(0, 2, 8))
+    _apart(memory[:0].view(0, 2, 8), memory[:0].view(0, 2, 8))
+
+
+@gpu
+def test_overlapping_outputs_are_refused() -> None:
+    from ivonar_inference_b200 import KV4Cache
+
+    cache = KV4Cache(3, 2, 64, 16)
+    at = torch.tensor([4, 5, 6], device="cuda")
+    memory = torch.zeros(4096, device="cuda")
+    q = torch.zeros(3, 2, 64, device="cuda")
+    for strides in ((64, 64, 1), (0, 64, 1), (128, 32, 1), (96, 64, 1)):
+        wrong = memory.as_strided((3, 2, 64), strides)
+        with pytest.raises(ValueError, match="overlap"):
+            cache.attention(q, at, out=wrong)
+        with pytest.raises(ValueError, match="overlap"):
+            cache.read(at, out=(q, wrong))
+        with pytest.raises(ValueError, match="overlap"):
+            cache.read(at, out=(wrong, q))
+    with pytest.raises(ValueError, match="overlap"):
+        cache.read(at, out=(q, q))
+    with pytest.raises(ValueError, match="overlap"):
+        cache.read(at, out=(memory[:384].view(3, 2, 64), memory[64:448].view(3, 2, 64)))
+    filled(cache, [10] * 3)
+    want = cache.read(at)
+    # rows within the step of heads, and keys and values side by side
+    turned = memory.as_strided((3, 2, 64), (64, 192, 1)), memory.as_strided((3, 2, 64), (64, 192, 1), 1024)
+    fused = memory[2048:].as_strided((3, 2, 64), (256, 64, 1)), memory[2048:].as_strided((3, 2, 64), (256, 64, 1), 2048 + 128)
+    for out in (turned, fused):
+        cache.read(at, out=out)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
