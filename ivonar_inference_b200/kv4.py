@@ -198,7 +198,10 @@ class KV4Cache:
             raise ValueError("window and sinks must not be negative")
         if out is None:
             out = torch.empty_like(q)
-            o_row, o_head, _ = out.stride()
+            o_row, o_head, channel = out.stride()
+            if channel != 1:  # of queries whose rows overlap, such as a sliding window's
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                o_row, o_head, _ = out.stride()
         else:
             o_row, o_head = self._values("out", out, heads, q.dtype)
             if out.shape[0] != rows:

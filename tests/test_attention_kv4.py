@@ -269,3 +269,19 @@ def test_overlapping_outputs_are_refused() -> None:
     for out in (turned, fused):
         cache.read(at, out=out)
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+# ---- queries whose rows overlap -----------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("rows,strides", [(4, (1, 64, 1)), (100, (1, 256, 1)), (100, (64, 1, 1)), (3, (2, 2, 1)), (100, (0, 0, 1)), (70, (64, 64, 1))])
+def test_queries_that_overlap(rows, strides) -> None:
+    """Sliding windows over one tensor: the result's channels are contiguous and its values those of the copied queries."""
+    from ivonar_inference_b200 import KV4Cache
+
+    cache = KV4Cache(1, 2, 64, 128)
+    filled(cache, [128])
+    memory = torch.randn(8192, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    q = memory.as_strided((rows, 2, 64), strides)
+    at, starts = rows_of(1, [5], [rows])
+    got, want = cache.attention(q, at, starts), cache.attention(q.contiguous(), at, starts)
+    assert got.stride(2) == 1 and torch.equal(got, want) and bool((want != 0).all())
