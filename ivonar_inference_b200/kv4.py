@@ -162,7 +162,7 @@ class KV4Cache:
                 raise ValueError("out and rows disagree")
             _writable(k)
             _writable(v)
-            _apart(k, v)
+            _apart(k, v, "the outputs")
             rows = k.shape[0]
         else:
             if rows is None:
@@ -186,7 +186,7 @@ class KV4Cache:
 
         `heads` is a multiple of `kv_heads`: query head h reads key/value head h // (heads // kv_heads). The row at position p
         sees the positions j <= p with j > p - window, and the first `sinks` positions (window 0: every j <= p). `scale` is
-        1 / sqrt(head_dim) by default. Products are summed and softmax statistics held in 32 bits.
+        1 / sqrt(head_dim) by default. `out` may be q itself, but not overlap it otherwise. Products are summed and softmax statistics held in 32 bits.
         """
 
         heads = q.shape[1] if q.ndim == 3 else 0
@@ -207,6 +207,8 @@ class KV4Cache:
             if out.shape[0] != rows:
                 raise ValueError("out and q disagree")
             _writable(out)
+            if out.data_ptr() != q.data_ptr() or out.stride() != q.stride():
+                _apart(out, q, "out and q")
         at = self._rows(rows, positions, starts)
         self._call("ivb_kv4_attention", self.lib.ivb_kv4_attention, self._ref, q.data_ptr(), _TYPES[q.dtype], q_row, q_head, heads,
                    at, positions.data_ptr(), rows, self.head_dim**-0.5 if scale is None else scale, window, sinks, out.data_ptr(), o_row,
@@ -240,8 +242,8 @@ def _writable(x: Tensor) -> None:
         raise ValueError("the rows of an output must not overlap")
 
 
-def _apart(a: Tensor, b: Tensor) -> None:
-    """Refuses two outputs of one shape and type that share memory."""
+def _apart(a: Tensor, b: Tensor, names: str) -> None:
+    """Refuses an output `a` that shares memory with `b`, another one or an input of the same shape and type."""
 
     rows, heads, dim = a.shape
     if rows == 0:
@@ -255,6 +257,8 @@ def _apart(a: Tensor, b: Tensor) -> None:
     # side by side in each row, as a fused projection has them
     if first.stride() == second.stride() and ((heads - 1) * head + dim) * size <= gap <= (row - (heads - 1) * head - dim) * size:
         return
-    at = torch.cat([_places(a), _places(b)]).sort().values
-    if bool((at.diff() < dim * size).any()):
-        raise ValueError("the outputs must not overlap")
+    at, other = _places(a), _places(b)
+    after = torch.searchsorted(at, other)
+    below, above = at[(after - 1).clamp(min=0)], at[after.clamp(max=at.numel() - 1)]
+    if bool(((other - below).abs() < dim * size).any()) or bool(((above - other).abs() < dim * size).any()):
+        raise ValueError(f"{names} must not overlap")

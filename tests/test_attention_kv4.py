@@ -234,11 +234,11 @@ def test_overlapping_outputs_are_found() -> None:
                     for pair in ((a, b), (b, a)):
                         if places.unique().numel() < places.numel():
                             with pytest.raises(ValueError, match="overlap"):
-                                _apart(*pair)
+                                _apart(*pair, "outputs")
                         else:
-                            _apart(*pair)
+                            _apart(*pair, "outputs")
     _writable(memory[:0].view(0, 2, 8))
-    _apart(memory[:0].view(0, 2, 8), memory[:0].view(0, 2, 8))
+    _apart(memory[:0].view(0, 2, 8), memory[:0].view(0, 2, 8), "outputs")
 
 
 @gpu
@@ -285,3 +285,27 @@ def test_queries_that_overlap(rows, strides) -> None:
     at, starts = rows_of(1, [5], [rows])
     got, want = cache.attention(q, at, starts), cache.attention(q.contiguous(), at, starts)
     assert got.stride(2) == 1 and torch.equal(got, want) and bool((want != 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 90])
+def test_an_output_is_the_queries_or_apart_from_them(rows) -> None:
+    from ivonar_inference_b200 import KV4Cache
+
+    cache = KV4Cache(1, 2, 64, 128)
+    filled(cache, [128])
+    at, starts = rows_of(1, [20], [rows])
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    memory = torch.randn(rows + 2, 8, 64, generator=gen, device="cuda")
+    q = memory[:rows, :4]
+    want = cache.attention(q, at, starts)
+    for wrong in (memory[1:rows + 1, :4], memory[:rows, 1:5], memory[:rows, 3:7], memory[:rows, :4].transpose(0, 1).reshape(-1)[:0]):
+        with pytest.raises(ValueError):
+            cache.attention(q, at, starts, out=wrong)
+    narrow = torch.randn(rows * 4 * 64 + 64, generator=gen, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        cache.attention(narrow[:-64].view(rows, 4, 64), at, starts, out=narrow[64:].view(rows, 4, 64))
+    # an input whose own rows overlap, and an output beside it
+    assert cache.attention(narrow[:256].view(1, 4, 64).expand(rows, 4, 64), at, starts, out=memory[:rows, 4:]).data_ptr() == memory[:, 4:].data_ptr()
+    for out in (memory[:rows, 4:], q):
+        assert torch.equal(cache.attention(q, at, starts, out=out), want) and torch.equal(out, want)
