@@ -54,7 +54,7 @@ __device__ __forceinline__ bool kv4_place(const IvbKv4Cache& C, const int32_t* s
                                           int& b, int64_t& pos) {
   b = kv4_sequence(starts, C.batch, row);
   if (b >= C.batch) return false;
-  pos = positions[b] + (starts == nullptr ? 0 : row - starts[b]);
+  pos = kv4_position(positions, b) + (starts == nullptr ? 0 : row - starts[b]);
   if (pos >= C.max_len && (threadIdx.x & 31) == 0 && error != nullptr) atomicCAS(error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
   return pos >= 0 && pos < C.max_len;
 }

@@ -49,6 +49,9 @@ __device__ __forceinline__ int kv4_sequence(const int32_t* starts, int batch, in
   return row < *starts ? batch : before;
 }
 
+// The position of a sequence's first row; far beyond any capacity it stays so for all of its rows.
+__device__ __forceinline__ int64_t kv4_position(const int64_t* positions, int b) { return min(positions[b], static_cast<int64_t>(1) << 62); }
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T x);
 template <>

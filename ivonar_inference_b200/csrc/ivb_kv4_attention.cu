@@ -107,7 +107,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
   const int items = max(count, 0) * A.group, i0 = tile * R;
   if (i0 >= items || items > A.few) return;  // the whole cluster
   const int live = min(R, items - i0);
-  const int64_t base = A.positions[b];
+  const int64_t base = kv4_position(A.positions, b);
   const int max_len = A.cache.max_len;
   // token and query head of an item of the sequence's head group
   auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };

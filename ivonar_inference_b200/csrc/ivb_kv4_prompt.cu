@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     count = min(A.rows, A.starts[b + 1]) - row0;
   }
   const int i0 = which[1] * G::rows, live = min(G::rows, count * A.group - i0), row_tiles = live > kRowsX ? 2 : 1;
-  const int64_t base = A.positions[b];
+  const int64_t base = kv4_position(A.positions, b);
   const int max_len = A.cache.max_len;
   const unsigned group_size = static_cast<unsigned>(A.group);
   auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };

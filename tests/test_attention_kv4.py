@@ -309,3 +309,37 @@ def test_an_output_is_the_queries_or_apart_from_them(rows) -> None:
     assert cache.attention(narrow[:256].view(1, 4, 64).expand(rows, 4, 64), at, starts, out=memory[:rows, 4:]).data_ptr() == memory[:, 4:].data_ptr()
     for out in (memory[:rows, 4:], q):
         assert torch.equal(cache.attention(q, at, starts, out=out), want) and torch.equal(out, want)
+
+
+# ---- positions and rows at the ends of their ranges ---------------------------------------------
+@gpu
+@pytest.mark.parametrize("rows", [3, 100])
+@pytest.mark.parametrize("position", [2**63 - 1, 2**63 - 2, 2**62, 2**31 - 1, -(2**63)])
+def test_positions_at_the_ends_of_their_range(position, rows) -> None:
+    from ivonar_inference_b200 import KV4Cache
+
+    cache = KV4Cache(2, 2, 64, 128)
+    filled(cache, [128, 128])
+    before = cache.data.clone()
+    at, starts = rows_of(2, [position, 20], [rows, 2])
+    x = torch.randn(rows + 2, 2, 64, device="cuda")
+    want = cache.attention(x[rows:], torch.tensor([200, 20], device="cuda"), torch.tensor([0, 0, 2], dtype=torch.int32, device="cuda"))
+    cache.check()
+
+    def reported():
+        if position < 0:
+            cache.check()
+        else:
+            with pytest.raises(ValueError, match="capacity"):
+                cache.check()
+
+    y = cache.attention(x, at, starts)
+    reported()
+    assert bool((y[:rows] == 0).all()) and torch.equal(y[rows:], want)
+    out = torch.full_like(x, 9.0), torch.full_like(x, 9.0)
+    cache.read(at, starts, out=out)
+    reported()
+    assert all(bool((o[:rows] == 9.0).all()) and bool((o[rows:] != 9.0).any()) for o in out)
+    cache.append(x, x, at, starts)
+    reported()
+    assert torch.equal(cache.data[0], before[0])
