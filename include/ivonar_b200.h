@@ -312,7 +312,8 @@ int32_t ivb_batch_sample_merge(const uint32_t* keys, const int32_t* ids, int32_t
  * Rows of a call: sequence b holds rows starts[b] .. starts[b + 1] - 1 (device int32 [batch + 1], ascending)
  * at positions positions[b], positions[b] + 1, ... (device int64 [batch]); starts NULL: row b is sequence
  * b's only row (rows == batch). `rows` is the number of rows that the arrays have; rows from starts[batch]
- * on are left as they are. A row at a negative position is idle: it is not written, not read, and attends to
+ * on are left as they are, and so are those before starts[0]. Rows of a sequence beyond either end of the arrays (negative starts: the
+ * call has a part of the rows that starts counts) are not there and keep the others' positions. A row at a negative position is idle: it is not written, not read, and attends to
  * nothing (zeros). A row at max_len or beyond sets *error (device word, may be NULL) to IVB_ECAPACITY and is
  * treated the same way. `dtype` is IVB_F32, IVB_F16 or IVB_BF16; strides are in values, channels contiguous.
  * Nothing is allocated and nothing is kept between calls; calls on one cache are ordered by their stream. */

@@ -100,14 +100,16 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
   const unsigned sh = cluster_id / static_cast<unsigned>(tiles_per_sequence);
   const int b = static_cast<int>(sh / static_cast<unsigned>(A.cache.kv_heads)), kvh = static_cast<int>(sh) - b * A.cache.kv_heads;
   int row0 = b, count = 1;
+  int64_t before = 0;  // rows of the sequence that the call does not have
   if (A.starts != nullptr) {
     row0 = max(0, A.starts[b]);
+    before = static_cast<int64_t>(row0) - A.starts[b];
     count = min(A.rows, A.starts[b + 1]) - row0;
   }
   const int items = max(count, 0) * A.group, i0 = tile * R;
   if (i0 >= items || items > A.few) return;  // the whole cluster
   const int live = min(R, items - i0);
-  const int64_t base = kv4_position(A.positions, b);
+  const int64_t base = kv4_position(A.positions, b) + before;
   const int max_len = A.cache.max_len;
   // token and query head of an item of the sequence's head group
   auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };

@@ -266,12 +266,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     pdl_trigger();  // not before this CTA has its tensor memory: the next grid may take some too, and waits for this one
   }
   int row0 = b, count = 1;
+  int64_t before = 0;  // rows of the sequence that the call does not have
   if (A.starts != nullptr) {
     row0 = max(0, A.starts[b]);
+    before = static_cast<int64_t>(row0) - A.starts[b];
     count = min(A.rows, A.starts[b + 1]) - row0;
   }
   const int i0 = which[1] * G::rows, live = min(G::rows, count * A.group - i0), row_tiles = live > kRowsX ? 2 : 1;
-  const int64_t base = kv4_position(A.positions, b);
+  const int64_t base = kv4_position(A.positions, b) + before;
   const int max_len = A.cache.max_len;
   const unsigned group_size = static_cast<unsigned>(A.group);
   auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };

@@ -7,8 +7,9 @@ token per sequence, a few drafted ones, whole prompts, or all of these in one ca
 
 A call's rows are those of its tensors' first axis. With `starts` (int32 [batch + 1] on the device, ascending) rows
 `starts[b] .. starts[b + 1] - 1` belong to sequence `b` and hold its positions `positions[b], positions[b] + 1, ...`
-(int64 [batch] on the device); without it there is one row per sequence. Rows from `starts[batch]` on are left as they are. A row
-at a negative position is idle: nothing is written or read for it and its attention is zero. A row at `max_len` or
+(int64 [batch] on the device); without it there is one row per sequence. Rows from `starts[batch]` on are left as they are.
+Rows that `starts` counts beyond either end of the tensors are not there (a call may have a part of the rows, with `starts` less the
+number of those before it). A row at a negative position is idle: nothing is written or read for it and its attention is zero. A row at `max_len` or
 beyond is treated the same way and reported by `check`. A token is attended to once it is written: `append` first,
 then `attention`, on one stream.
 

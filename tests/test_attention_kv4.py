@@ -343,3 +343,35 @@ def test_positions_at_the_ends_of_their_range(position, rows) -> None:
     cache.append(x, x, at, starts)
     reported()
     assert torch.equal(cache.data[0], before[0])
+
+
+@gpu
+@pytest.mark.parametrize("counts,cuts", [([3, 1, 5], [2, 6]), ([200, 1, 150, 40], [70, 201, 230, 300]), ([400], [1, 300])])
+def test_a_call_in_parts(counts, cuts) -> None:
+    """Slices of a call's rows with starts less the rows before: every part is what the whole call has there."""
+    from ivonar_inference_b200 import KV4Cache
+
+    batch, rows = len(counts), sum(counts)
+    whole, parts = (KV4Cache(batch, 2, 64, 600) for _ in range(2))
+    at, starts = rows_of(batch, [50] * batch, counts)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v = torch.randn(3, rows, 2, 64, generator=gen, device="cuda")
+    for cache in (whole, parts):
+        filled(cache, [50] * batch)
+    whole.append(k, v, at, starts)
+    bounds = list(zip([0] + cuts, cuts + [rows]))
+    for a, b in bounds:
+        parts.append(k[a:b], v[a:b], at, starts - a)
+    assert torch.equal(parts.data, whole.data)
+    want, held_ = whole.attention(q, at, starts), whole.read(at, starts, rows)
+    kk, vv, par = contents(whole.data, 64)
+    most, vmax = float((par[..., 1].abs() + 15 * par[..., 0]).max()), float(vv.abs().max())
+    for a, b in bounds:
+        for got, expected in zip(parts.read(at, starts - a, b - a), held_):
+            assert torch.equal(got, expected[a:b])
+        got = parts.attention(q[a:b], at, starts - a)
+        # other kernels and splits: both within the tolerance of the exact result
+        tol = tolerance(q, most, vmax, 0.125, want[a:b].double().cpu(), torch.float32)
+        assert bool(((got - want[a:b]).abs().double().cpu() <= 2 * tol).all())
+    whole.check()
+    parts.check()
