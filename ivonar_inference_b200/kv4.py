@@ -95,6 +95,8 @@ class KV4Cache:
         if (positions.dtype is not torch.int64 or positions.shape != self._sequences or positions.device != self.device
                 or not positions.is_contiguous()):
             raise ValueError(f"positions must be an int64 tensor [{self.batch}] on {self.device}")
+        if rows >= 2**31:
+            raise ValueError(f"{rows} rows in one call")
         if starts is None:
             if rows != self.batch:
                 raise ValueError(f"{rows} rows for {self.batch} sequences need starts")

@@ -375,3 +375,17 @@ def test_a_call_in_parts(counts, cuts) -> None:
         assert bool(((got - want[a:b]).abs().double().cpu() <= 2 * tol).all())
     whole.check()
     parts.check()
+
+
+@gpu
+def test_more_rows_than_32_bits_count_are_refused() -> None:
+    from ivonar_inference_b200 import KV4Cache
+
+    cache = KV4Cache(1, 1, 64, 16)
+    at, starts = rows_of(1, [0], [5])
+    x = torch.ones(1, 1, 64, device="cuda")
+    for rows in (2**31, 2**32 + 1):
+        many = x.expand(rows, 1, 64)
+        with pytest.raises(ValueError, match="rows"):
+            cache.append(many, many, at, starts)
+    assert bool((cache.data == 0).all())
