@@ -23,6 +23,7 @@ import ctypes
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _native as native
 
@@ -121,6 +122,8 @@ class KV4Cache:
             raise ValueError(f"the channels of {name} must be contiguous")
         if x.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires a gradient: the 4-bit cache has none")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+            raise ValueError(f"{name} has a tangent: the 4-bit cache has none")
         return row, head
 
     def _call(self, what: str, function, *args) -> None:

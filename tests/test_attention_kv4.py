@@ -389,3 +389,29 @@ def test_more_rows_than_32_bits_count_are_refused() -> None:
         with pytest.raises(ValueError, match="rows"):
             cache.append(many, many, at, starts)
     assert bool((cache.data == 0).all())
+
+
+@gpu
+def test_dual_tensors_are_refused() -> None:
+    """Forward-mode tangents would be lost; transforms of torch.func have no storage to read."""
+    from torch.autograd import forward_ad
+
+    from ivonar_inference_b200 import KV4Cache
+
+    cache = KV4Cache(2, 2, 64, 16)
+    at = torch.tensor([0, 0], device="cuda")
+    x = torch.ones(2, 2, 64, device="cuda")
+    with forward_ad.dual_level():
+        cache.append(x, x, at)
+        before = cache.data.clone()
+        dual = forward_ad.make_dual(x, x)
+        for grad in (torch.enable_grad, torch.no_grad):
+            with grad():
+                for call in (lambda: cache.append(dual, x, at), lambda: cache.append(x, dual, at), lambda: cache.attention(dual, at)):
+                    with pytest.raises(ValueError, match="tangent"):
+                        call()
+        assert torch.isfinite(cache.attention(x, at)).all()
+    for transform in (lambda f: torch.func.jvp(f, (x,), (x,)), lambda f: torch.func.grad(lambda y: f(y).sum())(x), lambda f: torch.func.vmap(f)(x[None])):
+        with pytest.raises((ValueError, RuntimeError)):
+            transform(lambda y: cache.attention(y, at))
+    assert torch.equal(cache.data, before)
