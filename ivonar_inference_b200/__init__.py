@@ -13,8 +13,9 @@ __all__ = ["B200Decoder", "KV4Cache", "KernelError", "build_decoder"]
 
 
 def __getattr__(name: str):
-    if name in ("B200Decoder", "build_decoder"):
-        from . import decoder
+    if name in ("B200Decoder", "build_decoder", "decoder", "_reference"):
+        import importlib
 
-        return getattr(decoder, name)
+        found = importlib.import_module("._reference" if name == "_reference" else ".decoder", __name__)
+        return found if name in ("decoder", "_reference") else getattr(found, name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
