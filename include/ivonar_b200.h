@@ -324,11 +324,12 @@ typedef struct IvbKv4Cache {
 } IvbKv4Cache;
 uint64_t ivb_kv4_bytes(int32_t batch, int32_t kv_heads, int32_t head_dim, int32_t max_len);
 /* Quantises key and value rows k, v [rows][kv_heads][head_dim] into the cache. A row with an infinity or a
- * NaN reads back as NaN; values beyond +-65504 are clipped. */
+ * NaN reads back as NaN. The offset is clipped to +-65504 and the scale to 65504; values below the offset or above offset + 15 scale are
+ * clipped to these. */
 int32_t ivb_kv4_append(const IvbKv4Cache* c, const void* k, const void* v, int32_t dtype, int64_t k_row, int64_t k_head,
                        int64_t v_row, int64_t v_head, const int32_t* starts, const int64_t* positions, int32_t rows,
                        uint32_t* error, void* stream);
-/* The rows as the cache holds them, into k, v [rows][kv_heads][head_dim]. */
+/* The rows as the cache holds them, into k, v [rows][kv_heads][head_dim]; what passes fp16 (offset + 15 scale can) is infinity there. */
 int32_t ivb_kv4_read(const IvbKv4Cache* c, void* k, void* v, int32_t dtype, int64_t k_row, int64_t k_head, int64_t v_row,
                      int64_t v_head, const int32_t* starts, const int64_t* positions, int32_t rows, uint32_t* error,
                      void* stream);

@@ -139,7 +139,8 @@ class KV4Cache:
     def append(self, k: Tensor, v: Tensor, positions: Tensor, starts: Tensor | None = None) -> None:
         """Quantise the key and value rows k, v [rows, kv_heads, head_dim] (fp32, fp16 or bf16) into the cache.
 
-        A row that holds an infinity or a NaN reads back as NaN; values beyond +-65504 are clipped.
+        A row that holds an infinity or a NaN reads back as NaN. The row's offset (its least value) is clipped to +-65504 and its
+        scale to 65504: values below the offset, or above it by more than 15 times the scale, are clipped to that.
         """
 
         k_row, k_head = self._values("k", k, self.kv_heads)
@@ -157,7 +158,8 @@ class KV4Cache:
 
         `rows` is the number of rows (`batch` by default; with `starts`, which lies on the device, it has to be given) or
         comes with `out`, a pair of tensors to write to; rows that the call does not read are left as they are there, and
-        hold nothing of use without `out`.
+        hold nothing of use without `out`. A row holds offset + 15 scale at most, which in fp16 may be infinity: a row from -65504
+        to 65504 has the scale 8736 and holds 65536.
         """
 
         if out is not None:
@@ -193,6 +195,7 @@ class KV4Cache:
         `heads` is a multiple of `kv_heads`: query head h reads key/value head h // (heads // kv_heads). The row at position p
         sees the positions j <= p with j > p - window, and the first `sinks` positions (window 0: every j <= p). `scale` is
         1 / sqrt(head_dim) by default. `out` may be q itself, but not overlap it otherwise. Products are summed and softmax statistics held in 32 bits.
+        Values that pass fp16 (see `read`) may give infinity in an fp16 result.
         """
 
         heads = q.shape[1] if q.ndim == 3 else 0

@@ -415,3 +415,26 @@ def test_dual_tensors_are_refused() -> None:
         with pytest.raises((ValueError, RuntimeError)):
             transform(lambda y: cache.attention(y, at))
     assert torch.equal(cache.data, before)
+
+
+# ---- rows at the ends of the types --------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_rows_of_the_whole_range(dtype) -> None:
+    """What is clipped and what is not: the offset to +-65504, the scale to 65504, values to offset and offset + 15 scale."""
+    from ivonar_inference_b200 import KV4Cache
+
+    T = TYPES[dtype]
+    ends = [(-65504.0, 65504.0)]
+    if dtype != "fp16":
+        ends += [(0.0, 2.0**20), (-(2.0**20), 1.0), (1e5, 2e5), (-3e38, 3e38)]
+    x = torch.stack([torch.linspace(0, 1, 64, dtype=torch.float64) * (high - low) + low for low, high in ends])[:, None].to(T).cuda()
+    cache = KV4Cache(1, 1, 64, 8)
+    at, starts = rows_of(1, [0], [len(ends)])
+    cache.append(x, -x, at, starts)
+    want = held(x)[:, 0], held(-x)[:, 0]
+    assert float(want[0][0].max()) == 65536.0 and (dtype == "fp16" or float(want[0][4].max()) == 65504.0 * 14)
+    for out in TYPES.values():
+        for got, w in zip(cache.read(at, starts, len(ends), dtype=out), want):
+            assert torch.equal(got[:, 0].cpu(), w.float().to(out))
+    assert bool(cache.read(at, starts, len(ends), dtype=torch.float16)[0][0].isinf().any())
