@@ -335,7 +335,8 @@ int32_t ivb_kv4_read(const IvbKv4Cache* c, void* k, void* v, int32_t dtype, int6
                      void* stream);
 /* Attention of the rows' queries q [rows][heads][head_dim] over their sequences' caches into out (same shape
  * and type); query head h reads key/value head h / (heads / kv_heads). The row at position p sees positions
- * j <= p with j > p - window or j < sinks (window 0: all j <= p). out = sum_j softmax_j(scale q.k_j) v_j.
+ * j <= p with j > p - window or j < sinks (window 0: all j <= p). out = sum_j softmax_j(scale q.k_j) v_j, summed
+ * in 32 bits; 16-bit queries: with weights rounded to fp16, but for single tokens (starts NULL) of up to four heads a key/value head.
  * A wait inside the prompts' kernel that runs out (2 s of wall time, in which the context may not have been scheduled) sets *error to
  * IVB_ETIMEOUT; the rows that it concerns are then NaN. */
 int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,

@@ -195,6 +195,8 @@ class KV4Cache:
         `heads` is a multiple of `kv_heads`: query head h reads key/value head h // (heads // kv_heads). The row at position p
         sees the positions j <= p with j > p - window, and the first `sinks` positions (window 0: every j <= p). `scale` is
         1 / sqrt(head_dim) by default. `out` may be q itself, but not overlap it otherwise. Products are summed and softmax statistics held in 32 bits.
+        With fp32 queries the softmax's weights keep 22 bits; with fp16 and bf16 ones they are rounded to fp16 (by 2^-11 of each at most)
+        before they meet the values, but for single tokens with up to four query heads a key/value head.
         Values that pass fp16 (see `read`) may give infinity in an fp16 result.
         """
 

@@ -438,3 +438,58 @@ def test_rows_of_the_whole_range(dtype) -> None:
         for got, w in zip(cache.read(at, starts, len(ends), dtype=out), want):
             assert torch.equal(got[:, 0].cpu(), w.float().to(out))
     assert bool(cache.read(at, starts, len(ends), dtype=torch.float16)[0][0].isinf().any())
+
+
+# ---- how near the result is, by its norm --------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim,kv_heads,group,first,counts,window,sinks", [
+    (64, 2, 1, [700, 30, 299], None, 0, 0),
+    (128, 2, 4, [511, 64], None, 200, 4),
+    (32, 2, 8, [400, 65, 7, 260], None, 0, 0),
+    (128, 1, 16, [300, 511], None, 0, 0),
+    (64, 2, 3, [200, 0, 77], [4, 7, 2], 0, 0),
+    (64, 6, 2, [0, 130, 300], [250, 1, 40], 0, 0),
+    (128, 2, 1, [300, 0], [150, 400], 120, 3),
+    (32, 1, 4, [64], [200], 0, 0),
+])
+def test_errors_by_their_norm(dim, kv_heads, group, first, counts, window, sinks, dtype) -> None:
+    """All outputs of a call against 64 bits. The scores here are sums of absolute products of up to about 16, each off by 2^-22 of that, in
+    both directions as their parts are; with the weights' split and the sums that is 2^-18 of the output, and twice that is allowed
+    (a weight held in 11 bits alone would be off by 2^-13 of it). 16 bits: a weight p_j is off by a rounding of 2^-11 at most, apart from the
+    others', on values s (u - c) about the codes' middle, and the result by half a step of its type: the norms of
+    2^-11 sqrt(sum_j (p_j s_j (u_j - c_j))^2) and of eps / 2 of the output are added, whose expected sizes are 0.58 of these."""
+    from ivonar_inference_b200 import KV4Cache
+
+    T, batch = TYPES[dtype], len(first)
+    n = [1] * batch if counts is None else counts
+    total = [a + c for a, c in zip(first, n)]
+    cache = KV4Cache(batch, kv_heads, dim, max(total))
+    filled(cache, total, seed=dim + group, spread=0.3)
+    at, starts = rows_of(batch, first, n)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(sum(n), kv_heads * group, dim, generator=gen, device="cuda").to(T)
+    got = cache.attention(q, at, None if counts is None else starts, window=window, sinks=sinks).double().cpu()
+    kk, vv, par = contents(cache.data, dim)
+    error = size = rounding = 0.0
+    r0 = 0
+    for b in range(batch):
+        L, mine = total[b], torch.arange(first[b], total[b])[:, None]
+        where = torch.arange(L)
+        hidden = where > mine
+        if window:
+            hidden |= (where <= mine - window) & (where >= sinks)
+        x = q[r0:r0 + n[b]].double().cpu().unflatten(1, (kv_heads, group))
+        score = torch.einsum("nhgd,hjd->hgnj", x, kk[b, :, :L]) * dim**-0.5
+        weight = torch.softmax(score.masked_fill(hidden, -math.inf), -1)
+        value, scale, offset = vv[b, :, :L], par[b, :, :L, 2:3], par[b, :, :L, 3:4]
+        want = torch.einsum("hgnj,hjd->nhgd", weight, value).flatten(1, 2)
+        about = value - offset - scale * (8.0 - (where % 2)[:, None])
+        error += float(((got[r0:r0 + n[b]] - want) ** 2).sum())
+        size += float((want**2).sum())
+        rounding += float(torch.einsum("hgnj,hjd->nhgd", weight**2, about**2).sum())
+        r0 += n[b]
+    bound = 2.0**-17 * size**0.5
+    if T != torch.float32:
+        bound += 2.0**-11 * rounding**0.5 + torch.finfo(T).eps / 2 * size**0.5
+    assert error**0.5 <= bound, (error**0.5 / size**0.5, bound / size**0.5)
