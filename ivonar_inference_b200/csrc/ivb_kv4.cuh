@@ -1,4 +1,4 @@
-// Layout and row lookup of the 4-bit key/value cache, shared by its kernels (ivb_kv4.cu, ivb_kv4_attention.cu).
+// Layout and row lookup of the 4-bit key/value cache, shared by its kernels (ivb_kv4.cu, ivb_kv4_attention.cu, ivb_kv4_prompt.cu).
 //
 // A row x of D values (one position of one key/value head) is kept as codes u in 0..15 with one fp16 scale s and
 // one fp16 offset m, x ~ m + s u. Sixteen positions of one head form a tile of 16 (D + 8) bytes:

@@ -1,5 +1,5 @@
-// tcgen05 (5th-generation tensor core) helpers shared by the prefill GEMM (ivb_gemm.cu) and the prefill
-// attention (ivb_prefill.cu): shared-memory matrix descriptors, MMA issue and commit, tensor-memory
+// tcgen05 (5th-generation tensor core) helpers shared by the prefill GEMM (ivb_gemm.cu), the prefill
+// attention (ivb_prefill.cu) and the 4-bit cache's attention for prompts (ivb_kv4_prompt.cu): shared-memory matrix descriptors, MMA issue and commit, tensor-memory
 // loads and stores, mbarrier transaction counts.
 #pragma once
 
@@ -69,16 +69,6 @@ __device__ __forceinline__ void tmem_st32(unsigned taddr, const uint32_t (&v)[32
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
       "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
-
-// 16 columns of this warp's lanes from 16 registers.
-__device__ __forceinline__ void tmem_st16(unsigned taddr, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 
