@@ -309,7 +309,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
 #pragma unroll
         for (int s = 0; s < kSets; ++s) {
           const float dot = kSplit ? s2[s][2 * h] + s2[s][2 * h + 1] : s2[s >> 1][2 * h + (s & 1)];
-          x[s][2 * t + h] = fmaf(dot * row_unit[s], pt.x, fmaf(sum_q[s], pt.y, pt.z));
+          x[s][2 * t + h] = fmaf(dot, row_unit[s] * pt.x, fmaf(sum_q[s], pt.y, pt.z));  // (dot * row_unit could overflow)
         }
       }
     }

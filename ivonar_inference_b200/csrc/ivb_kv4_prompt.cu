@@ -369,13 +369,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   }
   const bool even = least >= most * kEven;
   const int up = query_power(most);
-  // of the scores, in the positions' terms or (uneven) for each row
-  const float score_unit = even ? power_of_two(-up) * (A.scale * kLog2e) : 1.0f;
+  const float score_unit = power_of_two(-up) * (A.scale * kLog2e);  // in the positions' terms
   if (tid < kSoftmaxThreads && x < row_tiles) {
     unsigned char* dst = smem + G::q_at + x * G::parts * G::q_bytes;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int row = 32 * warp + 8 * g + row8, own = even ? up : query_power(row_units[row]);
+      const int row = 32 * warp + 8 * g + row8, own = even ? up : min(query_power(row_units[row]), up + 126);
       const float q_unit = power_of_two(own);
       float total = 0.0f;
 #pragma unroll
@@ -402,7 +401,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       }
       total += __shfl_xor_sync(0xFFFFFFFFu, total, 8);
       total += __shfl_xor_sync(0xFFFFFFFFu, total, 16);  // the lanes of the row have read row_units[row]
-      const float unit = even ? 1.0f : power_of_two(-own) * (A.scale * kLog2e);
+      const float unit = power_of_two(up - own);  // what is left to undo for the row
       if (chunk4 == 0) {
         row_units[row] = unit;
         sums[row] = total * unit;

@@ -493,3 +493,29 @@ def test_errors_by_their_norm(dim, kv_heads, group, first, counts, window, sinks
     if T != torch.float32:
         bound += 2.0**-11 * rounding**0.5 + torch.finfo(T).eps / 2 * size**0.5
     assert error**0.5 <= bound, (error**0.5 / size**0.5, bound / size**0.5)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("group,counts", [(1, None), (8, None), (2, [3, 2]), (1, [90, 1]), (4, [100, 70])])
+def test_queries_near_the_largest_of_their_type(group, counts, dtype) -> None:
+    """Queries of 2^124 beside others whose products with the codes pass 32 bits while the scores do not: as the same queries and scale
+    2^100 apart (the powers of two come off exactly)."""
+    from ivonar_inference_b200 import KV4Cache
+
+    T, n = TYPES[dtype], [1, 1] if counts is None else counts
+    cache = KV4Cache(2, 1, 64, 120)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    k = torch.randn(240, 1, 64, generator=gen, device="cuda") * 1e-4
+    at, starts = rows_of(2, [0, 0], [120, 120])
+    cache.append(k, torch.randn(240, 1, 64, generator=gen, device="cuda"), at, starts)
+    at, starts = rows_of(2, [15, 10], n)
+    q = torch.randn(sum(n), group, 64, generator=gen, device="cuda").clamp(-7, 7) * 2.0**24
+    q[::2, ::2] *= 2.0**-30
+    q = q.to(T)
+    for scale in (1e-3, 2.0**-22):
+        want = cache.attention(q, at, None if counts is None else starts, scale=scale)
+        got = cache.attention(q * 2.0**100, at, None if counts is None else starts, scale=scale * 2.0**-100)
+        assert torch.isfinite(want).all() and torch.equal(got, want)
+    # scores of 2^124 * 1e-4 * scale: finite
+    assert torch.isfinite(cache.attention(q * 2.0**100, at, None if counts is None else starts, scale=0.125)).all()
