@@ -519,3 +519,45 @@ def test_queries_near_the_largest_of_their_type(group, counts, dtype) -> None:
         assert torch.isfinite(want).all() and torch.equal(got, want)
     # scores of 2^124 * 1e-4 * scale: finite
     assert torch.isfinite(cache.attention(q * 2.0**100, at, None if counts is None else starts, scale=0.125)).all()
+
+
+# ---- the first call of a process ----------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("first", ["append", "read", "attention"])
+def test_the_first_call_of_a_process_can_be_captured(first) -> None:
+    """Before any eager call has loaded a kernel or allowed its shared memory: few rows, prompts and both in one graph."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = f"""
+import torch
+from ivonar_inference_b200 import KV4Cache
+cache = KV4Cache(2, 2, 64, 400)
+x = torch.randn(302, 2, 64, device="cuda")
+at = torch.tensor([0, 0], device="cuda")
+starts = torch.tensor([0, 300, 302], dtype=torch.int32, device="cuda")
+def step():
+    order = ["append", "read", "attention"]
+    order.remove({first!r})
+    out = []
+    for name in [{first!r}] + order:
+        if name == "append":
+            cache.append(x, x, at, starts)
+        elif name == "read":
+            out.append(cache.read(at, starts, 302)[0])
+        else:
+            out += [cache.attention(x, at, starts), cache.attention(x[:2], at), cache.attention(x[:40], at, starts)]
+    return out
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+for _ in range(2):
+    graph.replay()
+torch.cuda.synchronize()
+cache.check()
+for a, b in zip(got, step()):
+    assert torch.equal(a, b) and bool((a != 0).any())
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
