@@ -1010,8 +1010,9 @@ int32_t ivb_batch_qk(const IvbLayerDesc* L, const float* ent, int32_t ld, const 
                      float* q, float* k, void* stream) {
   using namespace ivb;
   if (L == nullptr || L->rope == nullptr || ent == nullptr || k_nope == nullptr || positions == nullptr || q == nullptr || k == nullptr ||
-      batch <= 0 || max_len <= 0 || channels != heads * head_dim || nope + rope != head_dim || (rope & 1) != 0 ||
-      ld < channels + latent + heads * rope)
+      batch <= 0 || max_len <= 0 || heads <= 0 || head_dim <= 0 || latent < 0 || rope < 0 || nope < 0 || (rope & 1) != 0 ||
+      static_cast<int64_t>(nope) + rope != head_dim || channels != static_cast<int64_t>(heads) * head_dim ||
+      ld < static_cast<int64_t>(channels) + latent + static_cast<int64_t>(heads) * rope)
     return fail(IVB_EINVAL, "ivb_batch_qk: bad argument");
   batch_qk_kernel<<<batch, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(L->rope, ent, ld, k_nope, positions, channels, latent, heads,
                                                                              head_dim, rope, nope, max_len, q, k);

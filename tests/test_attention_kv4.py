@@ -561,3 +561,27 @@ for a, b in zip(got, step()):
 """
     done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr
+
+
+# ---- refusals of the C entry points, before any launch ------------------------------------------
+def test_the_queries_and_keys_of_a_step_refuse_bad_sizes() -> None:
+    import ctypes
+
+    from ivonar_inference_b200 import _native as native
+
+    lib = native.library()
+    buffer = ctypes.create_string_buffer(64)
+    at = ctypes.addressof(buffer)  # never read: every call is refused before a launch
+    desc = native.IvbLayerDesc()
+    desc.rope = at
+    good = dict(ld=256, batch=1, channels=64, latent=16, heads=2, head_dim=32, rope=16, nope=16, max_len=8)
+
+    def call(entry=at, **kw):
+        g = {**good, **kw}
+        return lib.ivb_batch_qk(ctypes.byref(desc), entry, g["ld"], at, at, g["batch"], g["channels"], g["latent"], g["heads"], g["head_dim"], g["rope"],
+                                g["nope"], g["max_len"], at, at, None)
+
+    for wrong in (dict(batch=0), dict(max_len=0), dict(channels=32), dict(rope=15, nope=17), dict(rope=48, nope=-16), dict(rope=-16, nope=48), dict(ld=64 + 16 + 31),
+                  dict(heads=0, channels=0), dict(heads=-2, head_dim=-32, rope=-16, nope=-16), dict(latent=-64, ld=64), dict(rope=16, nope=8),
+                  dict(heads=2**26, channels=0, head_dim=64, rope=32, nope=32), dict(entry=None)):
+        assert call(**wrong) == native.IVB_EINVAL and "ivb_batch_qk" in native.last_error(), wrong
