@@ -322,6 +322,7 @@ typedef struct IvbKv4Cache {
   void* data;
   int32_t batch, kv_heads, head_dim, max_len;
 } IvbKv4Cache;
+/* 0 for sizes that are not above zero, other head_dim, and caches of over 2^63 bytes. */
 uint64_t ivb_kv4_bytes(int32_t batch, int32_t kv_heads, int32_t head_dim, int32_t max_len);
 /* Quantises key and value rows k, v [rows][kv_heads][head_dim] into the cache. A row with an infinity or a
  * NaN reads back as NaN. The offset is clipped to +-65504 and the scale to 65504; values below the offset or above offset + 15 scale are

@@ -174,10 +174,18 @@ bool aligned(const void* p, int64_t row, int64_t head, int size, int chunk) {
 
 }  // namespace
 
+// Bytes of a cache with sizes above zero; 0 where 63 bits do not count them.
+static uint64_t kv4_bytes(int32_t batch, int32_t kv_heads, int32_t head_dim, int32_t max_len) {
+  const unsigned __int128 bytes = static_cast<unsigned __int128>(static_cast<uint64_t>(batch) * static_cast<uint64_t>(kv_heads)) *
+                                  static_cast<uint64_t>(kv4_tiles(max_len) * kv4_tile_bytes(head_dim));
+  return bytes >> 63 == 0 ? static_cast<uint64_t>(bytes) : 0;
+}
+
 int32_t check_kv4(const IvbKv4Cache* c, const char* who) {
   if (c == nullptr || c->data == nullptr) return fail(IVB_EINVAL, "%s: null cache", who);
   if (c->batch <= 0 || c->kv_heads <= 0 || c->max_len <= 0) return fail(IVB_EINVAL, "%s: batch %d, kv_heads %d, max_len %d", who, c->batch, c->kv_heads, c->max_len);
   if (c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128) return fail(IVB_EINVAL, "%s: head_dim %d (32, 64 or 128)", who, c->head_dim);
+  if (kv4_bytes(c->batch, c->kv_heads, c->head_dim, c->max_len) == 0) return fail(IVB_EINVAL, "%s: a cache of over 2^63 bytes", who);
   if (reinterpret_cast<uintptr_t>(c->data) % 16 != 0) return fail(IVB_EINVAL, "%s: the cache must be 16-byte aligned", who);
   return IVB_OK;
 }
@@ -236,7 +244,7 @@ extern "C" {
 
 uint64_t ivb_kv4_bytes(int32_t batch, int32_t kv_heads, int32_t head_dim, int32_t max_len) {
   if (batch <= 0 || kv_heads <= 0 || max_len <= 0 || (head_dim != 32 && head_dim != 64 && head_dim != 128)) return 0;
-  return static_cast<uint64_t>(batch) * kv_heads * ivb::kv4_tiles(max_len) * ivb::kv4_tile_bytes(head_dim);
+  return ivb::kv4_bytes(batch, kv_heads, head_dim, max_len);
 }
 
 int32_t ivb_kv4_append(const IvbKv4Cache* c, const void* k, const void* v, int32_t dtype, int64_t k_row, int64_t k_head, int64_t v_row,

@@ -585,3 +585,19 @@ def test_the_queries_and_keys_of_a_step_refuse_bad_sizes() -> None:
                   dict(heads=0, channels=0), dict(heads=-2, head_dim=-32, rope=-16, nope=-16), dict(latent=-64, ld=64), dict(rope=16, nope=8),
                   dict(heads=2**26, channels=0, head_dim=64, rope=32, nope=32), dict(entry=None)):
         assert call(**wrong) == native.IVB_EINVAL and "ivb_batch_qk" in native.last_error(), wrong
+
+
+def test_caches_whose_bytes_64_bits_do_not_count() -> None:
+    import ctypes
+
+    from ivonar_inference_b200 import _native as native
+
+    lib, most = native.library(), 2**31 - 1
+    for batch, heads, dim, length in ((most, most, 128, most), (most, most, 32, 4), (2**30, 2**30, 64, 1), (2**16, 2**16, 128, 2**30), (1, 1, 128, most),
+                                      (2**10, 2**10, 128, most), (2**14, 1, 32, most)):
+        want = batch * heads * 2 * ((length + 31) // 32) * 16 * (dim + 8)
+        assert lib.ivb_kv4_bytes(batch, heads, dim, length) == (want if want < 2**63 else 0)
+        buffer = ctypes.create_string_buffer(64)
+        at = (ctypes.addressof(buffer) + 15) // 16 * 16  # never read: refused, or no rows
+        rc = lib.ivb_kv4_append(ctypes.byref(native.IvbKv4Cache(at, batch, heads, dim, length)), at, at, native.IVB_F32, 0, 0, 0, 0, at, at, 0, None, None)
+        assert rc == (native.IVB_OK if want < 2**63 else native.IVB_EINVAL)
