@@ -61,8 +61,9 @@ __device__ __forceinline__ bool kv4_place(const IvbKv4Cache& C, const int32_t* s
 
 // One warp per row and kHeads heads: lanes 0..15 the key rows, lanes 16..31 the value rows, D / 16 channels each. Four heads a
 // warp share the look-up of the row and keep their loads in flight together; one is for calls too small to fill the GPU with
-// the others (2048 rows of 32 heads x 128 in bf16: written in 25 us and read in 11 with four, 32 and 17 with one; bound by
-// the instructions of the writing, 140 a row, and the latency of the reading).
+// the others (2048 rows of 32 heads x 128 in bf16: written in 25 us and read in 11 with four, 32 and 17 with one; in fp32 written in 23
+// and read in 21. The writing takes 140 instructions a row, at 57 % of the issue slots; the reading 4 bytes a lane and load, each
+// from a sector of its own).
 template <int D, typename T, int kHeads>
 __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(IvbKv4Cache C, const T* k, const T* v, int64_t k_row, int64_t k_head,
                                                                  int64_t v_row, int64_t v_head, const int32_t* starts,

@@ -13,9 +13,9 @@
 // fp32 queries and weights are hi + lo fp16 pairs: two products each. The scores come 64 positions at a time (48 cycles a product
 // where 128 columns take 65), so that the next half's are there when a half's weights are done. With few CTAs a cluster of C shares
 // the rows: each takes every C-th tile, and they join what they found through one another's shared memory.
-// What bounds it is the latency of the softmax's instructions: 2048 rows at 6144 under a window of 4096, 32 heads x 128 in bf16, take
-// 228 us (0.60 PFLOP/s) with 47 % of the issue slots used; without its exponentials 203, with a sixth of the products 222, without the
-// producers' stores 226.
+// What takes the time is the softmax: 2048 rows at 6144 under a window of 4096, 32 heads x 128 in bf16, take 230 us (0.60 PFLOP/s). Measured
+// when it was 228: 47 % of the issue slots used; without the exponentials 203, with a sixth of the products 222, without the
+// producers' stores 226, without any of these and without the terms 168.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -913,7 +913,7 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   const int64_t tiles = items / G::rows + sequences;
   if (tiles * A.cache.kv_heads > 0x1fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(tiles));
   // a cluster where one CTA each would leave SMs without work (128 CTAs of a 2048-row causal prompt: 68 us, in pairs 56, in fours
-  // 88; 256 CTAs of a chunk under a window: 228, in pairs 275)
+  // 88; 256 CTAs of a chunk under a window: 228, in pairs 275; each pair measured on one day's kernel)
   int C = 1;
   while (C < 4 && tiles * A.cache.kv_heads * C < 148 && A.cache.max_len > 2 * C * kPos) C *= 2;
   cudaLaunchConfig_t cfg = {};

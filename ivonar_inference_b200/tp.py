@@ -24,7 +24,10 @@ the same step teacher-forced, one token per step.
 With `cache="kv4"` the attention blocks keep keys and values in 4 bits (`KV4Cache`) instead of the compressed latent: the
 latent of each new token is up-projected once, its keys and values are quantised as they are written, and the
 attention reads them, over all positions or a `window` with the first `sinks` visible. No query is absorbed and no value
-projected per step, at twice the latent cache's bytes and with 4-bit rounding of what is attended to.
+projected per step, at about the latent cache's bytes (whose rotated key channels are fp16 for each head: 1,152 a position and block
+against 1,284 with 16 heads x 64, 4,352 against 4,612 with 32 x 128) and with 4-bit rounding of what is attended to. A step of 24 blocks, 12
+of them attention, 16 heads x 64: 2.9 ms in place of 3.9 (256 sequences at positions 128-640), 2.7 in place of 18.0 (32 at 6,000-8,000;
+2.0 under a window of 1,024); of 4 blocks, 32 heads x 128: 1.0 ms in place of 3.0 (64 sequences at 300-1,900).
 """
 
 from __future__ import annotations
