@@ -348,6 +348,22 @@ int32_t ivb_probe_kv4_timeout(const IvbKv4Cache* c, const void* q, int32_t dtype
                               const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,
                               int32_t sinks, void* out, int64_t o_row, int64_t o_head, uint32_t* error, void* stream);
 
+/* ---- log probabilities --------------------------------------------------------------------------------
+ * Of rows of logits [rows][vocab] (IVB_F32, IVB_F16 or IVB_BF16, `stride` values from row to row), p = softmax(x / temperature):
+ * token_lp [rows][given] = ln p of the tokens [rows][given] (device int64; NaN for one outside the vocabulary),
+ * entropy [rows] = -sum p ln p, top_lp and top_ids [rows][top] = ln p of the `top` (0 to 256, at most vocab) likeliest tokens, in
+ * descending order of the logits, the lowest of equal ones first. Sums are held in 32 bits. A logit of -inf has no probability. A row
+ * that holds a NaN or +inf, or nothing but -inf, has NaN for its values; its ids are tokens of the vocabulary all the same. */
+int32_t ivb_log_probs(const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t stride, const int64_t* tokens, int32_t given,
+                      float temperature, int32_t top, float* token_lp, float* entropy, float* top_lp, int64_t* top_ids, void* stream);
+/* The same of a vocabulary that is cut into slices: logits of the tokens v0 .. v0 + vloc - 1 into parts [rows][3 + given + 2 top] (32-bit
+ * words), which `world` of (in any order, [world][rows][...], an all-gather's result) are merged into what ivb_log_probs
+ * gives for the whole one, up to the order of its sums. `top` is at most the whole vocabulary's size. */
+int32_t ivb_log_probs_slice(const void* logits, int32_t dtype, int32_t rows, int32_t vloc, int32_t v0, int64_t stride, const int64_t* tokens,
+                            int32_t given, float temperature, int32_t top, uint32_t* parts, void* stream);
+int32_t ivb_log_probs_merge(const uint32_t* parts, int32_t world, int32_t rows, int32_t given, float temperature, int32_t top, float* token_lp,
+                            float* entropy, float* top_lp, int64_t* top_ids, void* stream);
+
 /* Per-row max |x| (rows x n fp32) into amax [rows]; with ivb_quantize_rows_amax the quantisation of a
  * row-parallel shard uses the amax of the whole row (after an all-reduce MAX), so every shard's codes
  * equal the unsharded quantiser's: scale = max(amax / 127, act_eps), code = rint(x / scale). */

@@ -6,10 +6,11 @@ The decoder is imported on first use: it needs the reference package, the rest o
 
 from ._native import KernelError
 from .kv4 import KV4Cache
+from .logprobs import LogProbs, log_probs
 
 __version__ = "0.2.0"
 
-__all__ = ["B200Decoder", "KV4Cache", "KernelError", "build_decoder"]
+__all__ = ["B200Decoder", "KV4Cache", "KernelError", "LogProbs", "build_decoder", "log_probs"]
 
 
 def __getattr__(name: str):

@@ -202,6 +202,11 @@ SIGNATURES = {
                                c_void_p, c_int32, c_void_p, c_void_p]),
     "ivb_kv4_attention": (c_int32, [POINTER(IvbKv4Cache), c_void_p, c_int32, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_int32,
                                     c_float, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
+    "ivb_log_probs": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int64, c_void_p, c_int32, c_float, c_int32, c_void_p, c_void_p,
+                                c_void_p, c_void_p, c_void_p]),
+    "ivb_log_probs_slice": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_int64, c_void_p, c_int32, c_float, c_int32, c_void_p,
+                                      c_void_p]),
+    "ivb_log_probs_merge": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_float, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "ivb_decoder_check": (c_int32, [c_void_p, c_void_p]),
 }
 SIGNATURES["ivb_probe_kv4_timeout"] = SIGNATURES["ivb_kv4_attention"]

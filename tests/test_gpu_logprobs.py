@@ -1,0 +1,247 @@
+"""Log probabilities on a B200 against 64 bits.
+
+Tolerances, with V the vocabulary and n = V / 4096 + 1 turns of a thread (16 values each). A term e^d of S: d is off by 2^-22 of
+itself (the difference, the reciprocal temperature, its product with log2 e and the product are rounded), so S by
+2^-22 sum p |d| <= 2^-22 ln V of itself, and by 2^-22 for each exp2; a thread's sum has 16 n additions and n rescalings of two roundings
+and an exp2 (2^-21), lanes, warps, CTAs and slices join it 5 + 3 + 3 + 1 times with as much:
+    S is off by   s = 2^-22 (ln V + 1) + 16 n 2^-24 + (n + 12) 2^-21   of itself
+    ln p by       s + 2^-22 |ln p| + 2^-22 (|ln p| is at least the difference over the temperature; ln S, the sum)
+The entropy is ln S - sum p d: the second sum's terms are off by as much as S's and 2^-24 more, twice (of it and of S), and it is at most ln V:
+    the entropy by   s + 2 (s + 2^-22) ln V + 2^-22 ln V
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def logits_of(rows, vocab, seed=0, dtype=torch.float32, size=2.5):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = size * torch.randn(rows, vocab, generator=gen, device="cuda")
+    x.scatter_add_(1, torch.randint(0, vocab, (rows, 4), generator=gen, device="cuda"), 9 * torch.rand(rows, 4, generator=gen, device="cuda"))
+    return x.to(dtype), torch.randint(0, vocab, (rows,), generator=gen, device="cuda")
+
+
+def expected(x, tokens, top, temperature):
+    x = x.double()
+    order = x.nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf)
+    ids = torch.argsort(-order, dim=1, stable=True)[:, :top]
+    lp = torch.log_softmax(x / temperature, 1)
+    p = lp.exp()
+    entropy = -torch.where(p == 0, 0.0, p * lp).sum(1)
+    two = tokens if tokens.ndim == 2 else tokens[:, None]
+    inside = (two >= 0) & (two < x.shape[1])
+    given = torch.where(inside, lp.gather(1, two.clamp(0, x.shape[1] - 1)), math.nan).view(tokens.shape)
+    return given, entropy, lp.gather(1, ids), ids
+
+
+def close(got, want, tol):
+    got, want = got.double(), want.double()
+    finite = torch.isfinite(want)
+    assert torch.equal(got[~finite].nan_to_num(nan=7.0), want[~finite].nan_to_num(nan=7.0))
+    assert bool(((got - want).abs() <= tol)[finite].all()), float(((got - want).abs() - tol)[finite].max())
+
+
+def check(found, x, tokens, top=0, temperature=1.0):
+    given, entropy, best, ids = expected(x, tokens, top, temperature)
+    V = x.shape[1]
+    n = V // 4096 + 1
+    s = 2.0**-22 * (math.log(V) + 1) + 16 * n * 2.0**-24 + (n + 12) * 2.0**-21
+    for got, want in ((found.tokens, given), (found.top, best)):
+        assert got.dtype == torch.float32 and got.shape == want.shape
+        close(got, want, s + 2.0**-22 * (want.abs() + 1))
+    close(found.entropy, entropy, s + 2 * (s + 2.0**-22) * math.log(V) + 2.0**-22 * math.log(V))
+    assert torch.equal(found.ids, ids)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (3, 2, 2), (1, 31, 31), (5, 257, 0), (2, 300, 256), (70, 1000, 5), (1, 4096, 20), (3, 4097, 64),
+                                            (700, 8195, 3), (1, 32768, 5), (2, 32768, 256), (33, 32768, 20), (9, 100003, 1), (1, 200001, 64)])
+def test_against_64_bits(rows, vocab, top, dtype) -> None:
+    from ivonar_inference_b200 import log_probs
+
+    x, tokens = logits_of(rows, vocab, vocab + top, TYPES[dtype])
+    for temperature in (1.0, 0.7):
+        check(log_probs(x, tokens, top=top, temperature=temperature), x, tokens, top, temperature)
+
+
+@pytest.mark.parametrize("top", [1, 7, 256])
+@pytest.mark.parametrize("kind", ["equal", "levels", "ascending", "descending", "zeros", "last", "mostly banned"])
+def test_orders_that_a_bound_does_not_help(kind, top) -> None:
+    """Ties go to the lowest token, and rows whose every turn has larger values than the last are ranked all the same."""
+    from ivonar_inference_b200 import log_probs
+
+    for rows, vocab in ((2, 40007), (1, 9001), (600, 5000)):
+        gen = torch.Generator(device="cuda").manual_seed(top)
+        ramp = torch.arange(vocab, device="cuda") / vocab * 4
+        x = {"equal": torch.full((rows, vocab), 1.25, device="cuda"),
+             "levels": torch.randint(0, 3, (rows, vocab), generator=gen, device="cuda").float(),
+             "ascending": ramp.expand(rows, vocab).contiguous(),
+             "descending": -ramp.expand(rows, vocab).contiguous(),
+             "zeros": torch.randint(0, 2, (rows, vocab), generator=gen, device="cuda").float() * -0.0,
+             "last": torch.zeros(rows, vocab, device="cuda"),
+             "mostly banned": torch.full((rows, vocab), -math.inf, device="cuda")}[kind]
+        if kind == "zeros":
+            x = torch.where(torch.rand(rows, vocab, generator=gen, device="cuda") < 0.5, 0.0, -0.0)
+        if kind == "last":
+            x[:, -300:] = torch.rand(rows, 300, generator=gen, device="cuda")
+        if kind == "mostly banned":
+            x[:, 17::vocab // 5] = torch.rand(x[:, 17::vocab // 5].shape, generator=gen, device="cuda")
+        tokens = torch.randint(0, vocab, (rows,), generator=gen, device="cuda")
+        check(log_probs(x, tokens, top=top), x, tokens, top)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_rows_with_special_values(dtype) -> None:
+    from ivonar_inference_b200 import log_probs
+
+    T = TYPES[dtype]
+    x, _ = logits_of(12, 5003, 4, T)
+    least, most = torch.finfo(T).min, torch.finfo(T).max
+    x[0] = -math.inf                     # nothing is left
+    x[1] = -math.inf
+    x[1, 4001] = 3.0                     # one token is left
+    x[2] = least                         # the type's lowest value throughout: any token
+    x[3, ::2] = least
+    x[4, 77] = math.nan
+    x[5, 78] = math.inf
+    x[6] = most
+    x[7, 9] = most
+    x[8, :4999] = -math.inf
+    x[9, 100:] = least
+    x[9, :100] = -math.inf
+    x[10, 5] = -math.nan
+    tokens = torch.tensor([4001, 4001, 5, 6, 7, 78, 5002, 9, 5000, 3, 5, 0], device="cuda")
+    for temperature in (1.0, 1.5):
+        check(log_probs(x, tokens, top=9, temperature=temperature), x, tokens, 9, temperature)
+
+
+def test_tokens_of_every_kind() -> None:
+    from ivonar_inference_b200 import log_probs
+
+    x, _ = logits_of(5, 777, 1)
+    tokens = torch.tensor([[-1, 0, 776], [777, 5, 5], [2**40, -(2**62), 1], [3, 2, 1], [776, 776, 776]], device="cuda")
+    check(log_probs(x, tokens, top=2), x, tokens, 2)
+    none = torch.empty(5, 0, dtype=torch.int64, device="cuda")
+    found = log_probs(x, none, top=4)
+    check(found, x, none, 4)
+    many = torch.randint(0, 777, (5, 1000), device="cuda")
+    check(log_probs(x, many), x, many)
+    empty = log_probs(x[:0], tokens[:0], top=2)
+    assert [tuple(t.shape) for t in empty] == [(0, 3), (0,), (0, 2), (0, 2)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_strides_and_alignment(dtype) -> None:
+    from ivonar_inference_b200 import log_probs
+
+    wide, tokens = logits_of(40, 4500, 3, TYPES[dtype])
+    for cut in (wide[:, 1:4001], wide[::3, 3:1000], wide[:, 7:12], wide[5:6, 4:4404], wide[:1].expand(40, 4500), wide[:, 2:3]):
+        t = (tokens[: cut.shape[0]] % cut.shape[1]).contiguous()
+        check(log_probs(cut, t, top=min(4, cut.shape[1])), cut, t, min(4, cut.shape[1]))
+    odd, t = logits_of(9, 4501, 3, TYPES[dtype])   # every row begins elsewhere in its 16 bytes
+    check(log_probs(odd, t, top=6), odd, t, 6)
+
+
+def test_offsets_beyond_32_bits() -> None:
+    from ivonar_inference_b200 import log_probs
+
+    x = torch.empty(3, 1_500_000_001, dtype=torch.bfloat16, device="cuda")[:, :5000]
+    part, tokens = logits_of(3, 5000, 3, torch.bfloat16)
+    x.copy_(part)
+    check(log_probs(x, tokens, top=3), x, tokens, 3)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("vocab,cuts", [(5000, [0, 2500, 5000]), (300, [0, 7, 8, 200, 300]), (40001, [0, 128, 30000, 40001])])
+def test_slices_of_a_vocabulary(vocab, cuts, dtype) -> None:
+    from ivonar_inference_b200.logprobs import log_probs_merge, log_probs_slice
+
+    x, _ = logits_of(6, vocab, vocab, TYPES[dtype])
+    x[1, : vocab // 2] = x[1, 0]
+    x[2] = -math.inf
+    x[3, cuts[1]:cuts[2]] = -math.inf
+    tokens = torch.randint(-2, vocab + 2, (6, 3), device="cuda")
+    for top in (0, 1, 256):
+        parts = torch.stack([log_probs_slice(x[:, a:b], tokens, a, top, 0.9) for a, b in zip(cuts, cuts[1:])])
+        check(log_probs_merge(parts, tokens, top, 0.9), x, tokens, top, 0.9)
+        check(log_probs_merge(parts.flip(0).contiguous(), tokens, top, 0.9), x, tokens, top, 0.9)
+
+
+def test_many_slices() -> None:
+    from ivonar_inference_b200.logprobs import log_probs_merge, log_probs_slice
+
+    x, tokens = logits_of(2, 64 * 300, 1)
+    parts = torch.stack([log_probs_slice(x[:, a:a + 300], tokens, a, 256) for a in range(0, 64 * 300, 300)])
+    check(log_probs_merge(parts, tokens, 256), x, tokens, 256)
+
+
+def test_streams_graphs_and_repeated_calls() -> None:
+    from ivonar_inference_b200 import log_probs
+
+    x, tokens = logits_of(64, 32768, 2)
+    want = log_probs(x, tokens, top=20)
+    check(want, x, tokens, 20)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = log_probs(x, tokens, top=20)
+    side.synchronize()
+    # two calls at once, and the same bits each time
+    for a, b in zip(want, other):
+        assert torch.equal(a, b)
+    graph, still = torch.cuda.CUDAGraph(), x.clone()
+    with torch.cuda.graph(graph):
+        found = log_probs(still, tokens, top=20)
+    for seed in (5, 6):
+        fresh, _ = logits_of(64, 32768, seed)
+        still.copy_(fresh)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(found, fresh, tokens, 20)
+    reserved = torch.cuda.memory_allocated()
+    log_probs(x, tokens)
+    assert torch.cuda.memory_allocated() == reserved
+
+
+def test_refusals() -> None:
+    from ivonar_inference_b200 import KernelError, log_probs
+    from ivonar_inference_b200.logprobs import log_probs_merge, log_probs_slice
+
+    x, tokens = logits_of(4, 100)
+
+    def refused(match, *args, **kwargs):
+        with pytest.raises(ValueError, match=match):
+            log_probs(*args, **kwargs)
+
+    refused("contiguous", x.t(), tokens.new_zeros(100))
+    refused("contiguous", x, tokens.repeat(2).view(4, 2).t().contiguous().t())
+    refused("tokens must be", x, tokens.int())
+    refused("tokens must be", x, tokens[:3])
+    refused("tokens must be", x, tokens.cpu())
+    refused("tokens must be", x, tokens[:, None, None])
+    refused("top", x, tokens, top=-1)
+    refused("top", x, tokens, top=257)
+    refused("vocabulary of 100", x, tokens, top=101)
+    for t in (0.0, -1.0, math.nan, math.inf):
+        refused("temperature", x, tokens, temperature=t)
+    refused("gradient", x.clone().requires_grad_(), tokens)
+    with torch.no_grad():
+        log_probs(x.clone().requires_grad_(), tokens)
+    with torch.autograd.forward_ad.dual_level():
+        refused("tangent", torch.autograd.forward_ad.make_dual(x, x), tokens)
+    with pytest.raises(ValueError, match="from -1"):
+        log_probs_slice(x, tokens, -1)
+    parts = log_probs_slice(x, tokens, 0, 3)
+    for bad in (parts, parts[None].long(), parts[None, :3], parts[None, :, :5]):
+        with pytest.raises(ValueError, match="parts must be"):
+            log_probs_merge(bad, tokens, 3)
+    with pytest.raises((KernelError, ValueError)):
+        log_probs_merge(parts[None], tokens, 3, 0.0)
