@@ -334,6 +334,18 @@ int32_t ivb_kv4_append(const IvbKv4Cache* c, const void* k, const void* v, int32
 int32_t ivb_kv4_read(const IvbKv4Cache* c, void* k, void* v, int32_t dtype, int64_t k_row, int64_t k_head, int64_t v_row,
                      int64_t v_head, const int32_t* starts, const int64_t* positions, int32_t rows, uint32_t* error,
                      void* stream);
+/* Sequence b takes the first lengths[b] positions of sequence sources[b] (device int64 [batch] each) of `source`: another cache of the
+ * same kv_heads and head_dim that shares no memory with `c`, or `c` itself (also by NULL), whose sequences are read as they were
+ * before the call, of 4,096 at most; max_len may differ. Positions behind those taken stay as they are, and so does a sequence with
+ * a negative source, a length of zero or below, or itself as its source. A length beyond either cache's capacity sets *error to
+ * IVB_ECAPACITY and a source that `source` does not have sets it to IVB_EINVAL; nothing is taken for these. */
+int32_t ivb_kv4_fork(const IvbKv4Cache* c, const IvbKv4Cache* source, const int64_t* sources, const int64_t* lengths, uint32_t* error,
+                     void* stream);
+/* Row i of sequence b (rows as above) becomes a copy of the sequence's row at position index[starts[b] + i] (device int64 [rows]), as
+ * it was before the call: the row's own position or one behind it, in any order. A negative index leaves the row as it is. An index
+ * before the row's position sets *error to IVB_EINVAL, one beyond the capacity to IVB_ECAPACITY; these rows stay as they are too. */
+int32_t ivb_kv4_compact(const IvbKv4Cache* c, const int64_t* index, const int32_t* starts, const int64_t* positions, int32_t rows,
+                        uint32_t* error, void* stream);
 /* Attention of the rows' queries q [rows][heads][head_dim] over their sequences' caches into out (same shape
  * and type); query head h reads key/value head h / (heads / kv_heads). The row at position p sees positions
  * j <= p with j > p - window or j < sinks (window 0: all j <= p). out = sum_j softmax_j(scale q.k_j) v_j, summed

@@ -202,6 +202,8 @@ SIGNATURES = {
                                c_void_p, c_int32, c_void_p, c_void_p]),
     "ivb_kv4_attention": (c_int32, [POINTER(IvbKv4Cache), c_void_p, c_int32, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_int32,
                                     c_float, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
+    "ivb_kv4_fork": (c_int32, [POINTER(IvbKv4Cache), POINTER(IvbKv4Cache), c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ivb_kv4_compact": (c_int32, [POINTER(IvbKv4Cache), c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
     "ivb_log_probs": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int64, c_void_p, c_int32, c_float, c_int32, c_void_p, c_void_p,
                                 c_void_p, c_void_p, c_void_p]),
     "ivb_log_probs_slice": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_int64, c_void_p, c_int32, c_float, c_int32, c_void_p,

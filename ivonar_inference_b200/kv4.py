@@ -77,14 +77,16 @@ class KV4Cache:
         return KV4Cache(1, self.kv_heads, self.head_dim, self.max_len, data=self.data[index:index + 1], error=self.error)
 
     def check(self) -> None:
-        """Wait for the device; raises ValueError if a call since the last check met a row beyond the capacity, and KernelError
-        if a wait inside a kernel ran out (the rows that it concerns are then NaN)."""
+        """Wait for the device; raises ValueError if a call since the last check met a row beyond the capacity, or a source that
+        `fork` or `compact` refuse, and KernelError if a wait inside a kernel ran out (the rows that it concerns are then NaN)."""
 
         if self.error is None:
             raise RuntimeError("this cache was made without an error word")
         code = int(self.error.item())
         if code != native.IVB_OK:
             self.error.zero_()
+            if code == native.IVB_EINVAL:
+                raise ValueError("a sequence or a row that fork or compact cannot take")
             if code != native.IVB_ECAPACITY:
                 raise native.KernelError(f"the 4-bit attention reported error {code}")
             raise ValueError(f"a row lies beyond the cache's capacity of {self.max_len} positions")
@@ -187,6 +189,48 @@ class KV4Cache:
         self._call("ivb_kv4_read", self.lib.ivb_kv4_read, self._ref, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], k_row, k_head, v_row, v_head, at,
                    positions.data_ptr(), rows)
         return k, v
+
+    def _numbers(self, name: str, x: Tensor, count: int) -> int:
+        """Checks of numbers in device memory; their address."""
+
+        if x.dtype is not torch.int64 or x.shape != (count,) or x.device != self.device or not x.is_contiguous():
+            raise ValueError(f"{name} must be an int64 tensor [{count}] on {self.device}")
+        return x.data_ptr()
+
+    def fork(self, sources: Tensor, lengths: Tensor, source: KV4Cache | None = None) -> None:
+        """Sequence b takes the first lengths[b] positions of sequence sources[b] (int64 [batch] each, on the device), of this cache as
+        it was before the call or of `source`, another cache with the same heads that shares no memory with this one.
+
+        Any map: beams that change places, answers that begin as one did, sequences that move up to slots that others left; from another
+        cache a beginning that was shared, or what a cache of another capacity holds. Positions behind those taken stay as they are,
+        and so does a sequence with a negative source or itself, or a length of zero. Lengths beyond either cache's
+        capacity and sources that are not there are reported by `check`, and nothing is taken for them. Within one cache 4,096 sequences
+        at most.
+        """
+
+        at, n = self._numbers("sources", sources, self.batch), self._numbers("lengths", lengths, self.batch)
+        if source is None:
+            source = self
+        elif source.device != self.device or source.kv_heads != self.kv_heads or source.head_dim != self.head_dim:
+            raise ValueError(f"source must be a cache of {self.kv_heads} heads x {self.head_dim} on {self.device}")
+        elif (source.data.data_ptr() != self.data.data_ptr() or source.data.shape != self.data.shape or source.max_len != self.max_len) and (
+                source.data.data_ptr() < self.data.data_ptr() + self.nbytes and self.data.data_ptr() < source.data.data_ptr() + source.nbytes):
+            raise ValueError("source shares memory with the cache without being it")
+        self._call("ivb_kv4_fork", self.lib.ivb_kv4_fork, self._ref, source._ref, at, n)
+
+    def compact(self, index: Tensor, positions: Tensor, starts: Tensor | None = None) -> None:
+        """Row i of the call, at its position p, becomes a copy of the row of the same sequence at index[i] >= p (int64 [rows] on the
+        device), as that was before the call.
+
+        For drafted tokens that were accepted out of a tree, or a history of which a part is kept: the rows move up, in any order,
+        keys as they were rotated. A negative index leaves its row as it is. An index before the row's position or beyond
+        the capacity is reported by `check`, and its row stays as it is.
+        """
+
+        rows = index.shape[0] if index.ndim == 1 else -1
+        values = self._numbers("index", index, rows)
+        at = self._rows(rows, positions, starts)
+        self._call("ivb_kv4_compact", self.lib.ivb_kv4_compact, self._ref, values, at, positions.data_ptr(), rows)
 
     def attention(self, q: Tensor, positions: Tensor, starts: Tensor | None = None, scale: float | None = None, window: int = 0,
                   sinks: int = 0, out: Tensor | None = None) -> Tensor:
