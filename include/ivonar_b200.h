@@ -355,7 +355,25 @@ int32_t ivb_kv4_compact(const IvbKv4Cache* c, const int64_t* index, const int32_
 int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
                           const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,
                           int32_t sinks, void* out, int64_t o_row, int64_t o_head, uint32_t* error, void* stream);
-/* Failure-detection probe: the same call, but the prompts' kernel issues no products and its waits run out after 1 ms. */
+/* The same where sequences begin alike: sequences groups[g] .. groups[g + 1] - 1 (device int32 [cache.batch + 1], ascending; NULL: all
+ * of them, behind the one sequence of `cache`) begin with the first lengths[g] positions (device int64 [cache.batch]) of sequence g
+ * of `cache`, which is held once and read once for all of them; others begin with nothing. `positions` count from the end of that beginning, windows and
+ * sinks from its start. A length above the prefix's capacity sets *error to IVB_ECAPACITY and counts as that capacity, one below
+ * zero as zero. `cache` has the same kv_heads and head_dim; the two capacities' sum is below 2^31 - 256. `workspace`: device memory of
+ * ivb_kv4_prefix_workspace_bytes (0: none is needed) for the same arguments, 16-byte aligned, whose contents are of no use before
+ * and after the call. */
+typedef struct IvbKv4Prefix {
+  IvbKv4Cache cache;
+  const int64_t* lengths;
+  const int32_t* groups;
+} IvbKv4Prefix;
+uint64_t ivb_kv4_prefix_workspace_bytes(const IvbKv4Cache* c, const IvbKv4Prefix* prefix, int32_t dtype, int32_t heads, const int32_t* starts,
+                                        int32_t rows);
+int32_t ivb_kv4_attention_prefix(const IvbKv4Cache* c, const IvbKv4Prefix* prefix, const void* q, int32_t dtype, int64_t q_row, int64_t q_head,
+                                 int32_t heads, const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,
+                                 int32_t sinks, void* out, int64_t o_row, int64_t o_head, void* workspace, uint64_t workspace_bytes,
+                                 uint32_t* error, void* stream);
+/* Failure-detection probe: ivb_kv4_attention, but the prompts' kernel issues no products and its waits run out after 1 ms. */
 int32_t ivb_probe_kv4_timeout(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
                               const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,
                               int32_t sinks, void* out, int64_t o_row, int64_t o_head, uint32_t* error, void* stream);

@@ -154,6 +154,14 @@ class IvbKv4Cache(Structure):
     ]
 
 
+class IvbKv4Prefix(Structure):
+    _fields_ = [
+        ("cache", IvbKv4Cache),
+        ("lengths", c_void_p),
+        ("groups", c_void_p),
+    ]
+
+
 SIGNATURES = {
     "ivb_abi_version": (c_int32, []),
     "ivb_last_error": (c_char_p, []),
@@ -202,6 +210,10 @@ SIGNATURES = {
                                c_void_p, c_int32, c_void_p, c_void_p]),
     "ivb_kv4_attention": (c_int32, [POINTER(IvbKv4Cache), c_void_p, c_int32, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_int32,
                                     c_float, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
+    "ivb_kv4_prefix_workspace_bytes": (c_uint64, [POINTER(IvbKv4Cache), POINTER(IvbKv4Prefix), c_int32, c_int32, c_void_p, c_int32]),
+    "ivb_kv4_attention_prefix": (c_int32, [POINTER(IvbKv4Cache), POINTER(IvbKv4Prefix), c_void_p, c_int32, c_int64, c_int64, c_int32, c_void_p,
+                                           c_void_p, c_int32, c_float, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_uint64,
+                                           c_void_p, c_void_p]),
     "ivb_kv4_fork": (c_int32, [POINTER(IvbKv4Cache), POINTER(IvbKv4Cache), c_void_p, c_void_p, c_void_p, c_void_p]),
     "ivb_kv4_compact": (c_int32, [POINTER(IvbKv4Cache), c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
     "ivb_log_probs": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int64, c_void_p, c_int32, c_float, c_int32, c_void_p, c_void_p,

@@ -111,6 +111,10 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
   const int live = min(R, items - i0);
   const int64_t base = kv4_position(A.positions, b) + before;
   const int max_len = A.cache.max_len;
+  // a beginning that the sequence shares: its positions come first, and are joined from their parts at the end
+  int prefix_group;
+  const int shared_length = kv4_prefix(A, b, prefix_group), sinks = max(0, A.sinks - shared_length);
+  const bool joined = A.part_stats != nullptr && shared_length > 0;
   // token and query head of an item of the sequence's head group
   auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };
   // positions of the tile's first and last rows, -1 where idle and max_len where beyond the capacity
@@ -129,7 +133,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
   const int high = min(last, max_len - 1);  // negative: none
   const int low = A.window > 0 ? max(0, max(first, 0) - A.window + 1) : 0;
   const int window_group = low / kKv4Group;
-  const int sink_groups = A.window > 0 ? min((min(A.sinks, low) + kKv4Group - 1) / kKv4Group, window_group) : 0;
+  const int sink_groups = A.window > 0 ? min((min(sinks, low) + kKv4Group - 1) / kKv4Group, window_group) : 0;
   const int groups = high < 0 ? 0 : sink_groups + high / kKv4Group - window_group + 1;
   const int lanes_in = C * W, mine = rank * W + warp;
   const int steps = groups > mine ? (groups - mine + lanes_in - 1) / lanes_in : 0;
@@ -314,14 +318,14 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
       }
     }
     // a group that every row sees whole needs no masks
-    const bool whole = first >= p0 + kKv4Group - 1 && last < max_len && (A.window <= 0 || p0 > last - A.window || p0 <= A.sinks - kKv4Group);
+    const bool whole = first >= p0 + kKv4Group - 1 && last < max_len && (A.window <= 0 || p0 > last - A.window || p0 <= sinks - kKv4Group);
     if (!whole) {
 #pragma unroll
       for (int s = 0; s < kSets; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int p = p0 + 16 * (i >> 1) + mine_of + 2 * (i & 1);
-          const bool seen = p <= at[s] && (A.window <= 0 || p > at[s] - A.window || p < A.sinks);
+          const bool seen = p <= at[s] && (A.window <= 0 || p > at[s] - A.window || p < sinks);
           if (!seen) x[s][i] = -INFINITY;
         }
     }
@@ -437,9 +441,16 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
       off[s] += __shfl_xor_sync(0xFFFFFFFFu, off[s], d);
     }
   fold(true);
+  if (joined) pdl_wait();  // for the parts
+  auto head_of = [&](int row) { return kvh * A.group + i0 + row - token_of(i0 + row) * A.group; };
+  auto item_of = [&](int row) { return static_cast<int64_t>(row0 + token_of(i0 + row)) * A.heads + head_of(row); };
+  auto idle = [&](int row) {
+    const int p = clamp_position(base + token_of(i0 + row));
+    return p < 0 || p >= max_len;
+  };
   auto place = [&](int row) {
     const int t = token_of(i0 + row);
-    return static_cast<T*>(A.out) + (row0 + t) * A.o_row + (kvh * A.group + i0 + row - t * A.group) * A.o_head;
+    return static_cast<T*>(A.out) + (row0 + t) * A.o_row + head_of(row) * A.o_head;
   };
   if (C * W == 1) {
 #pragma unroll
@@ -451,7 +462,8 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
         for (int h = 0; h < kPlanes; ++h) {
           float y[kRun];
 #pragma unroll
-          for (int j = 0; j < kRun; ++j) y[j] = sum[s] == 0.0f ? 0.0f : (o[s][h][j] + off[s]) * inv;
+          for (int j = 0; j < kRun; ++j) y[j] = sum[s] == 0.0f ? 0.0f : (o[s][h][j] + off[s]) * (joined ? 1.0f : inv);
+          if (joined && at[s] >= 0) kv4_join_parts<D, kRun>(A, item_of(row_of(s)), ref[s], sum[s], y, [&](int j) { return channel(h, j); });
           if constexpr (D == 32) {
 #pragma unroll
             for (int j = 0; j < kRun; ++j) out[channel(h, j)] = from_f32<T>(y[j]);
@@ -494,7 +506,10 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
       }
     }
     if (C == 1) {
-      place(row)[i - row * D] = from_f32<T>(l == 0.0f ? 0.0f : (v + m) / l);
+      float y[1] = {v + m};
+      if (joined && !idle(row)) kv4_join_parts<D, 1>(A, item_of(row), top, l, y, [&](int) { return i - row * D; });
+      else y[0] = l == 0.0f ? 0.0f : y[0] / l;
+      place(row)[i - row * D] = from_f32<T>(y[0]);
     } else {
       comb[i] = v;
       if (i - row * D == 0) {
@@ -521,7 +536,10 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
         l = fmaf(part_sum, f, l);
       }
     }
-    place(row)[i - row * D] = from_f32<T>(l == 0.0f ? 0.0f : v / l);
+    float y[1] = {v};
+    if (joined && !idle(row)) kv4_join_parts<D, 1>(A, item_of(row), top, l, y, [&](int) { return i - row * D; });
+    else y[0] = l == 0.0f ? 0.0f : y[0] / l;
+    place(row)[i - row * D] = from_f32<T>(y[0]);
   }
   cluster.sync();  // no CTA leaves while another reads its shared memory
 }
@@ -529,7 +547,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
 template <int D, typename T, bool kSplit, int kTiles>
 __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int tiles_per_sequence) {
   kv4_rows<D, T, kSplit, kTiles>(A, tiles_per_sequence);
-  // whichever way the rows took: this grid does not end before the prompts' that it runs beside
+  // whichever way the rows took: this grid does not end before the ones that it runs beside
   if (A.beside_prompts && blockIdx.x == 0) pdl_wait();
 }
 
@@ -601,14 +619,45 @@ int32_t launch_attention(const Kv4Attention& A, cudaStream_t stream) {
   }
 }
 
-int32_t attention_call(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads, const int32_t* starts,
-                       const int64_t* positions, int32_t rows, float scale, int32_t window, int32_t sinks, void* out, int64_t o_row,
-                       int64_t o_head, uint32_t* error, void* stream, bool withhold) {
+// Which sequences are few rows' (those with so many items at most).
+int few_items(const IvbKv4Cache& c, int group, const int32_t* starts, int rows) {
+  const int64_t items = static_cast<int64_t>(rows) * group;
+  const int64_t tiles = items / 256 + std::min<int64_t>(c.batch, items / (kFewItems + 1));
+  const int few = tiles * c.kv_heads * 4 >= 148 ? kFewItems : kFewItemsSparse;
+  // a lone sequence that can have more takes the prompts' kernel however many it has: one launch
+  return starts == nullptr || items <= few ? 0x7fffffff : c.batch == 1 ? 0 : few;
+}
+
+// Bytes of the parts of a shared beginning: for each split, row and head its statistics and its values.
+uint64_t part_bytes(int splits, int rows, int heads, int dim) { return static_cast<uint64_t>(splits) * rows * heads * (8 + 4 * static_cast<uint64_t>(dim)); }
+
+int32_t check_heads(const IvbKv4Cache* c, int32_t heads, int32_t rows) {
+  if (heads <= 0 || heads % c->kv_heads != 0) return fail(IVB_EINVAL, "ivb_kv4_attention: %d query heads over %d key/value heads", heads, c->kv_heads);
+  if (static_cast<int64_t>(rows) * heads > 0x7fffffff - 1024) return fail(IVB_EINVAL, "ivb_kv4_attention: %d rows of %d heads", rows, heads);
+  return IVB_OK;
+}
+
+int32_t check_prefix(const IvbKv4Cache* c, const IvbKv4Prefix* prefix) {
+  if (prefix == nullptr) return fail(IVB_EINVAL, "ivb_kv4_attention_prefix: null prefix");
+  if (int32_t rc = check_kv4(&prefix->cache, "ivb_kv4_attention_prefix")) return rc;
+  if (prefix->cache.kv_heads != c->kv_heads || prefix->cache.head_dim != c->head_dim)
+    return fail(IVB_EINVAL, "ivb_kv4_attention_prefix: %d heads x %d behind a prefix of %d x %d", c->kv_heads, c->head_dim, prefix->cache.kv_heads,
+                prefix->cache.head_dim);
+  if (prefix->lengths == nullptr) return fail(IVB_EINVAL, "ivb_kv4_attention_prefix: null lengths");
+  if (prefix->groups == nullptr && prefix->cache.batch != 1)
+    return fail(IVB_EINVAL, "ivb_kv4_attention_prefix: %d prefixes without groups", prefix->cache.batch);
+  if (static_cast<int64_t>(prefix->cache.max_len) + c->max_len > 0x7fffffff - 256)
+    return fail(IVB_EINVAL, "ivb_kv4_attention_prefix: %d positions behind %d", c->max_len, prefix->cache.max_len);
+  return IVB_OK;
+}
+
+int32_t attention_call(const IvbKv4Cache* c, const IvbKv4Prefix* prefix, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
+                       const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window, int32_t sinks, void* out,
+                       int64_t o_row, int64_t o_head, void* workspace, uint64_t workspace_bytes, uint32_t* error, void* stream, bool withhold) {
   if (int32_t rc = check_kv4(c, "ivb_kv4_attention")) return rc;
   if (int32_t rc = check_kv4_rows(c, starts, positions, rows, dtype, "ivb_kv4_attention")) return rc;
-  if (heads <= 0 || heads % c->kv_heads != 0) return fail(IVB_EINVAL, "ivb_kv4_attention: %d query heads over %d key/value heads", heads, c->kv_heads);
+  if (int32_t rc = check_heads(c, heads, rows)) return rc;
   if (window < 0 || sinks < 0) return fail(IVB_EINVAL, "ivb_kv4_attention: window %d, sinks %d", window, sinks);
-  if (static_cast<int64_t>(rows) * heads > 0x7fffffff - 1024) return fail(IVB_EINVAL, "ivb_kv4_attention: %d rows of %d heads", rows, heads);
   if (rows == 0) return IVB_OK;
   if (q == nullptr || out == nullptr) return fail(IVB_EINVAL, "ivb_kv4_attention: null queries or output");
   Kv4Attention A{};
@@ -637,15 +686,28 @@ int32_t attention_call(const IvbKv4Cache* c, const void* q, int32_t dtype, int64
   A.q_vec = aligned(q, q_row, q_head);
   A.o_vec = aligned(out, o_row, o_head);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t items = static_cast<int64_t>(rows) * A.group;
-  const int64_t tiles = items / 256 + std::min<int64_t>(c->batch, items / (kFewItems + 1));
-  const int few = tiles * c->kv_heads * 4 >= 148 ? kFewItems : kFewItemsSparse;
-  // a lone sequence that can have more takes the prompts' kernel however many it has: one launch
-  A.few = starts == nullptr || items <= few ? 0x7fffffff : c->batch == 1 ? 0 : few;
+  A.few = few_items(*c, A.group, starts, rows);
+  if (prefix != nullptr) {
+    A.prefix = prefix->cache;
+    A.prefix_lengths = prefix->lengths;
+    A.prefix_groups = prefix->groups;
+    if (A.few != 0) {
+      A.splits = kv4_prefix_splits(*c, prefix->cache, dtype, A.group, rows);
+      if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < part_bytes(A.splits, rows, heads, c->head_dim))
+        return fail(IVB_EINVAL, "ivb_kv4_attention_prefix: a workspace of %llu bytes at %p, not 16-byte aligned or too small",
+                    static_cast<unsigned long long>(workspace_bytes), workspace);
+      A.part_values = static_cast<float*>(workspace);
+      A.part_stats = reinterpret_cast<float2*>(A.part_values + static_cast<int64_t>(A.splits) * rows * heads * c->head_dim);
+    }
+  }
   A.beside_prompts = A.few != 0x7fffffff;
-  if (A.few != 0x7fffffff)
+  if (A.beside_prompts)
     if (int32_t rc = launch_kv4_prompts(A, dtype, A.few, s)) return rc;
   if (A.few == 0) return IVB_OK;
+  if (prefix != nullptr) {
+    if (int32_t rc = launch_kv4_prefix(A, dtype, A.few, s)) return rc;
+    A.beside_prompts = true;  // beside the pass, and what that is beside
+  }
   if (dtype == IVB_F32) return launch_attention<float>(A, s);
   if (dtype == IVB_F16) return launch_attention<__half>(A, s);
   return launch_attention<__nv_bfloat16>(A, s);
@@ -659,14 +721,33 @@ extern "C" {
 int32_t ivb_kv4_attention(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
                           const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window, int32_t sinks, void* out,
                           int64_t o_row, int64_t o_head, uint32_t* error, void* stream) {
-  return ivb::attention_call(c, q, dtype, q_row, q_head, heads, starts, positions, rows, scale, window, sinks, out, o_row, o_head, error, stream,
-                             false);
+  return ivb::attention_call(c, nullptr, q, dtype, q_row, q_head, heads, starts, positions, rows, scale, window, sinks, out, o_row, o_head, nullptr, 0,
+                             error, stream, false);
+}
+
+uint64_t ivb_kv4_prefix_workspace_bytes(const IvbKv4Cache* c, const IvbKv4Prefix* prefix, int32_t dtype, int32_t heads, const int32_t* starts,
+                                        int32_t rows) {
+  if (ivb::check_kv4(c, "ivb_kv4_prefix_workspace_bytes") || rows <= 0 || ivb::check_heads(c, heads, rows) || ivb::check_prefix(c, prefix)) return 0;
+  const int group = heads / c->kv_heads;
+  if (ivb::few_items(*c, group, starts, rows) == 0) return 0;
+  return ivb::part_bytes(ivb::kv4_prefix_splits(*c, prefix->cache, dtype, group, rows), rows, heads, c->head_dim);
+}
+
+int32_t ivb_kv4_attention_prefix(const IvbKv4Cache* c, const IvbKv4Prefix* prefix, const void* q, int32_t dtype, int64_t q_row, int64_t q_head,
+                                 int32_t heads, const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,
+                                 int32_t sinks, void* out, int64_t o_row, int64_t o_head, void* workspace, uint64_t workspace_bytes, uint32_t* error,
+                                 void* stream) {
+  if (int32_t rc = ivb::check_kv4(c, "ivb_kv4_attention_prefix")) return rc;
+  if (int32_t rc = ivb::check_prefix(c, prefix)) return rc;
+  return ivb::attention_call(c, prefix, q, dtype, q_row, q_head, heads, starts, positions, rows, scale, window, sinks, out, o_row, o_head, workspace,
+                             workspace_bytes, error, stream, false);
 }
 
 int32_t ivb_probe_kv4_timeout(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
                               const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window, int32_t sinks,
                               void* out, int64_t o_row, int64_t o_head, uint32_t* error, void* stream) {
-  return ivb::attention_call(c, q, dtype, q_row, q_head, heads, starts, positions, rows, scale, window, sinks, out, o_row, o_head, error, stream, true);
+  return ivb::attention_call(c, nullptr, q, dtype, q_row, q_head, heads, starts, positions, rows, scale, window, sinks, out, o_row, o_head, nullptr, 0,
+                             error, stream, true);
 }
 
 }  // extern "C"

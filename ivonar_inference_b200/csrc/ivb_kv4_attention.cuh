@@ -42,6 +42,17 @@ struct Kv4Attention {
   // had ended then, with their writes in device memory, and a fence at its start keeps it from what an SM's cache may have from before.
   // The two write different rows. The first CTA waits at its end instead, so that who waits for this grid has waited for both.
   bool beside_prompts;
+  // Beginnings that sequences share: sequences prefix_groups[g] .. prefix_groups[g + 1] - 1 (nullptr: all) begin with the first
+  // prefix_lengths[g] positions of the prefix cache's sequence g; data is nullptr where there are none. Prompts' tiles take these
+  // positions before their sequence's own. For few rows another grid (the prompts' kernel as a pass over the prefix, all rows of a
+  // group together) leaves parts [split][row][head] of reference and sum (`part_stats`) and values (`part_values`, [head_dim] each), which the
+  // few rows' kernel joins at its end.
+  IvbKv4Cache prefix;
+  const int64_t* prefix_lengths;
+  const int32_t* prefix_groups;
+  float2* part_stats;
+  float* part_values;
+  int splits;
   unsigned long long wait_ns;  // the longest wait within the prompts' kernel
   bool withhold;               // issue no products, so that the waits for them run out (ivb_probe_kv4_timeout)
 };
@@ -131,7 +142,49 @@ __device__ __forceinline__ PositionTerms position_terms(uint2 par, float score_u
   return t;
 }
 
+// The group of sequence b, found by the whole warp, and the length of its beginning; 0 where there is none. A length beyond the
+// prefix's capacity is reported and counts as that.
+__device__ __forceinline__ int kv4_prefix(const Kv4Attention& A, int b, int& group) {
+  group = 0;
+  if (A.prefix.data == nullptr) return 0;
+  if (A.prefix_groups != nullptr) group = kv4_sequence(A.prefix_groups, A.prefix.batch, b);
+  if (group >= A.prefix.batch) return 0;
+  const int64_t n = A.prefix_lengths[group];
+  if (n > A.prefix.max_len && A.error != nullptr && (threadIdx.x & 31) == 0) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
+  return static_cast<int>(max(static_cast<int64_t>(0), min(n, static_cast<int64_t>(A.prefix.max_len))));
+}
+
+// Joins the parts of row x head `item` to its own reference, sum and values, and divides by the sum; channel(j) is value j's.
+template <int D, int n, typename Channel>
+__device__ __forceinline__ void kv4_join_parts(const Kv4Attention& A, int64_t item, float ref, float sum, float (&v)[n], Channel channel) {
+  const int64_t step = static_cast<int64_t>(A.rows) * A.heads;
+  float top = sum == 0.0f ? -INFINITY : ref;  // zero: nothing was seen
+  for (int k = 0; k < A.splits; ++k) {
+    const float2 s = __ldcg(A.part_stats + k * step + item);
+    if (s.y != 0.0f) top = fmaxf(top, s.x);
+  }
+  const float own = sum == 0.0f ? 0.0f : ex2(ref - top);
+  float l = sum * own;
+#pragma unroll
+  for (int j = 0; j < n; ++j) v[j] = sum == 0.0f ? 0.0f : v[j] * own;
+  for (int k = 0; k < A.splits; ++k) {
+    const float2 s = __ldcg(A.part_stats + k * step + item);
+    if (s.y == 0.0f) continue;
+    const float f = ex2(s.x - top);
+    l = fmaf(s.y, f, l);
+    const float* from = A.part_values + (k * step + item) * D;
+#pragma unroll
+    for (int j = 0; j < n; ++j) v[j] = fmaf(__ldcg(from + channel(j)), f, v[j]);
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int j = 0; j < n; ++j) v[j] = l == 0.0f ? 0.0f : v[j] * inv;
+}
+
 // Prompts: every sequence of the call with more than `few` items (tokens x query heads of a group).
 int32_t launch_kv4_prompts(const Kv4Attention& A, int32_t dtype, int few, cudaStream_t stream);
+// The prefix's parts of the rows of every other sequence, and in how many parts it comes.
+int32_t launch_kv4_prefix(const Kv4Attention& A, int32_t dtype, int few, cudaStream_t stream);
+int kv4_prefix_splits(const IvbKv4Cache& cache, const IvbKv4Cache& prefix, int32_t dtype, int group, int rows);
 
 }  // namespace ivb

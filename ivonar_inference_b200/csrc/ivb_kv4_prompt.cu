@@ -19,6 +19,7 @@
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -35,6 +36,7 @@ constexpr int kRowsX = 128, kRowsCta = 256, kPos = 128;
 // 12 warps: three on each of the SM's four parts have 168 registers a thread, for the scores of four rows at a time
 constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 32 * kSoftmaxWarps, kProducerWarps = 3, kProducers = 32 * kProducerWarps;
 constexpr int kIssueWarp = kSoftmaxWarps + kProducerWarps, kPromptThreads = 32 * (kIssueWarp + 1);
+constexpr int kMostSplits = 16;
 constexpr int kTermSets = 3;  // terms(it + 2) are written when S(it) is done, so when nobody reads terms(it - 1) any more
 constexpr float kWeightUnit = 64.0f;  // weights are at most 2 * 64 * 2^8 in fp16
 constexpr float kRaise = 8.0f;
@@ -190,7 +192,9 @@ __device__ __forceinline__ void store_codes_of_values(const RawChunks<D>& raw, i
   }
 }
 
-template <int D, typename T>
+// kPass: the pass over the prefix for the rows of sequences with no more than `few` items. Its "sequences" are the groups, its
+// items all rows of a group's sequences, each with a position of its own; the tiles are dealt out to A.splits CTAs a row tile.
+template <int D, typename T, bool kPass>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attention A, int few) {
   constexpr bool kSplit = std::is_same<T, float>::value;
   using G = PromptGeometry<D, kSplit>;
@@ -198,25 +202,39 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   __shared__ PromptBarriers bar;
   __shared__ unsigned tmem_base;
   __shared__ float largest[kSoftmaxWarps], smallest[kSoftmaxWarps], sums[kRowsCta], row_units[kRowsCta], refs_of[kRowsCta], totals[kRowsCta], offsets[kRowsCta];
-  __shared__ int which[3];  // sequence, tile of its rows; and whether a wait ran out
+  __shared__ int nearest[kSoftmaxWarps];
+  __shared__ int which[5];  // sequence, tile of its rows; whether a wait ran out; group of the prefix, its length
   const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
-  pdl_wait();
+  if (kPass && A.beside_prompts) __threadfence();
+  else pdl_wait();
   // which rows: the call's tiles of 256 items in the order of the sequences, the last ones (the longest rows) first
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int C = kPass ? A.splits : static_cast<int>(cluster.num_blocks());
+  const int rank = kPass ? static_cast<int>(blockIdx.x) % C : static_cast<int>(cluster.block_rank());
+  const int sequences = kPass ? A.prefix.batch : A.cache.batch;
+  // the rows of sequence, or group, b
+  auto rows_of = [&](int b, int& from) {
+    int b0 = b, b1 = b + 1;
+    if (kPass) {
+      b0 = A.prefix_groups == nullptr ? 0 : max(0, A.prefix_groups[b]);
+      b1 = A.prefix_groups == nullptr ? A.cache.batch : min(A.cache.batch, A.prefix_groups[b + 1]);
+      if (b1 <= b0) b0 = b1 = 0;
+    }
+    from = A.starts == nullptr ? b0 : max(0, A.starts[b0]);
+    return max(0, (A.starts == nullptr ? b1 : min(A.rows, A.starts[b1])) - from);
+  };
   const int unit = static_cast<int>(blockIdx.x) / C, units = static_cast<int>(gridDim.x) / C;
   const int kvh = unit % A.cache.kv_heads, order = units / A.cache.kv_heads - 1 - unit / A.cache.kv_heads;
   if (warp == 0) {
     int seen = 0, found = -1, tile = 0;
-    for (int b0 = 0; b0 < A.cache.batch && found < 0; b0 += 32) {
+    for (int b0 = 0; b0 < sequences && found < 0; b0 += 32) {
       const int b = b0 + lane;
       int n = 0;
-      if (b < A.cache.batch) {
-        int count = 1;
-        if (A.starts != nullptr) count = max(0, min(A.rows, A.starts[b + 1]) - max(0, A.starts[b]));
-        const int items = count * A.group;
-        n = items > few ? (items + G::rows - 1) / G::rows : 0;
+      if (b < sequences) {
+        int from;
+        const int items = rows_of(b, from) * A.group;
+        n = items > (kPass ? 0 : few) ? (items + G::rows - 1) / G::rows : 0;
       }
       int upto = n;
 #pragma unroll
@@ -232,10 +250,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       }
       seen += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
+    int group = found, length = 0;
+    if (found >= 0) {
+      if (kPass) length = static_cast<int>(max(static_cast<int64_t>(0), min(A.prefix_lengths[found], static_cast<int64_t>(A.prefix.max_len))));
+      else length = kv4_prefix(A, found, group);
+    }
     if (lane == 0) {
-      which[0] = found;
+      which[0] = kPass && length == 0 ? -1 : found;
       which[1] = tile;
       which[2] = 0;
+      which[3] = group;
+      which[4] = length;
     }
   }
   if (tid == 32) {
@@ -259,38 +284,56 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   }
   __syncthreads();
   const int b = which[0];
-  if (b < 0) return;
+  // a pass does not end before the prompts' grid that it runs beside, whichever way its first CTA takes
+  auto end = [&] {
+    if (kPass && A.beside_prompts && blockIdx.x == 0) pdl_wait();
+  };
+  if (b < 0) {
+    end();
+    return;
+  }
   if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)), "r"(G::columns));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     pdl_trigger();  // not before this CTA has its tensor memory: the next grid may take some too, and waits for this one
   }
-  int row0 = b, count = 1;
-  int64_t before = 0;  // rows of the sequence that the call does not have
-  if (A.starts != nullptr) {
-    row0 = max(0, A.starts[b]);
-    before = static_cast<int64_t>(row0) - A.starts[b];
-    count = min(A.rows, A.starts[b + 1]) - row0;
-  }
+  int row0;
+  const int count = rows_of(b, row0);
+  // rows of the sequence that the call does not have
+  const int64_t before = A.starts == nullptr || kPass ? 0 : static_cast<int64_t>(row0) - A.starts[b];
   const int i0 = which[1] * G::rows, live = min(G::rows, count * A.group - i0), row_tiles = live > kRowsX ? 2 : 1;
-  const int64_t base = kv4_position(A.positions, b) + before;
+  const int shared_length = which[4];  // positions of the prefix, which come before the sequence's own
   const int max_len = A.cache.max_len;
   const unsigned group_size = static_cast<unsigned>(A.group);
   auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };
   auto clamp_position = [&](int64_t p) { return static_cast<int>(max(static_cast<int64_t>(-1), min(p, static_cast<int64_t>(max_len)))); };
-  const int first = clamp_position(base + token_of(i0)), last = clamp_position(base + token_of(i0 + live - 1));
-  if (last >= max_len && tid == 0 && rank == 0 && A.error != nullptr) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
-  // the tiles of 128 positions that some row sees: the sinks' below the window, then the window's
-  const int high = min(last, max_len - 1);
-  const int low = A.window > 0 ? max(0, max(first, 0) - A.window + 1) : 0;
-  const int window_tile = low / kPos;
-  const int sink_tiles = A.window > 0 ? min((min(A.sinks, low) + kPos - 1) / kPos, window_tile) : 0;
-  const int all_tiles = high < 0 ? 0 : sink_tiles + high / kPos - window_tile + 1;
-  const int tiles = all_tiles > rank ? (all_tiles - rank + C - 1) / C : 0;  // this CTA's
-  auto tile_of = [&](int it) {
-    const int i = rank + it * C;
-    return i < sink_tiles ? i : window_tile + i - sink_tiles;
+  const int64_t base = kPass ? 0 : kv4_position(A.positions, b) + before;
+  // position of row r of the tile in its sequence's own cache, -1 where it sees nothing
+  auto own_position = [&](int r) {
+    if (r >= live) return -1;
+    int64_t p;
+    if constexpr (kPass) {
+      const int row = row0 + token_of(i0 + r);
+      int of = row;
+      if (A.starts != nullptr) {  // the last sequence of the group that starts at or before the row
+        int low = A.prefix_groups == nullptr ? 0 : max(0, A.prefix_groups[b]);
+        int high = A.prefix_groups == nullptr ? A.cache.batch : min(A.cache.batch, A.prefix_groups[b + 1]);
+        while (high - low > 1) {
+          const int middle = (low + high) >> 1;
+          if (A.starts[middle] <= row) low = middle;
+          else high = middle;
+        }
+        of = low;
+        if (static_cast<int64_t>(min(A.rows, A.starts[of + 1]) - max(0, A.starts[of])) * A.group > few) return -1;  // a prompt's
+      }
+      p = kv4_position(A.positions, of) + (A.starts == nullptr ? 0 : row - A.starts[of]);
+    } else {
+      p = base + token_of(i0 + r);
+    }
+    return p < 0 || p >= max_len ? -1 : static_cast<int>(p);
   };
+  if (!kPass && tid == 0 && rank == 0 && A.error != nullptr && clamp_position(base + token_of(i0 + live - 1)) >= max_len)
+    atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
 
   // queries: a warp takes 32 rows in 16-byte chunks, 8 rows and 4 chunks at a time (64 contiguous bytes of a row, and no bank
   // conflicts); the rows' largest first, then hi (and lo) parts as K-major operands, scaled by a power of two that brings the largest of
@@ -303,13 +346,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     return static_cast<const T*>(array) + (row0 + t) * row_stride + h * head_stride;
   };
   uint4 raw[4][kQuads];
+  int own_at = -1;  // of row 32 warp + lane
   if (tid < kSoftmaxThreads) {
+    own_at = own_position(tid);
+    if constexpr (kPass) {
+      const unsigned to_end = __reduce_min_sync(0xFFFFFFFFu, static_cast<unsigned>(own_at));  // -1 is the largest
+      if (lane == 0) nearest[warp] = static_cast<int>(to_end);
+    }
     const T* q[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int r = 32 * warp + 8 * g + row8;
-      const int p = clamp_position(base + token_of(i0 + r));
-      q[g] = r < live && p >= 0 && p < max_len ? item_row(A.q, i0 + r, A.q_row, A.q_head) + chunk4 * kPer : nullptr;
+      q[g] = __shfl_sync(0xFFFFFFFFu, own_at, 8 * g + row8) >= 0 ? item_row(A.q, i0 + r, A.q_row, A.q_head) + chunk4 * kPer : nullptr;
     }
     if (A.q_vec) {
 #pragma unroll
@@ -368,6 +416,38 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     least = fminf(least, smallest[w]);
   }
   const bool even = least >= most * kEven;
+  // The tiles of 128 positions that some row sees, of the prefix and then of the sequence's own: in each the sinks' below the window,
+  // then the window's. Positions count from the beginning, where the own ones' tiles stand at shared_length + 128 t.
+  int first, high;  // own positions: the rows' first, and the last that there is
+  if constexpr (kPass) {
+    unsigned low_at = 0xffffffffu;
+#pragma unroll
+    for (int w = 0; w < kSoftmaxWarps; ++w) low_at = min(low_at, static_cast<unsigned>(nearest[w]));
+    first = static_cast<int>(low_at);
+    high = -1;
+  } else {
+    first = clamp_position(base + token_of(i0));
+    high = min(clamp_position(base + token_of(i0 + live - 1)), max_len - 1);
+  }
+  const int low = A.window > 0 ? max(0, max(first, 0) + shared_length - A.window + 1) : 0;
+  const int own_low = max(0, low - shared_length), own_sinks = max(0, A.sinks - shared_length);
+  const int window_tile = own_low / kPos;
+  const int sink_tiles = A.window > 0 ? min((min(own_sinks, own_low) + kPos - 1) / kPos, window_tile) : 0;
+  const int own_tiles = high < 0 ? 0 : sink_tiles + high / kPos - window_tile + 1;
+  const bool any_row = kPass ? first >= 0 : high >= 0;
+  const int shared_all = any_row ? (shared_length + kPos - 1) / kPos : 0;
+  const int shared_window = min(low / kPos, shared_all);
+  const int shared_sinks = A.window > 0 ? min((min(A.sinks, low) + kPos - 1) / kPos, shared_window) : 0;
+  const int shared_tiles = shared_sinks + shared_all - shared_window;
+  const int all_tiles = shared_tiles + own_tiles;
+  const int tiles = all_tiles > rank ? (all_tiles - rank + C - 1) / C : 0;  // this CTA's
+  auto of_prefix = [&](int it) { return kPass || rank + it * C < shared_tiles; };
+  auto tile_of = [&](int it) {  // in its cache
+    int i = rank + it * C;
+    if (of_prefix(it)) return i < shared_sinks ? i : shared_window + i - shared_sinks;
+    i -= shared_tiles;
+    return i < sink_tiles ? i : window_tile + i - sink_tiles;
+  };
   const int up = query_power(most);
   const float score_unit = power_of_two(-up) * (A.scale * kLog2e);  // in the positions' terms
   if (tid < kSoftmaxThreads && x < row_tiles) {
@@ -424,11 +504,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     // ---- producers: 16-position tiles in turn ----
     constexpr int kTile = kv4_tile_bytes(D), kUnits = kPos / 16, kMine = (kUnits + kProducerWarps - 1) / kProducerWarps;
     const int unit0 = warp - kSoftmaxThreads / 32;
-    const int64_t tiles16 = kv4_tiles(max_len);
-    const unsigned char* codes = static_cast<const unsigned char*>(A.cache.data) + (static_cast<int64_t>(b) * A.cache.kv_heads + kvh) * tiles16 * kTile;
+    const int64_t own16 = kv4_tiles(max_len), shared16 = kv4_tiles(A.prefix.max_len);
+    const unsigned char* const own_codes = static_cast<const unsigned char*>(A.cache.data) + (static_cast<int64_t>(b) * A.cache.kv_heads + kvh) * own16 * kTile;
+    const unsigned char* const shared_codes = static_cast<const unsigned char*>(A.prefix.data) + (static_cast<int64_t>(which[3]) * A.cache.kv_heads + kvh) * shared16 * kTile;
     RawChunks<D> key[kMine], value[kMine];
     uint2 par[kMine];
     auto fetch = [&](int it, bool keys) {
+      const bool shared = of_prefix(it);
+      const unsigned char* const codes = shared ? shared_codes : own_codes;
+      const int64_t tiles16 = shared ? shared16 : own16;
 #pragma unroll
       for (int k = 0; k < kMine; ++k) {
         const int u = unit0 + k * kProducerWarps;
@@ -567,9 +651,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       const int n = kRowsX * x + row0x + 8 * i + r;
       sum_q[i] = sums[n];
       at[i] = -1;
+      const int p = __shfl_sync(0xFFFFFFFFu, own_at, 8 * i + r);
       if (n < live) {
-        const int p = clamp_position(base + token_of(i0 + n));
-        at[i] = p < max_len ? p : -1;
+        at[i] = p < 0 ? -1 : shared_length + p;
         live_rows = true;
         first_at = min(first_at, at[i]);
         last_at = max(last_at, at[i]);
@@ -587,11 +671,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     auto walk = [&](auto evenly) {
       bool stop = false;  // the same in all lanes, where `ok` is each lane's own between two votes
       for (int it = 0; it < tiles && !stop; ++it) {
-        const int p0 = tile_of(it) * kPos;
+        const bool shared = of_prefix(it);
+        const int p0 = tile_of(it) * kPos + (shared ? 0 : shared_length), end = shared ? shared_length - 1 : 0x7fffffff;
         const float* terms = terms_of(it);
         ok = ok && wait_for(&bar.terms_full[it % kTermSets], static_cast<unsigned>(it / kTermSets) & 1u);
         // what the warp's rows see of the tile: all of it, or nothing (first_at, last_at: the lowest and highest, -1 among them)
-        const bool whole = live_rows && first_at >= p0 + kPos - 1 && (A.window <= 0 || p0 > last_at - A.window || p0 <= A.sinks - kPos);
+        const bool whole = live_rows && min(first_at, end) >= p0 + kPos - 1 && (A.window <= 0 || p0 > last_at - A.window || p0 <= A.sinks - kPos);
         const bool none = last_at < p0 || (A.window > 0 && p0 + kPos - 1 <= first_at - A.window && p0 >= A.sinks);
         // 64 positions at a time: the next ones' scores and the last ones' product are computed meanwhile
 #pragma unroll 1
@@ -675,7 +760,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   const int p = p0 + h * (kPos / 2) + 8 * i + 2 * c + e;
-                  if (p > at[n] || (p <= from && p >= A.sinks)) s[n >> 1][4 * i + 2 * (n & 1) + e] = 0xff800000u;
+                  if (p > min(at[n], end) || (p <= from && p >= A.sinks)) s[n >> 1][4 * i + 2 * (n & 1) + e] = 0xff800000u;
                 }
             }
           }
@@ -791,7 +876,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float(f[j]));
     }
   };
-  if (C == 1) {
+  if constexpr (kPass) {
+    if (mine) {  // whole warps: they load from tensor memory together, also for rows that there are not
+      const bool there = row < live;
+      const int t = token_of(i0 + row), h = kvh * A.group + i0 + row - t * A.group;
+      const int64_t item = (static_cast<int64_t>(rank) * A.rows + row0 + t) * A.heads + h;
+      const float total = totals[row], offset = offsets[row];
+      if (there) A.part_stats[item] = make_float2(refs_of[row], total);
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 16) {
+        uint32_t o[16];
+        if (tiles > 0 && ok) load_o(c0, o);
+        else
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = 0u;
+        if (there && total != 0.0f) {
+          float4* const to = reinterpret_cast<float4*>(A.part_values + item * D + c0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            to[j] = make_float4(fmaf(__uint_as_float(o[4 * j]), 1.0f / kWeightUnit, offset), fmaf(__uint_as_float(o[4 * j + 1]), 1.0f / kWeightUnit, offset),
+                                fmaf(__uint_as_float(o[4 * j + 2]), 1.0f / kWeightUnit, offset), fmaf(__uint_as_float(o[4 * j + 3]), 1.0f / kWeightUnit, offset));
+        }
+      }
+    }
+  } else if (C == 1) {
     if (mine) {
       // through the place of its tile's queries, to leave in whole 16-byte chunks: 32 rows a warp
       const float total = totals[row], offset = offsets[row], inv = total == 0.0f ? 0.0f : 1.0f / total;
@@ -894,19 +1002,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::columns));
   }
+  end();
 }
 
-template <int D, typename T>
-int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
+// Opt-in shared memory, once per device.
+template <int D, typename T, bool kPass>
+int32_t allow_prompt() {
   using G = PromptGeometry<D, std::is_same<T, float>::value>;
   static std::atomic<uint64_t> done{0};
   int device = 0;
   IVB_CUDA(cudaGetDevice(&device));
   const uint64_t bit = device < 64 ? 1ull << device : 0;
   if ((done.load(std::memory_order_relaxed) & bit) == 0) {
-    IVB_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem));
+    IVB_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<D, T, kPass>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem));
     done.fetch_or(bit, std::memory_order_relaxed);
   }
+  return IVB_OK;
+}
+
+template <int D, typename T>
+int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
+  using G = PromptGeometry<D, std::is_same<T, float>::value>;
+  if (int32_t rc = allow_prompt<D, T, false>()) return rc;
   // as many tiles as the rows can make: each sequence of the call may leave one unfilled
   const int64_t items = static_cast<int64_t>(A.rows) * A.group;
   const int64_t sequences = std::min<int64_t>(A.cache.batch, items / (few + 1));
@@ -915,7 +1032,8 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   // a cluster where one CTA each would leave SMs without work (128 CTAs of a 2048-row causal prompt: 68 us, in pairs 56, in fours
   // 88; 256 CTAs of a chunk under a window: 228, in pairs 275; each pair measured on one day's kernel)
   int C = 1;
-  while (C < 4 && tiles * A.cache.kv_heads * C < 148 && A.cache.max_len > 2 * C * kPos) C *= 2;
+  const int64_t most = A.cache.max_len + (A.prefix.data == nullptr ? 0 : static_cast<int64_t>(A.prefix.max_len));
+  while (C < 4 && tiles * A.cache.kv_heads * C < 148 && most > 2 * C * kPos) C *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * A.cache.kv_heads * C));
   cfg.blockDim = dim3(kPromptThreads);
@@ -924,25 +1042,49 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
   cfg.numAttrs = kv4_attributes(C, attr);
-  IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<D, T>, A, few));
+  IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<D, T, false>, A, few));
+  return IVB_OK;
+}
+
+template <int D, typename T>
+int32_t launch_prefix(const Kv4Attention& A, int few, cudaStream_t stream) {
+  using G = PromptGeometry<D, std::is_same<T, float>::value>;
+  if (int32_t rc = allow_prompt<D, T, true>()) return rc;
+  // as many tiles as the rows can make: each group may leave one unfilled
+  const int64_t tiles = static_cast<int64_t>(A.rows) * A.group / G::rows + std::min<int64_t>(A.prefix.batch, A.rows);
+  const int64_t grid = tiles * A.cache.kv_heads * A.splits;
+  if (grid > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(tiles));
+  IVB_CUDA(launch_pdl(kv4_prompt_kernel<D, T, true>, dim3(static_cast<unsigned>(grid)), dim3(kPromptThreads), G::smem, stream, A, few));
   return IVB_OK;
 }
 
 template <typename T>
-int32_t launch_dim(const Kv4Attention& A, int few, cudaStream_t stream) {
+int32_t launch_dim(const Kv4Attention& A, bool pass, int few, cudaStream_t stream) {
   switch (A.cache.head_dim) {
-    case 32: return launch_prompts<32, T>(A, few, stream);
-    case 64: return launch_prompts<64, T>(A, few, stream);
-    default: return launch_prompts<128, T>(A, few, stream);
+    case 32: return pass ? launch_prefix<32, T>(A, few, stream) : launch_prompts<32, T>(A, few, stream);
+    case 64: return pass ? launch_prefix<64, T>(A, few, stream) : launch_prompts<64, T>(A, few, stream);
+    default: return pass ? launch_prefix<128, T>(A, few, stream) : launch_prompts<128, T>(A, few, stream);
   }
+}
+
+int32_t launch_type(const Kv4Attention& A, int32_t dtype, bool pass, int few, cudaStream_t stream) {
+  if (dtype == IVB_F32) return launch_dim<float>(A, pass, few, stream);
+  if (dtype == IVB_F16) return launch_dim<__half>(A, pass, few, stream);
+  return launch_dim<__nv_bfloat16>(A, pass, few, stream);
 }
 
 }  // namespace
 
-int32_t launch_kv4_prompts(const Kv4Attention& A, int32_t dtype, int few, cudaStream_t stream) {
-  if (dtype == IVB_F32) return launch_dim<float>(A, few, stream);
-  if (dtype == IVB_F16) return launch_dim<__half>(A, few, stream);
-  return launch_dim<__nv_bfloat16>(A, few, stream);
+int32_t launch_kv4_prompts(const Kv4Attention& A, int32_t dtype, int few, cudaStream_t stream) { return launch_type(A, dtype, false, few, stream); }
+int32_t launch_kv4_prefix(const Kv4Attention& A, int32_t dtype, int few, cudaStream_t stream) { return launch_type(A, dtype, true, few, stream); }
+
+// Parts of the prefix that fill the SMs, if the rows are spread evenly over its groups and it is as long as it can be.
+int kv4_prefix_splits(const IvbKv4Cache& cache, const IvbKv4Cache& prefix, int32_t dtype, int group, int rows) {
+  const int per_tile = dtype == IVB_F32 && cache.head_dim == 128 ? kRowsX : kRowsCta;
+  const int64_t groups = std::min(prefix.batch, rows), items = (static_cast<int64_t>(rows) * group + groups - 1) / groups;
+  const int64_t units = groups * ((items + per_tile - 1) / per_tile) * cache.kv_heads;
+  const int64_t most = std::min<int64_t>(kMostSplits, (static_cast<int64_t>(prefix.max_len) + kPos - 1) / kPos);
+  return static_cast<int>(std::max<int64_t>(1, std::min(most, 148 / units)));
 }
 
 }  // namespace ivb

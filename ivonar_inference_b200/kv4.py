@@ -13,8 +13,11 @@ number of those before it). A row at a negative position is idle: nothing is wri
 beyond is treated the same way and reported by `check`. A token is attended to once it is written: `append` first,
 then `attention`, on one stream.
 
-Inference only: nothing here is differentiable. The calls allocate nothing but the tensors they return, do not wait for the
-GPU, and can be captured in a CUDA graph.
+Sequences that answer one prompt need not hold it each: `attention` takes a second cache with what they begin with, held and read
+once (`prefix`), `fork` lets a sequence begin as another does, of this cache or of another one, and `compact` moves a sequence's rows up.
+
+Inference only: nothing here is differentiable. The calls allocate nothing but the tensors they return (with a prefix, a workspace for
+the call too), do not wait for the GPU, and can be captured in a CUDA graph.
 """
 
 from __future__ import annotations
@@ -233,7 +236,8 @@ class KV4Cache:
         self._call("ivb_kv4_compact", self.lib.ivb_kv4_compact, self._ref, values, at, positions.data_ptr(), rows)
 
     def attention(self, q: Tensor, positions: Tensor, starts: Tensor | None = None, scale: float | None = None, window: int = 0,
-                  sinks: int = 0, out: Tensor | None = None) -> Tensor:
+                  sinks: int = 0, out: Tensor | None = None, prefix: KV4Cache | None = None, prefix_lengths: Tensor | None = None,
+                  prefix_groups: Tensor | None = None) -> Tensor:
         """Causal attention of the queries q [rows, heads, head_dim] over their sequences' caches, in q's type.
 
         `heads` is a multiple of `kv_heads`: query head h reads key/value head h // (heads // kv_heads). The row at position p
@@ -242,6 +246,13 @@ class KV4Cache:
         With fp32 queries the softmax's weights keep 22 bits; with fp16 and bf16 ones they are rounded to fp16 (by 2^-11 of each at most)
         before they meet the values, but for single tokens with up to four query heads a key/value head.
         Values that pass fp16 (see `read`) may give infinity in an fp16 result.
+
+        With `prefix`, another cache with the same heads, sequences share what they begin with: the sequences prefix_groups[g] ..
+        prefix_groups[g + 1] - 1 (int32 [prefix.batch + 1] on the device, ascending; without it all of them, behind a prefix of one
+        sequence) begin with the first prefix_lengths[g] positions (int64 [prefix.batch] on the device) of its sequence g, and
+        sequences of no group with nothing. They are held once, and read once for all rows that are tokens or drafts. `positions` then count
+        from the end of that beginning, as in `append`, and windows and sinks from its start. A length beyond the prefix's capacity is reported
+        by `check` and counts as that capacity.
         """
 
         heads = q.shape[1] if q.ndim == 3 else 0
@@ -265,10 +276,39 @@ class KV4Cache:
             if out.data_ptr() != q.data_ptr() or out.stride() != q.stride():
                 _apart(out, q, "out and q")
         at = self._rows(rows, positions, starts)
-        self._call("ivb_kv4_attention", self.lib.ivb_kv4_attention, self._ref, q.data_ptr(), _TYPES[q.dtype], q_row, q_head, heads,
-                   at, positions.data_ptr(), rows, self.head_dim**-0.5 if scale is None else scale, window, sinks, out.data_ptr(), o_row,
-                   o_head)
+        if scale is None:
+            scale = self.head_dim**-0.5
+        dtype = _TYPES[q.dtype]
+        if prefix is None:
+            if prefix_lengths is not None or prefix_groups is not None:
+                raise ValueError("prefix_lengths and prefix_groups need a prefix")
+            self._call("ivb_kv4_attention", self.lib.ivb_kv4_attention, self._ref, q.data_ptr(), dtype, q_row, q_head, heads,
+                       at, positions.data_ptr(), rows, scale, window, sinks, out.data_ptr(), o_row, o_head)
+            return out
+        shared = ctypes.byref(self._prefix(prefix, prefix_lengths, prefix_groups))
+        nbytes = self.lib.ivb_kv4_prefix_workspace_bytes(self._ref, shared, dtype, heads, at, rows)
+        workspace = self.data.new_empty(nbytes) if nbytes else None  # a call's own: nothing is shared by calls at the same time
+        self._call("ivb_kv4_attention_prefix", self.lib.ivb_kv4_attention_prefix, self._ref, shared, q.data_ptr(), dtype, q_row, q_head, heads,
+                   at, positions.data_ptr(), rows, scale, window, sinks, out.data_ptr(), o_row, o_head, workspace.data_ptr() if nbytes else 0,
+                   nbytes)
         return out
+
+    def _prefix(self, prefix: KV4Cache, lengths: Tensor | None, groups: Tensor | None) -> native.IvbKv4Prefix:
+        """Checks of what the sequences begin with."""
+
+        if prefix.device != self.device or prefix.kv_heads != self.kv_heads or prefix.head_dim != self.head_dim:
+            raise ValueError(f"prefix must be a cache of {self.kv_heads} heads x {self.head_dim} on {self.device}")
+        if prefix.max_len + self.max_len >= 2**31 - 256:
+            raise ValueError(f"{self.max_len} positions behind {prefix.max_len}")
+        if lengths is None:
+            raise ValueError("a prefix needs prefix_lengths")
+        if groups is None:
+            if prefix.batch != 1:
+                raise ValueError(f"{prefix.batch} prefixes need prefix_groups")
+        elif (groups.dtype is not torch.int32 or groups.shape != (prefix.batch + 1,) or groups.device != self.device
+                or not groups.is_contiguous()):
+            raise ValueError(f"prefix_groups must be an int32 tensor [{prefix.batch + 1}] on {self.device}")
+        return native.IvbKv4Prefix(prefix._desc, prefix._numbers("prefix_lengths", lengths, prefix.batch), 0 if groups is None else groups.data_ptr())
 
 
 def _places(x: Tensor) -> Tensor:
