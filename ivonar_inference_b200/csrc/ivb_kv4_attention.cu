@@ -73,7 +73,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-template <int D, typename T, bool kSplit, int kTiles>
+template <int D, typename T, bool kSplit, int kTiles, bool kShared>
 __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_sequence) {
   using G = RowsGeometry<D, T, kSplit, kTiles>;
   constexpr int R = G::rows, kSteps = D / 16, kTile = kv4_tile_bytes(D);
@@ -111,10 +111,10 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
   const int live = min(R, items - i0);
   const int64_t base = kv4_position(A.positions, b) + before;
   const int max_len = A.cache.max_len;
-  // a beginning that the sequence shares: its positions come first, and are joined from their parts at the end
-  int prefix_group;
-  const int shared_length = kv4_prefix(A, b, prefix_group), sinks = max(0, A.sinks - shared_length);
-  const bool joined = A.part_stats != nullptr && shared_length > 0;
+  // a beginning that the sequence shares: joined from its parts at the end, or walked here, at positions below zero
+  int prefix_group = 0;
+  const int shared_length = kShared ? kv4_prefix(A, b, prefix_group) : 0, sinks = kShared ? A.sinks - shared_length : A.sinks;
+  const bool joined = kShared && shared_length > 0 && A.part_stats != nullptr, walked = kShared && shared_length > 0 && !joined;
   // token and query head of an item of the sequence's head group
   auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };
   // positions of the tile's first and last rows, -1 where idle and max_len where beyond the capacity
@@ -133,20 +133,33 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
   const int high = min(last, max_len - 1);  // negative: none
   const int low = A.window > 0 ? max(0, max(first, 0) - A.window + 1) : 0;
   const int window_group = low / kKv4Group;
-  const int sink_groups = A.window > 0 ? min((min(sinks, low) + kKv4Group - 1) / kKv4Group, window_group) : 0;
-  const int groups = high < 0 ? 0 : sink_groups + high / kKv4Group - window_group + 1;
+  const int sink_groups = A.window > 0 ? min((min(kShared ? max(0, sinks) : sinks, low) + kKv4Group - 1) / kKv4Group, window_group) : 0;
+  const int own_groups = high < 0 ? 0 : sink_groups + high / kKv4Group - window_group + 1;
+  int shared_groups = 0, shared_sinks = 0, shared_window = 0;  // of the beginning, before these
+  if (walked && own_groups > 0) {
+    const int all = (shared_length + kKv4Group - 1) / kKv4Group, from = A.window > 0 ? max(0, max(first, 0) + shared_length - A.window + 1) : 0;
+    shared_window = min(from / kKv4Group, all);
+    shared_sinks = A.window > 0 ? min((min(A.sinks, from) + kKv4Group - 1) / kKv4Group, shared_window) : 0;
+    shared_groups = shared_sinks + all - shared_window;
+  }
+  const int groups = shared_groups + own_groups;
   const int lanes_in = C * W, mine = rank * W + warp;
   const int steps = groups > mine ? (groups - mine + lanes_in - 1) / lanes_in : 0;
 
   const unsigned char* const codes = static_cast<const unsigned char*>(A.cache.data) +
                                      (static_cast<int64_t>(b) * A.cache.kv_heads + kvh) * kv4_tiles(max_len) * kTile + lane * 16;
-  auto group_of = [&](int step) {
-    const int i = mine + step * lanes_in;
+  const unsigned char* const shared_codes = static_cast<const unsigned char*>(A.prefix.data) +
+                                            (static_cast<int64_t>(prefix_group) * A.cache.kv_heads + kvh) * kv4_tiles(A.prefix.max_len) * kTile + lane * 16;
+  auto of_prefix = [&](int step) { return kShared && mine + step * lanes_in < shared_groups; };
+  auto group_of = [&](int step) {  // in its cache
+    int i = mine + step * lanes_in;
+    if (of_prefix(step)) return i < shared_sinks ? i : shared_window + i - shared_sinks;
+    if constexpr (kShared) i -= shared_groups;
     return i < sink_groups ? i : window_group + i - sink_groups;
   };
   auto issue = [&](int step, int stage) {
     if (step < steps) {
-      const unsigned char* src = codes + static_cast<int64_t>(group_of(step)) * G::group_bytes;
+      const unsigned char* src = (of_prefix(step) ? shared_codes : codes) + static_cast<int64_t>(group_of(step)) * G::group_bytes;
       unsigned char* dst = ring + stage * G::group_bytes + lane * 16;
 #pragma unroll
       for (int o = 0; o < G::group_bytes; o += 512)
@@ -261,7 +274,8 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
     cp_async_wait<G::stages - 2>();
     __syncwarp();
     const unsigned char* const stage = ring + at_stage * G::group_bytes;
-    const int p0 = group_of(step) * kKv4Group;
+    const bool shared = of_prefix(step);
+    const int p0 = group_of(step) * kKv4Group - (shared ? shared_length : 0);
     {
       const uint2 par = *reinterpret_cast<const uint2*>(stage + (lane >> 4) * kTile + 16 * D + (lane & 15) * 8);
       const PositionTerms t = position_terms(par, 1.0f, 16384.0f, lane);
@@ -318,14 +332,14 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
       }
     }
     // a group that every row sees whole needs no masks
-    const bool whole = first >= p0 + kKv4Group - 1 && last < max_len && (A.window <= 0 || p0 > last - A.window || p0 <= sinks - kKv4Group);
+    const bool whole = (shared ? first >= 0 && p0 + kKv4Group <= 0 : first >= p0 + kKv4Group - 1) && last < max_len && (A.window <= 0 || p0 > last - A.window || p0 <= sinks - kKv4Group);
     if (!whole) {
 #pragma unroll
       for (int s = 0; s < kSets; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int p = p0 + 16 * (i >> 1) + mine_of + 2 * (i & 1);
-          const bool seen = p <= at[s] && (A.window <= 0 || p > at[s] - A.window || p < sinks);
+          const bool seen = (shared ? p < 0 && at[s] >= 0 : p <= at[s]) && (A.window <= 0 || p > at[s] - A.window || p < sinks);
           if (!seen) x[s][i] = -INFINITY;
         }
     }
@@ -441,18 +455,11 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
       off[s] += __shfl_xor_sync(0xFFFFFFFFu, off[s], d);
     }
   fold(true);
-  if (joined) pdl_wait();  // for the parts
-  auto head_of = [&](int row) { return kvh * A.group + i0 + row - token_of(i0 + row) * A.group; };
-  auto item_of = [&](int row) { return static_cast<int64_t>(row0 + token_of(i0 + row)) * A.heads + head_of(row); };
-  auto idle = [&](int row) {
-    const int p = clamp_position(base + token_of(i0 + row));
-    return p < 0 || p >= max_len;
-  };
   auto place = [&](int row) {
     const int t = token_of(i0 + row);
-    return static_cast<T*>(A.out) + (row0 + t) * A.o_row + head_of(row) * A.o_head;
+    return static_cast<T*>(A.out) + (row0 + t) * A.o_row + (kvh * A.group + i0 + row - t * A.group) * A.o_head;
   };
-  if (C * W == 1) {
+  if (C * W == 1 && !joined) {
 #pragma unroll
     for (int s = 0; s < kSets; ++s)
       if (row_of(s) < live) {
@@ -462,8 +469,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
         for (int h = 0; h < kPlanes; ++h) {
           float y[kRun];
 #pragma unroll
-          for (int j = 0; j < kRun; ++j) y[j] = sum[s] == 0.0f ? 0.0f : (o[s][h][j] + off[s]) * (joined ? 1.0f : inv);
-          if (joined && at[s] >= 0) kv4_join_parts<D, kRun>(A, item_of(row_of(s)), ref[s], sum[s], y, [&](int j) { return channel(h, j); });
+          for (int j = 0; j < kRun; ++j) y[j] = sum[s] == 0.0f ? 0.0f : (o[s][h][j] + off[s]) * inv;
           if constexpr (D == 32) {
 #pragma unroll
             for (int j = 0; j < kRun; ++j) out[channel(h, j)] = from_f32<T>(y[j]);
@@ -490,6 +496,69 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
         for (int j = 0; j < kRun; ++j) part[row_of(s) * D + channel(h, j)] = o[s][h][j];
     }
   __syncthreads();
+  // what the CTA's warps found for a row and n of its channels: values with their offset, reference and sum
+  auto of_warps = [&](int row, int c0, auto& v, float& top, float& l) {
+    constexpr int n = sizeof(v) / sizeof(float);
+    top = -INFINITY;
+    l = 0.0f;
+    for (int w = 0; w < W; ++w) top = fmaxf(top, stats[(w * R + row) * 3]);
+#pragma unroll
+    for (int j = 0; j < n; ++j) v[j] = 0.0f;
+    for (int w = 0; w < W; ++w) {
+      const float* st = stats + (w * R + row) * 3;
+      if (st[1] == 0.0f) continue;  // the warp saw nothing for this row
+      const float f = ex2(st[0] - top);
+      l = fmaf(st[1], f, l);
+#pragma unroll
+      for (int j = 0; j < n; ++j) v[j] = fmaf(reinterpret_cast<const float*>(smem + w * G::warp_bytes)[row * D + c0 + j] + st[2], f, v[j]);
+    }
+  };
+  if (kShared && joined) {
+    // a warp a row, D / 32 neighbouring channels a lane
+    constexpr int n = D / 32;
+    float* const cref = comb + R * D;
+    if (C > 1) {
+      for (int row = warp; row < live; row += W) {
+        float v[n], top, l;
+        of_warps(row, n * lane, v, top, l);
+#pragma unroll
+        for (int j = 0; j < n; ++j) comb[row * D + n * lane + j] = v[j];
+        if (lane == 0) {
+          cref[row] = top;
+          cref[R + row] = l;
+        }
+      }
+      cluster.sync();
+    }
+    pdl_wait();  // for the parts
+    for (int row = rank + C * warp; row < live; row += C * W) {
+      float v[n], top = -INFINITY, l = 0.0f;
+      if (C == 1) {
+        of_warps(row, n * lane, v, top, l);
+      } else {
+        for (int k = 0; k < C; ++k) top = fmaxf(top, cluster.map_shared_rank(comb, k)[R * D + row]);
+#pragma unroll
+        for (int j = 0; j < n; ++j) v[j] = 0.0f;
+        for (int k = 0; k < C; ++k) {
+          const float* other = cluster.map_shared_rank(comb, k);
+          const float theirs = other[R * D + R + row];
+          if (theirs == 0.0f) continue;
+          const float f = ex2(other[R * D + row] - top);
+          l = fmaf(theirs, f, l);
+#pragma unroll
+          for (int j = 0; j < n; ++j) v[j] = fmaf(other[row * D + n * lane + j], f, v[j]);
+        }
+      }
+      const int p = clamp_position(base + token_of(i0 + row));
+      if (p >= 0 && p < max_len) {
+        const int t = token_of(i0 + row);
+        kv4_join_parts<D>(A, static_cast<int64_t>(row0 + t) * A.heads + kvh * A.group + i0 + row - t * A.group, top, l, v);
+      }  // an idle row: zeros
+      store_values<T, n>(place(row) + n * lane, A.o_vec && n > 1, v);
+    }
+    if (C > 1) cluster.sync();  // no CTA leaves while another reads its shared memory
+    return;
+  }
   float* const cref = comb + R * D;
   for (int i = threadIdx.x; i < live * D; i += 32 * W) {
     const int row = i / D;
@@ -506,10 +575,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
       }
     }
     if (C == 1) {
-      float y[1] = {v + m};
-      if (joined && !idle(row)) kv4_join_parts<D, 1>(A, item_of(row), top, l, y, [&](int) { return i - row * D; });
-      else y[0] = l == 0.0f ? 0.0f : y[0] / l;
-      place(row)[i - row * D] = from_f32<T>(y[0]);
+      place(row)[i - row * D] = from_f32<T>(l == 0.0f ? 0.0f : (v + m) / l);
     } else {
       comb[i] = v;
       if (i - row * D == 0) {
@@ -536,17 +602,15 @@ __device__ __forceinline__ void kv4_rows(const Kv4Attention& A, int tiles_per_se
         l = fmaf(part_sum, f, l);
       }
     }
-    float y[1] = {v};
-    if (joined && !idle(row)) kv4_join_parts<D, 1>(A, item_of(row), top, l, y, [&](int) { return i - row * D; });
-    else y[0] = l == 0.0f ? 0.0f : y[0] / l;
-    place(row)[i - row * D] = from_f32<T>(y[0]);
+    place(row)[i - row * D] = from_f32<T>(l == 0.0f ? 0.0f : v / l);
   }
   cluster.sync();  // no CTA leaves while another reads its shared memory
 }
 
-template <int D, typename T, bool kSplit, int kTiles>
+// kShared: behind beginnings that the sequences share. (Told apart as it runs, 39.4 us where 38.7 are kept for 256 sequences.)
+template <int D, typename T, bool kSplit, int kTiles, bool kShared>
 __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(Kv4Attention A, int tiles_per_sequence) {
-  kv4_rows<D, T, kSplit, kTiles>(A, tiles_per_sequence);
+  kv4_rows<D, T, kSplit, kTiles, kShared>(A, tiles_per_sequence);
   // whichever way the rows took: this grid does not end before the ones that it runs beside
   if (A.beside_prompts && blockIdx.x == 0) pdl_wait();
 }
@@ -563,12 +627,12 @@ int32_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
   return IVB_OK;
 }
 
-template <int D, typename T, bool kSplit, int kTiles>
+template <int D, typename T, bool kSplit, int kTiles, bool kShared>
 int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   using G = RowsGeometry<D, T, kSplit, kTiles>;
   constexpr int kMostWarps = 8;
   static std::atomic<uint64_t> done{0};
-  if (int32_t rc = allow_smem(kv4_rows_kernel<D, T, kSplit, kTiles>, G::smem(kMostWarps), done)) return rc;
+  if (int32_t rc = allow_smem(kv4_rows_kernel<D, T, kSplit, kTiles, kShared>, G::smem(kMostWarps), done)) return rc;
   const int64_t most = std::min<int64_t>(A.few, static_cast<int64_t>(A.starts == nullptr ? 1 : A.rows) * A.group);
   const int64_t tiles = (most + G::rows - 1) / G::rows;
   const int64_t grid = tiles * A.cache.kv_heads * A.cache.batch;
@@ -580,9 +644,10 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   // 128-640 51, 41, 49, 74 us; 1024 tiles at 300-1900 51, 36, 34, 38; 256 tiles of 1028 positions x 128 50, 30, 21, 17; 32 tiles
   // of 30000 x 128 with 8 warps, clusters of 1 and 8: 203 and 42.
   const int64_t slots = 148 * 16;  // warps of this kernel that the GPU holds
+  const int64_t reach = A.cache.max_len + (kShared && A.part_stats == nullptr ? static_cast<int64_t>(A.prefix.max_len) : 0);
   int W = 1, C = 1;
-  while (W < kMostWarps && base * W < 2 * slots && A.cache.max_len > W * kKv4Group) W *= 2;
-  while (C < 8 && W == kMostWarps && base * W * C * 2 <= slots && A.cache.max_len > 4 * C * W * kKv4Group) C *= 2;
+  while (W < kMostWarps && base * W < 2 * slots && reach > W * kKv4Group) W *= 2;
+  while (C < 8 && W == kMostWarps && base * W * C * 2 <= slots && reach > 4 * C * W * kKv4Group) C *= 2;
   if (grid * C > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(grid));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid * C));
@@ -592,22 +657,27 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
   cfg.numAttrs = kv4_attributes(C, attr);
-  IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_rows_kernel<D, T, kSplit, kTiles>, A, static_cast<int>(tiles)));
+  IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_rows_kernel<D, T, kSplit, kTiles, kShared>, A, static_cast<int>(tiles)));
   return IVB_OK;
 }
 
 // Rows of a tile by what a sequence can have: four as pairs of fp16 (for every type: no less exact, and as fast), then
 // eight; 16-bit queries with more in columns of their own.
+template <int D, typename T, bool kShared>
+int32_t launch_rows_of(const Kv4Attention& A, cudaStream_t stream) {
+  const bool one = A.starts == nullptr;
+  if (one && A.group <= 4) return launch_rows_attention<D, T, true, 1, kShared>(A, stream);
+  if constexpr (std::is_same<T, float>::value) {
+    return launch_rows_attention<D, T, true, 2, kShared>(A, stream);
+  } else {
+    if (one && A.group <= 8) return launch_rows_attention<D, T, false, 1, kShared>(A, stream);
+    return launch_rows_attention<D, T, false, 2, kShared>(A, stream);
+  }
+}
+
 template <int D, typename T>
 int32_t launch_dim(const Kv4Attention& A, cudaStream_t stream) {
-  const bool one = A.starts == nullptr;
-  if (one && A.group <= 4) return launch_rows_attention<D, T, true, 1>(A, stream);
-  if constexpr (std::is_same<T, float>::value) {
-    return launch_rows_attention<D, T, true, 2>(A, stream);
-  } else {
-    if (one && A.group <= 8) return launch_rows_attention<D, T, false, 1>(A, stream);
-    return launch_rows_attention<D, T, false, 2>(A, stream);
-  }
+  return A.prefix.data == nullptr ? launch_rows_of<D, T, false>(A, stream) : launch_rows_of<D, T, true>(A, stream);
 }
 
 template <typename T>
@@ -626,6 +696,15 @@ int few_items(const IvbKv4Cache& c, int group, const int32_t* starts, int rows) 
   const int few = tiles * c.kv_heads * 4 >= 148 ? kFewItems : kFewItemsSparse;
   // a lone sequence that can have more takes the prompts' kernel however many it has: one launch
   return starts == nullptr || items <= few ? 0x7fffffff : c.batch == 1 ? 0 : few;
+}
+
+// Whether few rows walk the beginning that they share each on their own, in one kernel, where that is less than a pass over it.
+#ifndef IVB_WALK
+#define IVB_WALK 300000
+#endif
+bool walks_prefix(const IvbKv4Cache& c, const IvbKv4Cache& prefix, int group, int rows) {
+  const int64_t tiles = std::max<int64_t>(std::min(rows, c.batch), static_cast<int64_t>(rows) * group / 8);
+  return tiles * c.kv_heads * prefix.max_len <= IVB_WALK;
 }
 
 // Bytes of the parts of a shared beginning: for each split, row and head its statistics and its values.
@@ -691,7 +770,7 @@ int32_t attention_call(const IvbKv4Cache* c, const IvbKv4Prefix* prefix, const v
     A.prefix = prefix->cache;
     A.prefix_lengths = prefix->lengths;
     A.prefix_groups = prefix->groups;
-    if (A.few != 0) {
+    if (A.few != 0 && !walks_prefix(*c, prefix->cache, A.group, rows)) {
       A.splits = kv4_prefix_splits(*c, prefix->cache, dtype, A.group, rows);
       if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < part_bytes(A.splits, rows, heads, c->head_dim))
         return fail(IVB_EINVAL, "ivb_kv4_attention_prefix: a workspace of %llu bytes at %p, not 16-byte aligned or too small",
@@ -704,7 +783,7 @@ int32_t attention_call(const IvbKv4Cache* c, const IvbKv4Prefix* prefix, const v
   if (A.beside_prompts)
     if (int32_t rc = launch_kv4_prompts(A, dtype, A.few, s)) return rc;
   if (A.few == 0) return IVB_OK;
-  if (prefix != nullptr) {
+  if (A.part_stats != nullptr) {
     if (int32_t rc = launch_kv4_prefix(A, dtype, A.few, s)) return rc;
     A.beside_prompts = true;  // beside the pass, and what that is beside
   }
@@ -729,7 +808,7 @@ uint64_t ivb_kv4_prefix_workspace_bytes(const IvbKv4Cache* c, const IvbKv4Prefix
                                         int32_t rows) {
   if (ivb::check_kv4(c, "ivb_kv4_prefix_workspace_bytes") || rows <= 0 || ivb::check_heads(c, heads, rows) || ivb::check_prefix(c, prefix)) return 0;
   const int group = heads / c->kv_heads;
-  if (ivb::few_items(*c, group, starts, rows) == 0) return 0;
+  if (ivb::few_items(*c, group, starts, rows) == 0 || ivb::walks_prefix(*c, prefix->cache, group, rows)) return 0;
   return ivb::part_bytes(ivb::kv4_prefix_splits(*c, prefix->cache, dtype, group, rows), rows, heads, c->head_dim);
 }
 

@@ -22,6 +22,7 @@
 namespace ivb {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMostSplits = 16;  // parts of a shared beginning
 constexpr unsigned long long kKv4WaitNs = 2000000000ull, kKv4ProbeNs = 1000000ull;
 
 struct Kv4Attention {
@@ -154,27 +155,56 @@ __device__ __forceinline__ int kv4_prefix(const Kv4Attention& A, int b, int& gro
   return static_cast<int>(max(static_cast<int64_t>(0), min(n, static_cast<int64_t>(A.prefix.max_len))));
 }
 
-// Joins the parts of row x head `item` to its own reference, sum and values, and divides by the sum; channel(j) is value j's.
-template <int D, int n, typename Channel>
-__device__ __forceinline__ void kv4_join_parts(const Kv4Attention& A, int64_t item, float ref, float sum, float (&v)[n], Channel channel) {
+// Joins the parts of row x head `item` to its own reference, sum and values, and divides by the sum. A whole warp: lane k has part
+// k's statistics, all lanes D / 32 neighbouring channels, and eight parts' values are on their way at a time.
+template <int D>
+__device__ __forceinline__ void kv4_join_parts(const Kv4Attention& A, int64_t item, float ref, float sum, float (&v)[D / 32]) {
+  constexpr int n = D / 32, kAt = 8;
+  static_assert(kMostSplits <= 32, "a lane for each part");
+  const int lane = threadIdx.x & 31;
   const int64_t step = static_cast<int64_t>(A.rows) * A.heads;
-  float top = sum == 0.0f ? -INFINITY : ref;  // zero: nothing was seen
-  for (int k = 0; k < A.splits; ++k) {
-    const float2 s = __ldcg(A.part_stats + k * step + item);
-    if (s.y != 0.0f) top = fmaxf(top, s.x);
-  }
-  const float own = sum == 0.0f ? 0.0f : ex2(ref - top);
-  float l = sum * own;
+  const float2 part = lane < A.splits ? __ldcg(A.part_stats + lane * step + item) : make_float2(0.0f, 0.0f);
+  float top = part.y == 0.0f ? -INFINITY : part.x;  // a sum of zero: nothing was seen
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+  if (sum != 0.0f) top = fmaxf(top, ref);
+  const float f = part.y == 0.0f ? 0.0f : ex2(part.x - top), own = sum == 0.0f ? 0.0f : ex2(ref - top);
+  float l = part.y == 0.0f ? 0.0f : part.y * f;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, d);
+  l = fmaf(sum, own, l);
 #pragma unroll
   for (int j = 0; j < n; ++j) v[j] = sum == 0.0f ? 0.0f : v[j] * own;
-  for (int k = 0; k < A.splits; ++k) {
-    const float2 s = __ldcg(A.part_stats + k * step + item);
-    if (s.y == 0.0f) continue;
-    const float f = ex2(s.x - top);
-    l = fmaf(s.y, f, l);
-    const float* from = A.part_values + (k * step + item) * D;
+  const float* const values = A.part_values + item * D + n * lane;
+  for (int k0 = 0; k0 < A.splits; k0 += kAt) {
+    float x[kAt][n], w[kAt];
 #pragma unroll
-    for (int j = 0; j < n; ++j) v[j] = fmaf(__ldcg(from + channel(j)), f, v[j]);
+    for (int k = 0; k < kAt; ++k) {
+      w[k] = __shfl_sync(0xFFFFFFFFu, f, k0 + k);
+      const float* const at = values + (k0 + k) * step * D;
+      if (w[k] != 0.0f) {  // zero: nothing seen, or nothing beside the others
+        if constexpr (n == 4) {
+          const float4 q = __ldcg(reinterpret_cast<const float4*>(at));
+          x[k][0] = q.x;
+          x[k][1] = q.y;
+          x[k][2] = q.z;
+          x[k][3] = q.w;
+        } else if constexpr (n == 2) {
+          const float2 q = __ldcg(reinterpret_cast<const float2*>(at));
+          x[k][0] = q.x;
+          x[k][1] = q.y;
+        } else {
+          x[k][0] = __ldcg(at);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < n; ++j) x[k][j] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAt; ++k)
+#pragma unroll
+      for (int j = 0; j < n; ++j) v[j] = fmaf(x[k][j], w[k], v[j]);
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll

@@ -36,8 +36,6 @@ constexpr int kRowsX = 128, kRowsCta = 256, kPos = 128;
 // 12 warps: three on each of the SM's four parts have 168 registers a thread, for the scores of four rows at a time
 constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 32 * kSoftmaxWarps, kProducerWarps = 3, kProducers = 32 * kProducerWarps;
 constexpr int kIssueWarp = kSoftmaxWarps + kProducerWarps, kPromptThreads = 32 * (kIssueWarp + 1);
-constexpr int kMostSplits = 16;
-constexpr int kTermSets = 3;  // terms(it + 2) are written when S(it) is done, so when nobody reads terms(it - 1) any more
 constexpr float kWeightUnit = 64.0f;  // weights are at most 2 * 64 * 2^8 in fp16
 constexpr float kRaise = 8.0f;
 // A tile's rows share the queries' power of two (no multiplication of the scores by a row's own) unless one's largest is so far below
@@ -47,8 +45,11 @@ constexpr float kEven = 0.000244140625f;
 // 1024 positions). fp32 outputs keep a second one, to which the threads add the first every so many tiles, rounding to nearest.
 constexpr int kFoldTiles = 2;
 
-template <int D, bool kSplit>
+template <int D, bool kSplit, bool kOfPass>
 struct PromptGeometry {
+  // terms(it + 2) are written when S(it) is done, so when nobody reads terms(it - 1) any more; in streams (below) when nobody
+  // reads terms(it - 2)
+  static constexpr int term_sets = kOfPass ? 4 : 3;
   static constexpr int parts = kSplit ? 2 : 1;
   static constexpr int stages = kSplit && D == 128 ? 1 : 2;  // of keys and of values
   static constexpr int q_bytes = kRowsX * D * 2;             // one part of one row tile
@@ -56,7 +57,7 @@ struct PromptGeometry {
   static constexpr int term_bytes = kPos * 24;
   static constexpr int q_at = 0, k_at = (kSplit && D == 128 ? 1 : 2) * parts * q_bytes, v_at = k_at + stages * kv_bytes, terms_at = v_at + stages * kv_bytes;
   // over half of an SM's at least: of two clusters sharing two SMs each could hold the tensor memory that the other waits for
-  static constexpr int used = terms_at + kTermSets * term_bytes, smem = used < 118 * 1024 ? 118 * 1024 : used;
+  static constexpr int used = terms_at + term_sets * term_bytes, smem = used < 118 * 1024 ? 118 * 1024 : used;
   // row tiles of a CTA: at fp32 and D = 128 tensor memory holds the accumulators of one
   static constexpr int row_tiles = kSplit && D == 128 ? 1 : 2, rows = row_tiles * kRowsX;
   // tensor memory columns: S_X, then P_X in its place (of every 64 columns 32 hi, 32 lo), O_X, and O_X's sums (fp32)
@@ -109,7 +110,7 @@ __device__ __forceinline__ void values_of_chunk(uint4 w, float (&v)[16 / sizeof(
 }
 
 struct PromptBarriers {
-  unsigned long long k_full[2], k_free[2], v_full[2], v_free[2], terms_full[kTermSets], s_full[2][2], p_full[2][2], p_free[2][2], drain;
+  unsigned long long k_full[2], k_free[2], v_full[2], v_free[2], terms_full[4], s_full[2][2], p_full[2][2], p_free[2][2], drain;
 };
 
 // What a lane of a producer warp holds of the keys or values of one tile of 16 positions (D = 32: values in lanes 0..15), dealt
@@ -192,31 +193,34 @@ __device__ __forceinline__ void store_codes_of_values(const RawChunks<D>& raw, i
   }
 }
 
-// kPass: the pass over the prefix for the rows of sequences with no more than `few` items. Its "sequences" are the groups, its
-// items all rows of a group's sequences, each with a position of its own; the tiles are dealt out to A.splits CTAs a row tile.
-template <int D, typename T, bool kPass>
+// kPlain: sequences that hold all of their positions. kBehind: behind a beginning that they share. kPass: the pass over the beginnings
+// for the rows of sequences with no more than `few` items; its "sequences" are the groups, its items all rows of a group's sequences,
+// each with a position of its own, and the tiles are dealt out to A.splits CTAs a row tile. (One kernel for the first two, told
+// apart as it runs, took 240 us where 230 are kept for a chunk of 2048 rows under a window.)
+enum PromptMode { kPlain, kBehind, kPass };
+
+template <int D, typename T, PromptMode kMode>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attention A, int few) {
   constexpr bool kSplit = std::is_same<T, float>::value;
-  using G = PromptGeometry<D, kSplit>;
+  using G = PromptGeometry<D, kSplit, kMode == kPass>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ PromptBarriers bar;
   __shared__ unsigned tmem_base;
   __shared__ float largest[kSoftmaxWarps], smallest[kSoftmaxWarps], sums[kRowsCta], row_units[kRowsCta], refs_of[kRowsCta], totals[kRowsCta], offsets[kRowsCta];
   __shared__ int nearest[kSoftmaxWarps];
-  __shared__ int which[5];  // sequence, tile of its rows; whether a wait ran out; group of the prefix, its length
+  __shared__ int which[8];  // sequence, tile of its rows; whether a wait ran out; group of the prefix, its length, its parts, which of them, head
   const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
-  if (kPass && A.beside_prompts) __threadfence();
+  if (kMode == kPass && A.beside_prompts) __threadfence();
   else pdl_wait();
   // which rows: the call's tiles of 256 items in the order of the sequences, the last ones (the longest rows) first
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = kPass ? A.splits : static_cast<int>(cluster.num_blocks());
-  const int rank = kPass ? static_cast<int>(blockIdx.x) % C : static_cast<int>(cluster.block_rank());
-  const int sequences = kPass ? A.prefix.batch : A.cache.batch;
+  int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int sequences = kMode == kPass ? A.prefix.batch : A.cache.batch;
   // the rows of sequence, or group, b
   auto rows_of = [&](int b, int& from) {
     int b0 = b, b1 = b + 1;
-    if (kPass) {
+    if (kMode == kPass) {
       b0 = A.prefix_groups == nullptr ? 0 : max(0, A.prefix_groups[b]);
       b1 = A.prefix_groups == nullptr ? A.cache.batch : min(A.cache.batch, A.prefix_groups[b + 1]);
       if (b1 <= b0) b0 = b1 = 0;
@@ -225,17 +229,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     return max(0, (A.starts == nullptr ? b1 : min(A.rows, A.starts[b1])) - from);
   };
   const int unit = static_cast<int>(blockIdx.x) / C, units = static_cast<int>(gridDim.x) / C;
-  const int kvh = unit % A.cache.kv_heads, order = units / A.cache.kv_heads - 1 - unit / A.cache.kv_heads;
+  int kvh = unit % A.cache.kv_heads;
+  const int order = kMode == kPass ? static_cast<int>(blockIdx.x) : units / A.cache.kv_heads - 1 - unit / A.cache.kv_heads;
   if (warp == 0) {
+    // the tiles of 128 positions and of rows of group g
+    auto length_of = [&](int g) { return static_cast<int>(max(static_cast<int64_t>(0), min(A.prefix_lengths[g], static_cast<int64_t>(A.prefix.max_len)))); };
+    auto tiles_of = [&](int g) { return (length_of(g) + kPos - 1) / kPos; };
+    auto row_tiles_of = [&](int b) {
+      int from;
+      const int items = rows_of(b, from) * A.group;
+      return items > (kMode == kPass ? 0 : few) ? (items + G::rows - 1) / G::rows : 0;
+    };
+    // A pass deals its CTAs out by the work: each row tile and head of a group gets so many parts that all of them fill the SMs once.
+    unsigned long long work = 0;
+    if constexpr (kMode == kPass) {
+      for (int b = lane; b < sequences; b += 32) work += static_cast<unsigned long long>(row_tiles_of(b)) * tiles_of(b);
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) work += __shfl_xor_sync(0xFFFFFFFFu, work, d);
+      work = max(1ull, work * A.cache.kv_heads);
+    }
+    auto parts_of = [&](int b) {
+      const int n = tiles_of(b);
+      return n == 0 ? 0 : static_cast<int>(max(1ull, min(static_cast<unsigned long long>(A.splits), 148ull * n / work)));
+    };
     int seen = 0, found = -1, tile = 0;
     for (int b0 = 0; b0 < sequences && found < 0; b0 += 32) {
       const int b = b0 + lane;
       int n = 0;
-      if (b < sequences) {
-        int from;
-        const int items = rows_of(b, from) * A.group;
-        n = items > (kPass ? 0 : few) ? (items + G::rows - 1) / G::rows : 0;
-      }
+      if (b < sequences) n = kMode == kPass ? row_tiles_of(b) * A.cache.kv_heads * parts_of(b) : row_tiles_of(b);
       int upto = n;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -251,12 +272,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       seen += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
     int group = found, length = 0;
-    if (found >= 0) {
-      if (kPass) length = static_cast<int>(max(static_cast<int64_t>(0), min(A.prefix_lengths[found], static_cast<int64_t>(A.prefix.max_len))));
-      else length = kv4_prefix(A, found, group);
+    if (kMode == kBehind && found >= 0) length = kv4_prefix(A, found, group);
+    if (kMode == kPass && found >= 0) {
+      length = length_of(found);
+      const int each = row_tiles_of(found) * A.cache.kv_heads;
+      if (lane == 0) {
+        which[5] = parts_of(found);
+        which[6] = tile / each;
+        which[7] = tile % each % A.cache.kv_heads;
+      }
+      tile = tile % each / A.cache.kv_heads;
     }
     if (lane == 0) {
-      which[0] = kPass && length == 0 ? -1 : found;
+      which[0] = found;
       which[1] = tile;
       which[2] = 0;
       which[3] = group;
@@ -278,7 +306,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       }
     }
 #pragma unroll
-    for (int i = 0; i < kTermSets; ++i) mbar_init(&bar.terms_full[i], kProducers);
+    for (int i = 0; i < G::term_sets; ++i) mbar_init(&bar.terms_full[i], kProducers);
     mbar_init(&bar.drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -286,11 +314,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   const int b = which[0];
   // a pass does not end before the prompts' grid that it runs beside, whichever way its first CTA takes
   auto end = [&] {
-    if (kPass && A.beside_prompts && blockIdx.x == 0) pdl_wait();
+    if (kMode == kPass && A.beside_prompts && blockIdx.x == 0) pdl_wait();
   };
   if (b < 0) {
     end();
     return;
+  }
+  if (kMode == kPass) {
+    C = which[5];
+    rank = which[6];
+    kvh = which[7];
+    if (rank == 0) {  // parts that the group does not have: nothing was seen
+      int row0;
+      const int items = rows_of(b, row0) * A.group, i = which[1] * G::rows + tid;
+      if (tid < G::rows && i < items)
+        for (int k = C; k < A.splits; ++k) {
+          const int t = i / A.group;
+          A.part_stats[(static_cast<int64_t>(k) * A.rows + row0 + t) * A.heads + kvh * A.group + i - t * A.group] = make_float2(-INFINITY, 0.0f);
+        }
+    }
   }
   if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)), "r"(G::columns));
@@ -300,20 +342,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   int row0;
   const int count = rows_of(b, row0);
   // rows of the sequence that the call does not have
-  const int64_t before = A.starts == nullptr || kPass ? 0 : static_cast<int64_t>(row0) - A.starts[b];
+  const int64_t before = A.starts == nullptr || kMode == kPass ? 0 : static_cast<int64_t>(row0) - A.starts[b];
   const int i0 = which[1] * G::rows, live = min(G::rows, count * A.group - i0), row_tiles = live > kRowsX ? 2 : 1;
-  const int shared_length = which[4];  // positions of the prefix, which come before the sequence's own
+  // With up to 128 rows a pass runs two streams: the tiles of positions in turn are row tile 0's and 1's, which hold the same rows and
+  // are joined at the end, so that one's softmax runs while the other waits for the tensor cores, and both have four warps.
+  const bool streams = kMode == kPass && G::row_tiles == 2 && row_tiles == 1;
+  // Few rows stand 8 or 16 to a warp (the 8 or 16 lower ones of its 32 lanes of tensor memory), so that all warps share the softmax.
+  const int spread = !streams || live > 64 ? 32 : live > 32 ? 16 : 8;
+  auto item_at = [&](int r) {  // of the row tiles' lane r; -1: none
+    if (kMode != kPass || !streams) return r < live ? r : -1;
+    const int i = (r >> 5) * spread + (r & 31);
+    return (r & 31) < spread && r < kRowsX && i < live ? i : -1;
+  };
+  const int shared_length = kMode == kPlain ? 0 : which[4];  // positions of the prefix, which come before the sequence's own
   const int max_len = A.cache.max_len;
   const unsigned group_size = static_cast<unsigned>(A.group);
   auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };
   auto clamp_position = [&](int64_t p) { return static_cast<int>(max(static_cast<int64_t>(-1), min(p, static_cast<int64_t>(max_len)))); };
-  const int64_t base = kPass ? 0 : kv4_position(A.positions, b) + before;
+  const int64_t base = kMode == kPass ? 0 : kv4_position(A.positions, b) + before;
   // position of row r of the tile in its sequence's own cache, -1 where it sees nothing
   auto own_position = [&](int r) {
-    if (r >= live) return -1;
+    const int item = item_at(r);
+    if (item < 0) return -1;
     int64_t p;
-    if constexpr (kPass) {
-      const int row = row0 + token_of(i0 + r);
+    if constexpr (kMode == kPass) {
+      const int row = row0 + token_of(i0 + item);
       int of = row;
       if (A.starts != nullptr) {  // the last sequence of the group that starts at or before the row
         int low = A.prefix_groups == nullptr ? 0 : max(0, A.prefix_groups[b]);
@@ -332,7 +385,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     }
     return p < 0 || p >= max_len ? -1 : static_cast<int>(p);
   };
-  if (!kPass && tid == 0 && rank == 0 && A.error != nullptr && clamp_position(base + token_of(i0 + live - 1)) >= max_len)
+  if (kMode != kPass && tid == 0 && rank == 0 && A.error != nullptr && clamp_position(base + token_of(i0 + live - 1)) >= max_len)
     atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
 
   // queries: a warp takes 32 rows in 16-byte chunks, 8 rows and 4 chunks at a time (64 contiguous bytes of a row, and no bank
@@ -346,10 +399,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     return static_cast<const T*>(array) + (row0 + t) * row_stride + h * head_stride;
   };
   uint4 raw[4][kQuads];
-  int own_at = -1;  // of row 32 warp + lane
+  int own_at = -1;  // of row 32 warp + lane, where it takes a search
+  auto position_of = [&](int of_warp) { return kMode == kPass ? __shfl_sync(0xFFFFFFFFu, own_at, of_warp) : own_position(32 * warp + of_warp); };
   if (tid < kSoftmaxThreads) {
-    own_at = own_position(tid);
-    if constexpr (kPass) {
+    if constexpr (kMode == kPass) {
+      own_at = own_position(tid);
       const unsigned to_end = __reduce_min_sync(0xFFFFFFFFu, static_cast<unsigned>(own_at));  // -1 is the largest
       if (lane == 0) nearest[warp] = static_cast<int>(to_end);
     }
@@ -357,7 +411,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int r = 32 * warp + 8 * g + row8;
-      q[g] = __shfl_sync(0xFFFFFFFFu, own_at, 8 * g + row8) >= 0 ? item_row(A.q, i0 + r, A.q_row, A.q_head) + chunk4 * kPer : nullptr;
+      q[g] = position_of(8 * g + row8) >= 0 ? item_row(A.q, i0 + item_at(r), A.q_row, A.q_head) + chunk4 * kPer : nullptr;
     }
     if (A.q_vec) {
 #pragma unroll
@@ -418,30 +472,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   const bool even = least >= most * kEven;
   // The tiles of 128 positions that some row sees, of the prefix and then of the sequence's own: in each the sinks' below the window,
   // then the window's. Positions count from the beginning, where the own ones' tiles stand at shared_length + 128 t.
-  int first, high;  // own positions: the rows' first, and the last that there is
-  if constexpr (kPass) {
-    unsigned low_at = 0xffffffffu;
+  int shared_sinks, shared_window, shared_tiles, sink_tiles, window_tile, tiles;
+  auto plan = [&](int first, int high) {  // own positions: the rows' first, and the last that there is
+    const int low = A.window > 0 ? max(0, max(first, 0) + shared_length - A.window + 1) : 0;
+    const int own_low = max(0, low - shared_length), own_sinks = max(0, A.sinks - shared_length);
+    window_tile = own_low / kPos;
+    sink_tiles = A.window > 0 ? min((min(own_sinks, own_low) + kPos - 1) / kPos, window_tile) : 0;
+    const int own_tiles = kMode == kPass || high < 0 ? 0 : sink_tiles + high / kPos - window_tile + 1;
+    const int shared_all = kMode != kPlain && (kMode == kPass ? first : high) >= 0 ? (shared_length + kPos - 1) / kPos : 0;
+    shared_window = min(low / kPos, shared_all);
+    shared_sinks = A.window > 0 ? min((min(A.sinks, low) + kPos - 1) / kPos, shared_window) : 0;
+    shared_tiles = kMode == kPlain ? 0 : shared_sinks + shared_all - shared_window;
+    const int all_tiles = shared_tiles + own_tiles;
+    tiles = all_tiles > rank ? (all_tiles - rank + C - 1) / C : 0;  // this CTA's
+  };
+  if constexpr (kMode == kPass) {
+    unsigned first = 0xffffffffu;
 #pragma unroll
-    for (int w = 0; w < kSoftmaxWarps; ++w) low_at = min(low_at, static_cast<unsigned>(nearest[w]));
-    first = static_cast<int>(low_at);
-    high = -1;
+    for (int w = 0; w < kSoftmaxWarps; ++w) first = min(first, static_cast<unsigned>(nearest[w]));
+    plan(static_cast<int>(first), -1);
   } else {
-    first = clamp_position(base + token_of(i0));
-    high = min(clamp_position(base + token_of(i0 + live - 1)), max_len - 1);
+    plan(clamp_position(base + token_of(i0)), min(clamp_position(base + token_of(i0 + live - 1)), max_len - 1));
   }
-  const int low = A.window > 0 ? max(0, max(first, 0) + shared_length - A.window + 1) : 0;
-  const int own_low = max(0, low - shared_length), own_sinks = max(0, A.sinks - shared_length);
-  const int window_tile = own_low / kPos;
-  const int sink_tiles = A.window > 0 ? min((min(own_sinks, own_low) + kPos - 1) / kPos, window_tile) : 0;
-  const int own_tiles = high < 0 ? 0 : sink_tiles + high / kPos - window_tile + 1;
-  const bool any_row = kPass ? first >= 0 : high >= 0;
-  const int shared_all = any_row ? (shared_length + kPos - 1) / kPos : 0;
-  const int shared_window = min(low / kPos, shared_all);
-  const int shared_sinks = A.window > 0 ? min((min(A.sinks, low) + kPos - 1) / kPos, shared_window) : 0;
-  const int shared_tiles = shared_sinks + shared_all - shared_window;
-  const int all_tiles = shared_tiles + own_tiles;
-  const int tiles = all_tiles > rank ? (all_tiles - rank + C - 1) / C : 0;  // this CTA's
-  auto of_prefix = [&](int it) { return kPass || rank + it * C < shared_tiles; };
+  auto of_prefix = [&](int it) { return kMode == kPass || (kMode == kBehind && rank + it * C < shared_tiles); };
   auto tile_of = [&](int it) {  // in its cache
     int i = rank + it * C;
     if (of_prefix(it)) return i < shared_sinks ? i : shared_window + i - shared_sinks;
@@ -495,8 +548,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   const unsigned tmem = __shfl_sync(0xFFFFFFFFu, tmem_base, 0);
   auto keys_of = [&](int it) { return smem + G::k_at + it % G::stages * G::kv_bytes; };
   auto values_of = [&](int it) { return smem + G::v_at + it % G::stages * G::kv_bytes; };
-  auto terms_of = [&](int it) { return reinterpret_cast<float*>(smem + G::terms_at + it % kTermSets * G::term_bytes); };
+  auto terms_of = [&](int it) { return reinterpret_cast<float*>(smem + G::terms_at + it % G::term_sets * G::term_bytes); };
   auto turn_of = [&](int it) { return static_cast<unsigned>(it / G::stages) & 1u; };  // parity of a stage's use
+  const int my_tiles = streams ? (tiles + 1 - x) >> 1 : tiles;  // of a softmax warp's row tile
   bool ok = true;
   auto wait_for = [&](unsigned long long* at, unsigned turn) { return mbar_wait_bounded(at, turn, A.wait_ns); };
 
@@ -550,7 +604,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           }
         }
       }
-      mbar_arrive(&bar.terms_full[it % kTermSets]);
+      mbar_arrive(&bar.terms_full[it % G::term_sets]);
 #pragma unroll
       for (int k = 0; k < kMine; ++k) {
         const int u = unit0 + k * kProducerWarps;
@@ -580,13 +634,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     // in 16 bytes.
     auto issue_s = [&](int it, int h) {
       const uint64_t k = k0 + (it % G::stages * G::kv_bytes + h * (G::kv_bytes / 2)) / 16;
-      for (int xx = 0; xx < row_tiles; ++xx) {
-        if (it > 0) {  // S takes the place of P
-          ok = ok && wait(&bar.p_free[xx][h], (it - 1) & 1);
+      const int turn = streams ? it >> 1 : it;
+      for (int xx = streams ? it & 1 : 0; xx < (streams ? (it & 1) + 1 : row_tiles); ++xx) {
+        if (turn > 0) {  // S takes the place of P
+          ok = ok && wait(&bar.p_free[xx][h], (turn - 1) & 1);
           if (!ok) return;
         }
         tc_fence_after();
-        const uint64_t q = q0 + xx * (G::parts * G::q_bytes / 16);
+        const uint64_t q = q0 + (streams ? 0 : xx) * (G::parts * G::q_bytes / 16);
         const unsigned t_s = tmem + G::s_at + xx * kPos + h * (kPos / 2);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
@@ -599,8 +654,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     };
     auto issue_o = [&](int it, int h) {
       const uint64_t v = v0 + (it % G::stages * G::kv_bytes + h * (G::kv_bytes / 2)) / 16;
-      for (int xx = 0; xx < row_tiles; ++xx) {
-        ok = ok && wait(&bar.p_full[xx][h], it & 1);
+      const int turn = streams ? it >> 1 : it;
+      for (int xx = streams ? it & 1 : 0; xx < (streams ? (it & 1) + 1 : row_tiles); ++xx) {
+        ok = ok && wait(&bar.p_full[xx][h], turn & 1);
         if (!ok) return;
         tc_fence_after();
         const unsigned t_p = tmem + G::s_at + xx * kPos + h * (kPos / 2), t_o = tmem + G::o_at + xx * D;
@@ -608,7 +664,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         for (int kk = 0; kk < kPos / 32; ++kk)
 #pragma unroll
           for (int part = 0; part < G::parts; ++part)
-            umma_f16_ts_warp(t_o, t_p + part * (kPos / 4) + kk * 8, v + kk * 2 * (D / 8) * 8, idesc_f16_bt(kRowsX, D), kk + part > 0 || h > 0 || (kSplit ? it % kFoldTiles != 0 : it > 0));
+            umma_f16_ts_warp(t_o, t_p + part * (kPos / 4) + kk * 8, v + kk * 2 * (D / 8) * 8, idesc_f16_bt(kRowsX, D), kk + part > 0 || h > 0 || (kSplit ? turn % kFoldTiles != 0 : turn > 0));
         umma_commit_warp(&bar.p_free[xx][h]);
       }
       if (h == 1) umma_commit_warp(&bar.v_free[it % G::stages]);
@@ -620,27 +676,37 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         issue_s(0, 1);
       }
     }
+    const int ahead = streams ? 2 : 1;
+    if (streams && tiles > 1 && ok) {
+      ok = wait(&bar.k_full[1], 0);
+      if (ok) {
+        issue_s(1, 0);
+        issue_s(1, 1);
+      }
+    }
     // both row tiles' weights of a half, then, while they are used up, their next scores in that half's place
     for (int it = 0; it < tiles && ok; ++it) {
       ok = wait(&bar.v_full[it % G::stages], turn_of(it));
       if (ok) issue_o(it, 0);
-      if (it + 1 < tiles) {
-        ok = ok && wait(&bar.k_full[(it + 1) % G::stages], turn_of(it + 1));
-        if (ok) issue_s(it + 1, 0);
+      if (it + ahead < tiles) {
+        ok = ok && wait(&bar.k_full[(it + ahead) % G::stages], turn_of(it + ahead));
+        if (ok) issue_s(it + ahead, 0);
       }
       if (ok) issue_o(it, 1);
-      if (ok && it + 1 < tiles) issue_s(it + 1, 1);
+      if (ok && it + ahead < tiles) issue_s(it + ahead, 1);
     }
     // what was issued ends before shared and tensor memory go, also where another warp's wait ran out
     umma_commit_warp(&bar.drain);
     ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&bar.drain, 0, kKv4WaitNs)) != 0 && ok;
-  } else if (x < row_tiles) {
+  } else if (streams || x < row_tiles) {
     // ---- softmax: a warp has 32 rows, a thread in each 8-row set the row r and every fourth pair of positions, so that a
     // position's terms are loaded once for four rows (loaded for each row they bound the kernel: 12 cycles of the SM's
     // shared memory pipe for 64 scores)
     const int r = lane >> 2, c = lane & 3, row0x = 32 * (warp & 3);
     const unsigned lanes = static_cast<unsigned>(row0x) << 16;
     const unsigned ts = tmem + lanes + G::s_at + x * kPos, to = tmem + lanes + G::o_at + x * D, tf = tmem + lanes + G::fold_at + x * D;
+    const int rows_at = streams ? 0 : kRowsX * x;  // of the tile's first row
+    if (streams && x > 0) own_at = own_position(row0x + lane);
     float sum_q[4], refs[4];
     int at[4];
     f32x2 sum2[4], off2[4];
@@ -648,11 +714,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     int first_at = 0x7fffffff, last_at = -1;  // of the warp's rows
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int n = kRowsX * x + row0x + 8 * i + r;
+      const int n = rows_at + row0x + 8 * i + r;
       sum_q[i] = sums[n];
       at[i] = -1;
-      const int p = __shfl_sync(0xFFFFFFFFu, own_at, 8 * i + r);
-      if (n < live) {
+      const int p = position_of(8 * i + r);
+      if (item_at(n) >= 0) {
         at[i] = p < 0 ? -1 : shared_length + p;
         live_rows = true;
         first_at = min(first_at, at[i]);
@@ -668,13 +734,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     }
     live_rows = __any_sync(0xFFFFFFFFu, live_rows);
     // a copy for each kind of rows: the test within costs a chunk 235 us in place of 230
-    auto walk = [&](auto evenly) {
+    auto walk = [&](auto evenly, auto sets) {
+      constexpr int kSets = decltype(sets)::value, kHalves = kSets == 4 ? 2 : 1;  // of 8 rows, and of 16
       bool stop = false;  // the same in all lanes, where `ok` is each lane's own between two votes
-      for (int it = 0; it < tiles && !stop; ++it) {
-        const bool shared = of_prefix(it);
-        const int p0 = tile_of(it) * kPos + (shared ? 0 : shared_length), end = shared ? shared_length - 1 : 0x7fffffff;
-        const float* terms = terms_of(it);
-        ok = ok && wait_for(&bar.terms_full[it % kTermSets], static_cast<unsigned>(it / kTermSets) & 1u);
+      for (int it = 0; it < my_tiles && !stop; ++it) {  // the row tile's own count
+        const int tile = streams ? 2 * it + x : it;
+        const bool shared = of_prefix(tile);
+        const int p0 = tile_of(tile) * kPos + (shared ? 0 : shared_length), end = shared ? shared_length - 1 : 0x7fffffff;
+        const float* terms = terms_of(tile);
+        ok = ok && wait_for(&bar.terms_full[tile % G::term_sets], static_cast<unsigned>(tile / G::term_sets) & 1u);
         // what the warp's rows see of the tile: all of it, or nothing (first_at, last_at: the lowest and highest, -1 among them)
         const bool whole = live_rows && min(first_at, end) >= p0 + kPos - 1 && (A.window <= 0 || p0 > last_at - A.window || p0 <= A.sinks - kPos);
         const bool none = last_at < p0 || (A.window > 0 && p0 + kPos - 1 <= first_at - A.window && p0 >= A.sinks);
@@ -711,7 +779,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll
             for (int i = 0; i < 16; ++i) zero[i] = 0u;
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
+            for (int g = 0; g < kHalves; ++g) {
               tmem_st_16x128b_x8(th + (static_cast<unsigned>(16 * g) << 16), zero);
               if constexpr (kSplit) tmem_st_16x128b_x8(th + kPos / 4 + (static_cast<unsigned>(16 * g) << 16), zero);
             }
@@ -722,12 +790,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           }
           uint32_t s[2][32];  // [16 rows][4 pair + 2 (8 rows) + position], scores in place
 #pragma unroll
-          for (int g = 0; g < 2; ++g) tmem_ld_16x256b_x8_begin(th + (static_cast<unsigned>(16 * g) << 16), s[g]);
-          tmem_ld_end(s[0], s[1]);
+          for (int g = 0; g < kHalves; ++g) tmem_ld_16x256b_x8_begin(th + (static_cast<unsigned>(16 * g) << 16), s[g]);
+          if constexpr (kHalves == 2) tmem_ld_end(s[0], s[1]);
+          else tmem_ld_end(s[0], s[0]);
           if constexpr (!decltype(evenly)::value) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              const float unit = row_units[kRowsX * x + row0x + 8 * n + r];
+            for (int n = 0; n < kSets; ++n) {
+              const float unit = row_units[rows_at + row0x + 8 * n + r];
 #pragma unroll
               for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -743,7 +812,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
             const float4 k = t4[12 * i];
             const float2 e = *reinterpret_cast<const float2*>(&t4[12 * i + 1]);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
+            for (int n = 0; n < kSets; ++n) {
               const int j = 4 * i + 2 * (n & 1);
               const float2 y = unpair(fma2(pair(__uint_as_float(s[n >> 1][j]), __uint_as_float(s[n >> 1][j + 1])), pair(k.x, k.y),
                                            fma2(pair(sum_q[n], sum_q[n]), pair(k.z, k.w), pair(e.x, e.y))));
@@ -753,7 +822,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           }
           if (!whole) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
+            for (int n = 0; n < kSets; ++n) {
               const int from = A.window > 0 ? at[n] - A.window : -1;
 #pragma unroll
               for (int i = 0; i < 8; ++i)
@@ -765,17 +834,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
             }
           }
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
+          for (int n = 0; n < kSets; ++n)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               top[n] = max3(top[n], __uint_as_float(s[n >> 1][4 * i + 2 * (n & 1)]), __uint_as_float(s[n >> 1][4 * i + 2 * (n & 1) + 1]));
           bool raise = false;
 #pragma unroll
-          for (int n = 0; n < 4; ++n) raise |= top[n] > refs[n] + kRaise;  // the first seen position too: the reference is -inf
+          for (int n = 0; n < kSets; ++n) raise |= top[n] > refs[n] + kRaise;  // the first seen position too: the reference is -inf
           if (__any_sync(0xFFFFFFFFu, raise)) {
-            float corr[4];
+            float corr[kSets];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
+            for (int n = 0; n < kSets; ++n) {
               top[n] = fmaxf(top[n], __shfl_xor_sync(0xFFFFFFFFu, top[n], 1));
               top[n] = fmaxf(top[n], __shfl_xor_sync(0xFFFFFFFFu, top[n], 2));
               const float next = fmaxf(refs[n], top[n]);
@@ -792,12 +861,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll 1
               for (int c0 = 0; c0 < D; c0 += 32)
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
+                for (int g = 0; g < kHalves; ++g) {
                   uint32_t o[16];
                   const unsigned at_o = from + c0 + (static_cast<unsigned>(16 * g) << 16);
                   tmem_ld_16x256b_x4(at_o, o);
 #pragma unroll
-                  for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr[2 * g + ((j >> 1) & 1)]);
+                  for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr[kSets == 1 ? 0 : 2 * g + ((j >> 1) & 1)]);
                   tmem_st_16x256b_x4(at_o, o);
                 }
             };
@@ -809,14 +878,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
           }
           f32x2 minus[4];  // a row that has seen nothing yet: its weights are 2^-inf
 #pragma unroll
-          for (int n = 0; n < 4; ++n) minus[n] = refs[n] == -INFINITY ? pair(0.0f, 0.0f) : pair(-refs[n], -refs[n]);
+          for (int n = 0; n < kSets; ++n) minus[n] = refs[n] == -INFINITY ? pair(0.0f, 0.0f) : pair(-refs[n], -refs[n]);
           uint32_t hi[2][16], lo[2][16];
+          if constexpr (kSets == 1) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) hi[0][i] = lo[0][i] = 0u;
+          }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float2 mu = reinterpret_cast<const float2*>(t4)[24 * i + 3];
             const float4 uo = t4[12 * i + 2];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
+            for (int n = 0; n < kSets; ++n) {
               const int j = 4 * i + 2 * (n & 1);
               const float2 d = unpair(add2(pair(__uint_as_float(s[n >> 1][j]), __uint_as_float(s[n >> 1][j + 1])), minus[n]));
               const f32x2 pw = pair(ex2(d.x), ex2(d.y));
@@ -831,7 +904,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
             }
           }
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
+          for (int g = 0; g < kHalves; ++g) {
             tmem_st_16x128b_x8(th + (static_cast<unsigned>(16 * g) << 16), hi[g]);
             if constexpr (kSplit) tmem_st_16x128b_x8(th + kPos / 4 + (static_cast<unsigned>(16 * g) << 16), lo[g]);
           }
@@ -841,9 +914,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         }
       }
     };
-    if (even) walk(std::true_type{});
-    else walk(std::false_type{});
-    if (tiles > 0) ok = __all_sync(0xFFFFFFFFu, ok && wait_for(&bar.p_free[x][1], (tiles - 1) & 1)) != 0;
+    auto walk_sets = [&](auto sets) {
+      if (even) walk(std::true_type{}, sets);
+      else walk(std::false_type{}, sets);
+    };
+    if (kMode == kPass && G::row_tiles == 2 && spread == 8) walk_sets(std::integral_constant<int, kMode == kPass ? 1 : 4>{});
+    else if (kMode == kPass && G::row_tiles == 2 && spread == 16) walk_sets(std::integral_constant<int, kMode == kPass ? 2 : 4>{});
+    else walk_sets(std::integral_constant<int, 4>{});
+    if (my_tiles > 0) ok = __all_sync(0xFFFFFFFFu, ok && wait_for(&bar.p_free[x][1], (my_tiles - 1) & 1)) != 0;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const float2 s = unpair(sum2[n]), f = unpair(off2[n]);
@@ -866,36 +944,66 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   // now a thread has a row of its own: tensor-memory lane tid % 128 of row tile x
   const int row = tid & (kRowsCta - 1);
   const unsigned to = tmem + (static_cast<unsigned>(32 * (warp & 3)) << 16) + G::o_at + x * D;
-  const bool mine = tid < kSoftmaxThreads && x < row_tiles;
+  const bool mine = tid < kSoftmaxThreads && (streams || x < row_tiles);
   auto load_o = [&](int c0, uint32_t (&o)[16]) {  // 16 channels of the row
     tmem_ld16(to + c0, o);
-    if (kSplit && tiles > kFoldTiles) {
+    if (kSplit && my_tiles > kFoldTiles) {
       uint32_t f[16];
       tmem_ld16(to + (G::fold_at - G::o_at) + c0, f);
 #pragma unroll
       for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float(f[j]));
     }
   };
-  if constexpr (kPass) {
-    if (mine) {  // whole warps: they load from tensor memory together, also for rows that there are not
-      const bool there = row < live;
-      const int t = token_of(i0 + row), h = kvh * A.group + i0 + row - t * A.group;
+  if constexpr (kMode == kPass) {
+    float* const other = reinterpret_cast<float*>(smem);  // the second stream's O [channel][row]
+    auto load_mine = [&](int c0, uint32_t (&o)[16]) {  // whole warps: they load from tensor memory together, also for rows that there are not
+      if (my_tiles > 0 && ok) load_o(c0, o);
+      else
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] = 0u;
+    };
+    if (streams) {
+      if (mine && x > 0) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 16) {
+          uint32_t o[16];
+          load_mine(c0, o);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) other[(c0 + j) * kRowsX + row - kRowsX] = __uint_as_float(o[j]);
+        }
+      }
+      __syncthreads();
+    }
+    if (mine && !(streams && x > 0)) {
+      const int found = item_at(row);
+      const bool there = found >= 0;
+      const int i = i0 + max(found, 0), t = token_of(i), h = kvh * A.group + i - t * A.group;
       const int64_t item = (static_cast<int64_t>(rank) * A.rows + row0 + t) * A.heads + h;
-      const float total = totals[row], offset = offsets[row];
-      if (there) A.part_stats[item] = make_float2(refs_of[row], total);
+      float total = totals[row], offset = offsets[row], ref = refs_of[row], f0 = 1.0f, f1 = 0.0f;
+      if (streams && totals[kRowsX + row] != 0.0f) {  // zero: the stream saw nothing for this row
+        const float theirs = refs_of[kRowsX + row], top = total == 0.0f ? theirs : fmaxf(ref, theirs);
+        f0 = total == 0.0f ? 0.0f : ex2(ref - top);
+        f1 = ex2(theirs - top);
+        total = fmaf(totals[kRowsX + row], f1, total * f0);
+        offset = fmaf(offsets[kRowsX + row], f1, offset * f0);
+        ref = top;
+      }
+      if (there) A.part_stats[item] = make_float2(ref, total);
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 16) {
         uint32_t o[16];
-        if (tiles > 0 && ok) load_o(c0, o);
-        else
+        load_mine(c0, o);
+        float y[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) o[j] = 0u;
+        for (int j = 0; j < 16; ++j) {
+          y[j] = f0 == 0.0f ? 0.0f : __uint_as_float(o[j]) * f0;
+          if (f1 != 0.0f) y[j] = fmaf(other[(c0 + j) * kRowsX + row], f1, y[j]);
+          y[j] = fmaf(y[j], 1.0f / kWeightUnit, offset);
+        }
         if (there && total != 0.0f) {
           float4* const to = reinterpret_cast<float4*>(A.part_values + item * D + c0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            to[j] = make_float4(fmaf(__uint_as_float(o[4 * j]), 1.0f / kWeightUnit, offset), fmaf(__uint_as_float(o[4 * j + 1]), 1.0f / kWeightUnit, offset),
-                                fmaf(__uint_as_float(o[4 * j + 2]), 1.0f / kWeightUnit, offset), fmaf(__uint_as_float(o[4 * j + 3]), 1.0f / kWeightUnit, offset));
+          for (int j = 0; j < 4; ++j) to[j] = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
         }
       }
     }
@@ -1006,24 +1114,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 }
 
 // Opt-in shared memory, once per device.
-template <int D, typename T, bool kPass>
+template <int D, typename T, PromptMode kMode>
 int32_t allow_prompt() {
-  using G = PromptGeometry<D, std::is_same<T, float>::value>;
+  using G = PromptGeometry<D, std::is_same<T, float>::value, kMode == kPass>;
   static std::atomic<uint64_t> done{0};
   int device = 0;
   IVB_CUDA(cudaGetDevice(&device));
   const uint64_t bit = device < 64 ? 1ull << device : 0;
   if ((done.load(std::memory_order_relaxed) & bit) == 0) {
-    IVB_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<D, T, kPass>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem));
+    IVB_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<D, T, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem));
     done.fetch_or(bit, std::memory_order_relaxed);
   }
   return IVB_OK;
 }
 
-template <int D, typename T>
+template <int D, typename T, PromptMode kMode>
 int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
-  using G = PromptGeometry<D, std::is_same<T, float>::value>;
-  if (int32_t rc = allow_prompt<D, T, false>()) return rc;
+  using G = PromptGeometry<D, std::is_same<T, float>::value, false>;
+  if (int32_t rc = allow_prompt<D, T, kMode>()) return rc;
   // as many tiles as the rows can make: each sequence of the call may leave one unfilled
   const int64_t items = static_cast<int64_t>(A.rows) * A.group;
   const int64_t sequences = std::min<int64_t>(A.cache.batch, items / (few + 1));
@@ -1042,28 +1150,35 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
   cfg.numAttrs = kv4_attributes(C, attr);
-  IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<D, T, false>, A, few));
+  IVB_CUDA(cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<D, T, kMode>, A, few));
   return IVB_OK;
 }
 
 template <int D, typename T>
 int32_t launch_prefix(const Kv4Attention& A, int few, cudaStream_t stream) {
-  using G = PromptGeometry<D, std::is_same<T, float>::value>;
-  if (int32_t rc = allow_prompt<D, T, true>()) return rc;
+  using G = PromptGeometry<D, std::is_same<T, float>::value, true>;
+  if (int32_t rc = allow_prompt<D, T, kPass>()) return rc;
   // as many tiles as the rows can make: each group may leave one unfilled
   const int64_t tiles = static_cast<int64_t>(A.rows) * A.group / G::rows + std::min<int64_t>(A.prefix.batch, A.rows);
-  const int64_t grid = tiles * A.cache.kv_heads * A.splits;
+  // the parts fill 148 CTAs at most, but for groups whose share is below one
+  const int64_t grid = tiles * A.cache.kv_heads + (A.splits > 1 ? 148 : 0);
   if (grid > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(tiles));
-  IVB_CUDA(launch_pdl(kv4_prompt_kernel<D, T, true>, dim3(static_cast<unsigned>(grid)), dim3(kPromptThreads), G::smem, stream, A, few));
+  IVB_CUDA(launch_pdl(kv4_prompt_kernel<D, T, kPass>, dim3(static_cast<unsigned>(grid)), dim3(kPromptThreads), G::smem, stream, A, few));
   return IVB_OK;
+}
+
+template <int D, typename T>
+int32_t launch_mode(const Kv4Attention& A, bool pass, int few, cudaStream_t stream) {
+  if (pass) return launch_prefix<D, T>(A, few, stream);
+  return A.prefix.data == nullptr ? launch_prompts<D, T, kPlain>(A, few, stream) : launch_prompts<D, T, kBehind>(A, few, stream);
 }
 
 template <typename T>
 int32_t launch_dim(const Kv4Attention& A, bool pass, int few, cudaStream_t stream) {
   switch (A.cache.head_dim) {
-    case 32: return pass ? launch_prefix<32, T>(A, few, stream) : launch_prompts<32, T>(A, few, stream);
-    case 64: return pass ? launch_prefix<64, T>(A, few, stream) : launch_prompts<64, T>(A, few, stream);
-    default: return pass ? launch_prefix<128, T>(A, few, stream) : launch_prompts<128, T>(A, few, stream);
+    case 32: return launch_mode<32, T>(A, pass, few, stream);
+    case 64: return launch_mode<64, T>(A, pass, few, stream);
+    default: return launch_mode<128, T>(A, pass, few, stream);
   }
 }
 
@@ -1078,13 +1193,14 @@ int32_t launch_type(const Kv4Attention& A, int32_t dtype, bool pass, int few, cu
 int32_t launch_kv4_prompts(const Kv4Attention& A, int32_t dtype, int few, cudaStream_t stream) { return launch_type(A, dtype, false, few, stream); }
 int32_t launch_kv4_prefix(const Kv4Attention& A, int32_t dtype, int few, cudaStream_t stream) { return launch_type(A, dtype, true, few, stream); }
 
-// Parts of the prefix that fill the SMs, if the rows are spread evenly over its groups and it is as long as it can be.
+// Parts of the prefix: how many CTAs may share a row tile and head at most. As many as fill the SMs if the rows are spread evenly over the
+// groups, twice as many where there are several, so that a long beginning can have more than a short one.
 int kv4_prefix_splits(const IvbKv4Cache& cache, const IvbKv4Cache& prefix, int32_t dtype, int group, int rows) {
   const int per_tile = dtype == IVB_F32 && cache.head_dim == 128 ? kRowsX : kRowsCta;
   const int64_t groups = std::min(prefix.batch, rows), items = (static_cast<int64_t>(rows) * group + groups - 1) / groups;
   const int64_t units = groups * ((items + per_tile - 1) / per_tile) * cache.kv_heads;
   const int64_t most = std::min<int64_t>(kMostSplits, (static_cast<int64_t>(prefix.max_len) + kPos - 1) / kPos);
-  return static_cast<int>(std::max<int64_t>(1, std::min(most, 148 / units)));
+  return static_cast<int>(std::max<int64_t>(1, std::min(most, (groups > 1 ? 296 : 148) / units)));
 }
 
 }  // namespace ivb
