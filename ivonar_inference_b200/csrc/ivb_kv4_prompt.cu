@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   __shared__ PromptBarriers bar;
   __shared__ unsigned tmem_base;
   __shared__ float largest[kSoftmaxWarps], smallest[kSoftmaxWarps], sums[kRowsCta], row_units[kRowsCta], refs_of[kRowsCta], totals[kRowsCta], offsets[kRowsCta];
-  __shared__ int nearest[kSoftmaxWarps];
+  __shared__ unsigned nearest[kSoftmaxWarps];
   __shared__ int which[8];  // sequence, tile of its rows; whether a wait ran out; group of the prefix, its length, its parts, which of them, head
   const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
@@ -385,8 +385,46 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     }
     return p < 0 || p >= max_len ? -1 : static_cast<int>(p);
   };
-  if (kMode != kPass && tid == 0 && rank == 0 && A.error != nullptr && clamp_position(base + token_of(i0 + live - 1)) >= max_len)
-    atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
+  const int last = kMode == kPass ? -1 : clamp_position(base + token_of(i0 + live - 1));  // own position of the rows' last
+  if (last >= max_len && tid == 0 && rank == 0 && A.error != nullptr) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
+
+  int own_at = -1;  // of row 32 warp + lane, where it takes a search
+  auto position_of = [&](int of_warp) { return kMode == kPass ? __shfl_sync(0xFFFFFFFFu, own_at, of_warp) : own_position(32 * warp + of_warp); };
+  int nearest_at = -1;
+  if constexpr (kMode == kPass) {
+    if (tid < kSoftmaxThreads) {
+      own_at = own_position(tid);
+      const unsigned to_end = __reduce_min_sync(0xFFFFFFFFu, static_cast<unsigned>(own_at));  // -1 is the largest
+      if (lane == 0) nearest[warp] = to_end;
+    }
+    __syncthreads();
+    unsigned least = 0xffffffffu;
+#pragma unroll
+    for (int w = 0; w < kSoftmaxWarps; ++w) least = min(least, nearest[w]);
+    nearest_at = static_cast<int>(least);
+  }
+  // The tiles of 128 positions that some row sees, of the prefix and then of the sequence's own: in each the sinks' below the window,
+  // then the window's. Positions count from the beginning, where the own ones' tiles stand at shared_length + 128 t.
+  const int first = kMode == kPass ? nearest_at : clamp_position(base + token_of(i0));  // own position of the rows' first
+  const int high = min(last, max_len - 1);
+  const int low = A.window > 0 ? max(0, max(first, 0) + shared_length - A.window + 1) : 0;
+  const int own_low = kMode == kPlain ? low : max(0, low - shared_length), own_sinks = kMode == kPlain ? A.sinks : max(0, A.sinks - shared_length);
+  const int window_tile = own_low / kPos;
+  const int sink_tiles = A.window > 0 ? min((min(own_sinks, own_low) + kPos - 1) / kPos, window_tile) : 0;
+  const int own_tiles = high < 0 ? 0 : sink_tiles + high / kPos - window_tile + 1;
+  const int shared_all = kMode != kPlain && (kMode == kPass ? first : high) >= 0 ? (shared_length + kPos - 1) / kPos : 0;
+  const int shared_window = min(low / kPos, shared_all);
+  const int shared_sinks = A.window > 0 ? min((min(A.sinks, low) + kPos - 1) / kPos, shared_window) : 0;
+  const int shared_tiles = kMode == kPlain ? 0 : shared_sinks + shared_all - shared_window;
+  const int all_tiles = shared_tiles + own_tiles;
+  const int tiles = all_tiles > rank ? (all_tiles - rank + C - 1) / C : 0;  // this CTA's
+  auto of_prefix = [&](int it) { return kMode == kPass || (kMode == kBehind && rank + it * C < shared_tiles); };
+  auto tile_of = [&](int it) {  // in its cache
+    int i = rank + it * C;
+    if (of_prefix(it)) return i < shared_sinks ? i : shared_window + i - shared_sinks;
+    i -= shared_tiles;
+    return i < sink_tiles ? i : window_tile + i - sink_tiles;
+  };
 
   // queries: a warp takes 32 rows in 16-byte chunks, 8 rows and 4 chunks at a time (64 contiguous bytes of a row, and no bank
   // conflicts); the rows' largest first, then hi (and lo) parts as K-major operands, scaled by a power of two that brings the largest of
@@ -399,14 +437,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     return static_cast<const T*>(array) + (row0 + t) * row_stride + h * head_stride;
   };
   uint4 raw[4][kQuads];
-  int own_at = -1;  // of row 32 warp + lane, where it takes a search
-  auto position_of = [&](int of_warp) { return kMode == kPass ? __shfl_sync(0xFFFFFFFFu, own_at, of_warp) : own_position(32 * warp + of_warp); };
   if (tid < kSoftmaxThreads) {
-    if constexpr (kMode == kPass) {
-      own_at = own_position(tid);
-      const unsigned to_end = __reduce_min_sync(0xFFFFFFFFu, static_cast<unsigned>(own_at));  // -1 is the largest
-      if (lane == 0) nearest[warp] = static_cast<int>(to_end);
-    }
     const T* q[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -470,37 +501,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     least = fminf(least, smallest[w]);
   }
   const bool even = least >= most * kEven;
-  // The tiles of 128 positions that some row sees, of the prefix and then of the sequence's own: in each the sinks' below the window,
-  // then the window's. Positions count from the beginning, where the own ones' tiles stand at shared_length + 128 t.
-  int shared_sinks, shared_window, shared_tiles, sink_tiles, window_tile, tiles;
-  auto plan = [&](int first, int high) {  // own positions: the rows' first, and the last that there is
-    const int low = A.window > 0 ? max(0, max(first, 0) + shared_length - A.window + 1) : 0;
-    const int own_low = max(0, low - shared_length), own_sinks = max(0, A.sinks - shared_length);
-    window_tile = own_low / kPos;
-    sink_tiles = A.window > 0 ? min((min(own_sinks, own_low) + kPos - 1) / kPos, window_tile) : 0;
-    const int own_tiles = kMode == kPass || high < 0 ? 0 : sink_tiles + high / kPos - window_tile + 1;
-    const int shared_all = kMode != kPlain && (kMode == kPass ? first : high) >= 0 ? (shared_length + kPos - 1) / kPos : 0;
-    shared_window = min(low / kPos, shared_all);
-    shared_sinks = A.window > 0 ? min((min(A.sinks, low) + kPos - 1) / kPos, shared_window) : 0;
-    shared_tiles = kMode == kPlain ? 0 : shared_sinks + shared_all - shared_window;
-    const int all_tiles = shared_tiles + own_tiles;
-    tiles = all_tiles > rank ? (all_tiles - rank + C - 1) / C : 0;  // this CTA's
-  };
-  if constexpr (kMode == kPass) {
-    unsigned first = 0xffffffffu;
-#pragma unroll
-    for (int w = 0; w < kSoftmaxWarps; ++w) first = min(first, static_cast<unsigned>(nearest[w]));
-    plan(static_cast<int>(first), -1);
-  } else {
-    plan(clamp_position(base + token_of(i0)), min(clamp_position(base + token_of(i0 + live - 1)), max_len - 1));
-  }
-  auto of_prefix = [&](int it) { return kMode == kPass || (kMode == kBehind && rank + it * C < shared_tiles); };
-  auto tile_of = [&](int it) {  // in its cache
-    int i = rank + it * C;
-    if (of_prefix(it)) return i < shared_sinks ? i : shared_window + i - shared_sinks;
-    i -= shared_tiles;
-    return i < sink_tiles ? i : window_tile + i - sink_tiles;
-  };
   const int up = query_power(most);
   const float score_unit = power_of_two(-up) * (A.scale * kLog2e);  // in the positions' terms
   if (tid < kSoftmaxThreads && x < row_tiles) {
@@ -561,9 +561,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     const int64_t own16 = kv4_tiles(max_len), shared16 = kv4_tiles(A.prefix.max_len);
     const unsigned char* const own_codes = static_cast<const unsigned char*>(A.cache.data) + (static_cast<int64_t>(b) * A.cache.kv_heads + kvh) * own16 * kTile;
     const unsigned char* const shared_codes = static_cast<const unsigned char*>(A.prefix.data) + (static_cast<int64_t>(which[3]) * A.cache.kv_heads + kvh) * shared16 * kTile;
-    RawChunks<D> key[kMine], value[kMine];
+    RawChunks<D> key[kMine], value[kMine], later[kMine];
     uint2 par[kMine];
-    auto fetch = [&](int it, bool keys) {
+    auto fetch = [&](int it, bool keys, RawChunks<D>(&value)[kMine]) {
       const bool shared = of_prefix(it);
       const unsigned char* const codes = shared ? shared_codes : own_codes;
       const int64_t tiles16 = shared ? shared16 : own16;
@@ -581,9 +581,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         }
       }
     };
-    if (tiles > 0) fetch(0, true);
+    // A pass has the next tile's values on their way as well as its keys while it expands one: its softmax leaves no time to wait for them.
+    constexpr bool kEarly = kMode == kPass;
+    if (tiles > 0) {
+      fetch(0, true, value);
+      if constexpr (kEarly) fetch(0, false, later);
+    }
     for (int it = 0; it < tiles; ++it) {
-      fetch(it, false);
+      if constexpr (kEarly) {
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) value[k] = later[k];
+        if (it + 1 < tiles) fetch(it + 1, false, later);
+      } else {
+        fetch(it, false, value);
+      }
       if (it >= G::stages && !wait_for(&bar.k_free[it % G::stages], turn_of(it) ^ 1u)) {
         ok = false;
         break;
@@ -612,7 +623,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       }
       fence_proxy_async();
       mbar_arrive(&bar.k_full[it % G::stages]);
-      if (it + 1 < tiles) fetch(it + 1, true);
+      if (it + 1 < tiles) fetch(it + 1, true, value);
       if (it >= G::stages && !wait_for(&bar.v_free[it % G::stages], turn_of(it) ^ 1u)) {
         ok = false;
         break;
