@@ -775,7 +775,7 @@ int32_t attention_call(const IvbKv4Cache* c, const IvbKv4Prefix* prefix, const v
     A.prefix_lengths = prefix->lengths;
     A.prefix_groups = prefix->groups;
     if (A.few != 0 && !walks_prefix(*c, prefix->cache, A.group, rows)) {
-      A.splits = kv4_prefix_splits(*c, prefix->cache, dtype, A.group, rows);
+      A.splits = kv4_prefix_splits(*c, prefix->cache, A.group, rows);
       if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < part_bytes(A.splits, rows, heads, c->head_dim))
         return fail(IVB_EINVAL, "ivb_kv4_attention_prefix: a workspace of %llu bytes at %p, not 16-byte aligned or too small",
                     static_cast<unsigned long long>(workspace_bytes), workspace);
@@ -813,7 +813,7 @@ uint64_t ivb_kv4_prefix_workspace_bytes(const IvbKv4Cache* c, const IvbKv4Prefix
   if (ivb::check_kv4(c, "ivb_kv4_prefix_workspace_bytes") || rows <= 0 || ivb::check_heads(c, heads, rows) || ivb::check_prefix(c, prefix)) return 0;
   const int group = heads / c->kv_heads;
   if (ivb::few_items(*c, group, starts, rows) == 0 || ivb::walks_prefix(*c, prefix->cache, group, rows)) return 0;
-  return ivb::part_bytes(ivb::kv4_prefix_splits(*c, prefix->cache, dtype, group, rows), rows, heads, c->head_dim);
+  return ivb::part_bytes(ivb::kv4_prefix_splits(*c, prefix->cache, group, rows), rows, heads, c->head_dim);
 }
 
 int32_t ivb_kv4_attention_prefix(const IvbKv4Cache* c, const IvbKv4Prefix* prefix, const void* q, int32_t dtype, int64_t q_row, int64_t q_head,

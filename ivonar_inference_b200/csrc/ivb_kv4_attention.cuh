@@ -215,6 +215,6 @@ __device__ __forceinline__ void kv4_join_parts(const Kv4Attention& A, int64_t it
 int32_t launch_kv4_prompts(const Kv4Attention& A, int32_t dtype, int few, cudaStream_t stream);
 // The prefix's parts of the rows of every other sequence, and in how many parts it comes.
 int32_t launch_kv4_prefix(const Kv4Attention& A, int32_t dtype, int few, cudaStream_t stream);
-int kv4_prefix_splits(const IvbKv4Cache& cache, const IvbKv4Cache& prefix, int32_t dtype, int group, int rows);
+int kv4_prefix_splits(const IvbKv4Cache& cache, const IvbKv4Cache& prefix, int group, int rows);
 
 }  // namespace ivb

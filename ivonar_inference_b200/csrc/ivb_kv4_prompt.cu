@@ -34,8 +34,21 @@ namespace cg = cooperative_groups;
 
 constexpr int kRowsX = 128, kRowsCta = 256, kPos = 128;
 // 12 warps: three on each of the SM's four parts have 168 registers a thread, for the scores of four rows at a time
-constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 32 * kSoftmaxWarps, kProducerWarps = 3, kProducers = 32 * kProducerWarps;
-constexpr int kIssueWarp = kSoftmaxWarps + kProducerWarps, kPromptThreads = 32 * (kIssueWarp + 1);
+constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 32 * kSoftmaxWarps;
+// kPlain: sequences that hold all of their positions. kBehind: behind a beginning that they share. kWide, kNarrow: a pass over the beginnings
+// for the rows of sequences with no more than `few` items; its "sequences" are the groups, its items all rows of a group's sequences,
+// each with a position of its own, and the tiles of positions are dealt out to several CTAs a row tile. (One kernel for the first two,
+// told apart as it runs, took 240 us where 230 are kept for a chunk of 2048 rows under a window.)
+//
+// With up to 128 rows a pass runs two streams where tensor memory has room for both: the tiles in turn are row tile 0's and 1's, which hold
+// the same rows and are joined at the end, so that one's softmax runs while the other waits for the tensor cores. Narrow ones have 64 rows,
+// 8 or 16 a warp (the lower ones of its 32 lanes of tensor memory), so that all warps share the softmax, and seven producer warps, four for
+// the keys and three for the values: 16 warps of 128 registers (17 would have 96). Behind 32,768 positions, narrow / wide: 16 heads x 64, 16
+// rows 38 / 52 us, 64 rows 48 / 57, 128 rows 85 / 64; 8 x 128, 256 rows 111 / 78.
+enum PromptMode { kPlain, kBehind, kWide, kNarrow };
+constexpr int kKeyWarps = 4, kValueWarps = 3, kNarrowRows = 64;
+constexpr int producer_warps(PromptMode mode) { return mode == kNarrow ? kKeyWarps + kValueWarps : 3; }
+constexpr int prompt_threads(PromptMode mode) { return 32 * (kSoftmaxWarps + producer_warps(mode) + 1); }
 constexpr float kWeightUnit = 64.0f;  // weights are at most 2 * 64 * 2^8 in fp16
 constexpr float kRaise = 8.0f;
 // A tile's rows share the queries' power of two (no multiplication of the scores by a row's own) unless one's largest is so far below
@@ -45,24 +58,29 @@ constexpr float kEven = 0.000244140625f;
 // 1024 positions). fp32 outputs keep a second one, to which the threads add the first every so many tiles, rounding to nearest.
 constexpr int kFoldTiles = 2;
 
-template <int D, bool kSplit, bool kOfPass>
+template <int D, bool kSplit, PromptMode kMode>
 struct PromptGeometry {
-  // terms(it + 2) are written when S(it) is done, so when nobody reads terms(it - 1) any more; in streams (below) when nobody
-  // reads terms(it - 2)
-  static constexpr int term_sets = kOfPass ? 4 : 3;
+  static constexpr bool narrow = kMode == kNarrow, pass = narrow || kMode == kWide;
   static constexpr int parts = kSplit ? 2 : 1;
-  static constexpr int stages = kSplit && D == 128 ? 1 : 2;  // of keys and of values
+  // Stages of keys and of values. Two streams want more of them than two (with two their tiles waited for one another: 1.3 us a tile).
+  static constexpr int k_stages = narrow ? (D < 128 ? 4 : kSplit ? 2 : 3) : kSplit && D == 128 ? 1 : 2, v_stages = narrow ? (D < 128 ? 4 : 2) : k_stages;
+  // The terms of tile it are written when S(it - k_stages) is done, which was issued when nobody read the terms of the tile before it, in
+  // streams of the one before that, any more.
+  static constexpr int term_sets = pass ? k_stages + 2 : 3;
   static constexpr int q_bytes = kRowsX * D * 2;             // one part of one row tile
   static constexpr int kv_bytes = kPos * D * 2;              // keys or values of a stage
   static constexpr int term_bytes = kPos * 24;
-  static constexpr int q_at = 0, k_at = (kSplit && D == 128 ? 1 : 2) * parts * q_bytes, v_at = k_at + stages * kv_bytes, terms_at = v_at + stages * kv_bytes;
+  static constexpr int q_at = 0, k_at = ((kSplit && D == 128) || narrow ? 1 : 2) * parts * q_bytes, v_at = k_at + k_stages * kv_bytes, terms_at = v_at + v_stages * kv_bytes;
   // over half of an SM's at least: of two clusters sharing two SMs each could hold the tensor memory that the other waits for
   static constexpr int used = terms_at + term_sets * term_bytes, smem = used < 118 * 1024 ? 118 * 1024 : used;
   // row tiles of a CTA: at fp32 and D = 128 tensor memory holds the accumulators of one
-  static constexpr int row_tiles = kSplit && D == 128 ? 1 : 2, rows = row_tiles * kRowsX;
+  static constexpr int row_tiles = kSplit && D == 128 ? 1 : 2, rows = narrow ? kNarrowRows : row_tiles * kRowsX;
   // tensor memory columns: S_X, then P_X in its place (of every 64 columns 32 hi, 32 lo), O_X, and O_X's sums (fp32)
   static constexpr int s_at = 0, o_at = row_tiles * kPos, fold_at = o_at + row_tiles * D, columns = 512;
   static_assert(fold_at + (kSplit ? row_tiles * D : 0) <= columns, "tensor memory");
+  // what a pass leaves at its end: the streams' O, rows of D values and 4 more, so that neighbouring rows' chunks lie on other banks
+  static constexpr int leave_row = D + 4, leave_stream = kRowsX * leave_row;
+  static_assert(!pass || row_tiles * leave_stream * 4 <= smem, "shared memory");
 };
 
 // kind::f16, fp32 result, A K-major, B MN-major.
@@ -110,7 +128,7 @@ __device__ __forceinline__ void values_of_chunk(uint4 w, float (&v)[16 / sizeof(
 }
 
 struct PromptBarriers {
-  unsigned long long k_full[2], k_free[2], v_full[2], v_free[2], terms_full[4], s_full[2][2], p_full[2][2], p_free[2][2], drain;
+  unsigned long long k_full[4], k_free[4], v_full[4], v_free[4], terms_full[6], s_full[2][2], p_full[2][2], p_free[2][2], drain;
 };
 
 // What a lane of a producer warp holds of the keys or values of one tile of 16 positions (D = 32: values in lanes 0..15), dealt
@@ -193,16 +211,14 @@ __device__ __forceinline__ void store_codes_of_values(const RawChunks<D>& raw, i
   }
 }
 
-// kPlain: sequences that hold all of their positions. kBehind: behind a beginning that they share. kPass: the pass over the beginnings
-// for the rows of sequences with no more than `few` items; its "sequences" are the groups, its items all rows of a group's sequences,
-// each with a position of its own, and the tiles are dealt out to A.splits CTAs a row tile. (One kernel for the first two, told
-// apart as it runs, took 240 us where 230 are kept for a chunk of 2048 rows under a window.)
-enum PromptMode { kPlain, kBehind, kPass };
-
 template <int D, typename T, PromptMode kMode>
-__global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attention A, int few) {
+__global__ void __launch_bounds__(prompt_threads(kMode), 1) kv4_prompt_kernel(Kv4Attention A, int few) {
+  constexpr bool kPass = kMode == kWide || kMode == kNarrow;
+  constexpr int kProducerWarps = producer_warps(kMode), kProducers = 32 * kProducerWarps;
+  constexpr int kKeyThreads = kMode == kNarrow ? 32 * kKeyWarps : kProducers, kValueThreads = kMode == kNarrow ? 32 * kValueWarps : kProducers;
+  constexpr int kIssueWarp = kSoftmaxWarps + kProducerWarps;
   constexpr bool kSplit = std::is_same<T, float>::value;
-  using G = PromptGeometry<D, kSplit, kMode == kPass>;
+  using G = PromptGeometry<D, kSplit, kMode>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ PromptBarriers bar;
   __shared__ unsigned tmem_base;
@@ -211,16 +227,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   __shared__ int which[8];  // sequence, tile of its rows; whether a wait ran out; group of the prefix, its length, its parts, which of them, head
   const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
-  if (kMode == kPass && A.beside_prompts) __threadfence();
+  if (kPass && A.beside_prompts) __threadfence();
   else pdl_wait();
   // which rows: the call's tiles of 256 items in the order of the sequences, the last ones (the longest rows) first
   cg::cluster_group cluster = cg::this_cluster();
   int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-  const int sequences = kMode == kPass ? A.prefix.batch : A.cache.batch;
+  const int sequences = kPass ? A.prefix.batch : A.cache.batch;
   // the rows of sequence, or group, b
   auto rows_of = [&](int b, int& from) {
     int b0 = b, b1 = b + 1;
-    if (kMode == kPass) {
+    if (kPass) {
       b0 = A.prefix_groups == nullptr ? 0 : max(0, A.prefix_groups[b]);
       b1 = A.prefix_groups == nullptr ? A.cache.batch : min(A.cache.batch, A.prefix_groups[b + 1]);
       if (b1 <= b0) b0 = b1 = 0;
@@ -230,33 +246,47 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   };
   const int unit = static_cast<int>(blockIdx.x) / C, units = static_cast<int>(gridDim.x) / C;
   int kvh = unit % A.cache.kv_heads;
-  const int order = kMode == kPass ? static_cast<int>(blockIdx.x) : units / A.cache.kv_heads - 1 - unit / A.cache.kv_heads;
+  const int order = kPass ? static_cast<int>(blockIdx.x) : units / A.cache.kv_heads - 1 - unit / A.cache.kv_heads;
   if (warp == 0) {
-    // the tiles of 128 positions and of rows of group g
     auto length_of = [&](int g) { return static_cast<int>(max(static_cast<int64_t>(0), min(A.prefix_lengths[g], static_cast<int64_t>(A.prefix.max_len)))); };
-    auto tiles_of = [&](int g) { return (length_of(g) + kPos - 1) / kPos; };
     auto row_tiles_of = [&](int b) {
       int from;
       const int items = rows_of(b, from) * A.group;
-      return items > (kMode == kPass ? 0 : few) ? (items + G::rows - 1) / G::rows : 0;
+      return items > (kPass ? 0 : few) ? (items + G::rows - 1) / G::rows : 0;
     };
     // A pass deals its CTAs out by the work: each row tile and head of a group gets so many parts that all of them fill the SMs once.
-    unsigned long long work = 0;
-    if constexpr (kMode == kPass) {
-      for (int b = lane; b < sequences; b += 32) work += static_cast<unsigned long long>(row_tiles_of(b)) * tiles_of(b);
+    // The lanes keep what they load of the first 32 groups.
+    int lane_length = 0, lane_tiles = 0;
+    float share = 0.0f;
+    if constexpr (kPass) {
+      unsigned long long work = 0;
+      for (int b = lane; b < sequences; b += 32) {
+        const int length = length_of(b), n = row_tiles_of(b);
+        if (b == lane) {
+          lane_length = length;
+          lane_tiles = n;
+        }
+        work += static_cast<unsigned long long>(n) * ((length + kPos - 1) / kPos);
+      }
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) work += __shfl_xor_sync(0xFFFFFFFFu, work, d);
-      work = max(1ull, work * A.cache.kv_heads);
+      share = 148.0f / (static_cast<float>(max(1ull, work)) * static_cast<float>(A.cache.kv_heads));  // CTAs a tile of positions
     }
-    auto parts_of = [&](int b) {
-      const int n = tiles_of(b);
-      return n == 0 ? 0 : static_cast<int>(max(1ull, min(static_cast<unsigned long long>(A.splits), 148ull * n / work)));
+    auto parts_of = [&](int length) {  // rounded down, with room for the quotient's rounding: no more than 148 in all
+      return length == 0 ? 0 : max(1, min(A.splits, static_cast<int>(static_cast<float>((length + kPos - 1) / kPos) * share * 0.99999f)));
     };
     int seen = 0, found = -1, tile = 0;
     for (int b0 = 0; b0 < sequences && found < 0; b0 += 32) {
       const int b = b0 + lane;
       int n = 0;
-      if (b < sequences) n = kMode == kPass ? row_tiles_of(b) * A.cache.kv_heads * parts_of(b) : row_tiles_of(b);
+      int length = 0, row_tiles = 0;
+      if (b < sequences) {
+        row_tiles = n = kPass && b0 == 0 ? lane_tiles : row_tiles_of(b);
+        if constexpr (kPass) {
+          length = b0 == 0 ? lane_length : length_of(b);
+          n *= A.cache.kv_heads * parts_of(length);
+        }
+      }
       int upto = n;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -268,16 +298,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
         const int l = __ffs(hit) - 1;
         found = b0 + l;
         tile = order - (seen + __shfl_sync(0xFFFFFFFFu, upto, l) - __shfl_sync(0xFFFFFFFFu, n, l));
+        if constexpr (kPass) {
+          lane_length = __shfl_sync(0xFFFFFFFFu, length, l);
+          lane_tiles = __shfl_sync(0xFFFFFFFFu, row_tiles, l);
+        }
       }
       seen += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
     int group = found, length = 0;
     if (kMode == kBehind && found >= 0) length = kv4_prefix(A, found, group);
-    if (kMode == kPass && found >= 0) {
-      length = length_of(found);
-      const int each = row_tiles_of(found) * A.cache.kv_heads;
+    if (kPass && found >= 0) {
+      length = lane_length;
+      const int each = lane_tiles * A.cache.kv_heads;
       if (lane == 0) {
-        which[5] = parts_of(found);
+        which[5] = parts_of(length);
         which[6] = tile / each;
         which[7] = tile % each % A.cache.kv_heads;
       }
@@ -293,11 +327,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   }
   if (tid == 32) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.k_full[i], kProducers);
+    for (int i = 0; i < G::k_stages; ++i) {
+      mbar_init(&bar.k_full[i], kKeyThreads);
       mbar_init(&bar.k_free[i], 1);
-      mbar_init(&bar.v_full[i], kProducers);
+    }
+#pragma unroll
+    for (int i = 0; i < G::v_stages; ++i) {
+      mbar_init(&bar.v_full[i], kValueThreads);
       mbar_init(&bar.v_free[i], 1);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         mbar_init(&bar.p_full[i][h], kSoftmaxThreads / 2);
@@ -306,7 +346,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       }
     }
 #pragma unroll
-    for (int i = 0; i < G::term_sets; ++i) mbar_init(&bar.terms_full[i], kProducers);
+    for (int i = 0; i < G::term_sets; ++i) mbar_init(&bar.terms_full[i], kKeyThreads);
     mbar_init(&bar.drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -314,13 +354,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   const int b = which[0];
   // a pass does not end before the prompts' grid that it runs beside, whichever way its first CTA takes
   auto end = [&] {
-    if (kMode == kPass && A.beside_prompts && blockIdx.x == 0) pdl_wait();
+    if (kPass && A.beside_prompts && blockIdx.x == 0) pdl_wait();
   };
   if (b < 0) {
     end();
     return;
   }
-  if (kMode == kPass) {
+  if (kPass) {
     C = which[5];
     rank = which[6];
     kvh = which[7];
@@ -342,15 +382,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   int row0;
   const int count = rows_of(b, row0);
   // rows of the sequence that the call does not have
-  const int64_t before = A.starts == nullptr || kMode == kPass ? 0 : static_cast<int64_t>(row0) - A.starts[b];
-  const int i0 = which[1] * G::rows, live = min(G::rows, count * A.group - i0), row_tiles = live > kRowsX ? 2 : 1;
-  // With up to 128 rows a pass runs two streams: the tiles of positions in turn are row tile 0's and 1's, which hold the same rows and
-  // are joined at the end, so that one's softmax runs while the other waits for the tensor cores, and both have four warps.
-  const bool streams = kMode == kPass && G::row_tiles == 2 && row_tiles == 1;
-  // Few rows stand 8 or 16 to a warp (the 8 or 16 lower ones of its 32 lanes of tensor memory), so that all warps share the softmax.
-  const int spread = !streams || live > 64 ? 32 : live > 32 ? 16 : 8;
+  const int64_t before = A.starts == nullptr || kPass ? 0 : static_cast<int64_t>(row0) - A.starts[b];
+  const int i0 = which[1] * G::rows, live = min(G::rows, count * A.group - i0), row_tiles = !G::narrow && live > kRowsX ? 2 : 1;
+  const bool streams = G::pass && G::row_tiles == 2 && (G::narrow || live <= kRowsX);
+  const int spread = !G::narrow ? 32 : live > 32 ? 16 : 8;  // rows of a warp
   auto item_at = [&](int r) {  // of the row tiles' lane r; -1: none
-    if (kMode != kPass || !streams) return r < live ? r : -1;
+    if (!G::narrow) return r < live ? r : -1;
     const int i = (r >> 5) * spread + (r & 31);
     return (r & 31) < spread && r < kRowsX && i < live ? i : -1;
   };
@@ -359,13 +396,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   const unsigned group_size = static_cast<unsigned>(A.group);
   auto token_of = [&](int i) { return static_cast<int>(static_cast<unsigned>(i) / group_size); };
   auto clamp_position = [&](int64_t p) { return static_cast<int>(max(static_cast<int64_t>(-1), min(p, static_cast<int64_t>(max_len)))); };
-  const int64_t base = kMode == kPass ? 0 : kv4_position(A.positions, b) + before;
+  const int64_t base = kPass ? 0 : kv4_position(A.positions, b) + before;
   // position of row r of the tile in its sequence's own cache, -1 where it sees nothing
   auto own_position = [&](int r) {
     const int item = item_at(r);
     if (item < 0) return -1;
     int64_t p;
-    if constexpr (kMode == kPass) {
+    if constexpr (kPass) {
       const int row = row0 + token_of(i0 + item);
       int of = row;
       if (A.starts != nullptr) {  // the last sequence of the group that starts at or before the row
@@ -385,13 +422,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     }
     return p < 0 || p >= max_len ? -1 : static_cast<int>(p);
   };
-  const int last = kMode == kPass ? -1 : clamp_position(base + token_of(i0 + live - 1));  // own position of the rows' last
+  const int last = kPass ? -1 : clamp_position(base + token_of(i0 + live - 1));  // own position of the rows' last
   if (last >= max_len && tid == 0 && rank == 0 && A.error != nullptr) atomicCAS(A.error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
 
   int own_at = -1;  // of row 32 warp + lane, where it takes a search
-  auto position_of = [&](int of_warp) { return kMode == kPass ? __shfl_sync(0xFFFFFFFFu, own_at, of_warp) : own_position(32 * warp + of_warp); };
+  auto position_of = [&](int of_warp) { return kPass ? __shfl_sync(0xFFFFFFFFu, own_at, of_warp) : own_position(32 * warp + of_warp); };
   int nearest_at = -1;
-  if constexpr (kMode == kPass) {
+  if constexpr (kPass) {
     if (tid < kSoftmaxThreads) {
       own_at = own_position(tid);
       const unsigned to_end = __reduce_min_sync(0xFFFFFFFFu, static_cast<unsigned>(own_at));  // -1 is the largest
@@ -402,23 +439,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 #pragma unroll
     for (int w = 0; w < kSoftmaxWarps; ++w) least = min(least, nearest[w]);
     nearest_at = static_cast<int>(least);
+    if (nearest_at < 0) {  // prompts' rows and idle ones: nobody reads their parts
+      if (warp == kIssueWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(G::columns));
+      end();
+      return;
+    }
   }
   // The tiles of 128 positions that some row sees, of the prefix and then of the sequence's own: in each the sinks' below the window,
   // then the window's. Positions count from the beginning, where the own ones' tiles stand at shared_length + 128 t.
-  const int first = kMode == kPass ? nearest_at : clamp_position(base + token_of(i0));  // own position of the rows' first
+  const int first = kPass ? nearest_at : clamp_position(base + token_of(i0));  // own position of the rows' first
   const int high = min(last, max_len - 1);
   const int low = A.window > 0 ? max(0, max(first, 0) + shared_length - A.window + 1) : 0;
   const int own_low = kMode == kPlain ? low : max(0, low - shared_length), own_sinks = kMode == kPlain ? A.sinks : max(0, A.sinks - shared_length);
   const int window_tile = own_low / kPos;
   const int sink_tiles = A.window > 0 ? min((min(own_sinks, own_low) + kPos - 1) / kPos, window_tile) : 0;
   const int own_tiles = high < 0 ? 0 : sink_tiles + high / kPos - window_tile + 1;
-  const int shared_all = kMode != kPlain && (kMode == kPass ? first : high) >= 0 ? (shared_length + kPos - 1) / kPos : 0;
+  const int shared_all = kMode != kPlain && (kPass ? first : high) >= 0 ? (shared_length + kPos - 1) / kPos : 0;
   const int shared_window = min(low / kPos, shared_all);
   const int shared_sinks = A.window > 0 ? min((min(A.sinks, low) + kPos - 1) / kPos, shared_window) : 0;
   const int shared_tiles = kMode == kPlain ? 0 : shared_sinks + shared_all - shared_window;
   const int all_tiles = shared_tiles + own_tiles;
   const int tiles = all_tiles > rank ? (all_tiles - rank + C - 1) / C : 0;  // this CTA's
-  auto of_prefix = [&](int it) { return kMode == kPass || (kMode == kBehind && rank + it * C < shared_tiles); };
+  auto of_prefix = [&](int it) { return kPass || (kMode == kBehind && rank + it * C < shared_tiles); };
   auto tile_of = [&](int it) {  // in its cache
     int i = rank + it * C;
     if (of_prefix(it)) return i < shared_sinks ? i : shared_window + i - shared_sinks;
@@ -426,6 +468,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     return i < sink_tiles ? i : window_tile + i - sink_tiles;
   };
 
+  if constexpr (kPass) {  // the first two tiles come into the second-level cache while the queries are loaded
+    constexpr int kLine = 128, kTileBytes = kPos / 16 * kv4_tile_bytes(D);
+    const unsigned char* const codes = static_cast<const unsigned char*>(A.prefix.data) +
+                                       (static_cast<int64_t>(which[3]) * A.cache.kv_heads + kvh) * kv4_tiles(A.prefix.max_len) * kv4_tile_bytes(D);
+    const int64_t end = kv4_tiles(A.prefix.max_len) * kv4_tile_bytes(D);
+    const int n = tid - kSoftmaxThreads;
+    if (n >= 0 && n < kProducers)
+      for (int it = 0; it < min(2, tiles); ++it)
+        for (int64_t at = static_cast<int64_t>(tile_of(it)) * kTileBytes + n * kLine; n * kLine < kTileBytes && at < end; at = end)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(codes + at));
+  }
   // queries: a warp takes 32 rows in 16-byte chunks, 8 rows and 4 chunks at a time (64 contiguous bytes of a row, and no bank
   // conflicts); the rows' largest first, then hi (and lo) parts as K-major operands, scaled by a power of two that brings the largest of
   // all rows to 2^13, or each row's own where they are uneven. Idle rows' queries are not read.
@@ -546,95 +599,139 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = __shfl_sync(0xFFFFFFFFu, tmem_base, 0);
-  auto keys_of = [&](int it) { return smem + G::k_at + it % G::stages * G::kv_bytes; };
-  auto values_of = [&](int it) { return smem + G::v_at + it % G::stages * G::kv_bytes; };
+  auto keys_of = [&](int it) { return smem + G::k_at + it % G::k_stages * G::kv_bytes; };
+  auto values_of = [&](int it) { return smem + G::v_at + it % G::v_stages * G::kv_bytes; };
   auto terms_of = [&](int it) { return reinterpret_cast<float*>(smem + G::terms_at + it % G::term_sets * G::term_bytes); };
-  auto turn_of = [&](int it) { return static_cast<unsigned>(it / G::stages) & 1u; };  // parity of a stage's use
+  // parities of a stage's use
+  auto k_turn = [&](int it) { return static_cast<unsigned>(it / G::k_stages) & 1u; };
+  auto v_turn = [&](int it) { return static_cast<unsigned>(it / G::v_stages) & 1u; };
   const int my_tiles = streams ? (tiles + 1 - x) >> 1 : tiles;  // of a softmax warp's row tile
   bool ok = true;
   auto wait_for = [&](unsigned long long* at, unsigned turn) { return mbar_wait_bounded(at, turn, A.wait_ns); };
 
   if (warp >= kSoftmaxWarps && warp < kIssueWarp) {
-    // ---- producers: 16-position tiles in turn ----
-    constexpr int kTile = kv4_tile_bytes(D), kUnits = kPos / 16, kMine = (kUnits + kProducerWarps - 1) / kProducerWarps;
-    const int unit0 = warp - kSoftmaxThreads / 32;
+    // ---- producers: 16-position tiles in turn; in a pass four warps the keys, three the values ----
+    constexpr int kTile = kv4_tile_bytes(D), kUnits = kPos / 16;
     const int64_t own16 = kv4_tiles(max_len), shared16 = kv4_tiles(A.prefix.max_len);
     const unsigned char* const own_codes = static_cast<const unsigned char*>(A.cache.data) + (static_cast<int64_t>(b) * A.cache.kv_heads + kvh) * own16 * kTile;
     const unsigned char* const shared_codes = static_cast<const unsigned char*>(A.prefix.data) + (static_cast<int64_t>(which[3]) * A.cache.kv_heads + kvh) * shared16 * kTile;
-    RawChunks<D> key[kMine], value[kMine], later[kMine];
-    uint2 par[kMine];
-    auto fetch = [&](int it, bool keys, RawChunks<D>(&value)[kMine]) {
+    // unit u of tile it, and whether there is one
+    auto unit_at = [&](int it, int u, bool& in) {
       const bool shared = of_prefix(it);
-      const unsigned char* const codes = shared ? shared_codes : own_codes;
-      const int64_t tiles16 = shared ? shared16 : own16;
-#pragma unroll
-      for (int k = 0; k < kMine; ++k) {
-        const int u = unit0 + k * kProducerWarps;
-        const int64_t t = static_cast<int64_t>(tile_of(it)) * kUnits + u;
-        const bool in = u < kUnits && t < tiles16;
-        const unsigned char* tile = codes + (in ? t : 0) * kTile;
-        if (keys) {
-          load_keys<D>(tile, in, lane, key[k]);
-          par[k] = in && lane < 16 ? *reinterpret_cast<const uint2*>(tile + 16 * D + lane * 8) : make_uint2(0u, 0u);
-        } else {
-          load_codes_of_values<D>(tile, in, lane, value[k]);
-        }
+      const int64_t t = static_cast<int64_t>(tile_of(it)) * kUnits + u;
+      in = u < kUnits && t < (shared ? shared16 : own16);
+      return (shared ? shared_codes : own_codes) + (in ? t : 0) * kTile;
+    };
+    auto load_unit_keys = [&](int it, int u, RawChunks<D>& key, uint2& par) {
+      bool in;
+      const unsigned char* const tile = unit_at(it, u, in);
+      load_keys<D>(tile, in, lane, key);
+      par = in && lane < 16 ? *reinterpret_cast<const uint2*>(tile + 16 * D + lane * 8) : make_uint2(0u, 0u);
+    };
+    auto load_unit_values = [&](int it, int u, RawChunks<D>& value) {
+      bool in;
+      const unsigned char* const tile = unit_at(it, u, in);
+      load_codes_of_values<D>(tile, in, lane, value);
+    };
+    auto store_unit_terms = [&](int it, int u, uint2 par) {
+      if (lane < 16) {
+        const PositionTerms p = position_terms(par, score_unit, kWeightUnit, lane);
+        float* at_terms = terms_of(it) + 12 * (8 * u + (lane >> 1)) + (lane & 1);
+        at_terms[0] = p.key_scale;
+        at_terms[2] = p.key_offset;
+        at_terms[4] = p.bias;
+        at_terms[6] = p.mantissa;
+        at_terms[8] = p.unbias;
+        at_terms[10] = p.value_offset;
       }
     };
-    // A pass has the next tile's values on their way as well as its keys while it expands one: its softmax leaves no time to wait for them.
-    constexpr bool kEarly = kMode == kPass;
-    if (tiles > 0) {
-      fetch(0, true, value);
-      if constexpr (kEarly) fetch(0, false, later);
-    }
-    for (int it = 0; it < tiles; ++it) {
-      if constexpr (kEarly) {
+    auto keys_may_go = [&](int it) { return it < G::k_stages || wait_for(&bar.k_free[it % G::k_stages], k_turn(it) ^ 1u); };
+    auto values_may_go = [&](int it) { return it < G::v_stages || wait_for(&bar.v_free[it % G::v_stages], v_turn(it) ^ 1u); };
+    if constexpr (G::narrow) {
+      // what a warp does for a tile is mostly waiting for its own instructions: keys and values one after the other took seven warps 1.1 us
+      const int w = warp - kSoftmaxWarps;
+      if (w < kKeyWarps) {
+        constexpr int kMine = kUnits / kKeyWarps;
+        RawChunks<D> key[kMine], next[kMine];
+        uint2 par[kMine], next_par[kMine];
+        auto load = [&](int it) {
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) value[k] = later[k];
-        if (it + 1 < tiles) fetch(it + 1, false, later);
-      } else {
-        fetch(it, false, value);
-      }
-      if (it >= G::stages && !wait_for(&bar.k_free[it % G::stages], turn_of(it) ^ 1u)) {
-        ok = false;
-        break;
-      }
-      if (lane < 16) {
+          for (int k = 0; k < kMine; ++k) load_unit_keys(it, w + k * kKeyWarps, next[k], next_par[k]);
+        };
+        if (tiles > 0) load(0);
+        for (int it = 0; it < tiles; ++it) {
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) {
-          const int u = unit0 + k * kProducerWarps;
-          if (u < kUnits) {
-            const PositionTerms p = position_terms(par[k], score_unit, kWeightUnit, lane);
-            float* at_terms = terms_of(it) + 12 * (8 * u + (lane >> 1)) + (lane & 1);
-            at_terms[0] = p.key_scale;
-            at_terms[2] = p.key_offset;
-            at_terms[4] = p.bias;
-            at_terms[6] = p.mantissa;
-            at_terms[8] = p.unbias;
-            at_terms[10] = p.value_offset;
+          for (int k = 0; k < kMine; ++k) {
+            key[k] = next[k];
+            par[k] = next_par[k];
           }
+          if (it + 1 < tiles) load(it + 1);
+          ok = keys_may_go(it);
+          if (!ok) break;
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) store_unit_terms(it, w + k * kKeyWarps, par[k]);
+          mbar_arrive(&bar.terms_full[it % G::term_sets]);
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) store_keys<D>(key[k], lane, keys_of(it) + (w + k * kKeyWarps) * 16 * D * 2);
+          fence_proxy_async();
+          mbar_arrive(&bar.k_full[it % G::k_stages]);
+        }
+      } else {
+        constexpr int kMine = (kUnits + kValueWarps - 1) / kValueWarps;
+        RawChunks<D> value[kMine], next[kMine];
+        auto load = [&](int it) {
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) load_unit_values(it, w - kKeyWarps + k * kValueWarps, next[k]);
+        };
+        if (tiles > 0) load(0);
+        for (int it = 0; it < tiles; ++it) {
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) value[k] = next[k];
+          if (it + 1 < tiles) load(it + 1);
+          ok = values_may_go(it);
+          if (!ok) break;
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) {
+            const int u = w - kKeyWarps + k * kValueWarps;
+            if (u < kUnits) store_codes_of_values<D>(value[k], lane, values_of(it) + u * 16 * D * 2);
+          }
+          fence_proxy_async();
+          mbar_arrive(&bar.v_full[it % G::v_stages]);
         }
       }
-      mbar_arrive(&bar.terms_full[it % G::term_sets]);
+    } else {
+      constexpr int kMine = (kUnits + kProducerWarps - 1) / kProducerWarps;
+      const int unit0 = warp - kSoftmaxWarps;
+      RawChunks<D> key[kMine], value[kMine];
+      uint2 par[kMine];
+      auto load = [&](int it) {
 #pragma unroll
-      for (int k = 0; k < kMine; ++k) {
-        const int u = unit0 + k * kProducerWarps;
-        if (u < kUnits) store_keys<D>(key[k], lane, keys_of(it) + u * 16 * D * 2);
-      }
-      fence_proxy_async();
-      mbar_arrive(&bar.k_full[it % G::stages]);
-      if (it + 1 < tiles) fetch(it + 1, true, value);
-      if (it >= G::stages && !wait_for(&bar.v_free[it % G::stages], turn_of(it) ^ 1u)) {
-        ok = false;
-        break;
-      }
+        for (int k = 0; k < kMine; ++k) load_unit_keys(it, unit0 + k * kProducerWarps, key[k], par[k]);
+      };
+      if (tiles > 0) load(0);
+      for (int it = 0; it < tiles; ++it) {
 #pragma unroll
-      for (int k = 0; k < kMine; ++k) {
-        const int u = unit0 + k * kProducerWarps;
-        if (u < kUnits) store_codes_of_values<D>(value[k], lane, values_of(it) + u * 16 * D * 2);
+        for (int k = 0; k < kMine; ++k) load_unit_values(it, unit0 + k * kProducerWarps, value[k]);
+        ok = keys_may_go(it);
+        if (!ok) break;
+#pragma unroll
+        for (int k = 0; k < kMine; ++k)
+          if (unit0 + k * kProducerWarps < kUnits) store_unit_terms(it, unit0 + k * kProducerWarps, par[k]);
+        mbar_arrive(&bar.terms_full[it % G::term_sets]);
+#pragma unroll
+        for (int k = 0; k < kMine; ++k)
+          if (unit0 + k * kProducerWarps < kUnits) store_keys<D>(key[k], lane, keys_of(it) + (unit0 + k * kProducerWarps) * 16 * D * 2);
+        fence_proxy_async();
+        mbar_arrive(&bar.k_full[it % G::k_stages]);
+        if (it + 1 < tiles) load(it + 1);
+        ok = values_may_go(it);
+        if (!ok) break;
+#pragma unroll
+        for (int k = 0; k < kMine; ++k)
+          if (unit0 + k * kProducerWarps < kUnits) store_codes_of_values<D>(value[k], lane, values_of(it) + (unit0 + k * kProducerWarps) * 16 * D * 2);
+        fence_proxy_async();
+        mbar_arrive(&bar.v_full[it % G::v_stages]);
       }
-      fence_proxy_async();
-      mbar_arrive(&bar.v_full[it % G::stages]);
     }
   } else if (warp >= kIssueWarp) {
     // ---- the warp that issues the products: all its lanes take the same way (ok is the same in each) ----
@@ -644,7 +741,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     // Half h of tile it: its 64 columns of S_X, and with P_X in their place its 64 positions' part of O_X. Descriptors count
     // in 16 bytes.
     auto issue_s = [&](int it, int h) {
-      const uint64_t k = k0 + (it % G::stages * G::kv_bytes + h * (G::kv_bytes / 2)) / 16;
+      const uint64_t k = k0 + (it % G::k_stages * G::kv_bytes + h * (G::kv_bytes / 2)) / 16;
       const int turn = streams ? it >> 1 : it;
       for (int xx = streams ? it & 1 : 0; xx < (streams ? (it & 1) + 1 : row_tiles); ++xx) {
         if (turn > 0) {  // S takes the place of P
@@ -661,10 +758,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
             umma_f16_ss_warp(t_s, q + (part * G::q_bytes + kk * 256) / 16, k + kk * 16, idesc_f16(kRowsX, kPos / 2), kk + part > 0);
         umma_commit_warp(&bar.s_full[xx][h]);
       }
-      if (h == 1) umma_commit_warp(&bar.k_free[it % G::stages]);
+      if (h == 1) umma_commit_warp(&bar.k_free[it % G::k_stages]);
     };
     auto issue_o = [&](int it, int h) {
-      const uint64_t v = v0 + (it % G::stages * G::kv_bytes + h * (G::kv_bytes / 2)) / 16;
+      const uint64_t v = v0 + (it % G::v_stages * G::kv_bytes + h * (G::kv_bytes / 2)) / 16;
       const int turn = streams ? it >> 1 : it;
       for (int xx = streams ? it & 1 : 0; xx < (streams ? (it & 1) + 1 : row_tiles); ++xx) {
         ok = ok && wait(&bar.p_full[xx][h], turn & 1);
@@ -678,7 +775,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
             umma_f16_ts_warp(t_o, t_p + part * (kPos / 4) + kk * 8, v + kk * 2 * (D / 8) * 8, idesc_f16_bt(kRowsX, D), kk + part > 0 || h > 0 || (kSplit ? turn % kFoldTiles != 0 : turn > 0));
         umma_commit_warp(&bar.p_free[xx][h]);
       }
-      if (h == 1) umma_commit_warp(&bar.v_free[it % G::stages]);
+      if (h == 1) umma_commit_warp(&bar.v_free[it % G::v_stages]);
     };
     if (tiles > 0) {
       ok = wait(&bar.k_full[0], 0) && !A.withhold;
@@ -689,7 +786,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     }
     const int ahead = streams ? 2 : 1;
     if (streams && tiles > 1 && ok) {
-      ok = wait(&bar.k_full[1], 0);
+      ok = wait(&bar.k_full[1 % G::k_stages], 0);
       if (ok) {
         issue_s(1, 0);
         issue_s(1, 1);
@@ -697,10 +794,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
     }
     // both row tiles' weights of a half, then, while they are used up, their next scores in that half's place
     for (int it = 0; it < tiles && ok; ++it) {
-      ok = wait(&bar.v_full[it % G::stages], turn_of(it));
+      ok = wait(&bar.v_full[it % G::v_stages], v_turn(it));
       if (ok) issue_o(it, 0);
       if (it + ahead < tiles) {
-        ok = ok && wait(&bar.k_full[(it + ahead) % G::stages], turn_of(it + ahead));
+        ok = ok && wait(&bar.k_full[(it + ahead) % G::k_stages], k_turn(it + ahead));
         if (ok) issue_s(it + ahead, 0);
       }
       if (ok) issue_o(it, 1);
@@ -929,9 +1026,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       if (even) walk(std::true_type{}, sets);
       else walk(std::false_type{}, sets);
     };
-    if (kMode == kPass && G::row_tiles == 2 && spread == 8) walk_sets(std::integral_constant<int, kMode == kPass ? 1 : 4>{});
-    else if (kMode == kPass && G::row_tiles == 2 && spread == 16) walk_sets(std::integral_constant<int, kMode == kPass ? 2 : 4>{});
-    else walk_sets(std::integral_constant<int, 4>{});
+    if constexpr (G::narrow) {
+      if (spread == 8) walk_sets(std::integral_constant<int, 1>{});
+      else walk_sets(std::integral_constant<int, 2>{});
+    } else {
+      walk_sets(std::integral_constant<int, 4>{});
+    }
     if (my_tiles > 0) ok = __all_sync(0xFFFFFFFFu, ok && wait_for(&bar.p_free[x][1], (my_tiles - 1) & 1)) != 0;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
@@ -965,58 +1065,48 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
       for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float(f[j]));
     }
   };
-  if constexpr (kMode == kPass) {
-    float* const other = reinterpret_cast<float*>(smem);  // the second stream's O [channel][row]
-    auto load_mine = [&](int c0, uint32_t (&o)[16]) {  // whole warps: they load from tensor memory together, also for rows that there are not
-      if (my_tiles > 0 && ok) load_o(c0, o);
-      else
-#pragma unroll
-        for (int j = 0; j < 16; ++j) o[j] = 0u;
-    };
-    if (streams) {
-      if (mine && x > 0) {
-#pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += 16) {
-          uint32_t o[16];
-          load_mine(c0, o);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) other[(c0 + j) * kRowsX + row - kRowsX] = __uint_as_float(o[j]);
-        }
-      }
-      __syncthreads();
-    }
-    if (mine && !(streams && x > 0)) {
-      const int found = item_at(row);
-      const bool there = found >= 0;
-      const int i = i0 + max(found, 0), t = token_of(i), h = kvh * A.group + i - t * A.group;
-      const int64_t item = (static_cast<int64_t>(rank) * A.rows + row0 + t) * A.heads + h;
-      float total = totals[row], offset = offsets[row], ref = refs_of[row], f0 = 1.0f, f1 = 0.0f;
-      if (streams && totals[kRowsX + row] != 0.0f) {  // zero: the stream saw nothing for this row
-        const float theirs = refs_of[kRowsX + row], top = total == 0.0f ? theirs : fmaxf(ref, theirs);
-        f0 = total == 0.0f ? 0.0f : ex2(ref - top);
-        f1 = ex2(theirs - top);
-        total = fmaf(totals[kRowsX + row], f1, total * f0);
-        offset = fmaf(offsets[kRowsX + row], f1, offset * f0);
-        ref = top;
-      }
-      if (there) A.part_stats[item] = make_float2(ref, total);
+  if constexpr (kPass) {
+    // Both streams' O into shared memory, then a warp an item: its channels leave in one row.
+    float* const left = reinterpret_cast<float*>(smem);
+    if (mine) {  // whole warps: they load from tensor memory together, also for rows that there are not
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 16) {
         uint32_t o[16];
-        load_mine(c0, o);
-        float y[16];
+        if (my_tiles > 0 && ok) load_o(c0, o);
+        else
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          y[j] = f0 == 0.0f ? 0.0f : __uint_as_float(o[j]) * f0;
-          if (f1 != 0.0f) y[j] = fmaf(other[(c0 + j) * kRowsX + row], f1, y[j]);
-          y[j] = fmaf(y[j], 1.0f / kWeightUnit, offset);
-        }
-        if (there && total != 0.0f) {
-          float4* const to = reinterpret_cast<float4*>(A.part_values + item * D + c0);
+          for (int j = 0; j < 16; ++j) o[j] = 0u;
+        uint4* const to = reinterpret_cast<uint4*>(left + x * G::leave_stream + (row & (kRowsX - 1)) * G::leave_row + c0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) to[j] = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
-        }
+        for (int j = 0; j < 4; ++j) to[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
       }
+    }
+    __syncthreads();
+    constexpr int n = D / 32;  // channels of a lane
+    for (int i = warp; i < live; i += prompt_threads(kMode) / 32) {
+      const int r = i / spread * 32 + i % spread;
+      float total = totals[r], offset = offsets[r], ref = refs_of[r], f0 = total == 0.0f ? 0.0f : 1.0f, f1 = 0.0f;
+      if (streams && totals[kRowsX + r] != 0.0f) {  // zero: the stream saw nothing for this row
+        const float theirs = refs_of[kRowsX + r], top = total == 0.0f ? theirs : fmaxf(ref, theirs);
+        f0 = total == 0.0f ? 0.0f : ex2(ref - top);
+        f1 = ex2(theirs - top);
+        total = f0 == 0.0f ? totals[kRowsX + r] * f1 : fmaf(totals[kRowsX + r], f1, total * f0);
+        offset = f0 == 0.0f ? offsets[kRowsX + r] * f1 : fmaf(offsets[kRowsX + r], f1, offset * f0);
+        ref = top;
+      }
+      const int t = token_of(i0 + i), h = kvh * A.group + i0 + i - t * A.group;
+      const int64_t item = (static_cast<int64_t>(rank) * A.rows + row0 + t) * A.heads + h;
+      if (lane == 0) A.part_stats[item] = make_float2(ref, total);
+      if (total == 0.0f) continue;
+      const float* const from = left + (r / kRowsX) * G::leave_stream + r % kRowsX * G::leave_row + n * lane;
+      float y[n];
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        y[j] = f0 == 0.0f ? 0.0f : from[j] * f0;
+        if (streams && f1 != 0.0f) y[j] = fmaf(from[G::leave_stream + j], f1, y[j]);
+        y[j] = fmaf(y[j], 1.0f / kWeightUnit, offset);
+      }
+      store_values<float, n>(A.part_values + item * D + n * lane, true, y);
     }
   } else if (C == 1) {
     if (mine) {
@@ -1127,7 +1217,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(Kv4Attent
 // Opt-in shared memory, once per device.
 template <int D, typename T, PromptMode kMode>
 int32_t allow_prompt() {
-  using G = PromptGeometry<D, std::is_same<T, float>::value, kMode == kPass>;
+  using G = PromptGeometry<D, std::is_same<T, float>::value, kMode>;
   static std::atomic<uint64_t> done{0};
   int device = 0;
   IVB_CUDA(cudaGetDevice(&device));
@@ -1141,7 +1231,7 @@ int32_t allow_prompt() {
 
 template <int D, typename T, PromptMode kMode>
 int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
-  using G = PromptGeometry<D, std::is_same<T, float>::value, false>;
+  using G = PromptGeometry<D, std::is_same<T, float>::value, kMode>;
   if (int32_t rc = allow_prompt<D, T, kMode>()) return rc;
   // as many tiles as the rows can make: each sequence of the call may leave one unfilled
   const int64_t items = static_cast<int64_t>(A.rows) * A.group;
@@ -1155,7 +1245,7 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   while (C < 4 && tiles * A.cache.kv_heads * C < 148 && most > 2 * C * kPos) C *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * A.cache.kv_heads * C));
-  cfg.blockDim = dim3(kPromptThreads);
+  cfg.blockDim = dim3(prompt_threads(kMode));
   cfg.dynamicSmemBytes = G::smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -1165,22 +1255,27 @@ int32_t launch_prompts(const Kv4Attention& A, int few, cudaStream_t stream) {
   return IVB_OK;
 }
 
-template <int D, typename T>
+// Whether a pass is narrow: the rows of a group, if they are spread evenly over the groups, are 64 at most.
+bool narrow_pass(const IvbKv4Cache& prefix, int group, int rows) {
+  return static_cast<int64_t>(rows) * group <= kNarrowRows * static_cast<int64_t>(std::min(prefix.batch, rows));
+}
+
+template <int D, typename T, PromptMode kMode>
 int32_t launch_prefix(const Kv4Attention& A, int few, cudaStream_t stream) {
-  using G = PromptGeometry<D, std::is_same<T, float>::value, true>;
-  if (int32_t rc = allow_prompt<D, T, kPass>()) return rc;
+  using G = PromptGeometry<D, std::is_same<T, float>::value, kMode>;
+  if (int32_t rc = allow_prompt<D, T, kMode>()) return rc;
   // as many tiles as the rows can make: each group may leave one unfilled
   const int64_t tiles = static_cast<int64_t>(A.rows) * A.group / G::rows + std::min<int64_t>(A.prefix.batch, A.rows);
   // the parts fill 148 CTAs at most, but for groups whose share is below one
   const int64_t grid = tiles * A.cache.kv_heads + (A.splits > 1 ? 148 : 0);
   if (grid > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(tiles));
-  IVB_CUDA(launch_pdl(kv4_prompt_kernel<D, T, kPass>, dim3(static_cast<unsigned>(grid)), dim3(kPromptThreads), G::smem, stream, A, few));
+  IVB_CUDA(launch_pdl(kv4_prompt_kernel<D, T, kMode>, dim3(static_cast<unsigned>(grid)), dim3(prompt_threads(kMode)), G::smem, stream, A, few));
   return IVB_OK;
 }
 
 template <int D, typename T>
 int32_t launch_mode(const Kv4Attention& A, bool pass, int few, cudaStream_t stream) {
-  if (pass) return launch_prefix<D, T>(A, few, stream);
+  if (pass) return narrow_pass(A.prefix, A.group, A.rows) ? launch_prefix<D, T, kNarrow>(A, few, stream) : launch_prefix<D, T, kWide>(A, few, stream);
   return A.prefix.data == nullptr ? launch_prompts<D, T, kPlain>(A, few, stream) : launch_prompts<D, T, kBehind>(A, few, stream);
 }
 
@@ -1206,9 +1301,9 @@ int32_t launch_kv4_prefix(const Kv4Attention& A, int32_t dtype, int few, cudaStr
 
 // Parts of the prefix: how many CTAs may share a row tile and head at most. As many as fill the SMs if the rows are spread evenly over the
 // groups, twice as many where there are several, so that a long beginning can have more than a short one.
-int kv4_prefix_splits(const IvbKv4Cache& cache, const IvbKv4Cache& prefix, int32_t dtype, int group, int rows) {
-  const int per_tile = dtype == IVB_F32 && cache.head_dim == 128 ? kRowsX : kRowsCta;
+int kv4_prefix_splits(const IvbKv4Cache& cache, const IvbKv4Cache& prefix, int group, int rows) {
   const int64_t groups = std::min(prefix.batch, rows), items = (static_cast<int64_t>(rows) * group + groups - 1) / groups;
+  const int64_t per_tile = narrow_pass(prefix, group, rows) ? kNarrowRows : kRowsCta;
   const int64_t units = groups * ((items + per_tile - 1) / per_tile) * cache.kv_heads;
   const int64_t most = std::min<int64_t>(kMostSplits, (static_cast<int64_t>(prefix.max_len) + kPos - 1) / kPos);
   return static_cast<int>(std::max<int64_t>(1, std::min(most, (groups > 1 ? 296 : 148) / units)));
