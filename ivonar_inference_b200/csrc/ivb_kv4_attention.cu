@@ -702,13 +702,14 @@ int few_items(const IvbKv4Cache& c, int group, const int32_t* starts, int rows) 
   return starts == nullptr || items <= few ? 0x7fffffff : c.batch == 1 ? 0 : few;
 }
 
-// Whether few rows walk the beginning that they share each on their own, in one kernel, where that is less than a pass over it.
-#ifndef IVB_WALK
-#define IVB_WALK 300000
-#endif
+// Whether few rows walk the beginning that they share each on their own, in one kernel, where that is less than a pass over it (whose
+// kernel takes 9 us at least): by row tiles x heads x its positions. Measured, walked / passed, us: 16 sequences x 16 heads x 64 in fp32,
+// 256k 10 / 18, 640k 17 / 18, 1,536k 33 / 22; 64 x 16 x 64 in bf16, 410k 20 / 19, 1,024k 30 / 18; 8 x 8 heads x 4 x 128, 160k 14 / 21,
+// 384k 19 / 22; 64 x 8 x 4 x 128, 204k 19 / 29, 512k 29 / 31, 1,280k 50 / 33; 32 x 8 x 32, 640k 13 / 16, 1,536k 24 / 17.
+constexpr int64_t kWalkReach = 500000;
 bool walks_prefix(const IvbKv4Cache& c, const IvbKv4Cache& prefix, int group, int rows) {
   const int64_t tiles = std::max<int64_t>(std::min(rows, c.batch), static_cast<int64_t>(rows) * group / 8);
-  return tiles * c.kv_heads * prefix.max_len <= IVB_WALK;
+  return tiles * c.kv_heads * prefix.max_len <= kWalkReach;
 }
 
 // Bytes of the parts of a shared beginning: for each split, row and head its statistics and its values.

@@ -5,9 +5,9 @@
 // lanes, warps, the CTAs of a cluster that share a row, and the ranks that share a vocabulary. Differences are taken before they
 // are scaled, so that a row of the type's lowest value is the uniform distribution that it stands for.
 //
-// The `top` largest ride along: after a CTA's first 4096 values the top-th largest of its threads' maxima bounds them from
-// below, what lies above is noted in shared memory (a test of each thread's maximum of 16, which the sums need anyway), and only
-// those few are ranked. Values are compared as they came, ties by the token, through one 64-bit key; NaN counts as -inf there.
+// The `top` largest ride along: a CTA's first 4096 values give a bound below which none of them is, what lies above is noted in shared
+// memory (a test of each thread's maximum of 16, which the sums need anyway), and only those few are ranked. Values are compared as
+// they came, ties by the token, through one 64-bit key; NaN counts as -inf there.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "ivb_common.h"
 #include "ivb_device.cuh"
@@ -26,7 +27,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kLogThreads = 256, kMostTop = 256, kBatch = 16;  // values of a thread at a time
-constexpr int kSpan = kLogThreads * kBatch, kNoted = kSpan + 1024;
+constexpr int kWarps = kLogThreads / 32, kSpan = kLogThreads * kBatch;
+constexpr int kSlack = 96, kRoom = 32 * kBatch + kSlack;  // a warp's list: one turn's values and what it had before
 constexpr int kRankAll = 512;  // so many are ranked each against all; more are first cut to the largest `top`
 constexpr unsigned kAbsent = 0x7fffffffu;  // of a slice that does not hold the token
 constexpr float kLeast = -200.0f;  // 2^-200 is zero in fp32: keeps -inf * 0 out of the third sum
@@ -76,53 +78,95 @@ __device__ __forceinline__ Stats join(Stats a, Stats b, float c) {
   return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// The largest keys so far in order (`have` of them, zeros behind), and what each warp has noted since.
 struct Shared {
-  Key noted[kNoted];
-  Key best[kMostTop], cut[kMostTop];
-  uint32_t maxima[kLogThreads];
-  Stats warps[kLogThreads / 32], all;
-  int count, found;
-  float bound;
-  int counts[2];
+  Key noted[kWarps][kRoom];
+  alignas(16) Key list[kRankAll];
+  Key best[kMostTop];
+  Stats warps[kWarps], all;
+  float bounds[kWarps];
+  int counts[kWarps], have, found, over, reached[2];
 };
 
-// The `top` largest of noted[0, n) into best[0, top), descending, zeros behind them. All threads; barriers on both sides.
-__device__ void rank_keys(Shared& sh, int n, int top) {
+// Ranks the best and all that is noted: the `top` largest become the best, nothing is noted then. All threads; barriers on both sides.
+__device__ void rank_keys(Shared& sh, int top) {
   const int tid = threadIdx.x;
-  const Key* from = sh.noted;
   __syncthreads();
-  if (n > kRankAll) {
+  const int have = sh.have;
+  int n = have, before = have;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    before += w < (tid >> 5) ? sh.counts[w] : 0;
+    n += sh.counts[w];
+  }
+  auto each = [&](auto f) {
+    for (int i = tid; i < have; i += kLogThreads) f(sh.best[i]);
+    for (int w = 0; w < kWarps; ++w)
+      for (int i = tid; i < sh.counts[w]; i += kLogThreads) f(sh.noted[w][i]);
+  };
+  if (n <= kRankAll) {
+    for (int i = tid; i < have; i += kLogThreads) sh.list[i] = sh.best[i];
+    for (int i = tid & 31; i < sh.counts[tid >> 5]; i += 32) sh.list[before + i] = sh.noted[tid >> 5][i];
+  } else {
     // the top-th largest key, bit by bit: the largest value that at least `top` keys reach
     Key at = 0;
-    if (tid < 2) sh.counts[tid] = 0;
+    if (tid < 2) sh.reached[tid] = 0;
+    if (tid == 2) sh.found = 0;
     __syncthreads();
     for (int bit = 63; bit >= 0; --bit) {
       const Key trial = at | Key(1) << bit;
       int mine = 0;
-      for (int i = tid; i < n; i += kLogThreads) mine += sh.noted[i] >= trial;
+      each([&](Key k) { mine += k >= trial; });
       mine = __reduce_add_sync(0xFFFFFFFFu, mine);
-      if ((tid & 31) == 0 && mine != 0) atomicAdd(&sh.counts[bit & 1], mine);
+      if ((tid & 31) == 0 && mine != 0) atomicAdd(&sh.reached[bit & 1], mine);
       __syncthreads();
-      if (sh.counts[bit & 1] >= top) at = trial;
-      if (tid == 0) sh.counts[(bit & 1) ^ 1] = 0;
+      if (sh.reached[bit & 1] >= top) at = trial;
+      if (tid == 0) sh.reached[(bit & 1) ^ 1] = 0;
       __syncthreads();
     }
-    if (tid == 0) sh.found = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kLogThreads)
-      if (sh.noted[i] >= at) sh.cut[atomicAdd(&sh.found, 1)] = sh.noted[i];  // keys differ: `top` of them
-    __syncthreads();
-    from = sh.cut;
+    each([&](Key k) {
+      if (k >= at) sh.list[atomicAdd(&sh.found, 1)] = k;  // keys differ: `top` of them
+    });
     n = top;
   }
-  for (int i = tid; i < n; i += kLogThreads) {
-    const Key k = from[i];
+  __syncthreads();
+  // each key against all, by 1 to 8 neighbouring lanes
+  const int lanes = n <= 32 ? 8 : n <= 64 ? 4 : n <= 128 ? 2 : 1, l = tid & (lanes - 1);
+  for (int i0 = 0; i0 < n; i0 += kLogThreads / lanes) {
+    const int i = i0 + tid / lanes;
+    const Key k = i < n ? sh.list[i] : 0;
     int above = 0;
-    for (int j = 0; j < n; ++j) above += from[j] > k;
-    if (above < top) sh.best[above] = k;
+#pragma unroll 4
+    for (int j = 2 * l; j + 1 < n; j += 2 * lanes) {
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(sh.list + j);
+      above += (two.x > k) + (two.y > k);
+    }
+    if ((n & 1) != 0 && l == 0) above += sh.list[n - 1] > k;
+    for (int d = 1; d < lanes; d <<= 1) above += __shfl_xor_sync(0xFFFFFFFFu, above, d);
+    if (i < n && l == 0 && above < top) sh.best[above] = k;
   }
   for (int i = n + tid; i < top; i += kLogThreads) sh.best[i] = 0;
+  if (tid < kWarps) sh.counts[tid] = 0;
+  if (tid == kWarps) sh.have = min(n, top);
   __syncthreads();
+}
+
+// Notes up to `top` keys of an ordered list that ends in zeros; a whole warp, its own list is empty.
+__device__ __forceinline__ void note_list(Shared& sh, int warp, int top, Key key_at(const void*, int, int), const void* from) {
+  const int lane = threadIdx.x & 31;
+  int count = 0;
+  for (int i0 = 0; i0 < top; i0 += 32) {
+    const Key k = i0 + lane < top ? key_at(from, i0 + lane, top) : 0;
+    if (k != 0) sh.noted[warp][i0 + lane] = k;
+    count += __popc(__ballot_sync(0xFFFFFFFFu, k != 0));
+  }
+  if (lane == 0) sh.counts[warp] = count;
 }
 
 // What one row's sums and largest keys say; all threads of a CTA.
@@ -159,98 +203,154 @@ __global__ void __launch_bounds__(kLogThreads, 4) log_probs_kernel(LogProbs p) {
   const int chunks = static_cast<int>((static_cast<int64_t>(shift) + p.vocab + E - 1) / E), per = (chunks + C - 1) / C;
   const int c0 = min(rank * per, chunks), c1 = min(c0 + per, chunks), turns = (c1 - c0 + kLogThreads * U - 1) / (kLogThreads * U);
   const float c = p.inv_t * 1.4426950408889634f;
-  auto first_of = [&](int chunk) { return static_cast<int64_t>(chunk) * E - shift; };
+  // Chunk c0 + (256 u + tid) of a turn; chunks from `whole0` to `whole1` lie in the row with all their values, as those of nearly all turns do.
+  const uint4* at = reinterpret_cast<const uint4*>(x - shift) + c0 + tid;
+  const int whole0 = shift > 0 ? 1 : 0, whole1 = min(c1, static_cast<int>((static_cast<int64_t>(shift) + p.vocab) / E));
+  constexpr int kTurn = kLogThreads * U;
   auto load = [&](int turn, uint4 (&to)[U]) {
+    const int first = c0 + turn * kTurn;
+    if (first >= whole0 && first + kTurn <= whole1) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t chunk = static_cast<int64_t>(c0) + (static_cast<int64_t>(turn) * U + u) * kLogThreads + tid;
-      const int64_t i0 = chunk * E - shift;
-      if (chunk < c1 && i0 >= 0 && i0 + E <= p.vocab) {
-        to[u] = __ldcs(reinterpret_cast<const uint4*>(x + i0));
-      } else {
+      for (int u = 0; u < U; ++u) to[u] = __ldcs(at + u * kLogThreads);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int chunk = first + u * kLogThreads + tid;
         union {
           uint4 w;
           T t[E];
         } e;
+        if (chunk >= whole0 && chunk < whole1) {
+          e.w = __ldcs(at + u * kLogThreads);
+        } else {
+          const int64_t i0 = static_cast<int64_t>(chunk) * E - shift;
 #pragma unroll
-        for (int i = 0; i < E; ++i) e.t[i] = chunk < c1 && i0 + i >= 0 && i0 + i < p.vocab ? x[i0 + i] : from_f32<T>(-INFINITY);
+          for (int i = 0; i < E; ++i) e.t[i] = chunk < c1 && i0 + i >= 0 && i0 + i < p.vocab ? x[i0 + i] : from_f32<T>(-INFINITY);
+        }
         to[u] = e.w;
       }
     }
+    at += kTurn;
   };
-  Stats mine = {-INFINITY, 0.0f, 0.0f};
+  // the row's first 256 tokens' logits are on their way meanwhile
+  const float first_logit = rank == 0 && tid < p.given ? logit_of_token<T>(p, row, tid) : 0.0f;
+  float m = -INFINITY;
+  float2 s2 = make_float2(0.0f, 0.0f), t2 = s2;  // of even and of odd values
   float bound = -INFINITY;
-  if (kTop && tid == 0) sh.count = 0;
+  int noted = 0;  // by this warp, since the last ranking
+  if (kTop && tid == 0) sh.have = sh.over = 0;
   uint4 next[U];
+  // What is noted is ranked, and the bound raised to the top-th largest, after the turns 0, 1, 3, 7, ...: between them warps need not wait
+  // for one another. A row that notes more than there is room for (one in ascending order does) is read again, and ranked after every turn.
+  bool careful = false;
+  const uint4* const begin = at;
+scan:
   if (turns > 0) load(0, next);
   for (int turn = 0; turn < turns; ++turn) {
     float v[kBatch];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      union {
-        uint4 w;
-        T t[E];
-      } e;
-      e.w = next[u];
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const uint32_t w[4] = {next[u].x, next[u].y, next[u].z, next[u].w};
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[u * E + i] = to_f32<T>(e.t[i]);
+        for (int i = 0; i < 4; ++i) {
+          v[u * E + 2 * i] = __uint_as_float(w[i] << 16);
+          v[u * E + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+      } else {
+        union {
+          uint4 w;
+          T t[E];
+        } e;
+        e.w = next[u];
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[u * E + i] = to_f32<T>(e.t[i]);
+      }
     }
     if (turn + 1 < turns) load(turn + 1, next);
-    float most = v[0];
+    float most = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < kBatch; ++i) most = fmaxf(most, v[i]);
-    most = fmaxf(most, -INFINITY);  // 16 NaN
-    if (most > mine.m) mine = join(mine, {most, 0.0f, 0.0f}, c);
-    const float m = mine.m == -INFINITY ? 0.0f : mine.m;
+    for (int i = 0; i < kBatch; i += 2) most = max3(most, v[i], v[i + 1]);
+    if (most > m) {
+      const float d = fmaxf((m - most) * c, kLeast), f = exp2_of(d);  // from nothing: sums of zero
+      t2 = make_float2(fmaf(s2.x, d, t2.x) * f, fmaf(s2.y, d, t2.y) * f);
+      s2 = make_float2(s2.x * f, s2.y * f);
+      m = most;
+    }
+    const float minus = m == -INFINITY ? 0.0f : -m;
+    const float2 minus2 = make_float2(minus, minus), c2 = make_float2(c, c);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const float d = (v[i] - m) * c, e = exp2_of(d);
-      mine.s += e;
-      mine.t = fmaf(fmaxf(d, kLeast), e, mine.t);
+    for (int i = 0; i < kBatch; i += 2) {
+      const float2 d = __fmul2_rn(__fadd2_rn(make_float2(v[i], v[i + 1]), minus2), c2), e = make_float2(exp2_of(d.x), exp2_of(d.y));
+      s2 = __fadd2_rn(s2, e);
+      t2 = __ffma2_rn(make_float2(fmaxf(d.x, kLeast), fmaxf(d.y, kLeast)), e, t2);
     }
     if constexpr (kTop) {
-      auto note = [&](bool all) {
+      // notes the values above the bound (or from it on, NaN too; a bound of -inf also takes places that are none), value after value
+      auto note = [&](auto from_it, auto checked) {
+        constexpr bool kFrom = decltype(from_it)::value, kChecked = decltype(checked)::value;
+        const uint32_t first = static_cast<uint32_t>((static_cast<int64_t>(c0) + turn * kTurn + tid) * E - shift);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int i = 0; i < E; ++i) {
-            const int chunk = c0 + (turn * U + u) * kLogThreads + tid;
-            const int64_t id = first_of(chunk) + i;
-            const float y = v[u * E + i] == v[u * E + i] ? v[u * E + i] : -INFINITY;
-            if (chunk < c1 && id >= 0 && id < p.vocab && (all ? y >= bound : y > bound))
-              sh.noted[atomicAdd(&sh.count, 1)] = key_of(ordered(y), static_cast<uint32_t>(id + p.v0));
+        for (int i = 0; i < kBatch; ++i) {
+          const uint32_t id = first + (i / E * kLogThreads * E + i % E);  // wraps below zero
+          bool in = kFrom ? !(v[i] < bound) : v[i] > bound;
+          if constexpr (kChecked) in = in && c0 + turn * kTurn + i / E * kLogThreads + tid < c1 && id < static_cast<uint32_t>(p.vocab);
+          const unsigned who = __ballot_sync(0xFFFFFFFFu, in);
+          if (who != 0) {
+            const int to = noted + __popc(who & ((1u << lane) - 1));
+            if (in && to < kRoom) sh.noted[warp][to] = key_of(ordered(v[i]), id + static_cast<uint32_t>(p.v0));
+            noted += __popc(who);
           }
+        }
+        if (noted > kRoom) {
+          noted = kRoom;
+          if (lane == 0) sh.over = 1;
+        }
       };
       if (turn == 0) {
-        sh.maxima[tid] = ordered(most);
-        __syncthreads();
-        int above = 0;
-        const uint32_t own = sh.maxima[tid];
-        for (int j = 0; j < kLogThreads; j += 4) {
-          const uint4 o = *reinterpret_cast<const uint4*>(sh.maxima + j);
-          above += (o.x > own || (o.x == own && j < tid)) + (o.y > own || (o.y == own && j + 1 < tid)) + (o.z > own || (o.z == own && j + 2 < tid)) +
-                   (o.w > own || (o.w == own && j + 3 < tid));
+        // each warp's r-th largest of its lanes' maxima, with r = top / 8 rounded up: `top` values at least reach the least of these.
+        // (The top-th largest of all 256, each ranked against all, is a closer bound, but took 1.6 us of each CTA.)
+        uint32_t own = ordered(most), reached = 0;
+        for (int r = 0; r < p.top; r += kWarps) {
+          reached = __reduce_max_sync(0xFFFFFFFFu, own);
+          const unsigned who = __ballot_sync(0xFFFFFFFFu, own == reached);
+          if (lane == __ffs(who) - 1) own = 0;
         }
-        if (above == p.top - 1) sh.bound = most;
+        if (lane == 0) sh.bounds[warp] = unordered(reached);
         __syncthreads();
-        bound = sh.bound;
-        if (most >= bound) note(true);
-      } else if (most > bound) {
-        note(false);  // later tokens: as large as the bound is too late
+        bound = sh.bounds[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) bound = fminf(bound, sh.bounds[w]);
+        if (bound == -INFINITY) note(std::true_type{}, std::true_type{});
+        else if (__any_sync(0xFFFFFFFFu, !(most < bound))) note(std::true_type{}, std::false_type{});
+      } else if (__any_sync(0xFFFFFFFFu, most > bound)) {
+        note(std::false_type{}, std::false_type{});  // later tokens: as large as the bound is too late
       }
-      if (turn + 1 < turns) {
-        __syncthreads();
-        const int n = sh.count;
-        if (n > kNoted - kSpan) {  // the next turn could note more than there is room for
-          rank_keys(sh, n, p.top);
-          for (int i = tid; i < p.top; i += kLogThreads) sh.noted[i] = sh.best[i];
-          bound = unordered(static_cast<uint32_t>(sh.best[p.top - 1] >> 32));
-          if (tid == 0) sh.count = p.top;
-          __syncthreads();
-        }
+      if (turn + 1 < turns && (careful || (turn & (turn + 1)) == 0)) {
+        if (lane == 0) sh.counts[warp] = noted;
+        noted = 0;
+        rank_keys(sh, p.top);
+        if (sh.have == p.top) bound = unordered(static_cast<uint32_t>(sh.best[p.top - 1] >> 32));
       }
     }
   }
+  if constexpr (kTop) {
+    if (lane == 0) sh.counts[warp] = noted;
+    __syncthreads();
+    const bool again = sh.over != 0;  // never when careful: a turn's values find room
+    __syncthreads();
+    if (again) {
+      if (tid == 0) sh.over = sh.have = 0;
+      careful = true;
+      noted = 0;
+      at = begin;
+      m = bound = -INFINITY;
+      s2 = t2 = make_float2(0.0f, 0.0f);
+      __syncthreads();
+      goto scan;
+    }
+  }
+  Stats mine = {m, s2.x + s2.y, t2.x + t2.y};
   // over lanes, warps and the cluster
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1)
@@ -259,29 +359,24 @@ __global__ void __launch_bounds__(kLogThreads, 4) log_probs_kernel(LogProbs p) {
   __syncthreads();
   Stats all = sh.warps[0];
 #pragma unroll
-  for (int w = 1; w < kLogThreads / 32; ++w) all = join(all, sh.warps[w], c);
-  if constexpr (kTop) rank_keys(sh, sh.count, p.top);
+  for (int w = 1; w < kWarps; ++w) all = join(all, sh.warps[w], c);
+  if constexpr (kTop) rank_keys(sh, p.top);
   if (C > 1) {
     if (tid == 0) sh.all = all;
     cluster.sync();
     if (rank == 0) {
       for (int k = 1; k < C; ++k) all = join(all, cluster.map_shared_rank(&sh, k)->all, c);
       if constexpr (kTop) {
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        for (int i = tid; i < C * p.top; i += kLogThreads) {
-          const Key k = cluster.map_shared_rank(&sh, i / p.top)->best[i % p.top];
-          if (k != 0) sh.noted[atomicAdd(&sh.count, 1)] = k;
-        }
-        __syncthreads();
-        rank_keys(sh, sh.count, p.top);
+        if (warp > 0 && warp < C)
+          note_list(sh, warp, p.top, [](const void* from, int i, int) { return static_cast<const Key*>(from)[i]; }, cluster.map_shared_rank(&sh, warp)->best);
+        rank_keys(sh, p.top);
       }
     }
     cluster.sync();  // no CTA leaves while another reads its shared memory
     if (rank != 0) return;
   }
   if (p.parts == nullptr) {
-    finish(p, sh, all, row, [&](int i) { return logit_of_token<T>(p, row, i); });
+    finish(p, sh, all, row, [&](int i) { return i == tid ? first_logit : logit_of_token<T>(p, row, i); });
     return;
   }
   uint32_t* const out = p.parts + row * (3 + p.given + 2 * p.top);
@@ -290,7 +385,7 @@ __global__ void __launch_bounds__(kLogThreads, 4) log_probs_kernel(LogProbs p) {
     out[1] = __float_as_uint(all.s);
     out[2] = __float_as_uint(all.t);
   }
-  for (int i = tid; i < p.given; i += kLogThreads) out[3 + i] = __float_as_uint(logit_of_token<T>(p, row, i));
+  for (int i = tid; i < p.given; i += kLogThreads) out[3 + i] = __float_as_uint(i == tid ? first_logit : logit_of_token<T>(p, row, i));
   for (int i = tid; i < p.top; i += kLogThreads) {
     out[3 + p.given + i] = static_cast<uint32_t>(sh.best[i] >> 32);
     out[3 + p.given + p.top + i] = id_of(sh.best[i]);
@@ -309,21 +404,16 @@ __global__ void __launch_bounds__(kLogThreads) log_probs_merge_kernel(LogProbs p
   for (int w = 0; w < world; ++w)
     all = join(all, {__uint_as_float(part[w * step]), __uint_as_float(part[w * step + 1]), __uint_as_float(part[w * step + 2])}, c);
   if (p.top > 0) {
-    int have = 0;
-    for (int w0 = 0; w0 < world;) {
-      const int n = min(world - w0, (kNoted - have) / p.top);
-      if (tid == 0) sh.count = have;
-      __syncthreads();
-      for (int i = tid; i < n * p.top; i += kLogThreads) {
-        const uint32_t* from = part + (w0 + i / p.top) * step + 3 + p.given + i % p.top;
-        if (from[0] != 0) sh.noted[atomicAdd(&sh.count, 1)] = key_of(from[0], from[p.top]);
-      }
-      __syncthreads();
-      have = min(sh.count, p.top);
-      rank_keys(sh, sh.count, p.top);
-      for (int i = tid; i < p.top; i += kLogThreads) sh.noted[i] = sh.best[i];
-      w0 += n;
-      __syncthreads();
+    const int warp = tid >> 5;
+    if (tid == 0) sh.have = 0;
+    for (int w0 = 0; w0 < world; w0 += kWarps) {  // a warp a slice's list
+      if (w0 + warp < world)
+        note_list(sh, warp, p.top, [](const void* from, int i, int top) {
+          const uint32_t* const list = static_cast<const uint32_t*>(from);
+          return list[i] == 0 ? Key(0) : key_of(list[i], list[top + i]);
+        }, part + (w0 + warp) * step + 3 + p.given);
+      else if ((tid & 31) == 0) sh.counts[warp] = 0;
+      rank_keys(sh, p.top);
     }
   }
   finish(p, sh, all, row, [&](int i) {
@@ -348,7 +438,7 @@ template <typename T, bool kTop>
 int32_t launch(const LogProbs& p, int rows, cudaStream_t stream) {
   // a cluster a row where the rows alone leave places on the GPU's SMs, four CTAs each, and the parts are a turn at least
   int C = 1;
-  while (C < 8 && static_cast<int64_t>(rows) * C < 148 * 4 && static_cast<int64_t>(C) * kSpan < p.vocab) C *= 2;
+  while (C < 8 && static_cast<int64_t>(rows) * C * 2 <= 148 * 4 && static_cast<int64_t>(C) * kSpan < p.vocab) C *= 2;
   if (static_cast<int64_t>(rows) * C > 0x7fffffff) return fail(IVB_EINVAL, "ivb_log_probs: %d rows in one call", rows);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * C));

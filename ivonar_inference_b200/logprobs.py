@@ -59,11 +59,20 @@ def _check(logits: Tensor, tokens: Tensor, top: int, temperature: float) -> tupl
     return rows, given
 
 
+def _call(what: str, index: int, *args) -> None:
+    function = getattr(native.library(), what)
+    if torch.cuda.current_device() == index:
+        rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    native.check(rc, what)
+
+
 def _empty(logits: Tensor, tokens: Tensor, top: int) -> LogProbs:
-    rows = logits.shape[0]
-    new = logits.new_empty
-    return LogProbs(new(tokens.shape, dtype=torch.float32), new((rows,), dtype=torch.float32), new((rows, top), dtype=torch.float32),
-                    new((rows, top), dtype=torch.int64))
+    rows, device, empty = logits.shape[0], logits.device, torch.empty
+    return LogProbs(empty(tokens.shape, dtype=torch.float32, device=device), empty(rows, dtype=torch.float32, device=device),
+                    empty(rows, top, dtype=torch.float32, device=device), empty(rows, top, dtype=torch.int64, device=device))
 
 
 def log_probs(logits: Tensor, tokens: Tensor, top: int = 0, temperature: float = 1.0) -> LogProbs:
@@ -78,12 +87,8 @@ def log_probs(logits: Tensor, tokens: Tensor, top: int = 0, temperature: float =
     if top > logits.shape[1]:
         raise ValueError(f"top {top} of a vocabulary of {logits.shape[1]}")
     out = _empty(logits, tokens, top)
-    with torch.cuda.device(logits.device):
-        rc = native.library().ivb_log_probs(
-            logits.data_ptr(), _TYPES[logits.dtype], rows, logits.shape[1], logits.stride(0), tokens.data_ptr(), given, temperature, top,
-            out.tokens.data_ptr(), out.entropy.data_ptr(), out.top.data_ptr(), out.ids.data_ptr(),
-            torch.cuda.current_stream(logits.device).cuda_stream)
-    native.check(rc, "ivb_log_probs")
+    _call("ivb_log_probs", logits.device.index, logits.data_ptr(), _TYPES[logits.dtype], rows, logits.shape[1], logits.stride(0), tokens.data_ptr(),
+          given, temperature, top, *(x.data_ptr() for x in out))
     return out
 
 
@@ -94,11 +99,8 @@ def log_probs_slice(logits: Tensor, tokens: Tensor, v0: int, top: int = 0, tempe
     if not 0 <= v0 < 2**31 - logits.shape[1]:
         raise ValueError(f"{logits.shape[1]} tokens from {v0} on")
     parts = logits.new_empty((rows, 3 + given + 2 * top), dtype=torch.int32)
-    with torch.cuda.device(logits.device):
-        rc = native.library().ivb_log_probs_slice(
-            logits.data_ptr(), _TYPES[logits.dtype], rows, logits.shape[1], v0, logits.stride(0), tokens.data_ptr(), given, temperature, top,
-            parts.data_ptr(), torch.cuda.current_stream(logits.device).cuda_stream)
-    native.check(rc, "ivb_log_probs_slice")
+    _call("ivb_log_probs_slice", logits.device.index, logits.data_ptr(), _TYPES[logits.dtype], rows, logits.shape[1], v0, logits.stride(0),
+          tokens.data_ptr(), given, temperature, top, parts.data_ptr())
     return parts
 
 
@@ -114,9 +116,5 @@ def log_probs_merge(parts: Tensor, tokens: Tensor, top: int = 0, temperature: fl
     if not 0 <= top <= MOST_TOP or not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"top {top}, temperature {temperature}")
     out = _empty(parts[0], tokens, top)
-    with torch.cuda.device(parts.device):
-        rc = native.library().ivb_log_probs_merge(
-            parts.data_ptr(), parts.shape[0], rows, given, temperature, top, out.tokens.data_ptr(), out.entropy.data_ptr(), out.top.data_ptr(),
-            out.ids.data_ptr(), torch.cuda.current_stream(parts.device).cuda_stream)
-    native.check(rc, "ivb_log_probs_merge")
+    _call("ivb_log_probs_merge", parts.device.index, parts.data_ptr(), parts.shape[0], rows, given, temperature, top, *(x.data_ptr() for x in out))
     return out
