@@ -32,30 +32,34 @@ __device__ __forceinline__ int kv4_position_of_word(int w) {
 }
 
 constexpr int kForkThreads = 512, kForkPer = 8;  // 16-byte pieces of a thread at a time
+constexpr int kForkPieces = kForkThreads * kForkPer;
 
-// A CTA takes pieces of a run of `across` x 16 bytes of one head at the same place of every sequence, kForkThreads * kForkPer
-// at a time: read all, a barrier, write all. In one cache `batch` x `across` pieces fit that, so whatever sequence another's
-// beginning comes from is read before any of its bytes at that place is written, in any permutation and without a copy elsewhere.
+// A CTA takes runs of `across` (a power of two) pieces of one head at the same place of every sequence, kForkPieces at a time: read all,
+// a barrier, write all. In one cache `batch` x `across` pieces fit that, so whatever sequence another's beginning comes from is read
+// before any of its bytes at that place is written, in any permutation and without a copy elsewhere. Two CTAs an SM: one reads while
+// the other writes.
 template <int D>
-__global__ void __launch_bounds__(kForkThreads) kv4_fork_kernel(IvbKv4Cache to, IvbKv4Cache from, const int64_t* sources,
-                                                                const int64_t* lengths, int across, uint32_t* error) {
-  constexpr int kTile = kv4_tile_bytes(D), kPieces = kTile / 16;  // of a tile
+__global__ void __launch_bounds__(kForkThreads, 2) kv4_fork_kernel(IvbKv4Cache to, IvbKv4Cache from, const int64_t* sources,
+                                                                   const int64_t* lengths, int across_log, uint32_t* error) {
+  constexpr int kPieces = kv4_tile_bytes(D) / 16;  // of a tile
   __shared__ int longest_of[kForkThreads / 32];
+  __shared__ int2 takes[kForkPieces];  // of the sequences at hand: source and length, 0 where nothing is taken
   const int tid = threadIdx.x;
   pdl_enter();
   const int64_t most = min(to.max_len, from.max_len);
-  // what a sequence takes: its source (-1: nothing) and its length
-  auto taken = [&](int b, int& source) {
+  auto taken = [&](int b) {
     const int64_t s = sources[b], n = lengths[b];
-    const bool there = s >= 0 && n > 0 && (s != b || to.data != from.data);
-    source = there && s < from.batch && n <= most ? static_cast<int>(s) : -1;
-    if (there && source < 0 && blockIdx.x == 0 && error != nullptr) atomicCAS(error, 0u, static_cast<unsigned>(n > most ? IVB_ECAPACITY : IVB_EINVAL));
-    return source < 0 ? 0 : static_cast<int>(n);
+    const bool wanted = s >= 0 && n > 0 && (s != b || to.data != from.data), there = wanted && s < from.batch && n <= most;
+    if (wanted && !there && blockIdx.x == 0 && error != nullptr) atomicCAS(error, 0u, static_cast<unsigned>(n > most ? IVB_ECAPACITY : IVB_EINVAL));
+    return there ? make_int2(static_cast<int>(s), static_cast<int>(n)) : make_int2(0, 0);
   };
+  const int across = 1 << across_log, together = kForkPieces >> across_log;  // sequences at a time
+  const int blocks = (to.batch + together - 1) / together;
   int longest = 0;
   for (int b = tid; b < to.batch; b += kForkThreads) {
-    int source;
-    longest = max(longest, taken(b, source));
+    const int2 t = taken(b);
+    longest = max(longest, t.y);
+    if (blocks == 1) takes[b] = t;
   }
   longest = __reduce_max_sync(0xFFFFFFFFu, longest);
   if ((tid & 31) == 0) longest_of[tid >> 5] = longest;
@@ -63,63 +67,63 @@ __global__ void __launch_bounds__(kForkThreads) kv4_fork_kernel(IvbKv4Cache to, 
 #pragma unroll
   for (int w = 0; w < kForkThreads / 32; ++w) longest = max(longest, longest_of[w]);
   const int64_t to_step = kv4_tiles(to.max_len) * kPieces, from_step = kv4_tiles(from.max_len) * kPieces;  // of a head
-  const int runs = static_cast<int>(((longest + 15) / 16 * static_cast<int64_t>(kPieces) + across - 1) / across);
-  const int together = kForkThreads * kForkPer / across;  // sequences
-  const int blocks = (to.batch + together - 1) / together;
+  const int runs = static_cast<int>(((longest + 15) / 16 * static_cast<int64_t>(kPieces) + across - 1) >> across_log);
   const int64_t items = static_cast<int64_t>(runs) * to.kv_heads * blocks;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int b0 = static_cast<int>(item % blocks) * together;
     const int64_t rest = item / blocks;
     const int run = static_cast<int>(rest % runs), head = static_cast<int>(rest / runs);
+    if (blocks > 1) {
+      __syncthreads();  // the last item's are no longer read
+      for (int i = tid; i < together && b0 + i < to.batch; i += kForkThreads) takes[i] = taken(b0 + i);
+      __syncthreads();
+    }
+    // a thread's pieces stand at one place of sequences kForkThreads / across apart
+    const int64_t piece = (static_cast<int64_t>(run) << across_log) + (tid & (across - 1));
+    const int first = static_cast<int>(piece / kPieces) * 16;  // position of the piece's tile
+    const int i0 = tid >> across_log, step = kForkThreads >> across_log;
     uint4 v[kForkPer];
-    uint4* at[kForkPer];
-    int left[kForkPer];  // positions taken, from the piece's tile's first on
 #pragma unroll
     for (int i = 0; i < kForkPer; ++i) {
-      const int n = i * kForkThreads + tid, b = b0 + n / across;
-      const int64_t piece = static_cast<int64_t>(run) * across + n % across;
-      left[i] = 0;
-      if (n < together * across && b < to.batch) {
-        int source;
-        const int length = taken(b, source);
-        left[i] = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(16), length - piece / kPieces * 16)));
-        if (left[i] > 0) {
-          v[i] = __ldcg(static_cast<const uint4*>(from.data) + (static_cast<int64_t>(source) * from.kv_heads + head) * from_step + piece);
-          at[i] = static_cast<uint4*>(to.data) + (static_cast<int64_t>(b) * to.kv_heads + head) * to_step + piece;
-        }
-      }
+      const int b = i0 + i * step;
+      if (b0 + b < to.batch && first < takes[b].y)
+        v[i] = __ldcg(static_cast<const uint4*>(from.data) + (static_cast<int64_t>(takes[b].x) * from.kv_heads + head) * from_step + piece);
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kForkPer; ++i) {
-      if (left[i] == 16) {
-        *at[i] = v[i];
-      } else if (left[i] > 0) {  // the positions behind stay as they are
-        const int n = i * kForkThreads + tid;
-        const int word = static_cast<int>((static_cast<int64_t>(run) * across + n % across) % kPieces) * 4;
-        uint32_t* w = reinterpret_cast<uint32_t*>(at[i]);
-        if (kv4_position_of_word<D>(word) < left[i]) w[0] = v[i].x;
-        if (kv4_position_of_word<D>(word + 1) < left[i]) w[1] = v[i].y;
-        if (kv4_position_of_word<D>(word + 2) < left[i]) w[2] = v[i].z;
-        if (kv4_position_of_word<D>(word + 3) < left[i]) w[3] = v[i].w;
+      const int b = i0 + i * step, left = b0 + b < to.batch ? takes[b].y - first : 0;  // positions taken from the tile's first on
+      if (left <= 0) continue;
+      uint4* const at = static_cast<uint4*>(to.data) + (static_cast<int64_t>(b0 + b) * to.kv_heads + head) * to_step + piece;
+      if (left >= 16) {
+        *at = v[i];
+      } else {  // the positions behind stay as they are
+        const int word = static_cast<int>(piece % kPieces) * 4;
+        uint32_t* const w = reinterpret_cast<uint32_t*>(at);
+        if (kv4_position_of_word<D>(word) < left) w[0] = v[i].x;
+        if (kv4_position_of_word<D>(word + 1) < left) w[1] = v[i].y;
+        if (kv4_position_of_word<D>(word + 2) < left) w[2] = v[i].z;
+        if (kv4_position_of_word<D>(word + 3) < left) w[3] = v[i].w;
       }
     }
   }
 }
 
-constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32;
+constexpr int kMoveWarps = 16;  // at most: so many tiles a CTA moves at a time
 
 // One cluster per (sequence, head), a tile of 16 destinations a warp at a time. A row comes from its own place or behind, so a turn's
 // destinations are no later turn's sources: a turn's reads come before its writes (a barrier of the cluster), and the next
-// turn's reads may come before these too.
+// turn's reads may come before these too, as the index of the one after that does. Lane l < 16 holds the source of the tile's position l;
+// a word finds its row's by a shuffle, and moves to the same word of another position: the keys' words are 4 c + w plus what depends on
+// the position alone (kv4_key_word), the values' 16 i + p, the scales' 2 p + w.
 template <int D>
-__global__ void __launch_bounds__(kMoveThreads) kv4_compact_kernel(IvbKv4Cache C, const int64_t* index, const int64_t* positions,
+__global__ void __launch_bounds__(32 * kMoveWarps) kv4_compact_kernel(IvbKv4Cache C, const int64_t* index, const int64_t* positions,
                                                                    const int32_t* starts, int rows, uint32_t* error) {
   constexpr int kTile = kv4_tile_bytes(D), kWords = kTile / 4, kPer = kWords / 32;  // words of a lane: 5, 9 or 17
   static_assert(kWords % 32 == 0, "words of a tile");
   cg::cluster_group cluster = cg::this_cluster();
   const int N = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
   const int unit = blockIdx.x / static_cast<unsigned>(N), b = unit / C.kv_heads, head = unit - b * C.kv_heads;
   pdl_enter();
   int row0 = b, count = 1;
@@ -131,66 +135,64 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_compact_kernel(IvbKv4Cache C
   }
   const int64_t base = kv4_position(positions, b) + before;  // of the first row
   unsigned char* const data = static_cast<unsigned char*>(C.data) + (static_cast<int64_t>(b) * C.kv_heads + head) * kv4_tiles(C.max_len) * kTile;
-  // destinations lo .. hi - 1, a tile of them a warp
-  const int64_t lo = max(base, static_cast<int64_t>(0)), hi = min(base + count, static_cast<int64_t>(C.max_len));
   if (base + count > C.max_len && head == 0 && rank == 0 && error != nullptr) {  // rows beyond the capacity, but for idle ones
-    for (int64_t i = max(static_cast<int64_t>(0), C.max_len - base) + threadIdx.x; i < count; i += kMoveThreads)
+    for (int64_t i = max(static_cast<int64_t>(0), C.max_len - base) + threadIdx.x; i < count; i += 32 * W)
       if (index[row0 + i] >= 0) atomicCAS(error, 0u, static_cast<unsigned>(IVB_ECAPACITY));
   }
-  const int64_t tile0 = lo >> 4, tiles = hi > lo ? ((hi + 15) >> 4) - tile0 : 0, turns = (tiles + N * kMoveWarps - 1) / (N * kMoveWarps);
-  // lane l < 16 has the source of the tile's position l, -1 where nothing is written
-  auto source_of = [&](int64_t turn) {
-    const int64_t t = turn * N * kMoveWarps + rank * kMoveWarps + warp, p = ((tile0 + t) << 4) + lane;
-    if (t >= tiles || lane >= 16 || p < lo || p >= hi) return static_cast<int64_t>(-1);
-    const int64_t s = index[row0 + (p - base)];
-    if (s < 0 || s == p) return static_cast<int64_t>(-1);
+  // destinations lo .. hi - 1, a tile of them a warp
+  const int64_t lo64 = max(base, static_cast<int64_t>(0)), hi64 = min(base + count, static_cast<int64_t>(C.max_len));
+  const int lo = static_cast<int>(min(lo64, static_cast<int64_t>(C.max_len))), hi = static_cast<int>(max(hi64, static_cast<int64_t>(0)));
+  const int tile0 = lo >> 4, tiles = hi > lo ? ((hi + 15) >> 4) - tile0 : 0, each = N * W, turns = (tiles + each - 1) / each;
+  auto tile_of = [&](int turn) { return turn * each + rank * W + warp; };
+  // -1: nothing is written; what index holds is checked when it is there
+  auto ask = [&](int turn) {
+    const int t = tile_of(turn), p = ((tile0 + t) << 4) + lane;
+    return t < tiles && lane < 16 && p >= lo && p < hi ? index[row0 + (p - base)] : static_cast<int64_t>(-1);
+  };
+  auto source_of = [&](int turn, int64_t s) {
+    const int p = ((tile0 + tile_of(turn)) << 4) + lane;
+    if (s < 0 || s == p) return -1;
     if (s < p || s >= C.max_len) {
       if (head == 0 && error != nullptr) atomicCAS(error, 0u, static_cast<unsigned>(s < p ? IVB_EINVAL : IVB_ECAPACITY));
-      return static_cast<int64_t>(-1);
+      return -1;
     }
-    return s;
+    return static_cast<int>(s);
   };
-  auto read = [&](int64_t source, uint32_t (&v)[kPer]) {
+  auto read = [&](int source, uint32_t (&v)[kPer]) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int w = 32 * i + lane, p = kv4_position_of_word<D>(w);
-      const int64_t s = __shfl_sync(0xFFFFFFFFu, source, p);
+      const int w = 32 * i + lane, s = __shfl_sync(0xFFFFFFFFu, source, kv4_position_of_word<D>(w)), q = s & 15;
       if (s >= 0) {
-        const int q = static_cast<int>(s & 15);
-        // the same word of position q (kv4_key_word, kv4_value_word, scales and offsets)
         int from;
         if (w < 2 * D) from = kv4_key_word<D>(q, (w >> (D == 32 ? 1 : 2) & 3) * (D / 32) + (w & (D / 32 - 1)));
         else if (w < 4 * D) from = (w & ~15) | q;
         else from = 4 * D + 2 * q + (w & 1);
-        v[i] = __ldcg(reinterpret_cast<const uint32_t*>(data + (s >> 4) * kTile) + from);
+        v[i] = __ldcg(reinterpret_cast<const uint32_t*>(data + static_cast<int64_t>(s >> 4) * kTile) + from);
       }
     }
   };
+  if (turns == 0) return;  // the whole cluster
   uint32_t next[kPer];
-  int64_t source = source_of(0);
+  int source = source_of(0, ask(0));
+  int64_t asked = ask(1);
   read(source, next);
-  for (int64_t turn = 0; turn < turns; ++turn) {
-    uint32_t v[kPer];
+  for (int turn = 0; turn < turns; ++turn) {
+    uint32_t v[kPer], any = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = next[i];
-    const int64_t mine = source;
-    // the words have to be there before another warp of the cluster writes: used, not only asked for
-    uint32_t any = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) any |= v[i];
-    asm volatile("" ::"r"(any) : "memory");
+    for (int i = 0; i < kPer; ++i) any |= v[i] = next[i];
+    asm volatile("" ::"r"(any) : "memory");  // the words are there
+    const int mine = source;
     if (turn + 1 < turns) {
-      source = source_of(turn + 1);
+      source = source_of(turn + 1, asked);
+      asked = ask(turn + 2);
       read(source, next);
     }
     cluster.sync();
-    const int64_t t = turn * N * kMoveWarps + rank * kMoveWarps + warp;
-    uint32_t* const to = reinterpret_cast<uint32_t*>(data + (tile0 + t) * kTile);
+    uint32_t* const to = reinterpret_cast<uint32_t*>(data + static_cast<int64_t>(tile0 + tile_of(turn)) * kTile);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int w = 32 * i + lane;
-      const int64_t s = __shfl_sync(0xFFFFFFFFu, mine, kv4_position_of_word<D>(w));
-      if (s >= 0) to[w] = v[i];
+      if (__shfl_sync(0xFFFFFFFFu, mine, kv4_position_of_word<D>(w)) >= 0) to[w] = v[i];
     }
   }
 }
@@ -201,14 +203,14 @@ int64_t bytes_of(const IvbKv4Cache& c) { return static_cast<int64_t>(c.batch) * 
 template <int D>
 int32_t launch_fork(const IvbKv4Cache& to, const IvbKv4Cache& from, const int64_t* sources, const int64_t* lengths, uint32_t* error,
                     cudaStream_t stream) {
-  constexpr int kPieces = kForkThreads * kForkPer;
-  int across = 64;
+  // runs of 1 KB, shorter ones where a cache's many sequences would not fit otherwise
+  int across_log = 6;
   if (to.data == from.data)
-    while (across * static_cast<int64_t>(to.batch) > kPieces) across /= 2;
-  const int64_t pieces = kv4_tiles(std::min(to.max_len, from.max_len)) * (kv4_tile_bytes(D) / 16), together = kPieces / across;
-  const int64_t items = (pieces + across - 1) / across * to.kv_heads * ((to.batch + together - 1) / together);
+    while ((static_cast<int64_t>(to.batch) << across_log) > kForkPieces) --across_log;
+  const int64_t pieces = kv4_tiles(std::min(to.max_len, from.max_len)) * (kv4_tile_bytes(D) / 16), together = kForkPieces >> across_log;
+  const int64_t items = ((pieces + (1 << across_log) - 1) >> across_log) * to.kv_heads * ((to.batch + together - 1) / together);
   IVB_CUDA(launch_pdl(kv4_fork_kernel<D>, dim3(static_cast<unsigned>(std::min<int64_t>(items, 148 * 2))), dim3(kForkThreads), 0, stream, to, from,
-                      sources, lengths, across, error));
+                      sources, lengths, across_log, error));
   return IVB_OK;
 }
 
@@ -216,13 +218,16 @@ template <int D>
 int32_t launch_compact(const IvbKv4Cache& c, const int64_t* index, const int64_t* positions, const int32_t* starts, int32_t rows, uint32_t* error,
                        cudaStream_t stream) {
   const int64_t units = static_cast<int64_t>(c.batch) * c.kv_heads;
-  // a cluster where a sequence may have more rows than a CTA moves at a time and the sequences alone leave SMs without work
-  int N = 1;
-  while (N < 8 && units * N < 148 * 4 && rows / c.batch > N * kMoveWarps * 16) N *= 2;
+  // Warps by the rows of a sequence, if they are spread evenly (64 x 16 heads of 1-6 rows: 10 us with 16 warps); a cluster where these are
+  // more than a CTA moves at a time and the sequences alone leave SMs without work.
+  const int64_t tiles = rows / c.batch / 16 + 2;
+  int W = 1, N = 1;
+  while (W < kMoveWarps && W < tiles) W *= 2;
+  while (N < 8 && units * N < 148 * 4 && tiles > N * W) N *= 2;
   if (units * N > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_compact: %d sequences of %d heads", c.batch, c.kv_heads);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(units * N));
-  cfg.blockDim = dim3(kMoveThreads);
+  cfg.blockDim = dim3(static_cast<unsigned>(32 * W));
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -254,8 +259,8 @@ int32_t ivb_kv4_fork(const IvbKv4Cache* c, const IvbKv4Cache* source, const int6
   const bool same = source->data == c->data && source->batch == c->batch && source->max_len == c->max_len;
   const char *a = static_cast<const char*>(c->data), *b = static_cast<const char*>(source->data);
   if (!same && a < b + bytes_of(*source) && b < a + bytes_of(*c)) return fail(IVB_EINVAL, "ivb_kv4_fork: the caches share memory");
-  if (same && c->batch > kForkThreads * kForkPer)
-    return fail(IVB_EINVAL, "ivb_kv4_fork: %d sequences within one cache (%d at most)", c->batch, kForkThreads * kForkPer);
+  if (same && c->batch > kForkPieces)
+    return fail(IVB_EINVAL, "ivb_kv4_fork: %d sequences within one cache (%d at most)", c->batch, kForkPieces);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c->head_dim == 32) return launch_fork<32>(*c, *source, sources, lengths, error, s);
   if (c->head_dim == 64) return launch_fork<64>(*c, *source, sources, lengths, error, s);

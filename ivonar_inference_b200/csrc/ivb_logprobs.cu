@@ -29,7 +29,9 @@ namespace cg = cooperative_groups;
 constexpr int kLogThreads = 256, kMostTop = 256, kBatch = 16;  // values of a thread at a time
 constexpr int kWarps = kLogThreads / 32, kSpan = kLogThreads * kBatch;
 constexpr int kSlack = 96, kRoom = 32 * kBatch + kSlack;  // a warp's list: one turn's values and what it had before
-constexpr int kRankAll = 512;  // so many are ranked each against all; more are first cut to the largest `top`
+constexpr int kFewTop = 64;
+// So many keys are ranked each against all; of more the largest `top` are found first, bit by bit (against all, 256 x 32768 with top = 128 took 164 us).
+constexpr int kRankAll = 384;
 constexpr unsigned kAbsent = 0x7fffffffu;  // of a slice that does not hold the token
 constexpr float kLeast = -200.0f;  // 2^-200 is zero in fp32: keeps -inf * 0 out of the third sum
 
@@ -91,15 +93,17 @@ struct Shared {
   Key best[kMostTop];
   Stats warps[kWarps], all;
   float bounds[kWarps];
-  int counts[kWarps], have, found, over, reached[2];
+  int counts[kWarps], have, found, over, reached[3];
 };
 
-// Ranks the best and all that is noted: the `top` largest become the best, nothing is noted then. All threads; barriers on both sides.
-__device__ void rank_keys(Shared& sh, int top) {
+// The `top` largest of the best and all that is noted become the best, in order if `in_order`; nothing is noted then. Returns a key
+// that `top` keys at least reach, 0 where there are fewer. All threads; barriers on both sides.
+__device__ Key rank_keys(Shared& sh, int top, bool in_order) {
   const int tid = threadIdx.x;
   __syncthreads();
   const int have = sh.have;
   int n = have, before = have;
+  Key at = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     before += w < (tid >> 5) ? sh.counts[w] : 0;
@@ -114,26 +118,52 @@ __device__ void rank_keys(Shared& sh, int top) {
     for (int i = tid; i < have; i += kLogThreads) sh.list[i] = sh.best[i];
     for (int i = tid & 31; i < sh.counts[tid >> 5]; i += 32) sh.list[before + i] = sh.noted[tid >> 5][i];
   } else {
-    // the top-th largest key, bit by bit: the largest value that at least `top` keys reach
-    Key at = 0;
-    if (tid < 2) sh.reached[tid] = 0;
-    if (tid == 2) sh.found = 0;
+    // the largest value that at least `top` keys reach, until just these do. A thread keeps its first keys.
+    constexpr int kKept = 5;
+    Key kept[kKept];
+    auto key_at = [&](int i) {
+      if (i < have) return sh.best[i];
+      i -= have;
+      int w = 0;
+      while (i >= sh.counts[w]) i -= sh.counts[w++];
+      return sh.noted[w][i];
+    };
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) kept[i] = i * kLogThreads + tid < n ? key_at(i * kLogThreads + tid) : 0;
+    const bool all_kept = n <= kKept * kLogThreads;
+    if (tid < 3) sh.reached[tid] = 0;
+    if (tid == 3) sh.found = 0;
     __syncthreads();
     for (int bit = 63; bit >= 0; --bit) {
       const Key trial = at | Key(1) << bit;
       int mine = 0;
-      each([&](Key k) { mine += k >= trial; });
+      if (all_kept) {
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) mine += kept[i] >= trial;
+      } else {
+        each([&](Key k) { mine += k >= trial; });
+      }
       mine = __reduce_add_sync(0xFFFFFFFFu, mine);
-      if ((tid & 31) == 0 && mine != 0) atomicAdd(&sh.reached[bit & 1], mine);
+      if ((tid & 31) == 0 && mine != 0) atomicAdd(&sh.reached[bit % 3], mine);
       __syncthreads();
-      if (sh.reached[bit & 1] >= top) at = trial;
-      if (tid == 0) sh.reached[(bit & 1) ^ 1] = 0;
-      __syncthreads();
+      const int reached = sh.reached[bit % 3];
+      if (reached >= top) at = trial;
+      if (reached == top) break;
+      if (tid == 0) sh.reached[(bit + 1) % 3] = 0;  // read before the barrier, and next used after another one
     }
+    __syncthreads();
     each([&](Key k) {
       if (k >= at) sh.list[atomicAdd(&sh.found, 1)] = k;  // keys differ: `top` of them
     });
     n = top;
+    __syncthreads();
+    if (!in_order) {
+      for (int i = tid; i < top; i += kLogThreads) sh.best[i] = sh.list[i];
+      if (tid < kWarps) sh.counts[tid] = 0;
+      if (tid == kWarps) sh.have = top;
+      __syncthreads();
+      return at;
+    }
   }
   __syncthreads();
   // each key against all, by 1 to 8 neighbouring lanes
@@ -155,6 +185,7 @@ __device__ void rank_keys(Shared& sh, int top) {
   if (tid < kWarps) sh.counts[tid] = 0;
   if (tid == kWarps) sh.have = min(n, top);
   __syncthreads();
+  return n < top ? 0 : sh.best[top - 1];
 }
 
 // Notes up to `top` keys of an ordered list that ends in zeros; a whole warp, its own list is empty.
@@ -240,7 +271,7 @@ __global__ void __launch_bounds__(kLogThreads, 4) log_probs_kernel(LogProbs p) {
   int noted = 0;  // by this warp, since the last ranking
   if (kTop && tid == 0) sh.have = sh.over = 0;
   uint4 next[U];
-  // What is noted is ranked, and the bound raised to the top-th largest, after the turns 0, 1, 3, 7, ...: between them warps need not wait
+  // What is noted is ranked, and the bound raised to the top-th largest, after the turns 0, 3, 15, ...: between them warps need not wait
   // for one another. A row that notes more than there is room for (one in ascending order does) is read again, and ranked after every turn.
   bool careful = false;
   const uint4* const begin = at;
@@ -308,29 +339,49 @@ scan:
         }
       };
       if (turn == 0) {
-        // each warp's r-th largest of its lanes' maxima, with r = top / 8 rounded up: `top` values at least reach the least of these.
-        // (The top-th largest of all 256, each ranked against all, is a closer bound, but took 1.6 us of each CTA.)
-        uint32_t own = ordered(most), reached = 0;
-        for (int r = 0; r < p.top; r += kWarps) {
-          reached = __reduce_max_sync(0xFFFFFFFFu, own);
-          const unsigned who = __ballot_sync(0xFFFFFFFFu, own == reached);
-          if (lane == __ffs(who) - 1) own = 0;
-        }
-        if (lane == 0) sh.bounds[warp] = unordered(reached);
-        __syncthreads();
-        bound = sh.bounds[0];
+        if (p.top <= kFewTop) {
+          // Each warp's r-th largest of its lanes' maxima, with r = top / 8 rounded up: `top` values at least reach the least of these.
+          // (The top-th largest of all 256, each ranked against all, is a closer bound, but took 1.6 us of each CTA.)
+          uint32_t own = ordered(most), reached = 0;
+          for (int r = 0; r < p.top; r += kWarps) {
+            reached = __reduce_max_sync(0xFFFFFFFFu, own);
+            const unsigned who = __ballot_sync(0xFFFFFFFFu, own == reached);
+            if (lane == __ffs(who) - 1) own = 0;
+          }
+          if (lane == 0) sh.bounds[warp] = unordered(reached);
+          __syncthreads();
+          bound = sh.bounds[0];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) bound = fminf(bound, sh.bounds[w]);
+          for (int w = 1; w < kWarps; ++w) bound = fminf(bound, sh.bounds[w]);
+        } else {
+          // the upper 16 bits of the top-th largest value's key, bit by bit (with as many maxima the bound would pass a third of all values:
+          // 338 us for 256 x 32768 with top = 256)
+          if (tid < 3) sh.reached[tid] = 0;
+          __syncthreads();
+          uint32_t key = 0;
+          for (int bit = 31; bit >= 16; --bit) {
+            const float trial = unordered(key | 1u << bit);  // a NaN above all: reached by none
+            int mine = 0;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) mine += v[i] >= trial;
+            mine = __reduce_add_sync(0xFFFFFFFFu, mine);
+            if (lane == 0 && mine != 0) atomicAdd(&sh.reached[bit % 3], mine);
+            __syncthreads();
+            if (sh.reached[bit % 3] >= p.top) key |= 1u << bit;
+            if (tid == 0) sh.reached[(bit + 1) % 3] = 0;
+          }
+          bound = key > ordered(-INFINITY) ? unordered(key) : -INFINITY;
+        }
         if (bound == -INFINITY) note(std::true_type{}, std::true_type{});
         else if (__any_sync(0xFFFFFFFFu, !(most < bound))) note(std::true_type{}, std::false_type{});
       } else if (__any_sync(0xFFFFFFFFu, most > bound)) {
         note(std::false_type{}, std::false_type{});  // later tokens: as large as the bound is too late
       }
-      if (turn + 1 < turns && (careful || (turn & (turn + 1)) == 0)) {
+      if (turn + 1 < turns && (careful || ((turn & (turn + 1)) == 0 && (turn + 1 & 0x55555555) != 0))) {
         if (lane == 0) sh.counts[warp] = noted;
         noted = 0;
-        rank_keys(sh, p.top);
-        if (sh.have == p.top) bound = unordered(static_cast<uint32_t>(sh.best[p.top - 1] >> 32));
+        const Key least = rank_keys(sh, p.top, false);
+        if (least != 0) bound = fmaxf(bound, unordered(static_cast<uint32_t>(least >> 32)));
       }
     }
   }
@@ -357,10 +408,13 @@ scan:
     mine = join(mine, {__shfl_xor_sync(0xFFFFFFFFu, mine.m, d), __shfl_xor_sync(0xFFFFFFFFu, mine.s, d), __shfl_xor_sync(0xFFFFFFFFu, mine.t, d)}, c);
   if (lane == 0) sh.warps[warp] = mine;
   __syncthreads();
-  Stats all = sh.warps[0];
+  Stats all = sh.warps[lane & (kWarps - 1)];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) all = join(all, sh.warps[w], c);
-  if constexpr (kTop) rank_keys(sh, p.top);
+  for (int d = 1; d < kWarps; d <<= 1)
+    all = join(all, {__shfl_xor_sync(0xFFFFFFFFu, all.m, d), __shfl_xor_sync(0xFFFFFFFFu, all.s, d), __shfl_xor_sync(0xFFFFFFFFu, all.t, d)}, c);
+  // one lane's, as the lanes' sums may differ in their last bits
+  all = {__shfl_sync(0xFFFFFFFFu, all.m, 0), __shfl_sync(0xFFFFFFFFu, all.s, 0), __shfl_sync(0xFFFFFFFFu, all.t, 0)};
+  if constexpr (kTop) rank_keys(sh, p.top, true);
   if (C > 1) {
     if (tid == 0) sh.all = all;
     cluster.sync();
@@ -369,7 +423,7 @@ scan:
       if constexpr (kTop) {
         if (warp > 0 && warp < C)
           note_list(sh, warp, p.top, [](const void* from, int i, int) { return static_cast<const Key*>(from)[i]; }, cluster.map_shared_rank(&sh, warp)->best);
-        rank_keys(sh, p.top);
+        rank_keys(sh, p.top, true);
       }
     }
     cluster.sync();  // no CTA leaves while another reads its shared memory
@@ -413,7 +467,7 @@ __global__ void __launch_bounds__(kLogThreads) log_probs_merge_kernel(LogProbs p
           return list[i] == 0 ? Key(0) : key_of(list[i], list[top + i]);
         }, part + (w0 + warp) * step + 3 + p.given);
       else if ((tid & 31) == 0) sh.counts[warp] = 0;
-      rank_keys(sh, p.top);
+      rank_keys(sh, p.top, true);
     }
   }
   finish(p, sh, all, row, [&](int i) {
