@@ -28,6 +28,10 @@ projected per step, at about the latent cache's bytes (whose rotated key channel
 against 1,284 with 16 heads x 64, 4,352 against 4,612 with 32 x 128) and with 4-bit rounding of what is attended to. A step of 24 blocks, 12
 of them attention, 16 heads x 64: 2.9 ms in place of 3.9 (256 sequences at positions 128-640), 2.7 in place of 18.0 (32 at 6,000-8,000;
 2.0 under a window of 1,024); of 4 blocks, 32 heads x 128: 1.0 ms in place of 3.0 (64 sequences at 300-1,900).
+
+Sequences that answer one prompt share what it begins with: `prefix_len` positions of the attention blocks are held once, `start(prefix=)`
+fills them, and every step attends to them and to the sequence's own. `fork` lets sequences go on from where others are (beams, several
+answers from one point on), and `log_probs` gives the log probabilities of given next tokens and the likeliest ones, from every rank's slice of the head.
 """
 
 from __future__ import annotations
@@ -41,6 +45,7 @@ from torch import Tensor
 
 from . import _native as native
 from .kv4 import KV4Cache
+from .logprobs import LogProbs, log_probs, log_probs_merge, log_probs_slice
 from .matrix import DeviceMatrix, rope_from_rotary
 
 
@@ -98,14 +103,16 @@ class B200TensorParallel:
 
     def __init__(self, model, rank: int, world: int, group=None, batch: int = 1, max_len: int = 1024,
                  device: str | torch.device | None = None, max_top_k: int = 256, history_len: int = 1024,
-                 graphs: bool = True, cache: str = "latent", window: int = 0, sinks: int = 0) -> None:
+                 graphs: bool = True, cache: str = "latent", window: int = 0, sinks: int = 0, prefix_len: int = 0) -> None:
         if cache not in ("latent", "kv4"):
             raise ValueError("cache must be 'latent' or 'kv4'")
         if cache == "latent" and (window != 0 or sinks != 0):
             raise ValueError("a window needs the kv4 cache")
         if window < 0 or sinks < 0:
             raise ValueError("window and sinks must not be negative")
-        self.cache, self.window, self.sinks = cache, int(window), int(sinks)
+        if prefix_len < 0 or (prefix_len > 0 and cache != "kv4"):
+            raise ValueError("a shared beginning needs the kv4 cache and a capacity")
+        self.cache, self.window, self.sinks, self.prefix_len = cache, int(window), int(sinks), int(prefix_len)
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         self.device, self.rank, self.world, self.group = dev, int(rank), int(world), group
         self.batch, self.max_len, self.max_top_k = int(batch), int(max_len), int(max_top_k)
@@ -194,7 +201,7 @@ class B200TensorParallel:
                 entry = DeviceMatrix([q, mixer.kv_down_proj, k_rope], dev)
                 kn = DeviceMatrix([row_slice(mixer.k_nope_up_proj, h0 * nope, h1 * nope)], dev, scale_align=8)
                 vu = DeviceMatrix([row_slice(mixer.v_up_proj, c0, c1)], dev, scale_align=8)
-                table = rope_from_rotary(mixer.rope, self.max_len).to(dev)
+                table = rope_from_rotary(mixer.rope, self.prefix_len + self.max_len).to(dev)
                 lpad, rpad = (Lt + 15) // 16 * 16, (rope + 7) // 8 * 8
                 if cache == "kv4":
                     store = KV4Cache(B, self.heads_local, hd, self.max_len, device=dev, error=self.error)
@@ -213,6 +220,8 @@ class B200TensorParallel:
                     state.latent_q, state.latent_scale, state.k_rope_cache = (c.data_ptr() for c in latents)
                 self.latent, self.rope, self.nope = Lt, rope, nope
                 layer = {"kind": "mla", "entry": entry, "k_nope_up": kn, "v_up": vu, "cache": store}
+                if self.prefix_len:
+                    layer["prefix"] = KV4Cache(1, self.heads_local, hd, self.prefix_len, device=dev, error=self.error)
             else:
                 raise native.KernelError(f"unsupported mixer for the B200 kernels: {type(mixer).__name__}")
             out = DeviceMatrix([col_slice(mixer.out_proj, c0, c1, keep_bias=rank == 0)], dev)
@@ -252,6 +261,10 @@ class B200TensorParallel:
         self.step_counter = torch.zeros(1, dtype=torch.int32, device=dev)
         self.sampling = torch.ones(3, **f32)
         self.top_k = torch.ones(1, dtype=torch.int64, device=dev)
+        # positions held in the shared beginning, and the sequences' positions from its start on
+        self.prefix_length = torch.zeros(1, dtype=torch.int64, device=dev)
+        self.places = torch.zeros(B, dtype=torch.int64, device=dev) if self.prefix_len else self.positions
+        self._sharing = False
         self.host_position = 0
         self.use_graphs = bool(graphs)
         self._graph: torch.cuda.CUDAGraph | None = None
@@ -324,22 +337,30 @@ class B200TensorParallel:
         self._quant(self.latents, self.latent, None, 0.0)
         self._gemm(layer["k_nope_up"], native.IVB_EPI_STORE, self.k_nope, self.k_nope.shape[1])
         self._gemm(layer["v_up"], native.IVB_EPI_STORE, self.v, self.channels)
-        rc = self.lib.ivb_batch_qk(ctypes.byref(desc), ent.data_ptr(), ld, self.k_nope.data_ptr(), self.positions.data_ptr(), self.batch,
-                                   self.channels, self.latent, self.heads_local, self.head_dim, self.rope, self.nope, self.max_len,
-                                   self.q.data_ptr(), self.k.data_ptr(), self._stream())
+        rc = self.lib.ivb_batch_qk(ctypes.byref(desc), ent.data_ptr(), ld, self.k_nope.data_ptr(), self.places.data_ptr(), self.batch,
+                                   self.channels, self.latent, self.heads_local, self.head_dim, self.rope, self.nope,
+                                   self.prefix_len + self.max_len, self.q.data_ptr(), self.k.data_ptr(), self._stream())
         native.check(rc, "ivb_batch_qk")
+        y, seen = self.y.view(self.batch, self.heads_local, self.head_dim), dict(scale=desc.attn_scale, window=self.window, sinks=self.sinks)
+        if self._sharing:  # a token of the beginning: the sequences are alike, the first one's is held
+            layer["prefix"].append(self.k[:1], self.v[:1], self.prefix_length)
+            layer["prefix"].attention(self.q[:1], self.prefix_length, out=y[:1], **seen)
+            y[1:].copy_(y[:1].expand_as(y[1:]))
+            return
         layer["cache"].append(self.k, self.v, self.positions)
-        layer["cache"].attention(self.q, self.positions, scale=desc.attn_scale, window=self.window, sinks=self.sinks,
-                                 out=self.y.view(self.batch, self.heads_local, self.head_dim))
+        shared = dict(prefix=layer["prefix"], prefix_lengths=self.prefix_length) if self.prefix_len else {}
+        layer["cache"].attention(self.q, self.positions, out=y, **seen, **shared)
 
     @torch.no_grad()
     def step(self, feed: Tensor | None = None, sample: bool = True) -> None:
         """One token for every sequence: `feed` [batch] teacher-forces the input tokens (no sampling)."""
 
-        if self.host_position >= self.max_len:
+        if self.host_position >= self.max_len and not self._sharing:
             raise ValueError("the decoder has no free position left (capacity)")
         if feed is not None:
             self.tokens.copy_(feed.to(self.device, torch.int64))
+        if self.prefix_len:
+            torch.add(self.positions, self.prefix_length, out=self.places)
         st = self._stream()
         head = self.head.desc()
         native.check(self.lib.ivb_batch_embed(ctypes.byref(head), self.tokens.data_ptr(), self.batch, self.hidden,
@@ -371,6 +392,9 @@ class B200TensorParallel:
             self._row_parallel(layer["down"])
         self._quant(self.resid, self.hidden, self.final_norm.data_ptr(), self.final_eps)
         self._gemm(self.head_shard, native.IVB_EPI_STORE, self.logits, self.vloc)
+        if self._sharing:
+            self.prefix_length.add_(1)
+            return
         if sample:
             self._sample(history=True)
         else:
@@ -378,19 +402,33 @@ class B200TensorParallel:
         self.host_position += 1
 
     @torch.no_grad()
-    def start(self, prompts: Tensor, seeds, temperature: float, top_k: int, repetition_penalty: float = 1.0) -> None:
-        """Run the prompts [batch, T] teacher-forced, then configure sampling (per-sequence seeds)."""
+    def start(self, prompts: Tensor, seeds, temperature: float, top_k: int, repetition_penalty: float = 1.0,
+              prefix: Tensor | None = None) -> None:
+        """Run the prompts [batch, T] teacher-forced, then configure sampling (per-sequence seeds).
+
+        `prefix` [n] are the tokens that all prompts begin with, before `prompts`: they take n steps, and the attention blocks hold
+        their keys and values once (`prefix_len` at most).
+        """
 
         if prompts.shape[0] != self.batch:
             raise ValueError(f"prompts must have {self.batch} rows")
+        if prefix is not None and (prefix.ndim != 1 or prefix.shape[0] > self.prefix_len):
+            raise ValueError(f"prefix must be up to {self.prefix_len} tokens (capacity)")
         if temperature <= 0 or repetition_penalty <= 0:
             raise ValueError("temperature and repetition_penalty must be positive")
-        for t in (self.positions, self.seen, self.step_counter, self.error):
+        for t in (self.positions, self.seen, self.step_counter, self.error, self.prefix_length):
             t.zero_()
         for layer in self.layers:
             for buf in layer.get("state", {}).values():
                 buf.zero_()
         self.host_position = 0
+        if prefix is not None:
+            self._sharing = True
+            try:
+                for token in prefix:
+                    self.step(token.expand(self.batch), sample=False)
+            finally:
+                self._sharing = False
         for t in range(int(prompts.shape[1])):
             self.step(prompts[:, t], sample=False)
         self.sampling[0], self.sampling[1], self.sampling[2] = float(temperature), float(repetition_penalty), 1.0 / float(repetition_penalty)
@@ -400,6 +438,41 @@ class B200TensorParallel:
         # the first sampled token comes from the prompt's last logits
         self._sample(history=False)
         self.positions.sub_(1)  # the sampler advanced the position; the sampled token is fed at the same slot
+
+    @torch.no_grad()
+    def fork(self, sources: Tensor) -> None:
+        """Sequence b goes on from where sequence sources[b] is (int64 [batch]; negative or b itself: from where it is): beams that
+        change places, several answers from one point on. What it keeps of its own are its random numbers."""
+
+        if sources.dtype is not torch.int64 or sources.shape != (self.batch,):
+            raise ValueError(f"sources must be an int64 tensor [{self.batch}]")
+        if int(sources.max()) >= self.batch:
+            raise ValueError(f"sources must be below {self.batch}")
+        sources = sources.to(self.device)
+        sources = torch.where(sources < 0, torch.arange(self.batch, device=self.device), sources)
+        lengths = self.positions[sources]
+        for layer in self.layers:
+            if layer["kind"] == "mla" and self.cache == "kv4":
+                layer["cache"].fork(sources, lengths)
+                continue
+            for state in layer["state"].values() if layer["kind"] == "mamba" else layer["cache"]:
+                state.copy_(state[sources])
+        for state in (self.tokens, self.positions, self.seen, self.history, self.logits):
+            state.copy_(state[sources])
+
+    @torch.no_grad()
+    def log_probs(self, tokens: Tensor, top: int = 0, temperature: float = 1.0) -> LogProbs:
+        """`log_probs` of the last step's logits (as the head gives them, without the sampler's penalty): ln p of `tokens` (int64 [batch]
+        or [batch, n] on the device) as the next ones, the entropy, and the `top` likeliest. The same on every rank."""
+
+        if self.world == 1:
+            return log_probs(self.logits, tokens, top, temperature)
+        if top > self.vocab:
+            raise ValueError(f"top {top} of a vocabulary of {self.vocab}")
+        part = log_probs_slice(self.logits, tokens, self.v_range[0], top, temperature)
+        parts = part.new_empty((self.world, *part.shape))
+        torch.distributed.all_gather_into_tensor(parts, part, group=self.group)
+        return log_probs_merge(parts, tokens, top, temperature)
 
     @torch.no_grad()
     def decode(self, steps: int) -> Tensor:

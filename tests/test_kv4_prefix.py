@@ -12,7 +12,7 @@ def test_the_c_entry_points_refuse_bad_arguments() -> None:
     buffer = ctypes.create_string_buffer(1 << 12)
     at = (ctypes.addressof(buffer) + 15) // 16 * 16   # never read: every call is refused before a launch
     cache = native.IvbKv4Cache
-    good, other = cache(at, 2, 2, 64, 16), cache(at, 1, 2, 64, 400)
+    good, other = cache(at, 2, 2, 64, 16), cache(at, 1, 2, 64, 1_000_000)   # long enough for a pass of its own
 
     def call(c=good, prefix=other, lengths=at, groups=None, q=at, dtype=native.IVB_F32, heads=4, starts=None, positions=at, rows=2, window=0, sinks=0,
              out=at, workspace=at, nbytes=1 << 40):
@@ -56,10 +56,12 @@ def test_workspace_sizes() -> None:
         p = native.IvbKv4Prefix(native.IvbKv4Cache(1 << 20, prefixes, kv_heads, dim, prefix_len), 1 << 20, 1 << 20)
         return lib.ivb_kv4_prefix_workspace_bytes(ctypes.byref(c), ctypes.byref(p), dtype, heads, starts, rows)
 
-    for rows, heads, dim in ((4, 16, 64), (64, 16, 64), (96, 32, 128)):
-        n = size(rows, 8, dim, 10000, native.IVB_F32, heads, None, rows)
+    for rows, heads, dim in ((4, 16, 64), (64, 16, 64), (96, 32, 128), (3000, 8, 32)):
+        n = size(rows, 8, dim, 20000, native.IVB_F32, heads, None, rows)
         assert n > 0 and n % (rows * heads * (8 + 4 * dim)) == 0 and n // (rows * heads * (8 + 4 * dim)) <= 16
-        assert size(rows, 8, dim, 100, native.IVB_F32, heads, None, rows) == rows * heads * (8 + 4 * dim)
+        # short beginnings are walked by each row's kernel
+        assert size(rows, 8, dim, 10, native.IVB_F32, heads, None, rows) == 0
+    assert size(3000, 8, 32, 100, native.IVB_F32, 8, None, 3000) == 3000 * 8 * (8 + 4 * 32)
     # a lone sequence's prompt needs none, nor do calls that are refused
     assert size(1, 8, 64, 1000, native.IVB_BF16, 8, 1 << 20, 500) == 0
     assert size(2, 8, 64, 1000, native.IVB_BF16, 9, None, 2) == 0 and size(2, 8, 64, 1000, native.IVB_BF16, 8, None, 0) == 0
