@@ -67,43 +67,50 @@ __global__ void __launch_bounds__(kForkThreads, 2) kv4_fork_kernel(IvbKv4Cache t
 #pragma unroll
   for (int w = 0; w < kForkThreads / 32; ++w) longest = max(longest, longest_of[w]);
   const int64_t to_step = kv4_tiles(to.max_len) * kPieces, from_step = kv4_tiles(from.max_len) * kPieces;  // of a head
-  const int runs = static_cast<int>(((longest + 15) / 16 * static_cast<int64_t>(kPieces) + across - 1) >> across_log);
-  const int64_t items = static_cast<int64_t>(runs) * to.kv_heads * blocks;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int b0 = static_cast<int>(item % blocks) * together;
-    const int64_t rest = item / blocks;
-    const int run = static_cast<int>(rest % runs), head = static_cast<int>(rest / runs);
+  const unsigned runs = static_cast<unsigned>(((longest + 15) / 16 * static_cast<int64_t>(kPieces) + across - 1) >> across_log);
+  const unsigned items = runs * static_cast<unsigned>(to.kv_heads) * static_cast<unsigned>(blocks);  // of 1 KB at least: below 2^32
+  for (unsigned item = blockIdx.x; item < items; item += gridDim.x) {
+    const unsigned rest = item / static_cast<unsigned>(blocks);
+    const int b0 = static_cast<int>(item - rest * blocks) * together;
+    const int head = static_cast<int>(rest / runs), run = static_cast<int>(rest - head * runs);
     if (blocks > 1) {
       __syncthreads();  // the last item's are no longer read
       for (int i = tid; i < together && b0 + i < to.batch; i += kForkThreads) takes[i] = taken(b0 + i);
       __syncthreads();
     }
-    // a thread's pieces stand at one place of sequences kForkThreads / across apart
+    // A thread's pieces stand at one place of sequences kForkThreads / across apart; what has the last one's source, as the answers to one
+    // prompt have, is not read again.
     const int64_t piece = (static_cast<int64_t>(run) << across_log) + (tid & (across - 1));
     const int first = static_cast<int>(piece / kPieces) * 16;  // position of the piece's tile
     const int i0 = tid >> across_log, step = kForkThreads >> across_log;
-    uint4 v[kForkPer];
+    uint4 v[kForkPer], held = make_uint4(0u, 0u, 0u, 0u);
+    unsigned reads = 0;  // which of them are read
+    int last = -1;       // the source at hand
 #pragma unroll
     for (int i = 0; i < kForkPer; ++i) {
       const int b = i0 + i * step;
-      if (b0 + b < to.batch && first < takes[b].y)
-        v[i] = __ldcg(static_cast<const uint4*>(from.data) + (static_cast<int64_t>(takes[b].x) * from.kv_heads + head) * from_step + piece);
+      if (b0 + b < to.batch && first < takes[b].y && takes[b].x != last) {
+        last = takes[b].x;
+        reads |= 1u << i;
+        v[i] = __ldcg(static_cast<const uint4*>(from.data) + (static_cast<int64_t>(last) * from.kv_heads + head) * from_step + piece);
+      }
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kForkPer; ++i) {
       const int b = i0 + i * step, left = b0 + b < to.batch ? takes[b].y - first : 0;  // positions taken from the tile's first on
+      if (reads >> i & 1) held = v[i];
       if (left <= 0) continue;
       uint4* const at = static_cast<uint4*>(to.data) + (static_cast<int64_t>(b0 + b) * to.kv_heads + head) * to_step + piece;
       if (left >= 16) {
-        *at = v[i];
+        *at = held;
       } else {  // the positions behind stay as they are
         const int word = static_cast<int>(piece % kPieces) * 4;
         uint32_t* const w = reinterpret_cast<uint32_t*>(at);
-        if (kv4_position_of_word<D>(word) < left) w[0] = v[i].x;
-        if (kv4_position_of_word<D>(word + 1) < left) w[1] = v[i].y;
-        if (kv4_position_of_word<D>(word + 2) < left) w[2] = v[i].z;
-        if (kv4_position_of_word<D>(word + 3) < left) w[3] = v[i].w;
+        if (kv4_position_of_word<D>(word) < left) w[0] = held.x;
+        if (kv4_position_of_word<D>(word + 1) < left) w[1] = held.y;
+        if (kv4_position_of_word<D>(word + 2) < left) w[2] = held.z;
+        if (kv4_position_of_word<D>(word + 3) < left) w[3] = held.w;
       }
     }
   }

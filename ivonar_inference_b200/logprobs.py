@@ -70,9 +70,10 @@ def _call(what: str, index: int, *args) -> None:
 
 
 def _empty(logits: Tensor, tokens: Tensor, top: int) -> LogProbs:
-    rows, device, empty = logits.shape[0], logits.device, torch.empty
-    return LogProbs(empty(tokens.shape, dtype=torch.float32, device=device), empty(rows, dtype=torch.float32, device=device),
-                    empty(rows, top, dtype=torch.float32, device=device), empty(rows, top, dtype=torch.int64, device=device))
+    # of other types by their own new_empty, and few keywords: each keyword of a creation costs as much as the kernel's launch
+    rows, shape = logits.shape[0], tokens.shape
+    like = logits if logits.dtype is torch.float32 else logits.new_empty(0, dtype=torch.float32)
+    return LogProbs(like.new_empty(shape), like.new_empty(rows), like.new_empty((rows, top)), torch.empty_strided((rows, top), (max(top, 1), 1), dtype=torch.int64, device=logits.device))
 
 
 def log_probs(logits: Tensor, tokens: Tensor, top: int = 0, temperature: float = 1.0) -> LogProbs:
