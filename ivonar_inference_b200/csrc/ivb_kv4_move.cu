@@ -83,25 +83,32 @@ __global__ void __launch_bounds__(kForkThreads, 2) kv4_fork_kernel(IvbKv4Cache t
     const int64_t piece = (static_cast<int64_t>(run) << across_log) + (tid & (across - 1));
     const int first = static_cast<int>(piece / kPieces) * 16;  // position of the piece's tile
     const int i0 = tid >> across_log, step = kForkThreads >> across_log;
+    const int64_t from_stride = from.kv_heads * from_step, to_stride = to.kv_heads * to_step;  // of a sequence
+    const uint4* const source = static_cast<const uint4*>(from.data) + head * from_step + piece;
+    uint4* at = static_cast<uint4*>(to.data) + (b0 + i0) * to_stride + head * to_step + piece;
+    const int there = min(together, to.batch - b0);
     uint4 v[kForkPer], held = make_uint4(0u, 0u, 0u, 0u);
     unsigned reads = 0;  // which of them are read
     int last = -1;       // the source at hand
 #pragma unroll
     for (int i = 0; i < kForkPer; ++i) {
       const int b = i0 + i * step;
-      if (b0 + b < to.batch && first < takes[b].y && takes[b].x != last) {
-        last = takes[b].x;
+      if (b >= there) break;
+      const int2 t = takes[b];
+      if (first < t.y && t.x != last) {
+        last = t.x;
         reads |= 1u << i;
-        v[i] = __ldcg(static_cast<const uint4*>(from.data) + (static_cast<int64_t>(last) * from.kv_heads + head) * from_step + piece);
+        v[i] = __ldcg(source + last * from_stride);
       }
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kForkPer; ++i) {
-      const int b = i0 + i * step, left = b0 + b < to.batch ? takes[b].y - first : 0;  // positions taken from the tile's first on
+    for (int i = 0; i < kForkPer; ++i, at += step * to_stride) {
+      const int b = i0 + i * step;
+      if (b >= there) break;
+      const int left = takes[b].y - first;  // positions taken from the tile's first on
       if (reads >> i & 1) held = v[i];
       if (left <= 0) continue;
-      uint4* const at = static_cast<uint4*>(to.data) + (static_cast<int64_t>(b0 + b) * to.kv_heads + head) * to_step + piece;
       if (left >= 16) {
         *at = held;
       } else {  // the positions behind stay as they are
