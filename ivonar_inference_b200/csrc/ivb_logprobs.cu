@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kLogThreads, 4) log_probs_kernel(LogProbs p) {
   int noted = 0;  // by this warp, since the last ranking
   if (kTop && tid == 0) sh.have = sh.over = 0;
   uint4 next[U];
-  // What is noted is ranked, and the bound raised to the top-th largest, after the turns 0, 7, 63, ...: between them warps need not wait
+  // What is noted is ranked, and the bound raised to the top-th largest, after the turns 0, 3, 15, ...: between them warps need not wait
   // for one another. A row that notes more than there is room for (one in ascending order does) is read again, and ranked after every turn.
   bool careful = false;
   const uint4* const begin = at;
@@ -377,7 +377,7 @@ scan:
       } else if (__any_sync(0xFFFFFFFFu, most > bound)) {
         note(std::false_type{}, std::false_type{});  // later tokens: as large as the bound is too late
       }
-      if (turn + 1 < turns && (careful || ((turn & (turn + 1)) == 0 && (turn + 1 & 0x49249249) != 0))) {
+      if (turn + 1 < turns && (careful || ((turn & (turn + 1)) == 0 && (turn + 1 & 0x55555555) != 0))) {
         if (lane == 0) sh.counts[warp] = noted;
         noted = 0;
         const Key least = rank_keys(sh, p.top, false);
