@@ -194,14 +194,15 @@ __global__ void __launch_bounds__(32 * kMoveWarps) kv4_compact_kernel(IvbKv4Cach
     uint32_t v[kPer], any = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) any |= v[i] = next[i];
-    asm volatile("" ::"r"(any) : "memory");  // the words are there
+    asm volatile("" ::"r"(any) : "memory");  // the words are in registers: no write behind the barrier can change them
     const int mine = source;
     if (turn + 1 < turns) {
       source = source_of(turn + 1, asked);
       asked = ask(turn + 2);
       read(source, next);
     }
-    cluster.sync();
+    // without the fence of a barrier with release, which nobody needs here (with it 31 us for 54,800 rows x 8 heads x 128)
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
     uint32_t* const to = reinterpret_cast<uint32_t*>(data + static_cast<int64_t>(tile0 + tile_of(turn)) * kTile);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
