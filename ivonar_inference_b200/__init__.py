@@ -1,6 +1,6 @@
 """B200-native (sm_100a) Ivonar token loop: decode step, prefill and sampler behind the reference
 decoder interface. The compute path is libivonar_b200.so (include/ivonar_b200.h); see
-``B200Decoder`` (a subclass of the reference's ``StaticDecoder``), ``build_decoder`` and ``KV4Cache``.
+``B200Decoder`` (a subclass of the reference's ``StaticDecoder``), ``build_decoder``, ``KV4Cache`` and ``log_probs``.
 
 The decoder is imported on first use: it needs the reference package, the rest of this one does not."""
 
