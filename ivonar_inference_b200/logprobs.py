@@ -109,7 +109,9 @@ def log_probs_merge(parts: Tensor, tokens: Tensor, top: int = 0, temperature: fl
     """What `log_probs` gives over the whole vocabulary, of the slices' parts [slices, rows, 3 + n + 2 top]; `tokens`, `top` and
     `temperature` are those of the slices' calls. The slices hold `top` tokens at least between them."""
 
-    given = 1 if tokens.ndim == 1 else tokens.shape[-1]
+    if tokens.ndim not in (1, 2):
+        raise ValueError("tokens must be those of the slices' calls")
+    given = 1 if tokens.ndim == 1 else tokens.shape[1]
     rows = tokens.shape[0]
     if (parts.dtype is not torch.int32 or parts.ndim != 3 or parts.shape[0] == 0 or tuple(parts.shape[1:]) != (rows, 3 + given + 2 * top)
             or not parts.is_contiguous() or not parts.is_cuda):

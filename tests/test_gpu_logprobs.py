@@ -78,7 +78,7 @@ def test_orders_that_a_bound_does_not_help(kind, top) -> None:
     """Ties go to the lowest token, and rows whose every turn has larger values than the last are ranked all the same."""
     from ivonar_inference_b200 import log_probs
 
-    for rows, vocab in ((2, 40007), (1, 9001), (600, 5000)):
+    for rows, vocab in ((2, 40007), (1, 9001), (600, 5000), (300, 33001), (1, 300001)):   # up to ten turns a CTA
         gen = torch.Generator(device="cuda").manual_seed(top)
         ramp = torch.arange(vocab, device="cuda") / vocab * 4
         x = {"equal": torch.full((rows, vocab), 1.25, device="cuda"),
