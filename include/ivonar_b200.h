@@ -373,6 +373,12 @@ int32_t ivb_kv4_attention_prefix(const IvbKv4Cache* c, const IvbKv4Prefix* prefi
                                  int32_t heads, const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,
                                  int32_t sinks, void* out, int64_t o_row, int64_t o_head, void* workspace, uint64_t workspace_bytes,
                                  uint32_t* error, void* stream);
+/* Failure-detection probe: ivb_kv4_attention_prefix, but the prompts' kernels, the pass over the prefix among them, issue
+ * no products and their waits run out after 1 ms. */
+int32_t ivb_probe_kv4_prefix_timeout(const IvbKv4Cache* c, const IvbKv4Prefix* prefix, const void* q, int32_t dtype, int64_t q_row, int64_t q_head,
+                                     int32_t heads, const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,
+                                     int32_t sinks, void* out, int64_t o_row, int64_t o_head, void* workspace, uint64_t workspace_bytes,
+                                     uint32_t* error, void* stream);
 /* Failure-detection probe: ivb_kv4_attention, but the prompts' kernel issues no products and its waits run out after 1 ms. */
 int32_t ivb_probe_kv4_timeout(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
                               const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,

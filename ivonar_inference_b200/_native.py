@@ -224,6 +224,7 @@ SIGNATURES = {
     "ivb_decoder_check": (c_int32, [c_void_p, c_void_p]),
 }
 SIGNATURES["ivb_probe_kv4_timeout"] = SIGNATURES["ivb_kv4_attention"]
+SIGNATURES["ivb_probe_kv4_prefix_timeout"] = SIGNATURES["ivb_kv4_attention_prefix"]
 
 _lib: ctypes.CDLL | None = None
 

@@ -827,6 +827,16 @@ int32_t ivb_kv4_attention_prefix(const IvbKv4Cache* c, const IvbKv4Prefix* prefi
                              workspace_bytes, error, stream, false);
 }
 
+int32_t ivb_probe_kv4_prefix_timeout(const IvbKv4Cache* c, const IvbKv4Prefix* prefix, const void* q, int32_t dtype, int64_t q_row, int64_t q_head,
+                                     int32_t heads, const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window,
+                                     int32_t sinks, void* out, int64_t o_row, int64_t o_head, void* workspace, uint64_t workspace_bytes,
+                                     uint32_t* error, void* stream) {
+  if (int32_t rc = ivb::check_kv4(c, "ivb_kv4_attention_prefix")) return rc;
+  if (int32_t rc = ivb::check_prefix(c, prefix)) return rc;
+  return ivb::attention_call(c, prefix, q, dtype, q_row, q_head, heads, starts, positions, rows, scale, window, sinks, out, o_row, o_head, workspace,
+                             workspace_bytes, error, stream, true);
+}
+
 int32_t ivb_probe_kv4_timeout(const IvbKv4Cache* c, const void* q, int32_t dtype, int64_t q_row, int64_t q_head, int32_t heads,
                               const int32_t* starts, const int64_t* positions, int32_t rows, float scale, int32_t window, int32_t sinks,
                               void* out, int64_t o_row, int64_t o_head, uint32_t* error, void* stream) {

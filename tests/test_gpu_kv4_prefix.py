@@ -379,6 +379,37 @@ def test_a_shared_beginning_is_what_each_sequence_could_have_held(room) -> None:
     assert float((got - whole.attention(q[:5], at + 115)).abs().max()) < 1e-5
 
 
+@pytest.mark.parametrize("dtype,dim,heads", [("fp32", 64, 4), ("bf16", 128, 4), ("fp32", 128, 2), ("fp16", 64, 96)])
+def test_waits_of_a_pass_that_run_out_are_reported_and_the_gpu_stays_usable(dtype, dim, heads) -> None:
+    """No products are issued, so that every wait for them gives up after 1 ms: NaN for the rows behind the beginning, and the error word."""
+    import ctypes
+
+    from ivonar_inference_b200 import KernelError, KV4Cache
+    from ivonar_inference_b200 import _native as native
+
+    cache, prefix = KV4Cache(6, 2, dim, 64), KV4Cache(1, 2, dim, 600_000)
+    filled(cache, [64] * 6)
+    filled(prefix, [900], seed=1)
+    q, at, lengths, groups = queries(6, heads, dim, TYPES[dtype]), device([5, 9, 63, 0, -1, 7]), device([900]), device([0, 5], torch.int32)
+    args = dict(prefix=prefix, prefix_lengths=lengths, prefix_groups=groups)
+    want = cache.attention(q, at, **args)
+    out = torch.empty_like(q)
+    shared = native.IvbKv4Prefix(prefix._desc, lengths.data_ptr(), groups.data_ptr())
+    lib, T = native.library(), {"fp32": native.IVB_F32, "fp16": native.IVB_F16, "bf16": native.IVB_BF16}[dtype]
+    nbytes = lib.ivb_kv4_prefix_workspace_bytes(cache._ref, ctypes.byref(shared), T, heads, None, 6)
+    assert nbytes > 0
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    rc = lib.ivb_probe_kv4_prefix_timeout(
+        cache._ref, ctypes.byref(shared), q.data_ptr(), T, q.stride(0), q.stride(1), heads, None, at.data_ptr(), 6, dim**-0.5, 0, 0, out.data_ptr(),
+        out.stride(0), out.stride(1), workspace.data_ptr(), nbytes, cache.error.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert rc == native.IVB_OK
+    with pytest.raises(KernelError, match="error"):
+        cache.check()
+    assert bool(out[:4].isnan().all()) and bool((out[4] == 0).all()) and torch.equal(out[5], want[5])
+    assert torch.equal(cache.attention(q, at, **args), want)
+    cache.check()
+
+
 def test_refusals() -> None:
     from ivonar_inference_b200 import KV4Cache
 
