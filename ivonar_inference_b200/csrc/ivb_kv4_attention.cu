@@ -646,10 +646,11 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   const int64_t slots = 148 * 16;  // warps of this kernel that the GPU holds
   const int64_t reach = A.cache.max_len + (kShared && A.part_stats == nullptr ? static_cast<int64_t>(A.prefix.max_len) : 0);
   int W = 1, C = 1;
-  // Joined, a CTA is a warp for each row and head of its tile at least, up to four, and fills the GPU once: 64 sequences x 16 heads of 10-500
-  // positions behind 8192 40 us with 2 warps, 51 with 8; 96 x 8 heads x 4 of 17-900 behind 30,000 118 with 2, 110 with 4, 115 with 8.
-  const bool joined = kShared && A.part_stats != nullptr;
-  const int64_t fill = joined ? slots : 2 * slots;
+  // Joined behind short histories of their own, a CTA has a warp for each row and head of its tile at least, up to four, and else so many
+  // that all CTAs are on the GPU at once: 64 sequences x 16 heads of 10-500 positions behind 8192 38 us with 2 warps, 39 with 4, 51 with 8 (at
+  // that time); 96 x 8 heads x 4 of 17-900 behind 30,000 118 with 2, 110 with 4, 115 with 8.
+  const bool joined = kShared && A.part_stats != nullptr, brief = joined && A.cache.max_len <= 1024;
+  const int64_t fill = brief ? slots / 2 + 1 : 2 * slots;
   while (W < kMostWarps && ((base * W < fill && reach > W * kKv4Group) || (joined && W < std::min(4, A.group)))) W *= 2;
   while (C < 8 && W == kMostWarps && base * W * C * 2 <= slots && reach > 4 * C * W * kKv4Group) C *= 2;
   if (grid * C > 0x7fffffff) return fail(IVB_EINVAL, "ivb_kv4_attention: %lld tiles of rows in one call", static_cast<long long>(grid));
