@@ -392,7 +392,7 @@ int32_t ivb_probe_kv4_timeout(const IvbKv4Cache* c, const void* q, int32_t dtype
  * that holds a NaN or +inf, or nothing but -inf, has NaN for its values; its ids are tokens of the vocabulary all the same. */
 int32_t ivb_log_probs(const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t stride, const int64_t* tokens, int32_t given,
                       float temperature, int32_t top, float* token_lp, float* entropy, float* top_lp, int64_t* top_ids, void* stream);
-/* The same of a vocabulary that is cut into slices: logits of the tokens v0 .. v0 + vloc - 1 into parts [rows][3 + given + 2 top] (32-bit
+/* The same of a vocabulary that is cut into slices: logits of the tokens v0 .. v0 + vloc - 1 into parts [rows][4 + given + 2 top] (32-bit
  * words), which `world` of (in any order, [world][rows][...], an all-gather's result) are merged into what ivb_log_probs
  * gives for the whole one, up to the order of its sums. `top` is at most the whole vocabulary's size. */
 int32_t ivb_log_probs_slice(const void* logits, int32_t dtype, int32_t rows, int32_t vloc, int32_t v0, int64_t stride, const int64_t* tokens,

@@ -94,28 +94,28 @@ def log_probs(logits: Tensor, tokens: Tensor, top: int = 0, temperature: float =
 
 
 def log_probs_slice(logits: Tensor, tokens: Tensor, v0: int, top: int = 0, temperature: float = 1.0) -> Tensor:
-    """The part of a rank whose `logits` are those of the tokens v0, v0 + 1, ...: int32 [rows, 3 + n + 2 top], for `log_probs_merge`."""
+    """The part of a rank whose `logits` are those of the tokens v0, v0 + 1, ...: int32 [rows, 4 + n + 2 top], for `log_probs_merge`."""
 
     rows, given = _check(logits, tokens, top, temperature)
     if not 0 <= v0 < 2**31 - logits.shape[1]:
         raise ValueError(f"{logits.shape[1]} tokens from {v0} on")
-    parts = logits.new_empty((rows, 3 + given + 2 * top), dtype=torch.int32)
+    parts = logits.new_empty((rows, 4 + given + 2 * top), dtype=torch.int32)
     _call("ivb_log_probs_slice", logits.device.index, logits.data_ptr(), _TYPES[logits.dtype], rows, logits.shape[1], v0, logits.stride(0),
           tokens.data_ptr(), given, temperature, top, parts.data_ptr())
     return parts
 
 
 def log_probs_merge(parts: Tensor, tokens: Tensor, top: int = 0, temperature: float = 1.0) -> LogProbs:
-    """What `log_probs` gives over the whole vocabulary, of the slices' parts [slices, rows, 3 + n + 2 top]; `tokens`, `top` and
+    """What `log_probs` gives over the whole vocabulary, of the slices' parts [slices, rows, 4 + n + 2 top]; `tokens`, `top` and
     `temperature` are those of the slices' calls. The slices hold `top` tokens at least between them."""
 
     if tokens.ndim not in (1, 2):
         raise ValueError("tokens must be those of the slices' calls")
     given = 1 if tokens.ndim == 1 else tokens.shape[1]
     rows = tokens.shape[0]
-    if (parts.dtype is not torch.int32 or parts.ndim != 3 or parts.shape[0] == 0 or tuple(parts.shape[1:]) != (rows, 3 + given + 2 * top)
+    if (parts.dtype is not torch.int32 or parts.ndim != 3 or parts.shape[0] == 0 or tuple(parts.shape[1:]) != (rows, 4 + given + 2 * top)
             or not parts.is_contiguous() or not parts.is_cuda):
-        raise ValueError(f"parts must be a contiguous int32 CUDA tensor [slices, {rows}, {3 + given + 2 * top}]")
+        raise ValueError(f"parts must be a contiguous int32 CUDA tensor [slices, {rows}, {4 + given + 2 * top}]")
     if not 0 <= top <= MOST_TOP or not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"top {top}, temperature {temperature}")
     out = _empty(parts[0], tokens, top)

@@ -123,6 +123,29 @@ def test_rows_with_special_values(dtype) -> None:
         check(log_probs(x, tokens, top=9, temperature=temperature), x, tokens, 9, temperature)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,vocab", [(1, 32768), (300, 9001), (3, 500)])
+def test_tokens_that_are_nearly_certain(rows, vocab, dtype) -> None:
+    """ln p of a token with nearly all of the probability, and the entropy then, to their own last bits: the others' sum r is off by s (above)
+    of itself, ln(1 + r) by that and a rounding, and so is r's part of the entropy, whose terms d e^d have |d| of under 40 here (2^-22 each
+    of d, twice, and of r)."""
+    from ivonar_inference_b200 import log_probs
+    from ivonar_inference_b200.logprobs import log_probs_merge, log_probs_slice
+
+    x, _ = logits_of(rows, vocab, 5, TYPES[dtype], size=1.0)
+    x = x.clamp(-6, 6)
+    tokens = torch.randint(0, vocab, (rows,), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    x[torch.arange(rows, device="cuda"), tokens] = torch.linspace(17, 30, rows, device="cuda").to(x.dtype)
+    given, entropy, _, _ = expected(x, tokens, 0, 1.0)
+    assert float(given.min()) > -32768 * math.exp(0.5 - 17) - 1e-3  # of normal logits e^x is e^0.5 on average
+    n = vocab // 4096 + 1
+    s = 2.0**-22 * (math.log(vocab) + 40) + 16 * n * 2.0**-24 + (n + 13) * 2.0**-21
+    parts = torch.stack([log_probs_slice(x[:, a:b], tokens, a) for a, b in ((0, 100), (100, vocab))])
+    for found in (log_probs(x, tokens), log_probs_merge(parts, tokens)):
+        assert bool(((found.tokens.double() - given).abs() <= s * given.abs()).all())
+        assert bool(((found.entropy.double() - entropy).abs() <= 2 * s * entropy.abs()).all())
+
+
 def test_tokens_of_every_kind() -> None:
     from ivonar_inference_b200 import log_probs
 
