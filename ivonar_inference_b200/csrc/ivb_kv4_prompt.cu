@@ -1,7 +1,8 @@
 // Causal attention over the 4-bit key/value cache for prompts: many rows a sequence, on the 5th-generation tensor cores.
 //
-// One CTA per (sequence, key/value head, 256 rows), 12 warps (narrow passes over shared beginnings differ: PromptMode). Row i of a sequence's head group is token i / group, query head
-// i % group; rows 0..127 and 128..255 are two tiles X of the tensor cores' 128 lanes. Per tile of 128 positions:
+// One CTA per (sequence, key/value head, 256 rows), 12 warps (the narrow passes over shared beginnings differ: PromptMode). Row i of a
+// sequence's head group is token i / group, query head i % group; rows 0..127 and 128..255 are two tiles X of the tensor cores' 128
+// lanes. Per tile of 128 positions:
 //   warps 8..10 (producers) read the codes, expand them to fp16 in shared memory (keys as a K-major operand, values as an
 //     MN-major one: both are position rows of 16-byte channel chunks, so neither is transposed) and compute each
 //     position's terms (scales and offsets; ivb_kv4_attention.cuh);

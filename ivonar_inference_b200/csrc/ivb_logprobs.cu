@@ -10,8 +10,9 @@
 // The `top` largest ride along: a CTA's first 4096 values give a bound below which none of them is, what lies above is noted in shared
 // memory (a test of each thread's maximum of 16, which the sums need anyway), and only those few are ranked. Values are compared as
 // they came, ties by the token, through one 64-bit key; NaN counts as -inf there.
-// Without alternatives the reading bounds it: 2048 x 32768 in fp32 47 us (5.7 TB/s), 1500 x 100003 in bf16 62 (4.8 TB/s). With them noting and ranking do: 84
-// with top = 20 and 100 with top = 2; one row of 32768 6.7 us, 3.4 without.
+// Without alternatives the reading bounds it: 2048 x 32768 in fp32 47 us (5.7 TB/s), 1500 x 100003 in bf16 62 (4.8 TB/s). With them noting and ranking do: 75
+// with top = 20 and 95 with top = 2; one row of 32768 6.5 us, 3.5 without. Rows that rise from token to token (read again) or are constant (all
+// values reach the bound) are the slowest: 256 x 32768 in bf16 265 and 190 us, 20 otherwise.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -70,6 +71,8 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
+// The next float above x; of infinity NaN, which none reaches.
+__device__ __forceinline__ float above(float x) { return unordered(ordered(x) + 1); }
 __device__ __forceinline__ Key key_of(uint32_t value, uint32_t id) { return static_cast<Key>(value) << 32 | (0xffffffffu - id); }
 __device__ __forceinline__ uint32_t id_of(Key k) { return 0xffffffffu - static_cast<uint32_t>(k); }
 
@@ -304,7 +307,7 @@ __global__ void __launch_bounds__(kLogThreads, 4) log_probs_kernel(LogProbs p) {
   const float first_logit = rank == 0 && tid < p.given ? logit_of_token<T>(p, row, tid) : 0.0f;
   float m = -INFINITY;
   float2 s2 = make_float2(0.0f, 0.0f), t2 = s2;  // of even and of odd values
-  float bound = -INFINITY;
+  float edge = -INFINITY;  // the first value that is noted: above the bound, as later tokens as large as it are too late
   int noted = 0;  // by this warp, since the last ranking
   if (kTop && tid == 0) sh.have = sh.over = 0;
   uint4 next[U];
@@ -316,7 +319,10 @@ scan:
   if (turns > 0) load(0, tid, next);
   for (int turn = 0; turn < turns; ++turn) {
     float v[kBatch];
-    unpack(next, v);
+    uint4 now[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = next[u];
+    unpack(now, v);
     if (turn + 1 < turns) load(turn + 1, tid, next);
     float most = -INFINITY;
 #pragma unroll
@@ -336,21 +342,32 @@ scan:
       t2 = __ffma2_rn(make_float2(fmaxf(d.x, kLeast), fmaxf(d.y, kLeast)), e, t2);
     }
     if constexpr (kTop) {
-      // notes the values above the bound (or from it on, NaN too; a bound of -inf also takes places that are none), value after value
-      auto note = [&](auto from_it, auto checked) {
-        constexpr bool kFrom = decltype(from_it)::value, kChecked = decltype(checked)::value;
-        const uint32_t first = static_cast<uint32_t>((static_cast<int64_t>(c0) + turn * kTurn + tid) * E - shift);
+      const uint32_t first = static_cast<uint32_t>((static_cast<int64_t>(c0) + turn * kTurn + tid) * E - shift);  // value 0's place; wraps below zero
+      auto again = [&] {
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const uint32_t id = first + (i / E * kLogThreads * E + i % E);  // wraps below zero
-          bool in = kFrom ? !(v[i] < bound) : v[i] > bound;
-          if constexpr (kChecked) in = in && c0 + turn * kTurn + i / E * kLogThreads + tid < c1 && id < static_cast<uint32_t>(p.vocab);
-          const unsigned who = __ballot_sync(0xFFFFFFFFu, in);
-          if (who != 0) {
-            const int to = noted + __popc(who & ((1u << lane) - 1));
-            if (in && to < kRoom) sh.noted[warp][to] = key_of(ordered(v[i]), id + static_cast<uint32_t>(p.v0));
-            noted += __popc(who);
-          }
+        for (int u = 0; u < U; ++u) asm volatile("" : "+r"(now[u].x), "+r"(now[u].y), "+r"(now[u].z), "+r"(now[u].w));
+        unpack(now, v);
+      };
+      auto place = [&](int i) { return first + i / E * (kLogThreads * E) + i % E; };
+      auto keep = [&](bool in, unsigned who, float value, uint32_t id) {
+        const int to = noted + __popc(who & ((1u << lane) - 1));
+        if (in && to < kRoom) sh.noted[warp][to] = key_of(ordered(value), id + static_cast<uint32_t>(p.v0));
+        noted += __popc(who);
+      };
+      // Notes the values from `edge` on: all lanes' first ones, then their second ones, as they seldom have more than one (the 16 values in turn, a
+      // vote and a branch apiece: 76.9 us for 74.6 with 2048 x 32768 in fp32, top = 20).
+      auto note = [&](float edge) {
+        // unpacked again: values kept for this in each turn took 91 us there
+        again();
+        unsigned mine = 0;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) mine |= v[i] >= edge ? 1u << i : 0u;
+        for (unsigned who; (who = __ballot_sync(0xFFFFFFFFu, mine != 0)) != 0; mine &= mine - 1) {
+          const int at_hand = __ffs(mine) - 1;
+          float value = v[0];
+#pragma unroll
+          for (int i = 1; i < kBatch; ++i) value = at_hand == i ? v[i] : value;
+          keep(mine != 0, who, value, place(at_hand));
         }
         if (noted > kRoom) {
           noted = kRoom;
@@ -358,6 +375,7 @@ scan:
         }
       };
       if (turn == 0) {
+        float bound = -INFINITY;
         if (p.top <= kFewTop) {
           // Each warp's r-th largest of its lanes' maxima, with r = top / 8 rounded up: `top` values at least reach the least of these.
           // (The top-th largest of all 256, each ranked against all, is a closer bound, but took 1.6 us of each CTA.)
@@ -372,9 +390,11 @@ scan:
           bound = sh.bounds[0];
 #pragma unroll
           for (int w = 1; w < kWarps; ++w) bound = fminf(bound, sh.bounds[w]);
-        } else {
-          // the upper 16 bits of the top-th largest value's key, bit by bit (with as many maxima the bound would pass a third of all values:
-          // 338 us for 256 x 32768 with top = 256)
+        }
+        if (bound == -INFINITY) {
+          // Of more, and where a mask leaves warps nothing: the upper 16 bits of the top-th largest value's key, bit by bit (with as many maxima the bound would pass a third of all values:
+          // 338 us for 256 x 32768 with top = 256).
+          again();
           if (tid < 3) sh.reached[tid] = 0;
           __syncthreads();
           uint32_t key = 0;
@@ -391,16 +411,28 @@ scan:
           }
           bound = key > ordered(-INFINITY) ? unordered(key) : -INFINITY;
         }
-        if (bound == -INFINITY) note(std::true_type{}, std::true_type{});
-        else if (__any_sync(0xFFFFFFFFu, !(most < bound))) note(std::true_type{}, std::false_type{});
-      } else if (__any_sync(0xFFFFFFFFu, most > bound)) {
-        note(std::false_type{}, std::false_type{});  // later tokens: as large as the bound is too late
+        if (bound == -INFINITY) {
+          // Fewer than `top` values above -inf, which are noted, and of those that count as -inf the `top` tokens the CTA begins with: what
+          // comes behind these is less than all of them (all noted, a row with 100 tokens allowed took 115 us in place of 9).
+          again();
+          const uint32_t begins = static_cast<uint32_t>(max(static_cast<int64_t>(c0) * E - shift, static_cast<int64_t>(0)));
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const bool in = c0 + i / E * kLogThreads + tid < c1 && place(i) < static_cast<uint32_t>(p.vocab) &&
+                            (v[i] > -INFINITY || place(i) - begins < static_cast<uint32_t>(p.top));
+            const unsigned who = __ballot_sync(0xFFFFFFFFu, in);
+            if (who != 0) keep(in, who, v[i], place(i));
+          }
+        } else if (__any_sync(0xFFFFFFFFu, most >= bound)) note(bound);
+        edge = above(bound);
+      } else if (__any_sync(0xFFFFFFFFu, most >= edge)) {
+        note(edge);
       }
       if (turn + 1 < turns && (careful || ((turn & (turn + 1)) == 0 && (turn + 1 & 0x55555555) != 0))) {
         if (lane == 0) sh.counts[warp] = noted;
         noted = 0;
         const Key least = rank_keys(sh, p.top, false);
-        if (least != 0) bound = fmaxf(bound, unordered(static_cast<uint32_t>(least >> 32)));
+        if (least != 0) edge = fmaxf(edge, above(unordered(static_cast<uint32_t>(least >> 32))));
       }
     }
   }
@@ -414,7 +446,7 @@ scan:
       careful = true;
       noted = 0;
       at = begin;
-      m = bound = -INFINITY;
+      m = -INFINITY;
       s2 = t2 = make_float2(0.0f, 0.0f);
       __syncthreads();
       goto scan;

@@ -146,6 +146,31 @@ def test_tokens_that_are_nearly_certain(rows, vocab, dtype) -> None:
         assert bool(((found.entropy.double() - entropy).abs() <= 2 * s * entropy.abs()).all())
 
 
+@pytest.mark.parametrize("top", [1, 20, 64, 65, 256])
+@pytest.mark.parametrize("rows,vocab", [(1, 32768), (2, 32768), (256, 32768), (3, 300)])
+def test_rows_of_which_a_mask_leaves_little(rows, vocab, top) -> None:
+    """Runs and single tokens allowed, fewer than `top` or more, at the beginning, the end, and where the warps' and the CTAs' parts meet."""
+    from ivonar_inference_b200 import log_probs
+    from ivonar_inference_b200.logprobs import log_probs_merge, log_probs_slice
+
+    for step, (begin, end, every) in enumerate(((0, 7, 1), (0, 100, 1), (vocab - 30, vocab, 1), (vocab // 8 - 3, vocab // 8 + 300, 1), (5, vocab, 1024),
+                                                (vocab // 2, vocab, 2), (0, 1, 1))):
+        for dtype, fill in ((torch.float32, -math.inf), (torch.bfloat16, -math.inf), (torch.float32, math.nan)):
+            x, tokens = logits_of(rows, vocab, 40 + step, dtype, 2)
+            masked = torch.ones(vocab, dtype=torch.bool, device="cuda")
+            masked[begin:end:every] = False
+            if fill == fill:
+                x[:, masked] = fill
+            else:  # these rows have no distribution, and NaN ranks with -inf
+                x[:, masked] = -math.inf
+                x[:, vocab // 3] = fill
+            found = log_probs(x, tokens, top=top)
+            check(found, x, tokens, top, 1.0)
+            cut = vocab // 3 + 1
+            parts = torch.stack([log_probs_slice(x[:, a:b], tokens, a, top) for a, b in ((0, cut), (cut, vocab)) if b > a])
+            assert torch.equal(log_probs_merge(parts, tokens, top).ids, found.ids)
+
+
 def test_tokens_of_every_kind() -> None:
     from ivonar_inference_b200 import log_probs
 
