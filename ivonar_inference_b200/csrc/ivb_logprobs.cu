@@ -458,7 +458,8 @@ scan:
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1)
     mine = join(mine, {__shfl_xor_sync(0xFFFFFFFFu, mine.m, d), 0.0f, __shfl_xor_sync(0xFFFFFFFFu, mine.s, d), __shfl_xor_sync(0xFFFFFFFFu, mine.t, d)}, c);
-  if (mine.s < kSure && mine.m > -INFINITY) {  // NaN: not
+  // By one lane's sum, as the lanes' own may differ in their last bits and what follows needs the whole warp; all have the same maximum.
+  if (__shfl_sync(0xFFFFFFFFu, mine.s, 0) < kSure && mine.m > -INFINITY) {  // NaN: not
     // one lane has the largest, once: the warp's lanes take a turn of that lane's each again, and sum what is not it
     const int sure = __ffs(__ballot_sync(0xFFFFFFFFu, m == mine.m)) - 1;
     float others = 0.0f;

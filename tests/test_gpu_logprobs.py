@@ -146,6 +146,30 @@ def test_tokens_that_are_nearly_certain(rows, vocab, dtype) -> None:
         assert bool(((found.entropy.double() - entropy).abs() <= 2 * s * entropy.abs()).all())
 
 
+@pytest.mark.parametrize("top", [0, 3])
+def test_sums_at_the_border_of_what_counts_as_certain(top) -> None:
+    """Warps whose sums lie within a few steps of 1.125 on both sides, where a lane's sum may be below it and its neighbour's not: a warp holds
+    every eighth run of 128 values of a row of 4096, and each has one large value here."""
+    from ivonar_inference_b200 import log_probs
+
+    rows, vocab = 3000, 4096
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, 4, 8, 128, generator=gen, device="cuda", dtype=torch.float64)
+    sure = torch.randint(0, 512, (rows, 8, 1), generator=gen, device="cuda")
+    x = x.transpose(1, 2).reshape(rows, 8, 512)
+    x.scatter_(2, sure, -math.inf)
+    steps = torch.randint(-3, 4, (rows, 8, 1), generator=gen, device="cuda") * 2.0**-23
+    x += torch.log(0.125 + steps) - torch.logsumexp(x, 2, keepdim=True)
+    x.scatter_(2, sure, 0.0)
+    x = x.view(rows, 8, 4, 128).transpose(1, 2).reshape(rows, vocab).float()
+    # rounded to fp32 the logits move their sum by 2^-24 |x| of each term at most, |x| < 16 here: 0.125 * 16 * 2^-24 = 2^-23
+    sums = x.double().view(rows, 4, 8, 128).exp().sum((1, 3))
+    assert float((sums - 1.125).abs().max()) <= 5 * 2.0**-23 and bool((sums < 1.125).any()) and bool((sums > 1.125).any())
+    tokens = torch.randint(0, vocab, (rows,), generator=gen, device="cuda")
+    tokens[::2] = x[::2].argmax(1)
+    check(log_probs(x, tokens, top=top), x, tokens, top)
+
+
 @pytest.mark.parametrize("top", [1, 20, 64, 65, 256])
 @pytest.mark.parametrize("rows,vocab", [(1, 32768), (2, 32768), (256, 32768), (3, 300)])
 def test_rows_of_which_a_mask_leaves_little(rows, vocab, top) -> None:
