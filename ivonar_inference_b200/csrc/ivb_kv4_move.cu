@@ -131,7 +131,7 @@ constexpr int kMoveWarps = 16;  // at most: so many tiles a CTA moves at a time
 // turn's reads may come before these too, as the index of the one after that does. Lane l < 16 holds the source of the tile's position l;
 // a word finds its row's by a shuffle, and moves to the same word of another position: the keys' words are 4 c + w plus what depends on
 // the position alone (kv4_key_word), the values' 16 i + p, the scales' 2 p + w. Bound by a turn's latency where sequences x heads are few: 54,800
-// rows of four sequences x 8 heads x 128 28.3 us (118 MB, 4.2 TB/s), 64 sequences x 16 heads x 64 of 1-6 rows 2.9.
+// rows of four sequences x 8 heads x 128 29.1 us (118 MB, 4.1 TB/s), 64 sequences x 16 heads x 64 of 1-6 rows 2.9.
 template <int D>
 __global__ void __launch_bounds__(32 * kMoveWarps) kv4_compact_kernel(IvbKv4Cache C, const int64_t* index, const int64_t* positions,
                                                                    const int32_t* starts, int rows, uint32_t* error) {
@@ -193,18 +193,20 @@ __global__ void __launch_bounds__(32 * kMoveWarps) kv4_compact_kernel(IvbKv4Cach
   int64_t asked = ask(1);
   read(source, next);
   for (int turn = 0; turn < turns; ++turn) {
-    uint32_t v[kPer], any = 0;
+    uint32_t v[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) any |= v[i] = next[i];
-    asm volatile("" ::"r"(any) : "memory");  // the words are in registers: no write behind the barrier can change them
+    for (int i = 0; i < kPer; ++i) v[i] = next[i];
     const int mine = source;
+    // This turn's reads are ordered before all of its writes, other warps' and CTAs' too: by a barrier with release and acquire, on the two
+    // sides of what the next turn asks and reads.
+    if (N > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     if (turn + 1 < turns) {
       source = source_of(turn + 1, asked);
       asked = ask(turn + 2);
       read(source, next);
     }
-    // without the fence of a barrier with release, which nobody needs here (with it 31 us for 54,800 rows x 8 heads x 128)
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+    if (N > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else __syncthreads();
     uint32_t* const to = reinterpret_cast<uint32_t*>(data + static_cast<int64_t>(tile0 + tile_of(turn)) * kTile);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {

@@ -188,6 +188,29 @@ def test_rows_move_up(counts, first, max_len, dim) -> None:
         assert np.array_equal(words(cache), want), kind
 
 
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("batch,rows", [(1, 30_000), (3, 9000), (300, 200), (700, 40)])
+def test_sources_that_are_written_in_the_same_turn(batch, rows, dim) -> None:
+    """Rows that move up by less than what is moved at a time: what one warp, or another CTA of the cluster, reads is written by its neighbour
+    in the same turn. Many times over, as an order that is missing shows now and then."""
+    cache = random_cache(batch, 2, dim, rows + 2200, 5)
+    words_of = [np.flatnonzero(places(dim) == p) for p in range(16)]
+    word = torch.from_numpy(np.stack(words_of)).cuda()   # [16 positions, words]
+    at, starts = rows_of(batch, [0] * batch, [rows] * batch)
+
+    def positions(data):   # [batch, heads, positions, words of one]
+        return data.view(torch.int32)[..., word].flatten(2, 3)
+
+    for by in (1, 15, 16, 17, 33, 250, 256, 2047, 2048):
+        before = positions(cache.data)
+        index = torch.arange(by, rows + by, device="cuda").repeat(batch)
+        for _ in range(5):
+            before[:, :, :rows] = before[:, :, by:rows + by].clone()
+            cache.compact(index, at, starts)
+        cache.check()
+        assert torch.equal(positions(cache.data), before), by
+
+
 def test_one_row_a_sequence() -> None:
     cache = random_cache(5, 3, 64, 40, 2)
     before = words(cache)
