@@ -394,7 +394,8 @@ int32_t ivb_log_probs(const void* logits, int32_t dtype, int32_t rows, int32_t v
                       float temperature, int32_t top, float* token_lp, float* entropy, float* top_lp, int64_t* top_ids, void* stream);
 /* The same of a vocabulary that is cut into slices: logits of the tokens v0 .. v0 + vloc - 1 into parts [rows][4 + given + 2 top] (32-bit
  * words), which `world` of (in any order, [world][rows][...], an all-gather's result) are merged into what ivb_log_probs
- * gives for the whole one, up to the order of its sums. `top` is at most the whole vocabulary's size. */
+ * gives for the whole one, up to the order of its sums. `top` is at most the whole vocabulary's size; where the slices hold fewer
+ * tokens between them, the places behind these have token -1 and NaN. */
 int32_t ivb_log_probs_slice(const void* logits, int32_t dtype, int32_t rows, int32_t vloc, int32_t v0, int64_t stride, const int64_t* tokens,
                             int32_t given, float temperature, int32_t top, uint32_t* parts, void* stream);
 int32_t ivb_log_probs_merge(const uint32_t* parts, int32_t world, int32_t rows, int32_t given, float temperature, int32_t top, float* token_lp,

@@ -228,7 +228,7 @@ __device__ __forceinline__ void finish(const LogProbs& p, const Shared& sh, Stat
   for (int i = tid; i < p.given; i += kLogThreads) p.token_lp[row * p.given + i] = fmaf(token_logit(i) - all.m, p.inv_t, -ln_s);
   for (int i = tid; i < p.top; i += kLogThreads) {
     p.top_lp[row * p.top + i] = fmaf(unordered(static_cast<uint32_t>(sh.best[i] >> 32)) - all.m, p.inv_t, -ln_s);
-    p.top_ids[row * p.top + i] = id_of(sh.best[i]);
+    p.top_ids[row * p.top + i] = sh.best[i] == 0 ? -1 : static_cast<int64_t>(id_of(sh.best[i]));  // none: slices of fewer tokens than that
   }
 }
 

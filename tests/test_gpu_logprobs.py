@@ -255,6 +255,19 @@ def test_many_slices() -> None:
     check(log_probs_merge(parts, tokens, 256), x, tokens, 256)
 
 
+def test_slices_of_fewer_tokens_than_alternatives() -> None:
+    from ivonar_inference_b200.logprobs import log_probs_merge, log_probs_slice
+
+    x, tokens = logits_of(5, 30, 1)
+    x[1, :20] = -math.inf
+    for top in (31, 64, 256):
+        for cuts in ([0, 30], [0, 1, 17, 30], list(range(31))):
+            parts = torch.stack([log_probs_slice(x[:, a:b], tokens, a, top) for a, b in zip(cuts, cuts[1:])])
+            found = log_probs_merge(parts, tokens, top)
+            check(found._replace(top=found.top[:, :30], ids=found.ids[:, :30]), x, tokens, 30)
+            assert bool((found.ids[:, 30:] == -1).all()) and bool(found.top[:, 30:].isnan().all())
+
+
 def test_streams_graphs_and_repeated_calls() -> None:
     from ivonar_inference_b200 import log_probs
 
