@@ -115,7 +115,9 @@ struct Shared {
 };
 
 // The `top` largest of the best and all that is noted become the best, in order if `in_order`; nothing is noted then. Returns a key
-// that `top` keys at least reach, 0 where there are fewer. All threads; barriers on both sides.
+// that `top` keys at least reach, 0 where there are fewer. All threads; barriers on both sides. kDistinct: a token is there once, as within a
+// row; slices that were handed in may overlap.
+template <bool kDistinct>
 __device__ Key rank_keys(Shared& sh, int top, bool in_order) {
   const int tid = threadIdx.x;
   __syncthreads();
@@ -171,10 +173,14 @@ __device__ Key rank_keys(Shared& sh, int top, bool in_order) {
     }
     __syncthreads();
     each([&](Key k) {
-      if (k >= at) sh.list[atomicAdd(&sh.found, 1)] = k;  // keys differ: `top` of them
+      if (kDistinct ? k >= at : k > at) sh.list[atomicAdd(&sh.found, 1)] = k;  // `top` of them, or fewer and all others the same
     });
     n = top;
     __syncthreads();
+    if constexpr (!kDistinct) {
+      for (int i = sh.found + tid; i < top; i += kLogThreads) sh.list[i] = at;
+      __syncthreads();
+    }
     if (!in_order) {
       for (int i = tid; i < top; i += kLogThreads) sh.best[i] = sh.list[i];
       if (tid < kWarps) sh.counts[tid] = 0;
@@ -194,8 +200,9 @@ __device__ Key rank_keys(Shared& sh, int top, bool in_order) {
     for (int j = 2 * l; j + 1 < n; j += 2 * lanes) {
       const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(sh.list + j);
       above += (two.x > k) + (two.y > k);
+      if constexpr (!kDistinct) above += (two.x == k && j < i) + (two.y == k && j + 1 < i);
     }
-    if ((n & 1) != 0 && l == 0) above += sh.list[n - 1] > k;
+    if ((n & 1) != 0 && l == 0) above += sh.list[n - 1] > k;  // of equal ones it is the last
     for (int d = 1; d < lanes; d <<= 1) above += __shfl_xor_sync(0xFFFFFFFFu, above, d);
     if (i < n && l == 0 && above < top) sh.best[above] = k;
   }
@@ -431,7 +438,7 @@ scan:
       if (turn + 1 < turns && (careful || ((turn & (turn + 1)) == 0 && (turn + 1 & 0x55555555) != 0))) {
         if (lane == 0) sh.counts[warp] = noted;
         noted = 0;
-        const Key least = rank_keys(sh, p.top, false);
+        const Key least = rank_keys<true>(sh, p.top, false);
         if (least != 0) edge = fmaxf(edge, above(unordered(static_cast<uint32_t>(least >> 32))));
       }
     }
@@ -485,7 +492,7 @@ scan:
     all = join(all, from_lane(all, lane ^ d), c);
   // one lane's, as the lanes' sums may differ in their last bits
   all = from_lane(all, 0);
-  if constexpr (kTop) rank_keys(sh, p.top, true);
+  if constexpr (kTop) rank_keys<true>(sh, p.top, true);
   if (C > 1) {
     if (tid == 0) sh.all = all;
     cluster.sync();
@@ -494,7 +501,7 @@ scan:
       if constexpr (kTop) {
         if (warp > 0 && warp < C)
           note_list(sh, warp, p.top, [](const void* from, int i, int) { return static_cast<const Key*>(from)[i]; }, cluster.map_shared_rank(&sh, warp)->best);
-        rank_keys(sh, p.top, true);
+        rank_keys<true>(sh, p.top, true);
       }
     }
     cluster.sync();  // no CTA leaves while another reads its shared memory
@@ -540,7 +547,7 @@ __global__ void __launch_bounds__(kLogThreads) log_probs_merge_kernel(LogProbs p
           return list[i] == 0 ? Key(0) : key_of(list[i], list[top + i]);
         }, part + (w0 + warp) * step + kHead + p.given);
       else if ((tid & 31) == 0) sh.counts[warp] = 0;
-      rank_keys(sh, p.top, true);
+      rank_keys<false>(sh, p.top, true);
     }
   }
   finish(p, sh, all, row, [&](int i) {

@@ -108,7 +108,7 @@ def log_probs_slice(logits: Tensor, tokens: Tensor, v0: int, top: int = 0, tempe
 def log_probs_merge(parts: Tensor, tokens: Tensor, top: int = 0, temperature: float = 1.0) -> LogProbs:
     """What `log_probs` gives over the whole vocabulary, of the slices' parts [slices, rows, 4 + n + 2 top]; `tokens`, `top` and
     `temperature` are those of the slices' calls. Where the slices hold fewer than `top` tokens between them, the places behind these
-    have the token -1 and NaN."""
+    have the token -1 and NaN. A slice that comes twice counts twice."""
 
     if tokens.ndim not in (1, 2):
         raise ValueError("tokens must be those of the slices' calls")

@@ -268,6 +268,26 @@ def test_slices_of_fewer_tokens_than_alternatives() -> None:
             assert bool((found.ids[:, 30:] == -1).all()) and bool(found.top[:, 30:].isnan().all())
 
 
+def test_slices_that_are_handed_in_more_than_once() -> None:
+    """A part that comes `times` times: each alternative stands there as often, and each token counts as often in the sums."""
+    from ivonar_inference_b200.logprobs import log_probs_merge, log_probs_slice
+
+    for vocab, top, times in ((5000, 256, 2), (5000, 256, 13), (5000, 20, 3), (5000, 200, 2), (300, 1, 9), (5000, 255, 8), (40, 256, 20)):
+        x, tokens = logits_of(4, vocab, 2)
+        x[1] = 0.0
+        part = log_probs_slice(x, tokens, 0, top)
+        found = log_probs_merge(part.expand(times, *part.shape).contiguous(), tokens, top)
+        many = min(vocab, -(-top // times))
+        given, _, best, ids = expected(x, tokens, many, 1.0)
+        have = min(top, times * many)
+        assert torch.equal(found.ids[:, :have], ids.repeat_interleave(times, 1)[:, :have]), (vocab, top, times)
+        assert bool((found.ids[:, have:] == -1).all())
+        # s of `check` is 1.1e-5 here, up to 20 joins of slices add 2^-21 each, and |ln p| < 30 adds 2^-22 of itself: 2.8e-5
+        tol = 2.0**-15
+        close(found.tokens, given - math.log(times), tol)
+        close(found.top[:, :have], (best - math.log(times)).repeat_interleave(times, 1)[:, :have], tol)
+
+
 def test_streams_graphs_and_repeated_calls() -> None:
     from ivonar_inference_b200 import log_probs
 
