@@ -114,6 +114,8 @@ def log_probs_merge(parts: Tensor, tokens: Tensor, top: int = 0, temperature: fl
         raise ValueError("tokens must be those of the slices' calls")
     given = 1 if tokens.ndim == 1 else tokens.shape[1]
     rows = tokens.shape[0]
+    if rows >= 2**28 or given >= 2**24:
+        raise ValueError(f"{rows} rows of {given} tokens in one call")
     if (parts.dtype is not torch.int32 or parts.ndim != 3 or parts.shape[0] == 0 or tuple(parts.shape[1:]) != (rows, 4 + given + 2 * top)
             or not parts.is_contiguous() or not parts.is_cuda):
         raise ValueError(f"parts must be a contiguous int32 CUDA tensor [slices, {rows}, {4 + given + 2 * top}]")

@@ -60,3 +60,14 @@ def test_refusals() -> None:
     for bad in (x[0], x.double(), x.long(), x[:, :0], x[None]):
         with pytest.raises(ValueError, match="logits must be"):
             log_probs(bad, tokens)
+
+
+def test_a_merge_refuses_sizes_that_a_slice_refuses() -> None:
+    """Sizes that 32 bits do not hold would be cut to their low ones in the call."""
+    from ivonar_inference_b200.logprobs import log_probs_merge
+
+    for shape in ((2**28,), (2**32 + 1,), (2, 2**24), (1, 2**32)):
+        tokens = torch.empty(shape, dtype=torch.int64, device="meta")
+        words = 4 + (shape[1] if len(shape) == 2 else 1)
+        with pytest.raises(ValueError, match="in one call"):
+            log_probs_merge(torch.empty(1, shape[0], words, dtype=torch.int32, device="meta"), tokens)
