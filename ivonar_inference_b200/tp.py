@@ -442,12 +442,15 @@ class B200TensorParallel:
     @torch.no_grad()
     def fork(self, sources: Tensor) -> None:
         """Sequence b goes on from where sequence sources[b] is (int64 [batch]; negative or b itself: from where it is): beams that
-        change places, several answers from one point on. What it keeps of its own are its random numbers."""
+        change places, several answers from one point on. What it keeps of its own are its random numbers. Over the 4-bit cache 4,096
+        sequences at most."""
 
         if sources.dtype is not torch.int64 or sources.shape != (self.batch,):
             raise ValueError(f"sources must be an int64 tensor [{self.batch}]")
         if int(sources.max()) >= self.batch:
             raise ValueError(f"sources must be below {self.batch}")
+        if self.cache == "kv4" and self.latent and self.batch > 4096:  # before anything has changed places
+            raise ValueError(f"{self.batch} sequences over the 4-bit cache (4,096 at most)")
         sources = sources.to(self.device)
         sources = torch.where(sources < 0, torch.arange(self.batch, device=self.device), sources)
         lengths = self.positions[sources]

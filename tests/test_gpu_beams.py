@@ -162,3 +162,13 @@ def test_refusals() -> None:
     for bad in (torch.tensor([0, 1], dtype=torch.int32), torch.tensor([0]), torch.tensor([0, 2])):
         with pytest.raises(ValueError, match="sources"):
             tp.fork(bad)
+
+
+def test_a_fork_of_more_sequences_than_a_cache_takes_is_refused_before_anything_moves() -> None:
+    many = decoder(layers=1, batch=4097, max_len=2, history_len=4)
+    many.step(torch.arange(4097) % VOCAB, sample=False)
+    before = [t.clone() for t in (many.tokens, many.positions, many.logits, many.layers[0]["cache"].data)]
+    with pytest.raises(ValueError, match="4097 sequences"):
+        many.fork(torch.zeros(4097, dtype=torch.int64))
+    for was, now in zip(before, (many.tokens, many.positions, many.logits, many.layers[0]["cache"].data)):
+        assert torch.equal(was, now)
