@@ -671,7 +671,7 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
 template <int D, typename T, bool kShared>
 int32_t launch_rows_of(const Kv4Attention& A, cudaStream_t stream) {
   const bool one = A.starts == nullptr;
-  if (one && A.group <= 4) return launch_rows_attention<D, T, true, 1, kShared>(A, stream);
+  if (keeps_rest(A)) return launch_rows_attention<D, T, true, 1, kShared>(A, stream);
   if constexpr (std::is_same<T, float>::value) {
     return launch_rows_attention<D, T, true, 2, kShared>(A, stream);
   } else {

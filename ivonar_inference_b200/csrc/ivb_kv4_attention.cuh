@@ -211,6 +211,9 @@ __device__ __forceinline__ void kv4_join_parts(const Kv4Attention& A, int64_t it
   for (int j = 0; j < n; ++j) v[j] = l == 0.0f ? 0.0f : v[j] * inv;
 }
 
+// Whether 16-bit queries' weights keep their remainder: single tokens of up to four query heads, whose tiles of four rows hold it anyway.
+inline bool keeps_rest(const Kv4Attention& A) { return A.starts == nullptr && A.group <= 4; }
+
 // Prompts: every sequence of the call with more than `few` items (tokens x query heads of a group).
 int32_t launch_kv4_prompts(const Kv4Attention& A, int32_t dtype, int few, cudaStream_t stream);
 // The prefix's parts of the rows of every other sequence, and in how many parts it comes.

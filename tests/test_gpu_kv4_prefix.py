@@ -1,8 +1,7 @@
 """Attention over the 4-bit cache behind beginnings that sequences share, on a B200 against 64 bits.
 
 Tolerances: those of test_gpu_kv4.py, and for the join of up to 17 parts (the prefix's splits and the sequence's own) an exp2 (2^-22) and
-three roundings (2^-24 each) a part, 2^-17.5 in all, twice as it enters values and sums: 2 vmax 2^-17 more. 16-bit queries' weights over a
-prefix are rounded to fp16 however few the rows are.
+three roundings (2^-24 each) a part, 2^-17.5 in all, twice as it enters values and sums: 2 vmax 2^-17 more.
 """
 
 from __future__ import annotations
@@ -130,6 +129,38 @@ def test_long_beginnings_are_split_and_joined(batch, kv_heads, group, length, di
     q = queries(batch, kv_heads * group, dim, TYPES[dtype])
     check(cache, prefix, [length], None, q, [n - 1 for n in own], None, TYPES[dtype])
     check(cache, prefix, [length], None, q, [n - 1 for n in own], None, TYPES[dtype], window=600, sinks=5)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("batch,group,length", [(9, 1, 301), (9, 4, 1281), (70, 4, 1000), (300, 3, 130)])
+def test_single_tokens_weights_keep_their_remainder(batch, group, length, dim, dtype, room) -> None:
+    """16-bit single tokens of up to four query heads a key/value head, whose weights are not rounded, walked or passed: half the positions
+    have the values of the other half with the other sign, so that what is left of them shows a rounding of the weights (2^-11, of values of 1).
+    The tolerance is that of fp32 queries, and half a step of the output: tanh(0.03 / 2), and 1 / 131 where one half has a position more, times
+    1.01 is under 2^-5."""
+    from ivonar_inference_b200 import KV4Cache
+
+    T = TYPES[dtype]
+    cache, prefix = KV4Cache(batch, 2, dim, 20), KV4Cache(1, 2, dim, length + room)
+    channel = (1.0 - 2.0 * (torch.arange(dim, device="cuda") % 3 == 0)).expand(2, dim)
+    for to, n in ((prefix, length), (cache, 20)):
+        k = (torch.arange(n, device="cuda") % 2).float()[:, None, None].expand(n, 2, dim)
+        at, starts = rows_of(to.batch, [0] * to.batch, [n] * to.batch)
+        to.append(k.repeat(to.batch, 1, 1), ((2 * k - 1) * channel).repeat(to.batch, 1, 1), at, starts)
+    gen = torch.Generator(device="cuda").manual_seed(batch)
+    q = (0.06 * torch.rand(batch, 2 * group, 1, generator=gen, device="cuda") - 0.03).expand(batch, 2 * group, dim).to(T) * dim**-0.5
+    own = [b % 20 for b in range(batch)]
+    got = cache.attention(q, device(own), prefix=prefix, prefix_lengths=device([length]))
+    k, v, par = contents(cache.data, dim)
+    pk, pv, _ = contents(prefix.data[:, :, : 2 * ((length + 31) // 32)].contiguous(), dim)
+    for b in range(batch):
+        kk, vv = torch.cat([pk[0][:, :length], k[b]], 1), torch.cat([pv[0][:, :length], v[b]], 1)
+        want = attended(q[b:b + 1], kk, vv, [length + own[b]], dim**-0.5, 0, 0)
+        assert float(want.abs().max()) < 2.0**-5
+        tol = tolerance(q[b:b + 1], 1.0, 1.01, dim**-0.5, want, torch.float32) + 2 * 2.0**-17 + torch.finfo(T).eps / 2 * want.abs()
+        diff = (got[b:b + 1].double().cpu() - want).abs()
+        assert bool((diff <= tol).all()), (b, float((diff - tol).max()), float(diff.max()))
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "fp16"])
