@@ -232,9 +232,14 @@ __device__ __forceinline__ void finish(const LogProbs& p, const Shared& sh, Stat
   const float sum = all.n + all.s;
   const float ln_s = !(sum > 0.0f) ? __uint_as_float(0x7fffffffu) : all.n == 1.0f ? log1pf(all.s) : logf(sum);  // nothing but -inf: no distribution
   if (tid == 0) p.entropy[row] = ln_s - all.t / sum * 0.6931471805599453f;
-  for (int i = tid; i < p.given; i += kLogThreads) p.token_lp[row * p.given + i] = fmaf(token_logit(i) - all.m, p.inv_t, -ln_s);
+  auto log_p = [&](float x) {
+    const float d = x - all.m;
+    if (d > -INFINITY || x == -INFINITY) return fmaf(d, p.inv_t, -ln_s);
+    return x * p.inv_t - all.m * p.inv_t - ln_s;  // further apart than fp32 reaches, which their quotients by T need not be
+  };
+  for (int i = tid; i < p.given; i += kLogThreads) p.token_lp[row * p.given + i] = log_p(token_logit(i));
   for (int i = tid; i < p.top; i += kLogThreads) {
-    p.top_lp[row * p.top + i] = fmaf(unordered(static_cast<uint32_t>(sh.best[i] >> 32)) - all.m, p.inv_t, -ln_s);
+    p.top_lp[row * p.top + i] = log_p(unordered(static_cast<uint32_t>(sh.best[i] >> 32)));
     p.top_ids[row * p.top + i] = sh.best[i] == 0 ? -1 : static_cast<int64_t>(id_of(sh.best[i]));  // none: slices of fewer tokens than that
   }
 }

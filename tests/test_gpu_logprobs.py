@@ -123,6 +123,23 @@ def test_rows_with_special_values(dtype) -> None:
         check(log_probs(x, tokens, top=9, temperature=temperature), x, tokens, 9, temperature)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("temperature", [4.0, 1e30])
+def test_logits_further_apart_than_fp32_reaches(temperature, dtype) -> None:
+    """The lowest and the largest value of the type in one row: their difference is no fp32 number, that over the temperature is one."""
+    from ivonar_inference_b200 import log_probs
+    from ivonar_inference_b200.logprobs import log_probs_merge, log_probs_slice
+
+    x, tokens = logits_of(4, 5000, 6, TYPES[dtype])
+    x[:, ::3] = torch.finfo(TYPES[dtype]).min
+    x[:2, 70] = torch.finfo(TYPES[dtype]).max
+    x[1, 9] = -math.inf
+    given = torch.tensor([0, 9, 70, 71], device="cuda").expand(4, 4).contiguous()
+    check(log_probs(x, given, 5, temperature), x, given, 5, temperature)
+    parts = torch.stack([log_probs_slice(x[:, a:b], given, a, 5, temperature) for a, b in ((0, 60), (60, 5000))])
+    check(log_probs_merge(parts, given, 5, temperature), x, given, 5, temperature)
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("rows,vocab", [(1, 32768), (300, 9001), (3, 500)])
 def test_tokens_that_are_nearly_certain(rows, vocab, dtype) -> None:
