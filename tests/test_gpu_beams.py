@@ -172,3 +172,30 @@ def test_a_fork_of_more_sequences_than_a_cache_takes_is_refused_before_anything_
         many.fork(torch.zeros(4097, dtype=torch.int64))
     for was, now in zip(before, (many.tokens, many.positions, many.logits, many.layers[0]["cache"].data)):
         assert torch.equal(was, now)
+
+
+@pytest.mark.parametrize("cache,prefix_len", [("kv4", 9), ("kv4", 0), ("latent", 0)])
+def test_a_fork_takes_recurrent_states_too(cache, prefix_len) -> None:
+    """Sequences that change places between recurrent and attention blocks go on as if each had read its tokens itself."""
+    from ivonar_inference_b200.tp import B200TensorParallel
+    from test_attention_kv4_decode import hybrid
+
+    model, text = hybrid(["mamba", "mla", "mamba"], 4), tokens(prefix_len, seed=9) if prefix_len else None
+    tp, anew = (B200TensorParallel(model, 0, 1, batch=4, max_len=24, device="cuda:0", cache=cache, prefix_len=prefix_len) for _ in range(2))
+    read = tokens(4, 11, seed=1)
+    tp.start(read[:, :6], [1, 2, 3, 4], 1.0, 1, prefix=text)
+    for t in range(6, 11):
+        tp.step(read[:, t], sample=False)
+    sources = torch.tensor([2, 0, -1, 1])
+    tp.fork(sources)
+    mine = read[torch.tensor([2, 0, 2, 1])]
+    anew.start(mine[:, :6], [1, 2, 3, 4], 1.0, 1, prefix=text)
+    for t in range(6, 11):
+        anew.step(mine[:, t], sample=False)
+    assert torch.equal(tp.logits, anew.logits) and tp.positions.tolist() == anew.positions.tolist()
+    for t in range(5):
+        both = tokens(4, seed=20 + t)
+        tp.step(both, sample=False)
+        anew.step(both, sample=False)
+        assert torch.equal(tp.logits, anew.logits), t
+    assert int(tp.error.item()) == 0
