@@ -647,8 +647,9 @@ int32_t launch_rows_attention(const Kv4Attention& A, cudaStream_t stream) {
   const int64_t reach = A.cache.max_len + (kShared && A.part_stats == nullptr ? static_cast<int64_t>(A.prefix.max_len) : 0);
   int W = 1, C = 1;
   // Joined behind short histories of their own, a CTA has a warp for each row and head of its tile at least, up to four, and else so many
-  // that all CTAs are on the GPU at once: 64 sequences x 16 heads of 10-500 positions behind 8192 38 us with 2 warps, 39 with 4, 51 with 8 (at
-  // that time); 96 x 8 heads x 4 of 17-900 behind 30,000 118 with 2, 110 with 4, 115 with 8.
+  // that all CTAs are on the GPU at once. How long the histories are is known by the cache's capacity alone. Brief / not, the same content: 64
+  // sequences x 16 heads x 64 of 10-500 positions behind 8192 37.7 us (2 warps) / 48.7 (8), in bf16 35.6 / 45.7, 128 of them 52.7 / 57.3; 96 x
+  // 8 heads x 4 of 17-900 behind 30,000 118 (4 warps) / 123; but 64 x 16 heads of 1,000-4,000 behind 8192 99 / 91.
   const bool joined = kShared && A.part_stats != nullptr, brief = joined && A.cache.max_len <= 1024;
   const int64_t fill = brief ? slots / 2 + 1 : 2 * slots;
   while (W < kMostWarps && ((base * W < fill && reach > W * kKv4Group) || (joined && W < std::min(4, A.group)))) W *= 2;

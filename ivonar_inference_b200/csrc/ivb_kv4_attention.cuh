@@ -12,7 +12,8 @@
 // 2^-11 of each at most (the sums that divide them are not), but for the few rows' tiles of four, which hold the remainder anyway. With it
 // the prompts' fp16 calls would be as near as fp32 ones before the output's rounding, but take a second product: a causal prompt of
 // 2048 x 16 heads x 64 53 us in place of 49, a chunk of 2048 under a window of 4096 x 32 heads x 128 267 in place of 230, a mixed call 74
-// in place of 67; for few rows it would take the columns of other rows. Who needs the bits hands in fp32 queries.
+// in place of 67; for few rows it would take the columns of other rows. Who needs the bits hands in fp32 queries. A pass over a shared
+// beginning holds it for the rows whose own tiles do.
 #pragma once
 
 #include "ivb_common.h"

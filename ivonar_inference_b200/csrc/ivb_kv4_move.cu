@@ -127,11 +127,11 @@ __global__ void __launch_bounds__(kForkThreads, 2) kv4_fork_kernel(IvbKv4Cache t
 constexpr int kMoveWarps = 16;  // at most: so many tiles a CTA moves at a time
 
 // One cluster per (sequence, head), a tile of 16 destinations a warp at a time. A row comes from its own place or behind, so a turn's
-// destinations are no later turn's sources: a turn's reads come before its writes (a barrier of the cluster), and the next
+// destinations are no later turn's sources: a turn's reads come before its writes (a barrier with release and acquire), and the next
 // turn's reads may come before these too, as the index of the one after that does. Lane l < 16 holds the source of the tile's position l;
 // a word finds its row's by a shuffle, and moves to the same word of another position: the keys' words are 4 c + w plus what depends on
 // the position alone (kv4_key_word), the values' 16 i + p, the scales' 2 p + w. Bound by a turn's latency where sequences x heads are few: 54,800
-// rows of four sequences x 8 heads x 128 29.1 us (118 MB, 4.1 TB/s), 64 sequences x 16 heads x 64 of 1-6 rows 2.9.
+// rows of four sequences x 8 heads x 128 27.9 us (118 MB, 4.2 TB/s), 64 sequences x 16 heads x 64 of 1-6 rows 2.9.
 template <int D>
 __global__ void __launch_bounds__(32 * kMoveWarps) kv4_compact_kernel(IvbKv4Cache C, const int64_t* index, const int64_t* positions,
                                                                    const int32_t* starts, int rows, uint32_t* error) {

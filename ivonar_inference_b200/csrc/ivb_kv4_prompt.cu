@@ -44,8 +44,9 @@ constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 32 * kSoftmaxWarps;
 // With up to 128 rows a pass runs two streams where tensor memory has room for both: the tiles in turn are row tile 0's and 1's, which hold
 // the same rows and are joined at the end, so that one's softmax runs while the other waits for the tensor cores. Narrow ones have 64 rows,
 // 8 or 16 a warp (the lower ones of its 32 lanes of tensor memory), so that all warps share the softmax, and seven producer warps, four for
-// the keys and three for the values: 16 warps of 128 registers (17 would have 96). Behind 32,768 positions, narrow / wide: 16 heads x 64, 16
-// rows 38 / 52 us, 64 rows 48 / 57, 128 rows 85 / 64; 8 x 128, 256 rows 111 / 78.
+// the keys and three for the values: 16 warps of 128 registers (17 would have 96). Tokens behind 32,768 positions, narrow / wide: in bf16 16 heads
+// x 64, 16 rows 42 / 65 us, 64 rows 51 / 68, 128 rows 92 / 72; 8 x 128, 64 rows 47 / 58, 256 rows 119 / 91; in fp32 47 / 68, 57 / 72, 108 / 77, 62 / 72 and
+// 173 / 114.
 enum PromptMode { kPlain, kBehind, kWide, kNarrow };
 constexpr int kKeyWarps = 4, kValueWarps = 3, kNarrowRows = 64;
 constexpr int producer_warps(PromptMode mode) { return mode == kNarrow ? kKeyWarps + kValueWarps : 3; }

@@ -244,7 +244,7 @@ class KV4Cache:
         sees the positions j <= p with j > p - window, and the first `sinks` positions (window 0: every j <= p). `scale` is
         1 / sqrt(head_dim) by default. `out` may be q itself, but not overlap it otherwise. Products are summed and softmax statistics held in 32 bits.
         With fp32 queries the softmax's weights keep 22 bits; with fp16 and bf16 ones they are rounded to fp16 (by 2^-11 of each at most)
-        before they meet the values, but for single tokens with up to four query heads a key/value head.
+        before they meet the values, but for single tokens (no `starts`) with up to four query heads a key/value head.
         Values that pass fp16 (see `read`) may give infinity in an fp16 result.
 
         With `prefix`, another cache with the same heads, sequences share what they begin with: the sequences prefix_groups[g] ..
