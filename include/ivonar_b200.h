@@ -388,7 +388,7 @@ int32_t ivb_probe_kv4_timeout(const IvbKv4Cache* c, const void* q, int32_t dtype
  * Of rows of logits [rows][vocab] (IVB_F32, IVB_F16 or IVB_BF16, `stride` values from row to row), p = softmax(x / temperature):
  * token_lp [rows][given] = ln p of the tokens [rows][given] (device int64; NaN for one outside the vocabulary),
  * entropy [rows] = -sum p ln p, top_lp and top_ids [rows][top] = ln p of the `top` (0 to 256, at most vocab) likeliest tokens, in
- * descending order of the logits, the lowest of equal ones first. Sums are held in 32 bits. A logit of -inf has no probability. A row
+ * descending order of the logits, the lowest of equal ones first. Sums are held in 32 bits, of exponentials within 2^-22. A logit of -inf has no probability. A row
  * that holds a NaN or +inf, or nothing but -inf, has NaN for its values; its ids are tokens of the vocabulary all the same. */
 int32_t ivb_log_probs(const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t stride, const int64_t* tokens, int32_t given,
                       float temperature, int32_t top, float* token_lp, float* entropy, float* top_lp, int64_t* top_ids, void* stream);

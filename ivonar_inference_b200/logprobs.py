@@ -79,7 +79,7 @@ def _empty(logits: Tensor, tokens: Tensor, top: int) -> LogProbs:
 def log_probs(logits: Tensor, tokens: Tensor, top: int = 0, temperature: float = 1.0) -> LogProbs:
     """ln p of `tokens` (int64 [rows] or [rows, n]) under p = softmax(logits / temperature), with the entropy and the `top` likeliest.
 
-    `logits` is [rows, vocabulary] in fp32, fp16 or bf16, each row contiguous; sums are held in 32 bits. A token outside the
+    `logits` is [rows, vocabulary] in fp32, fp16 or bf16, each row contiguous; sums are held in 32 bits, of exponentials within 2^-22. A token outside the
     vocabulary (padding, such as -1) has NaN. A logit of -inf has no probability; a row that holds a NaN or +inf, or nothing but
     -inf, has NaN for its values and ids that are tokens all the same.
     """
